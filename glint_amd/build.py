@@ -6,6 +6,7 @@
 Outputs (git-ignored, shipped with the tree):
     glint_amd/lib/libglint_encode.so   encode / expand / H-TILE (include/glint_encode.h, glint_htile.h)
     glint_amd/lib/libp7_kernels.so     attach ABI: INT8 GEMM (include/int8_mma_gemm.h, p7_attach.h)
+    glint_amd/lib/libglint_serve.so    4-bit key/value cache, attention, token scores (include/glint_serve.h)
     glint_amd/lib/libglint_probe.so    bench.py's HBM read ceiling (measurement only)
     glint_amd/lib/libglint_encode_tl.so  libglint_encode.so with the decode GEMV's per-wave
                                        timeline stamps (bench.py --timeline; measurement only)
@@ -41,6 +42,7 @@ HIP_FLAGS = [
 LIBS = {
     "libglint_encode.so": ["glint_encode.hip", "glint_htile.hip", "glint_select.hip", "glint_noalloc.hip"],
     "libp7_kernels.so": ["int8_mma_gemm.hip", "int8_tile_gemm.hip", "p7_abi.cpp", "glint_plug_streamer.cpp", "p7_selftest.cpp"],
+    "libglint_serve.so": ["glint_kv4.hip", "glint_kv4_attend.hip", "glint_attend_prompt.hip", "glint_logprobs.hip"],
     # measurement only (bench.py's read ceiling), not part of the GLINT ABI
     "libglint_probe.so": ["hbm_probe.hip"],
     # measurement only (bench.py --timeline): libglint_encode.so with the decode GEMV's

@@ -1,10 +1,10 @@
-"""ctypes bindings to the GLINT C ABI (libglint_encode.so, libp7_kernels.so).
+"""ctypes bindings to the GLINT C ABI (libglint_encode.so, libp7_kernels.so, libglint_serve.so).
 
 Two layers:
 
-* ``EncodeLib`` / ``P7Lib``: the raw C entry points with their argtypes, as a caller of
+* ``EncodeLib`` / ``P7Lib`` / ``ServeLib``: the raw C entry points with their argtypes, as a caller of
   the reference's ``glint_cuda.py`` would bind them (the host-pointer ABI takes bytes);
-* tensor helpers (``encode_bf16`` ... ``int8_gemm_i32``) that pass torch device tensors
+* tensor helpers (``encode_bf16`` ... ``token_logprobs``) that pass torch device tensors
   and torch's current stream straight to the device entry points. torch is only the
   allocator and stream here; every result is computed by the HIP kernels.
 
@@ -13,9 +13,10 @@ A missing library raises RuntimeError: there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 from pathlib import Path
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Tuple
 
 PKG = Path(__file__).resolve().parent
 LIB_DIR = PKG / "lib"
@@ -40,6 +41,15 @@ def p7_lib_path() -> Optional[Path]:
         p = Path(env)
         return p if p.is_file() else None
     p = LIB_DIR / "libp7_kernels.so"
+    return p if p.is_file() else None
+
+
+def serve_lib_path() -> Optional[Path]:
+    env = os.environ.get("GLINT_SERVE_SO")
+    if env:
+        p = Path(env)
+        return p if p.is_file() else None
+    p = LIB_DIR / "libglint_serve.so"
     return p if p.is_file() else None
 
 
@@ -107,8 +117,20 @@ _P7_SIGS = {
     "glint_plug_streamer_reset_stats": ([VP], None),
 }
 
+_SERVE_SIGS = {
+    "glint_kv4_append": ([VP, VP, I32, I64, I64, I64, I64, VP, I64, I32, I32, VP, VP, VP, VP, I64, VP], I32),
+    "glint_kv4_gather": ([VP, I64, I32, I32, VP, VP, VP, VP, I64, VP, VP, VP], I32),
+    "glint_kv4_attend_part": ([I32, I32, I32, I32, I32, I32], I64),
+    "glint_kv4_attend": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32,
+                          _c.c_float, VP, VP, VP], I32),
+    "glint_attend_prompt": ([VP, I64, I64, VP, I64, I64, VP, I64, I64, VP, VP, I64, I64, I32, I32, I32, I32, I32,
+                             _c.c_float, VP, VP], I32),
+    "glint_token_logprobs": ([VP, I32, I64, VP, I64, I64, I32, VP, VP, VP, VP, VP, VP], I32),
+}
+
 ENCODE_SYMBOLS = tuple(_ENCODE_SIGS)
 P7_SYMBOLS = tuple(_P7_SIGS)
+SERVE_SYMBOLS = tuple(_SERVE_SIGS)
 
 
 def _bind(path: Path, sigs: dict) -> ctypes.CDLL:
@@ -129,6 +151,7 @@ def _bind(path: Path, sigs: dict) -> ctypes.CDLL:
 
 _ENC: Optional[ctypes.CDLL] = None
 _P7: Optional[ctypes.CDLL] = None
+_SERVE: Optional[ctypes.CDLL] = None
 
 
 def encode_lib() -> ctypes.CDLL:
@@ -163,6 +186,16 @@ def p7_lib() -> ctypes.CDLL:
             raise RuntimeError("libp7_kernels.so not built: run `python -m glint_amd.build`")
         _P7 = _bind(p, _P7_SIGS)
     return _P7
+
+
+def serve_lib() -> ctypes.CDLL:
+    global _SERVE
+    if _SERVE is None:
+        p = serve_lib_path()
+        if p is None:
+            raise RuntimeError("libglint_serve.so not built: run `python -m glint_amd.build`")
+        _SERVE = _bind(p, _SERVE_SIGS)
+    return _SERVE
 
 
 def _check(rc: int, what: str) -> None:
@@ -474,6 +507,234 @@ def int8_gemm_scaled_bf16(A, B, sa, sb, out=None, stream=None):
     _check(p7_lib().glint_int8_gemm_scaled_bf16(A.data_ptr(), B.data_ptr(), sa.data_ptr(), sb.data_ptr(),
                                                 out.data_ptr(), M, N, K, _sh(stream)), "glint_int8_gemm_scaled_bf16")
     return out
+
+
+# ------------------------------------------------- between the linears (glint_serve.h)
+# Every helper here takes stream= (default: the current stream).
+KV_PAGE = 64
+
+
+def _on_stream(f):
+    """With a stream given, the whole call (its outputs, scratch and copies too) belongs to it."""
+    @functools.wraps(f)
+    def call(*args, stream=None, **kw):
+        if stream is None:
+            return f(*args, **kw)
+        with _torch().cuda.stream(stream):
+            return f(*args, **kw)
+    return call
+
+
+def _on_gpu(*tensors) -> None:
+    if not all(t.is_cuda for t in tensors):
+        raise ValueError(f"tensors on {', '.join(str(t.device) for t in tensors)}: all must be on the GPU")
+
+
+class Kv4Cache(NamedTuple):
+    """The 4-bit key/value cache's planes (glint_serve.h); any four tensors in this order do."""
+    k_hole: "object"    # u8 [pages, H, 64, D / 2]
+    k_absmax: "object"  # f32 [pages, H, D / 64, 64]
+    v_hole: "object"    # u8 [pages, H, D / 2, 64]
+    v_absmax: "object"  # f32 [pages, H, D / 64, 64]
+
+
+def kv4_cache(pages: int, heads: int, dim: int, device="cuda") -> Kv4Cache:
+    """An empty cache of pages of 64 tokens (every element zero)."""
+    torch = _torch()
+    if dim not in (64, 128):
+        raise ValueError(f"head dimension {dim}: 64 or 128")
+    scales = lambda: torch.zeros((pages, heads, dim // 64, KV_PAGE), dtype=torch.float32, device=device)
+    return Kv4Cache(torch.zeros((pages, heads, KV_PAGE, dim // 2), dtype=torch.uint8, device=device), scales(),
+                    torch.zeros((pages, heads, dim // 2, KV_PAGE), dtype=torch.uint8, device=device), scales())
+
+
+def _planes(cache):
+    """(pages, H, D, the four data pointers) of a cache whose planes agree."""
+    kh, ka, vh, va = cache
+    _on_gpu(kh, ka, vh, va)
+    torch = _TORCH or _torch()
+    pages, heads, page, half = kh.shape
+    scales = (pages, heads, half // 32, page)
+    if page != KV_PAGE or half not in (32, 64) or vh.shape != (pages, heads, half, page) or ka.shape != scales or \
+            va.shape != scales:
+        raise ValueError(f"cache planes {tuple(kh.shape)}, {tuple(ka.shape)}, {tuple(vh.shape)}, {tuple(va.shape)}")
+    if not (kh.dtype is torch.uint8 and vh.dtype is torch.uint8 and ka.dtype is torch.float32 and
+            va.dtype is torch.float32):
+        raise TypeError("cache planes are uint8 holes and float32 absmax")
+    if not (kh.is_contiguous() and ka.is_contiguous() and vh.is_contiguous() and va.is_contiguous()):
+        raise ValueError("cache planes are contiguous")
+    return pages, heads, 2 * half, kh.data_ptr(), ka.data_ptr(), vh.data_ptr(), va.data_ptr()
+
+
+def _rows(t, align: int):
+    """A [tokens, heads, D] tensor whose rows the kernels can load: itself, or a copy where D is
+    strided or an address or stride is no multiple of `align` elements."""
+    s = t.stride()
+    if s[2] != 1 or s[0] % align or s[1] % align or t.data_ptr() % (align * t.element_size()):
+        t = t.contiguous()
+        if t.data_ptr() % (align * t.element_size()):
+            t = t.clone()
+        s = t.stride()
+    return t, s[0], s[1]
+
+
+def _kv_elt(t) -> int:
+    torch = _TORCH or _torch()
+    if t.dtype is torch.bfloat16:
+        return 0
+    if t.dtype is torch.float32:
+        return 1
+    raise TypeError(f"expected bfloat16 or float32, got {t.dtype}")
+
+
+def _ints(t, dtype, n: int, what: str):
+    """t's data pointer, for a contiguous vector of n."""
+    if t.dtype is not dtype or t.dim() != 1 or t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{what}: a contiguous {dtype} vector of {n}, got {t.dtype} {tuple(t.shape)}")
+    return t.data_ptr()
+
+
+@_on_stream
+def kv4_append(k, v, slots, cache) -> None:
+    """Encode keys and values [T, H, D] (bf16 or f32) into the cache at slots [T] (int64: page * 64
+    + place; negative ones are skipped)."""
+    torch = _TORCH or _torch()
+    pages, heads, dim, *planes = _planes(cache)
+    T = k.shape[0]
+    if k.shape != (T, heads, dim) or v.shape != k.shape or v.dtype is not k.dtype:
+        raise ValueError(f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, cache of {heads} heads of {dim}")
+    elt = _kv_elt(k)
+    _on_gpu(k, v, slots)
+    k, kt, kh = _rows(k, 4)
+    v, vt, vh = _rows(v, 4)
+    at = _ints(slots, torch.int64, T, "slots")
+    if T == 0:
+        return
+    _check(serve_lib().glint_kv4_append(k.data_ptr(), v.data_ptr(), elt, kt, kh, vt, vh, at, T, heads, dim, *planes,
+                                        pages, _sh(None)), "glint_kv4_append")
+
+
+@_on_stream
+def kv4_gather(slots, cache, out=None):
+    """The cache's tokens at slots [T] (int64) as bf16 (k, v), each [T, H, D]; zeros for negative slots."""
+    torch = _TORCH or _torch()
+    pages, heads, dim, *planes = _planes(cache)
+    T = slots.numel()
+    _on_gpu(slots)
+    at = _ints(slots, torch.int64, T, "slots")
+    if out is None:
+        k = slots.new_empty((T, heads, dim), dtype=torch.bfloat16)
+        v = torch.empty_like(k)
+    else:
+        k, v = out
+        if any(t.shape != (T, heads, dim) or t.dtype is not torch.bfloat16 or not t.is_contiguous() for t in (k, v)):
+            raise ValueError(f"out: two contiguous bfloat16 tensors of {(T, heads, dim)}")
+    if T:
+        _check(serve_lib().glint_kv4_gather(at, T, heads, dim, *planes, pages, k.data_ptr(), v.data_ptr(), _sh(None)),
+               "glint_kv4_gather")
+    return k, v
+
+
+@_on_stream
+def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Optional[float] = None, out=None):
+    """Attention of the newest tokens over the cache: q bf16 [rows, Hq, D] -> bf16 [rows, Hq, D].
+
+    page_table int32 [B, max_pages] and lens int32 [B] (tokens in the cache, the new ones
+    included) say what each sequence sees; its rows are cu_q[b] .. cu_q[b + 1] (int32, at most
+    max_q each), or max_q each where cu_q is None. A row sees the positions up to its own."""
+    torch = _TORCH or _torch()
+    pages, heads, dim, *planes = _planes(cache)
+    rows, hq, d = q.shape
+    B, wide = page_table.shape
+    _on_gpu(q, page_table, lens, *(() if cu_q is None else (cu_q,)))
+    if d != dim or hq % heads:
+        raise ValueError(f"q {tuple(q.shape)}, cache of {heads} heads of {dim}")
+    if q.dtype is not torch.bfloat16:
+        raise TypeError(f"expected bfloat16, got {q.dtype}")
+    if max_q < 1 or (cu_q is None and rows != B * max_q):
+        raise ValueError(f"{rows} query rows, {B} sequences of {max_q}")
+    if page_table.dtype is not torch.int32 or page_table.stride(1) != 1:
+        raise ValueError("page_table: int32 with adjacent columns")
+    q, qt, qh = _rows(q, 8)
+    n = _ints(lens, torch.int32, B, "lens")
+    cu = None if cu_q is None else _ints(cu_q, torch.int32, B + 1, "cu_q")
+    out = _attend_out(out, q, rows, hq, dim)
+    if rows == 0 or B == 0:
+        return out
+    if wide == 0:
+        return out.zero_()
+    lib = serve_lib()
+    need = lib.glint_kv4_attend_part(B, max_q, hq, heads, dim, wide)
+    part = q.new_empty(need, dtype=torch.float32) if need > 0 else None
+    _check(lib.glint_kv4_attend(q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(), page_table.stride(0),
+                                wide, n, cu, B, max_q, hq, heads, dim, dim ** -0.5 if scale is None else scale,
+                                out.data_ptr(), None if part is None else part.data_ptr(), _sh(None)),
+           "glint_kv4_attend")
+    return out
+
+
+def _attend_out(out, q, rows: int, hq: int, dim: int):
+    if out is None:
+        return q.new_empty((rows, hq, dim))
+    if out.shape != (rows, hq, dim) or out.dtype is not q.dtype or not out.is_contiguous():
+        raise ValueError(f"out: a contiguous bfloat16 tensor of {(rows, hq, dim)}")
+    return out
+
+
+@_on_stream
+def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: Optional[float] = None, out=None):
+    """Causal attention over packed sequences: q bf16 [Tq, Hq, D], k and v bf16 [Tk, H, D] -> bf16 [Tq, Hq, D].
+
+    cu_q, cu_k int32 [B + 1]: where each sequence's queries and keys start (cu_k is cu_q where
+    None); a sequence's last query sees its last key. max_q: no sequence has more queries
+    (Tq where None)."""
+    torch = _TORCH or _torch()
+    Tq, hq, dim = q.shape
+    Tk, heads, _ = k.shape
+    _on_gpu(q, k, v, cu_q, *(() if cu_k is None else (cu_k,)))
+    if k.shape != v.shape or k.shape[2] != dim or heads == 0 or hq % heads:
+        raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
+    if any(t.dtype is not torch.bfloat16 for t in (q, k, v)):
+        raise TypeError(f"expected bfloat16, got {q.dtype}, {k.dtype}, {v.dtype}")
+    B = cu_q.numel() - 1
+    cq = _ints(cu_q, torch.int32, B + 1, "cu_q")
+    ck = cq if cu_k is None else _ints(cu_k, torch.int32, B + 1, "cu_k")
+    q, qt, qh = _rows(q, 8)
+    k, kt, kh = _rows(k, 8)
+    v, vt, vh = _rows(v, 8)
+    out = _attend_out(out, q, Tq, hq, dim)
+    if Tq == 0 or B <= 0:
+        return out
+    if Tk == 0:
+        return out.zero_()
+    _check(serve_lib().glint_attend_prompt(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cq, ck, Tq,
+                                           Tk, B, Tq if max_q is None else max_q, hq, heads, dim,
+                                           dim ** -0.5 if scale is None else scale, out.data_ptr(), _sh(None)),
+           "glint_attend_prompt")
+    return out
+
+
+@_on_stream
+def token_logprobs(logits, tokens, top: int = 0) -> dict:
+    """Scores of tokens [T] (int64) under logits [T, V] (bf16 or f32): f32 "logprob" and "entropy"
+    [T], int32 "rank" [T] (entries ahead of the token; 0 where it is the likeliest), and the
+    `top` likeliest entries, "top_logprob" f32 and "top_index" int32 [T, top], equal ones by
+    index. A negative token gives logprob 0 and rank -1."""
+    torch = _TORCH or _torch()
+    T, V = logits.shape
+    elt = _kv_elt(logits)
+    _on_gpu(logits, tokens)
+    if logits.stride(1) != 1 and V > 1:
+        logits = logits.contiguous()
+    at = _ints(tokens, torch.int64, T, "tokens")
+    new = lambda dtype, *s: logits.new_empty(s, dtype=dtype)
+    r = {"logprob": new(torch.float32, T), "entropy": new(torch.float32, T), "rank": new(torch.int32, T),
+         "top_logprob": new(torch.float32, T, top), "top_index": new(torch.int32, T, top)}
+    if T:
+        _check(serve_lib().glint_token_logprobs(logits.data_ptr(), elt, logits.stride(0), at, T, V, top,
+                                                *(t.data_ptr() for t in r.values()), _sh(None)),
+               "glint_token_logprobs")
+    return r
 
 
 # ------------------------------------------------------------- host-pointer wrappers
