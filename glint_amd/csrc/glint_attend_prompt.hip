@@ -6,6 +6,9 @@
  *   query row: maximum and sum are in-lane but for one exchange of the wave's halves, and the
  *   weights feed O^T = V^T P^T as they lie (the order of the keys inside a product is free).
  *   V^T operands come from the row-major V tile by the transposing LDS read. */
+#include <cfloat>
+#include <cmath>
+
 #include "glint_common.h"
 #include "glint_serve.h"
 
@@ -18,6 +21,8 @@ typedef __attribute__((address_space(3))) ap_s16x4 ap_lds_s16x4;
 #define AP_T (64 * AP_WAVES)
 #define AP_ROWS (32 * AP_WAVES)
 #define AP_KEYS 64
+#define AP_STRIDE (1 << 24) /* elements: a tile's bytes fit 32 bits */
+#define AP_SLACK 8.f /* a maximum may lag this far (in powers of two) before outputs are rescaled */
 
 union ApFrag {
     uint32_t u[4];
@@ -32,15 +37,149 @@ struct ApArgs {
     const int32_t *cu_q, *cu_k;
     int64_t Tq, Tk;
     int max_q, Hq, G;
-    float scale2; /* scale * log2 e */
+    uint32_t q_sign; /* 0x80008000 where the scale is negative */
+    float scale2;    /* |scale| log2 e, above 0 */
     uint16_t *out;
 };
 
+/* Where 16-B chunk c of row r lies in an LDS tile's row: keys so that 8 lanes reading one
+ * chunk of 8 rows touch 8 places, values so that the 64-B pieces of 4 rows that one transposing
+ * read takes lie in different 64-B quarters of 256 B. */
+__device__ __forceinline__ int ap_k_chunk(int r, int c) { return c ^ (r & 7); }
 template <int D>
-__global__ __launch_bounds__(AP_T) void k_attend_prompt(ApArgs A) {
-    constexpr int CH = D / 8; /* 16-B chunks of a row */
-    __shared__ __attribute__((aligned(16))) uint16_t kt[AP_KEYS * D], vt[AP_KEYS * D];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+__device__ __forceinline__ int ap_v_chunk(int r, int c) { return D == 128 ? c ^ ((r & 3) << 2) : c ^ ((r & 2) << 1); }
+
+typedef __attribute__((address_space(3))) char ap_lds;
+
+/* 16 B per lane from the buffer to LDS at `to` + 16 lane (not in a template: the host pass refuses
+ * the builtin where its arguments depend on one, and then leaves the kernel's stub out) */
+__device__ __forceinline__ void ap_dma(__amdgpu_buffer_rsrc_t from, ap_lds *to, uint32_t offset, uint32_t more) {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, offset, more, 0, 0);
+}
+
+/* What a wave carries from tile to tile for its 32 rows. */
+template <int D>
+struct ApRows {
+    ApFrag q[D / 16];
+    ap_f32x16 o[D / 32];
+    float m, l;
+    int last;        /* this lane's row sees the keys up to here */
+    uint32_t kat[4]; /* where the lane reads keys (by the chunk's low bits) and values (by dimension part) */
+    uint32_t vat[D / 32];
+};
+
+__device__ __forceinline__ uint32_t ap_pack(float a, float b) { /* two BF16, round to nearest even */
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+    union {
+        bf16x2 b;
+        uint32_t u;
+    } r;
+    r.b = __builtin_convertvector((f32x2{a, b}), bf16x2);
+    return r.u;
+}
+
+/* One tile of keys. */
+template <int D>
+__device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int t, ApRows<D> &w, float scale2, bool masked,
+                                        int half) {
+    ap_f32x16 sc[2];
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sc[a][i] = 0.f;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+            ApFrag f;
+            f.v = *(const __attribute__((address_space(3))) glint_u32x4 *)(kl + w.kat[s & 3] + 128 * (s >> 2) + a * 32 * D * 2);
+            sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.f, w.q[s].f, sc[a], 0, 0, 0);
+        }
+    /* element i of part a is key 32 a + 8 (i / 4) + 4 half + i % 4 */
+    if (masked) {
+        const int first = t * AP_KEYS + 4 * half;
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                sc[a][i] = first + 32 * a + 8 * (i >> 2) + (i & 3) <= w.last ? sc[a][i] : -INFINITY;
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            top = fmaxf(top, sc[a][i]);
+    top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale2;
+    if (__any(top > w.m + AP_SLACK)) {
+        const float mn = fmaxf(w.m, top);
+        const float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
+        w.m = mn;
+        w.l *= keep;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                w.o[d][i] *= keep;
+    }
+    const float base = w.m == -INFINITY ? 0.f : w.m;
+    ApFrag pf[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+#pragma unroll
+            for (int x = i; x < i + 2; ++x) {
+                sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], scale2, -base));
+                sum += sc[a][x];
+            }
+            pf[2 * a + (i >> 3)].u[(i & 7) >> 1] = ap_pack(sc[a][i], sc[a][i + 1]);
+        }
+    w.l += sum;
+    /* Step s multiplies the keys that pf[s] holds: 16 s + 4 half + 0..3, and 8 on. */
+    auto values = [&](int s, int d) {
+        ApFrag f;
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_lds_s16x4 *)(vl + w.vat[d] + (16 * s + 8 * x) * D * 2));
+        return f;
+    };
+    /* A weight's bf16 rounding (2^-8) averages out over many keys and does not where few hold
+     * the sum: a tile with a weight above 1 / 16 of some row's sum so far is multiplied by
+     * what the rounding left as well. */
+    if (__any(__builtin_amdgcn_exp2f(top - base) * 16.f > w.l + __shfl_xor(w.l, 32, 64))) {
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            ApFrag rest;
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int i = 8 * (s & 1) + 2 * x;
+                rest.u[x] = ap_pack(sc[s >> 1][i] - glint_bf16lo(pf[s].u[x]), sc[s >> 1][i + 1] - glint_bf16hi(pf[s].u[x]));
+            }
+#pragma unroll
+            for (int d = 0; d < D / 32; ++d)
+                w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(s, d).f, rest.f, w.o[d], 0, 0, 0);
+        }
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+            w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(s, d).f, pf[s].f, w.o[d], 0, 0, 0);
+}
+
+template <int D>
+__global__ __launch_bounds__(AP_T, 2) void k_attend_prompt(ApArgs A) {
+    constexpr int CH = D / 8;                  /* 16-B chunks of a row */
+    constexpr int LOADS = AP_KEYS * CH / AP_T; /* of a thread, per tile of keys or values */
+    constexpr int STEP = AP_T / CH;            /* rows that one load of every thread covers */
+    constexpr int TILE = AP_KEYS * D * 2;      /* bytes */
+    /* two tiles of each; arrays of their own, so that reads of one do not wait for loads into the other */
+    __shared__ __attribute__((aligned(16))) char k0t[TILE], k1t[TILE], v0t[TILE], v1t[TILE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     const int hq = blockIdx.y, h = hq / A.G, b = blockIdx.z;
     const int64_t q0 = A.cu_q[b], k0 = A.cu_k[b];
@@ -54,117 +193,91 @@ __global__ __launch_bounds__(AP_T) void k_attend_prompt(ApArgs A) {
         return;
     const int row = r0 + 32 * wave + col;
     const int64_t gap = nk - (q1 - q0); /* row i's last key is i + gap */
-    const int last = row < nq ? (int)max((int64_t)-1, row + gap) : -1;
+    /* the wave's first and last row's last keys: tiles up to the one need no mask, tiles past
+     * the other nothing at all */
+    const int wave_low = (int)max((int64_t)-1, r0 + 32 * wave + gap);
+    const int wave_high = r0 + 32 * wave < nq ? (int)max((int64_t)-1, min(r0 + 32 * wave + 31, nq - 1) + gap) : -1;
 
-    ApFrag qf[D / 16];
+    ApRows<D> w;
+    w.m = -INFINITY;
+    w.l = 0.f;
+    w.last = row < nq ? (int)max((int64_t)-1, row + gap) : -1;
     {
         const uint16_t *qr = A.q + (q0 + min(row, nq - 1)) * A.q_st + hq * A.q_sh;
 #pragma unroll
-        for (int s = 0; s < D / 16; ++s)
-            qf[s].v = *(const glint_u32x4 *)(qr + 16 * s + 8 * half);
+        for (int s = 0; s < D / 16; ++s) {
+            w.q[s].v = *(const glint_u32x4 *)(qr + 16 * s + 8 * half);
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                w.q[s].u[x] ^= A.q_sign;
+        }
     }
-    ap_f32x16 o[D / 32];
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
 #pragma unroll
         for (int i = 0; i < 16; ++i)
-            o[d][i] = 0.f;
-    float m = -INFINITY, l = 0.f;
+            w.o[d][i] = 0.f;
+    /* Keys: row col (and col + 32), chunk 2 s + half. Values: a 16-lane group of the transposing
+     * read takes 4 keys x 16 dimensions; lane i addresses key i / 4, dimensions 4 (i % 4), and
+     * receives dimension i of the 4 keys. */
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        w.kat[j] = col * D * 2 + 16 * ap_k_chunk(col, 2 * j + half);
+    const int vkey = 4 * half + ((lane & 15) >> 2), vdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+        w.vat[d] = vkey * D * 2 + 16 * ap_v_chunk<D>(vkey, (32 * d + vdim) >> 3) + 2 * (vdim & 7);
 
     const int64_t far = min(r0 + AP_ROWS, nq) - 1 + gap; /* the last key of the last row */
     const int ntiles = far < 0 ? 0 : (int)(far / AP_KEYS) + 1;
     const uint16_t *kb = A.k + k0 * A.k_st + h * A.k_sh, *vb = A.v + k0 * A.v_st + h * A.v_sh;
-    for (int t = 0; t < ntiles; ++t) {
+
+    /* Tiles go to LDS by the loads' direct path. Place p of a tile is chunk p % CH of row p / CH;
+     * thread t fills places t + i AP_T, so its lane's global chunk carries the swizzle (the same
+     * for every i). Rows past the sequence take an offset past the buffer's end: zeros. */
+    const int my_row = threadIdx.x / CH, my_chunk = threadIdx.x % CH;
+    const uint32_t ko = (uint32_t)(my_row * A.k_st * 2) + 16 * ap_k_chunk(my_row, my_chunk);
+    const uint32_t vo = (uint32_t)(my_row * A.v_st * 2) + 16 * ap_v_chunk<D>(my_row, my_chunk);
+    const uint32_t kstep = (uint32_t)(STEP * A.k_st * 2), vstep = (uint32_t)(STEP * A.v_st * 2);
+    auto fetch = [&](int t, ap_lds *kt, ap_lds *vt) {
+        const __amdgpu_buffer_rsrc_t rk = __builtin_amdgcn_make_buffer_rsrc((void *)(kb + (int64_t)t * AP_KEYS * A.k_st),
+                                                                            (short)0, 0x7FFFFFFF, GLINT_BUF_DWORD3);
+        const __amdgpu_buffer_rsrc_t rv = __builtin_amdgcn_make_buffer_rsrc((void *)(vb + (int64_t)t * AP_KEYS * A.v_st),
+                                                                            (short)0, 0x7FFFFFFF, GLINT_BUF_DWORD3);
+        const int rows = nk - t * AP_KEYS;
+        if (rows >= AP_KEYS) {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                ap_dma(rk, kt + (i * AP_T + wave * 64) * 16, ko, i * kstep);
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i)
+                ap_dma(rv, vt + (i * AP_T + wave * 64) * 16, vo, i * vstep);
+        } else {
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                const bool in = my_row + i * STEP < rows;
+                ap_dma(rk, kt + (i * AP_T + wave * 64) * 16, in ? ko + i * kstep : 0xFFFFFF00u, 0);
+                ap_dma(rv, vt + (i * AP_T + wave * 64) * 16, in ? vo + i * vstep : 0xFFFFFF00u, 0);
+            }
+        }
+    };
+
+    auto step = [&](int t, ap_lds *kt, ap_lds *vt, ap_lds *kn, ap_lds *vn) {
+        __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0); /* this wave's part of tile t */
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < AP_KEYS * CH / AP_T; ++i) {
-            const int u = threadIdx.x + i * AP_T, r = u / CH, c = u % CH;
-            const int key = t * AP_KEYS + r;
-            glint_u32x4 kv = {0, 0, 0, 0}, vv = {0, 0, 0, 0};
-            if (key < nk) {
-                kv = *(const glint_u32x4 *)(kb + key * A.k_st + 8 * c);
-                vv = *(const glint_u32x4 *)(vb + key * A.v_st + 8 * c);
-            }
-            *(glint_u32x4 *)(kt + r * D + 8 * (c ^ (r & 7))) = kv;
-            *(glint_u32x4 *)(vt + r * D + 8 * c) = vv;
-        }
-        __syncthreads();
-        ap_f32x16 sc[2];
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                sc[a][i] = 0.f;
-            const int r = 32 * a + col;
-#pragma unroll
-            for (int s = 0; s < D / 16; ++s) {
-                ApFrag f;
-                f.v = *(const glint_u32x4 *)(kt + r * D + 8 * ((2 * s + half) ^ (r & 7)));
-                sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.f, qf[s].f, sc[a], 0, 0, 0);
-            }
-        }
-        /* element i of tile a is key 32 a + 8 (i / 4) + 4 half + i % 4 */
-        const int first = t * AP_KEYS + 4 * half;
-        float top = -INFINITY;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = first + 32 * a + 8 * (i >> 2) + (i & 3);
-                const float x = key <= last ? sc[a][i] * A.scale2 : -INFINITY;
-                sc[a][i] = x;
-                top = fmaxf(top, x);
-            }
-        top = fmaxf(top, __shfl_xor(top, 32, 64));
-        const float mn = fmaxf(m, top), base = mn == -INFINITY ? 0.f : mn;
-        const float keep = __builtin_amdgcn_exp2f(m - base);
-        m = mn;
-        float sum = 0.f, high = 0.f;
-        ApFrag pf[4], rest[4];
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const float p = __builtin_amdgcn_exp2f(sc[a][i] - base);
-                sum += p;
-                high = fmaxf(high, p);
-                pf[2 * a + (i >> 3)].f[i & 7] = (__bf16)p;
-                sc[a][i] = p;
-            }
-        l = fmaf(l, keep, sum);
-        /* A weight's bf16 rounding (2^-8) averages out over many keys and does not where few hold
-         * the sum: a tile with a weight above 1 / 16 of some row's sum so far is multiplied by
-         * what the rounding left as well. */
-        const bool few = __any(high * 16.f > l + __shfl_xor(l, 32, 64));
-        if (few) {
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    rest[2 * a + (i >> 3)].f[i & 7] = (__bf16)(sc[a][i] - (float)pf[2 * a + (i >> 3)].f[i & 7]);
-        }
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                o[d][i] *= keep;
-        /* step s multiplies keys 16 s + 8 j / 4 ... as the weights lie: keys 16 s + 4 half +
-         * 0..3, then 8 on. A 16-lane group reads 4 keys x 16 dimensions: lane i addresses key
-         * i / 4, dimensions 4 (i % 4), and receives dimension i of the 4 keys. */
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d) {
-                ApFrag f;
-                const int key = 16 * s + 4 * half + ((lane & 15) >> 2);
-                const int dim = 32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
-                f.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_lds_s16x4 *)(vt + key * D + dim));
-                f.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_lds_s16x4 *)(vt + (key + 8) * D + dim));
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.f, pf[s].f, o[d], 0, 0, 0);
-                if (few)
-                    o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.f, rest[s].f, o[d], 0, 0, 0);
-            }
+        if (t + 1 < ntiles)
+            fetch(t + 1, kn, vn); /* over tile t - 1, which every wave has left */
+        if (t * AP_KEYS <= wave_high)
+            ap_tile<D>(kt, vt, t, w, A.scale2, t * AP_KEYS + AP_KEYS - 1 > wave_low, half);
+    };
+    if (ntiles > 0)
+        fetch(0, (ap_lds *)k0t, (ap_lds *)v0t);
+    for (int t = 0; t < ntiles; t += 2) {
+        step(t, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t, (ap_lds *)v1t);
+        if (t + 1 < ntiles)
+            step(t + 1, (ap_lds *)k1t, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t);
     }
+    float l = w.l;
     l += __shfl_xor(l, 32, 64);
     if (row >= nq)
         return;
@@ -175,8 +288,8 @@ __global__ __launch_bounds__(AP_T) void k_attend_prompt(ApArgs A) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             glint_u32x2 two;
-            two.x = glint_f32_to_bf16(o[d][i] * inv) | (uint32_t)glint_f32_to_bf16(o[d][i + 1] * inv) << 16;
-            two.y = glint_f32_to_bf16(o[d][i + 2] * inv) | (uint32_t)glint_f32_to_bf16(o[d][i + 3] * inv) << 16;
+            two.x = ap_pack(w.o[d][i] * inv, w.o[d][i + 1] * inv);
+            two.y = ap_pack(w.o[d][i + 2] * inv, w.o[d][i + 3] * inv);
             *(glint_u32x2 *)(dst + 32 * d + 2 * i + 4 * half) = two;
         }
 }
@@ -192,12 +305,14 @@ GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t
         (D != 64 && D != 128) || Tq < 0 || Tk < 0)
         return -2;
     if (!glint_aligned(q, 16) || !glint_aligned(k, 16) || !glint_aligned(v, 16) || !glint_aligned(out, 8) ||
-        ((q_stride_t | q_stride_h | k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7))
+        ((q_stride_t | q_stride_h | k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7) || k_stride_t < D ||
+        v_stride_t < D || k_stride_t > AP_STRIDE || v_stride_t > AP_STRIDE)
         return -2;
     if (B == 0 || Tq == 0 || max_q == 0)
         return 0;
+    const float scale2 = fabsf(scale) * 1.44269504088896341f;
     const ApArgs a{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk,
-                   max_q, Hq, Hq / H, scale * 1.44269504088896341f, out};
+                   max_q, Hq, Hq / H, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out};
     const dim3 grid((unsigned)((max_q + AP_ROWS - 1) / AP_ROWS), Hq, B);
     if (D == 64)
         k_attend_prompt<64><<<grid, AP_T, 0, stream>>>(a);

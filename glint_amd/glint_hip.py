@@ -700,8 +700,8 @@ def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: 
     cq = _ints(cu_q, torch.int32, B + 1, "cu_q")
     ck = cq if cu_k is None else _ints(cu_k, torch.int32, B + 1, "cu_k")
     q, qt, qh = _rows(q, 8)
-    k, kt, kh = _rows(k, 8)
-    v, vt, vh = _rows(v, 8)
+    k, kt, kh = _rows(k if dim <= k.stride(0) <= 1 << 24 else k.contiguous(), 8)
+    v, vt, vh = _rows(v if dim <= v.stride(0) <= 1 << 24 else v.contiguous(), 8)
     out = _attend_out(out, q, Tq, hq, dim)
     if Tq == 0 or B <= 0:
         return out

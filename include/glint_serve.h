@@ -67,8 +67,8 @@ int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, 
 /* Causal attention of B packed sequences. Sequence b has queries cu_q[b] .. cu_q[b + 1] of
  * q [Tq] (at most max_q) and keys cu_k[b] .. cu_k[b + 1] of k, v [Tk]; the last query sees
  * the last key, each earlier query one key less, and a query before the first key gives
- * zeros. Hq % H == 0; BF16 in and out, out [Tq][Hq][D]; strides multiples of 8, addresses
- * 16-B aligned. f32 scores, softmax and sums; the softmax weights enter the second product
+ * zeros. Hq % H == 0; BF16 in and out, out [Tq][Hq][D]; strides multiples of 8, k's and v's
+ * stride_t from D to 2^24, addresses 16-B aligned. f32 scores, softmax and sums; the softmax weights enter the second product
  * in BF16. */
 int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
                         int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
