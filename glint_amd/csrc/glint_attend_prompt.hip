@@ -36,7 +36,9 @@ struct ApArgs {
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;
     const int32_t *cu_q, *cu_k;
     int64_t Tq, Tk;
-    int max_q, Hq, G;
+    int max_q, Hq, H, G;
+    int nblk; /* row blocks of a head */
+    int ngroups;
     uint32_t q_sign; /* 0x80008000 where the scale is negative */
     float scale2;    /* |scale| log2 e, above 0 */
     uint16_t *out;
@@ -181,14 +183,37 @@ __global__ __launch_bounds__(AP_T, 2) void k_attend_prompt(ApArgs A) {
     __shared__ __attribute__((aligned(16))) char k0t[TILE], k1t[TILE], v0t[TILE], v1t[TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    const int hq = blockIdx.y, h = hq / A.G, b = blockIdx.z;
+    /* Work items are the row blocks of a group's heads, a group being one sequence and key head;
+     * the longest rows come first. A workgroup's XCD is its index modulo 8, and each XCD's L2
+     * should hold few groups' keys: as many groups as share out evenly go whole to one XCD
+     * each; of the rest, where they divide 8, each goes to 8 / rest XCDs. 8192 tokens of 32
+     * heads over 8 key heads: 555 us, 773 with every group on every XCD. */
+    const int per = A.nblk * A.G, whole = A.ngroups & ~7, rest = A.ngroups & 7;
+    int group, item;
+    if ((int)blockIdx.x < whole * per) {
+        const int on = (int)blockIdx.x >> 3;
+        group = (on / per) * 8 + ((int)blockIdx.x & 7);
+        item = on % per;
+    } else {
+        const int at = (int)blockIdx.x - whole * per;
+        if (8 % rest == 0) {
+            group = whole + (at & 7) % rest;
+            item = (at >> 3) * (8 / rest) + (at & 7) / rest;
+            if (item >= per)
+                return;
+        } else {
+            group = whole + at % rest;
+            item = at / rest;
+        }
+    }
+    const int b = group / A.H, h = group % A.H, hq = h * A.G + item % A.G;
     const int64_t q0 = A.cu_q[b], k0 = A.cu_k[b];
     const int64_t q1 = A.cu_q[b + 1], k1 = A.cu_k[b + 1];
     if (q0 < 0 || q1 <= q0 || q1 > A.Tq)
         return;
     const int nq = (int)min(q1 - q0, (int64_t)A.max_q);
     const int nk = k0 >= 0 && k1 > k0 && k1 <= A.Tk ? (int)(k1 - k0) : 0;
-    const int r0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * AP_ROWS; /* the longest rows first */
+    const int r0 = (A.nblk - 1 - item / A.G) * AP_ROWS;
     if (r0 >= nq)
         return;
     const int row = r0 + 32 * wave + col;
@@ -310,10 +335,15 @@ GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t
         return -2;
     if (B == 0 || Tq == 0 || max_q == 0)
         return 0;
+    const int nblk = (max_q + AP_ROWS - 1) / AP_ROWS;
     const float scale2 = fabsf(scale) * 1.44269504088896341f;
     const ApArgs a{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk,
-                   max_q, Hq, Hq / H, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out};
-    const dim3 grid((unsigned)((max_q + AP_ROWS - 1) / AP_ROWS), Hq, B);
+                   max_q, Hq, H, Hq / H, nblk, B * H, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out};
+    if ((int64_t)B * H > INT32_MAX || ((int64_t)nblk * Hq * B + 8) > INT32_MAX / AP_T)
+        return -2;
+    const int per = a.nblk * a.G, rest = a.ngroups & 7; /* 8 % rest == 0: whole rounds of 8 workgroups */
+    const int tail = rest == 0 ? 0 : 8 % rest == 0 ? (per + 8 / rest - 1) / (8 / rest) * 8 : rest * per;
+    const unsigned grid = (unsigned)((a.ngroups - rest) * per + tail);
     if (D == 64)
         k_attend_prompt<64><<<grid, AP_T, 0, stream>>>(a);
     else
