@@ -174,7 +174,7 @@ __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int 
 }
 
 template <int D>
-__global__ __launch_bounds__(AP_T, 2) void k_attend_prompt(ApArgs A) {
+__global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs A) {
     constexpr int CH = D / 8;                  /* 16-B chunks of a row */
     constexpr int LOADS = AP_KEYS * CH / AP_T; /* of a thread, per tile of keys or values */
     constexpr int STEP = AP_T / CH;            /* rows that one load of every thread covers */
