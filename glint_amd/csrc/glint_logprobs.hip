@@ -1,9 +1,9 @@
 /* Log probabilities of given tokens (include/glint_serve.h).
  *
  * k_token_logprobs — one workgroup per row, one pass: a thread keeps a running maximum m,
- *   s = sum e^(x - m) and t = sum e^(x - m) (x - m) of its elements, counts those that come
- *   before the token, and remembers the 16-B load that held its largest element. Then
- *     lse = m + log s,  entropy = log s - t / s.
+ *   s = sum 2^(u - m) and t = sum 2^(u - m) (u - m) of its elements' u = x log2 e, counts those
+ *   that come before the token, and remembers the 16-B load that held its largest element. Then
+ *     lse = ln 2 (m + log2 s),  entropy = ln 2 (log2 s - t / s).
  *   The top list needs no second pass over the row: with T the top-th largest of the threads'
  *   own maxima, every entry of the list is at least T and sits in one of the `top` threads
  *   whose maximum is at least T, so those threads look at their elements again and put
@@ -33,7 +33,8 @@ struct LpRow {
         nvec = (v - head) / PER;
     }
     __device__ float at(int64_t j) const;
-    __device__ void load(int64_t vec, float (&w)[PER]) const;
+    __device__ glint_u32x4 raw(int vec) const { return *(const glint_u32x4 *)(x + head + (int64_t)vec * PER); }
+    __device__ void unpack(const glint_u32x4 u, float (&w)[PER]) const;
     /* the element of this thread's that lies outside the 16-B loads: before (thread j < head)
      * and after them, or -1 */
     __device__ int64_t before() const { return (int)threadIdx.x < head ? (int64_t)threadIdx.x : -1; }
@@ -47,15 +48,13 @@ __device__ __forceinline__ float LpRow<float>::at(int64_t j) const { return x[j]
 template <>
 __device__ __forceinline__ float LpRow<uint16_t>::at(int64_t j) const { return __uint_as_float((uint32_t)x[j] << 16); }
 template <>
-__device__ __forceinline__ void LpRow<float>::load(int64_t vec, float (&w)[4]) const {
-    const glint_f32x4 u = *(const glint_f32x4 *)(x + head + vec * 4);
+__device__ __forceinline__ void LpRow<float>::unpack(const glint_u32x4 u, float (&w)[4]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-        w[i] = u[i];
+        w[i] = __uint_as_float(u[i]);
 }
 template <>
-__device__ __forceinline__ void LpRow<uint16_t>::load(int64_t vec, float (&w)[8]) const {
-    const glint_u32x4 u = *(const glint_u32x4 *)(x + head + vec * 8);
+__device__ __forceinline__ void LpRow<uint16_t>::unpack(const glint_u32x4 u, float (&w)[8]) const {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         w[2 * i] = glint_bf16lo(u[i]);
@@ -70,132 +69,229 @@ __device__ __forceinline__ uint64_t lp_key(float x, int64_t j) {
     return (uint64_t)u << 32 | (0xFFFFFFFFu - (uint32_t)j);
 }
 __device__ __forceinline__ uint32_t lp_key_index(uint64_t k) { return 0xFFFFFFFFu - (uint32_t)k; }
-__device__ __forceinline__ uint64_t lp_wave_max(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint64_t w = __shfl_xor(v, o, 64);
-        v = w > v ? w : v;
-    }
-    return v;
+__device__ __forceinline__ float lp_key_value(uint64_t k) {
+    const uint32_t u = (uint32_t)(k >> 32);
+    return __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~u);
+}
+/* The next float above x; NaN above +inf and NaN. */
+__device__ __forceinline__ float lp_next_up(float x) {
+    const float y = x + 0.f;
+    const int32_t i = __float_as_int(y);
+    return y != y ? y : __int_as_float(i >= 0 ? i + 1 : i - 1);
 }
 
+/* Running sums of a set of elements, in powers of two: with u = x log2 e and a reference m (not
+ * below any u by more than LP_SLACK), s = sum 2^(u - m), t = sum 2^(u - m) (u - m). */
+#define LP_LOG2E 1.44269504088896341f
+#define LP_LN2 0.69314718055994531f
+#define LP_SLACK 20.f
 struct LpSum {
     float m, s, t;
-    /* one more element; -inf adds nothing */
-    __device__ void shift(float to) { /* to >= m */
-        if (to > m) {
-            if (m != -INFINITY) {
-                const float d = m - to, f = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
-                t = f * fmaf(d, s, t);
-                s = f * s;
-            }
-            m = to;
+    __device__ void shift(float to) { /* to > m */
+        if (m != -INFINITY) {
+            const float d = m - to, f = __builtin_amdgcn_exp2f(d);
+            t = f * fmaf(d, s, t);
+            s = f * s;
         }
+        m = to;
     }
-    __device__ void add(float x) {
-        const float d = x - m, e = __builtin_amdgcn_exp2f(d * 1.44269504088896341f);
+    __device__ void add(float x) { /* m is finite, or x makes s NaN */
+        const float d = fmaf(x, LP_LOG2E, -m), e = __builtin_amdgcn_exp2f(d);
         s += e;
-        t = fmaf(e, x == -INFINITY ? 0.f : d, t);
+        t = fmaf(e, fmaxf(d, -1024.f), t); /* 0 times -inf counts 0 */
     }
 };
-__device__ __forceinline__ void lp_join(LpSum &a, float m, float s, float t) {
-    const float to = fmaxf(a.m, m);
-    if (to == -INFINITY) {
-        a.s += s; /* NaN stays NaN */
-        return;
-    }
-    const float da = a.m - to, db = m - to;
-    const float fa = __builtin_amdgcn_exp2f(da * 1.44269504088896341f), fb = __builtin_amdgcn_exp2f(db * 1.44269504088896341f);
-    const float ta = a.m == -INFINITY ? a.t : fmaf(da, a.s, a.t), tb = m == -INFINITY ? t : fmaf(db, s, t);
-    a.s = fmaf(fa, a.s, fb * s);
-    a.t = fmaf(fa, ta, fb * tb);
+/* Over each row of 16 lanes, left in every lane of the row. */
+template <class F>
+__device__ __forceinline__ float lp_row16(float v, F op) {
+    v = op(v, __int_as_float(glint_dpp<GLINT_DPP_QUAD_1032>(__float_as_int(v))));
+    v = op(v, __int_as_float(glint_dpp<GLINT_DPP_QUAD_2301>(__float_as_int(v))));
+    v = op(v, __int_as_float(glint_dpp<GLINT_DPP_ROW_HALF_MIRROR>(__float_as_int(v))));
+    return op(v, __int_as_float(glint_dpp<GLINT_DPP_ROW_MIRROR>(__float_as_int(v))));
+}
+__device__ __forceinline__ int lp_row16_sum(int v) {
+    v += glint_dpp<GLINT_DPP_QUAD_1032>(v);
+    v += glint_dpp<GLINT_DPP_QUAD_2301>(v);
+    v += glint_dpp<GLINT_DPP_ROW_HALF_MIRROR>(v);
+    return v + glint_dpp<GLINT_DPP_ROW_MIRROR>(v);
+}
+__device__ __forceinline__ float lp_lane(float v, int lane) {
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+/* Over the wave: the four rows. The reads of other lanes stand here, in code that every lane
+ * runs: a sum that only a branch uses may be computed inside it, for the branch's lanes alone. */
+template <class F>
+__device__ __forceinline__ float lp_wave(float v, F op) {
+    v = lp_row16(v, op);
+    return op(op(lp_lane(v, 0), lp_lane(v, 16)), op(lp_lane(v, 32), lp_lane(v, 48)));
+}
+__device__ __forceinline__ int lp_wave_sum(int v) {
+    v = lp_row16_sum(v);
+    return __builtin_amdgcn_readlane(v, 0) + __builtin_amdgcn_readlane(v, 16) + __builtin_amdgcn_readlane(v, 32) +
+           __builtin_amdgcn_readlane(v, 48);
+}
+struct LpMax {
+    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct LpAdd {
+    __device__ float operator()(float a, float b) const { return a + b; }
+};
+/* The sums under another reference `to` >= m; nothing but NaN is left of a set without one. */
+__device__ __forceinline__ void lp_refer(LpSum &a, float to) {
+    const float d = a.m - to, f = a.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(d);
+    a.t = a.m == -INFINITY ? 0.f : f * fmaf(d, a.s, a.t);
+    a.s = a.m == -INFINITY && a.s == a.s ? 0.f : f * a.s;
     a.m = to;
 }
 
+/* Largest of the wave's keys, in every lane: the upper words' maximum by DPP, then, where more
+ * than one lane has it, the lower words'. */
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t lp_dpp_max(uint32_t v) {
+    const uint32_t w = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+    return w > v ? w : v;
+}
+__device__ __forceinline__ uint32_t lp_wave_max32(uint32_t v) {
+    v = lp_dpp_max<0x111, 0xF>(v); /* row_shr 1, 2, 4, 8 */
+    v = lp_dpp_max<0x112, 0xF>(v);
+    v = lp_dpp_max<0x114, 0xF>(v);
+    v = lp_dpp_max<0x118, 0xF>(v);
+    v = lp_dpp_max<0x142, 0xA>(v); /* row_bcast 15, 31 */
+    v = lp_dpp_max<0x143, 0xC>(v);
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+__device__ __forceinline__ uint64_t lp_wave_max(uint64_t v) {
+    const uint32_t hi = lp_wave_max32((uint32_t)(v >> 32));
+    const bool has = (uint32_t)(v >> 32) == hi;
+    const uint64_t who = __ballot(has);
+    uint32_t lo;
+    if ((who & (who - 1)) == 0)
+        lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, __builtin_ctzll(who));
+    else
+        lo = lp_wave_max32(has ? (uint32_t)v : 0u);
+    return (uint64_t)hi << 32 | lo;
+}
+
+#define LP_U 4 /* 16-B loads of a thread in flight, twice */
+
 template <class E>
-__global__ __launch_bounds__(LP_T) void k_token_logprobs(const E *__restrict__ logits, int64_t stride,
-                                                         const int64_t *__restrict__ tokens, int64_t V, int top,
-                                                         float *__restrict__ logprob, float *__restrict__ entropy,
-                                                         int32_t *__restrict__ rank, float *__restrict__ top_logprob,
-                                                         int32_t *__restrict__ top_index) {
+__global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict__ logits, int64_t stride,
+                                                            const int64_t *__restrict__ tokens, int64_t V, int top,
+                                                            float *__restrict__ logprob, float *__restrict__ entropy,
+                                                            int32_t *__restrict__ rank, float *__restrict__ top_logprob,
+                                                            int32_t *__restrict__ top_index) {
     constexpr int PER = LpRow<E>::PER;
     __shared__ float sm[LP_WAVES], ss[LP_WAVES], st[LP_WAVES];
     __shared__ int sr[LP_WAVES];
     __shared__ uint64_t best[LP_WAVES * LP_TOP], cand[LP_CAND];
     __shared__ uint64_t floor_key;
     __shared__ int ncand;
-    __shared__ float s_lse;
+    __shared__ float s_ref, s_ls;
     const int64_t row = blockIdx.x;
     const LpRow<E> r(logits + row * stride, V);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+
+    /* vectors threadIdx.x + k LP_T; one past the end repeats the last and counts as -inf */
+    const int nvec = (int)r.nvec, rounds = (nvec + LP_T - 1) / LP_T;
+    glint_u32x4 now[LP_U], next[LP_U];
+    auto fetch = [&](int k0, glint_u32x4 (&w)[LP_U]) {
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+            w[u] = r.raw(min((int)threadIdx.x + (k0 + u) * LP_T, nvec - 1));
+    };
+    if (rounds > 0)
+        fetch(0, now);
+
     const int64_t tok = tokens[row];
     const bool is_tok = tok >= 0 && tok < V;
-    const float xt = is_tok ? r.at(tok) : INFINITY;
+    const float xt = is_tok ? r.at(tok) : NAN; /* NaN: nothing comes before it */
+    /* entries that come before the token reach xt at indices below it and the next float above it */
+    const float xt_up = lp_next_up(xt);
 
     LpSum a{-INFINITY, 0.f, 0.f};
     int before = 0;
-    uint64_t mine = 0;
     float high = -INFINITY;
-    int64_t where = -1;
-    bool bad = false; /* NaN or +inf */
-    for (int64_t vec = threadIdx.x; vec < r.nvec; vec += LP_T) {
+    int where = -1;
+    auto take = [&](int vec, const glint_u32x4 raw) {
         float w[PER];
-        r.load(vec, w);
+        r.unpack(raw, w);
         float mx = w[0];
 #pragma unroll
         for (int i = 1; i < PER; ++i)
             mx = fmaxf(mx, w[i]);
-        a.shift(mx);
+        if (__any(fmaf(mx, LP_LOG2E, -LP_SLACK) > a.m)) {
+            const float to = mx * LP_LOG2E;
+            if (to > a.m)
+                a.shift(to);
+        }
         if (a.m != -INFINITY) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
                 a.add(w[i]);
-        }
-        const int64_t j = r.head + vec * PER;
+        } else { /* nothing but -inf and NaN so far */
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-            before += w[i] > xt || (w[i] == xt && j + i < tok) ? 1 : 0;
-            bad |= !(w[i] < INFINITY);
+            for (int i = 0; i < PER; ++i)
+                a.s += w[i] != w[i] ? NAN : 0.f;
         }
-        if (mx > high || where < 0) {
-            high = fmaxf(high, mx); /* not NaN */
-            where = vec;
+        const int64_t j = r.head + (int64_t)vec * PER;
+        const float reach = j < tok ? xt : xt_up;
+        if (__any(mx >= reach || (j < tok && tok < j + PER))) {
+#pragma unroll
+            for (int i = 0; i < PER; ++i)
+                before += w[i] >= (j + i < tok ? xt : xt_up) ? 1 : 0;
         }
+        const bool more = mx > high || where < 0;
+        high = fmaxf(high, mx);
+        where = more ? vec : where;
+    };
+    for (int k0 = 0; k0 < rounds; k0 += LP_U) {
+        if (k0 + LP_U < rounds)
+            fetch(k0 + LP_U, next);
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u) {
+            const int vec = (int)threadIdx.x + (k0 + u) * LP_T;
+            if (vec < nvec)
+                take(vec, now[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < LP_U; ++u)
+            now[u] = next[u];
     }
-    int64_t ends[2] = {r.before(), r.after()};
+    uint64_t mine = 0;
+    const int64_t ends[2] = {r.before(), r.after()};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         if (ends[k] >= 0) {
-            const float x = r.at(ends[k]);
-            a.shift(x);
+            const float x = r.at(ends[k]), to = x * LP_LOG2E;
+            if (to > a.m)
+                a.shift(to);
             if (a.m != -INFINITY)
                 a.add(x);
-            before += x > xt || (x == xt && ends[k] < tok) ? 1 : 0;
-            bad |= !(x < INFINITY);
+            else
+                a.s += x != x ? NAN : 0.f;
+            before += x >= (ends[k] < tok ? xt : xt_up) ? 1 : 0;
             const uint64_t key = lp_key(x, ends[k]);
             mine = key > mine ? key : mine;
         }
     if (top > 0 && where >= 0) {
         float w[PER];
-        r.load(where, w);
+        r.unpack(r.raw(where), w);
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const uint64_t key = lp_key(w[i], r.head + where * PER + i);
+            const uint64_t key = lp_key(w[i], r.head + (int64_t)where * PER + i);
             mine = key > mine ? key : mine;
         }
     }
-    if (bad)
-        a.s = NAN;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        lp_join(a, __shfl_xor(a.m, o, 64), __shfl_xor(a.s, o, 64), __shfl_xor(a.t, o, 64));
-        before += __shfl_xor(before, o, 64);
-    }
+    /* the wave's sums under its largest reference */
+    const float wm = lp_wave(a.m, LpMax());
+    lp_refer(a, wm);
+    const float ws = lp_wave(a.s, LpAdd()), wt = lp_wave(a.t, LpAdd());
+    const int wr = lp_wave_sum(before);
     if (lane == 0) {
-        sm[wave] = a.m;
-        ss[wave] = a.s;
-        st[wave] = a.t;
-        sr[wave] = before;
+        sm[wave] = wm;
+        ss[wave] = ws;
+        st[wave] = wt;
+        sr[wave] = wr;
     }
     /* this wave's `top` largest thread maxima, in order */
     uint64_t rest = mine;
@@ -210,28 +306,30 @@ __global__ __launch_bounds__(LP_T) void k_token_logprobs(const E *__restrict__ l
         ncand = 0;
     __syncthreads();
     if (wave == 0) {
-        LpSum z{-INFINITY, 0.f, 0.f};
-        int n = 0;
-        for (int i = 0; i < LP_WAVES; ++i) {
-            lp_join(z, sm[i], ss[i], st[i]);
-            n += sr[i];
-        }
+        static_assert(LP_WAVES == 16, "one row of lanes holds every wave's sums");
+        LpSum z{sm[lane & 15], ss[lane & 15], st[lane & 15]};
+        const int n = lp_row16_sum(sr[lane & 15]);
+        lp_refer(z, lp_row16(z.m, LpMax()));
+        z.s = lp_row16(z.s, LpAdd());
+        z.t = lp_row16(z.t, LpAdd());
         if (z.m == -INFINITY)
             z.s = NAN; /* nothing is possible */
-        const float ls = logf(z.s);
-        const float lse = z.m + ls;
+        const float ls = log2f(z.s);
         if (lane == 0) {
-            logprob[row] = tok < 0 ? 0.f : is_tok ? (xt - z.m) - ls : NAN;
+            /* x - lse, in powers of two up to the last product */
+            logprob[row] = tok < 0 ? 0.f : is_tok ? (fmaf(xt, LP_LOG2E, -z.m) - ls) * LP_LN2 : NAN;
             if (entropy)
-                entropy[row] = ls - z.t / z.s;
+                entropy[row] = (ls - z.t / z.s) * LP_LN2;
             if (rank)
                 rank[row] = is_tok ? n : -1;
-            s_lse = lse;
+            s_ref = z.m;
+            s_ls = ls;
         }
         /* the top-th largest over the waves */
-        uint64_t v[(LP_WAVES * LP_TOP + 63) / 64];
+        constexpr int LISTS = (LP_WAVES * LP_TOP + 63) / 64;
+        uint64_t v[LISTS];
 #pragma unroll
-        for (int i = 0; i < (LP_WAVES * LP_TOP + 63) / 64; ++i) {
+        for (int i = 0; i < LISTS; ++i) {
             const int k = lane + 64 * i;
             v[i] = k < LP_WAVES * LP_TOP && k % LP_TOP < top ? best[k] : 0;
         }
@@ -239,11 +337,11 @@ __global__ __launch_bounds__(LP_T) void k_token_logprobs(const E *__restrict__ l
         for (int i = 0; i < top; ++i) {
             k = 0;
 #pragma unroll
-            for (int u = 0; u < (LP_WAVES * LP_TOP + 63) / 64; ++u)
+            for (int u = 0; u < LISTS; ++u)
                 k = v[u] > k ? v[u] : k;
             k = lp_wave_max(k);
 #pragma unroll
-            for (int u = 0; u < (LP_WAVES * LP_TOP + 63) / 64; ++u)
+            for (int u = 0; u < LISTS; ++u)
                 v[u] = v[u] == k ? 0 : v[u];
         }
         if (lane == 0)
@@ -253,17 +351,22 @@ __global__ __launch_bounds__(LP_T) void k_token_logprobs(const E *__restrict__ l
         return;
     __syncthreads();
     const uint64_t least = floor_key;
-    if (mine != 0 && mine >= least) {
-        for (int64_t vec = threadIdx.x; vec < r.nvec; vec += LP_T) {
+    /* the elements of each thread whose maximum counts, a load per lane of its wave */
+    for (uint64_t who = __ballot(mine != 0 && mine >= least); who; who &= who - 1) {
+        const int owner = wave * 64 + __builtin_ctzll(who);
+        const int vec = owner + lane * LP_T;
+        if (vec < nvec) { /* at most 64 rounds: V <= LP_V_TOP */
             float w[PER];
-            r.load(vec, w);
+            r.unpack(r.raw(vec), w);
 #pragma unroll
             for (int i = 0; i < PER; ++i) {
-                const uint64_t key = lp_key(w[i], r.head + vec * PER + i);
+                const uint64_t key = lp_key(w[i], r.head + (int64_t)vec * PER + i);
                 if (key >= least)
                     cand[atomicAdd(&ncand, 1)] = key;
             }
         }
+    }
+    if (mine != 0 && mine >= least) {
 #pragma unroll
         for (int k = 0; k < 2; ++k)
             if (ends[k] >= 0) {
@@ -274,16 +377,16 @@ __global__ __launch_bounds__(LP_T) void k_token_logprobs(const E *__restrict__ l
     }
     __syncthreads();
     const int n = ncand;
-    const float lse = s_lse;
+    const float m = s_ref, ls = s_ls;
     for (int c = threadIdx.x; c < n; c += LP_T) {
         const uint64_t key = cand[c];
         int place = 0;
+#pragma unroll 8
         for (int i = 0; i < n; ++i)
             place += cand[i] > key ? 1 : 0;
         if (place < top) {
-            const uint32_t j = lp_key_index(key);
-            top_logprob[row * top + place] = r.at(j) - lse;
-            top_index[row * top + place] = (int32_t)j;
+            top_logprob[row * top + place] = (fmaf(lp_key_value(key), LP_LOG2E, -m) - ls) * LP_LN2;
+            top_index[row * top + place] = (int32_t)lp_key_index(key);
         }
     }
 }
