@@ -1,9 +1,15 @@
 /* Attention over the 4-bit cache (include/glint_serve.h).
  *
- * k_kv4_attend — a workgroup takes a run of pages of one sequence and head for up to 16 NT
- *   query rows (the heads that share the key head, times the new tokens); its 8 waves take
- *   the run's pages in turn, each with a running maximum, sum and output of its own, and meet
- *   in LDS at the end. Per page of 64 tokens a wave forms scores transposed, S^T = K q^T, on
+ * k_kv4_attend — the work is a list of rounds: a group is one sequence, key head and block of
+ *   up to 16 NT query rows (the heads that share the key head, times the new tokens), and a
+ *   round is KA_WAVES pages of a group, one a wave. Every workgroup takes an equal run of the
+ *   list, whatever the lengths, so that a batch of short and long sequences fills the device
+ *   evenly and the table below is filled once per workgroup. A wave keeps a running maximum,
+ *   sum and output of its own; the waves meet in LDS at the end of a group, and the workgroups
+ *   that share one in the last of them to arrive (partials in the stream's workspace, added in
+ *   the groups' order, so the result does not depend on the arrival).
+ *
+ *   Per page of 64 tokens a wave forms scores transposed, S^T = K q^T, on
  *   the 16x16x32 f16 matrix instruction, so that a lane ends up with 16 tokens of one row,
  *   exponentiates in place and feeds them as they lie to O^T = V^T P^T: the order of the
  *   tokens inside a product is free, so the cache's rows are read in the order in which the
@@ -20,11 +26,11 @@
  *   (8 bits) fits f16 exactly once its row is scaled by a power of two; the weights are
  *   scaled by a power of two per row and 64-block that follows the largest value scale
  *   seen, so that they stay inside f16's range whatever the scales' size.
- *
- * k_kv4_join — adds the runs' outputs where a sequence was split over workgroups. */
+ */
 #include <algorithm>
 
 #include "kv4.h"
+#include "tile_mfma.h"
 
 typedef _Float16 kv4_f16x8 __attribute__((ext_vector_type(8)));
 
@@ -60,25 +66,34 @@ struct Kv4AttendArgs {
     int B, max_q, Hq, H, G;
     float scale;
     uint16_t *out;
-    float *part;
-    int nsplit, chunk; /* pages of a workgroup's run */
-    int nrb;           /* row blocks of 16 NT */
+    float *part; /* two partials per workgroup; NULL: groups are not split */
+    unsigned *ctr;
+    int least; /* fewest rounds of a workgroup's run */
 };
 
 /* The sequence's rows and length, with every device value bounded. */
 struct Kv4Seq {
     int64_t q0;
-    int nq, len, npages;
+    int nq, rows, len, npages;
+    int rounds; /* of a group; one at least: a group without pages writes zeros */
+    int blocks; /* row blocks */
+    int units;  /* of the list that the sequence takes */
 };
+template <int COLS>
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttendArgs &a, int b) {
     Kv4Seq s;
     s.q0 = a.cu_q ? a.cu_q[b] : (int64_t)b * a.max_q;
     const int64_t q1 = a.cu_q ? a.cu_q[b + 1] : s.q0 + a.max_q;
     s.nq = s.q0 >= 0 && q1 > s.q0 && q1 <= a.Tq ? (int)(q1 - s.q0) : 0;
+    s.rows = a.G * min(s.nq, a.max_q);
     s.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * KV4_PAGE);
     s.npages = (s.len + KV4_PAGE - 1) / KV4_PAGE;
+    s.rounds = a.part ? max(1, (s.npages + KA_WAVES - 1) / KA_WAVES) : 1;
+    s.blocks = (s.rows + COLS - 1) / COLS;
+    s.units = s.rounds * s.blocks * a.H;
     return s;
 }
+__device__ __forceinline__ int kv4_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 /* Some row's value scales leave f16's range: rows whose largest finite one does take a power
  * of two that puts it at 2^KA_VSTART and carry their outputs over. An infinite scale stays
@@ -109,36 +124,69 @@ __device__ __forceinline__ void kv4_new_power(const glint_f32x4 (&vscale)[4], fl
 template <int D, int NT>
 __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     constexpr int NB = D / 64, COLS = 16 * NT;
-    /* the table, then the waves' outputs over it: [wave][COLS][D + 4], m and l after each row */
-    constexpr int ROW = D + 4;
-    constexpr int LDS_WORDS = KA_WAVES * 16 * ROW > KA_TABLE_WORDS ? KA_WAVES * 16 * ROW : KA_TABLE_WORDS;
-    __shared__ __attribute__((aligned(16))) uint32_t lds[LDS_WORDS];
+    constexpr int ROW = D + 4; /* a row's output, then its maximum and sum */
+    __shared__ __attribute__((aligned(16))) uint32_t lds[KA_TABLE_WORDS];
+    __shared__ __attribute__((aligned(16))) float meet[KA_WAVES * 16 * ROW];
     __shared__ __attribute__((aligned(16))) float scales[KA_WAVES * 2 * NB * KV4_PAGE];
+    __shared__ unsigned s_last;
 
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63, wave = kv4_uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
-    const int split = (int)blockIdx.x % A.nsplit, rb = (int)blockIdx.x / A.nsplit;
-    const int h = blockIdx.y, b = blockIdx.z;
-    const Kv4Seq s = kv4_seq(A, b);
-    const int rows = A.G * min(s.nq, A.max_q);
-    if (rb * COLS >= rows)
-        return;
-    const int p0 = split * A.chunk, p1 = min(p0 + A.chunk, s.npages);
-    if (p0 >= p1 && split > 0)
-        return;
 
-    for (int i = threadIdx.x; i < 256 * KA_COPIES / 4; i += KA_T) {
-        const int byte = i / (KA_COPIES / 4);
-        union { _Float16 f[2]; uint32_t u; } e;
-        e.f[0] = (_Float16)(kKv4Parent[byte & 15] * KA_ALPHA);
-        e.f[1] = (_Float16)(kKv4Parent[byte >> 4] * KA_ALPHA);
-        ((glint_u32x4 *)lds)[byte * 16 + i % (KA_COPIES / 4)] = glint_u32x4{e.u, e.u, e.u, e.u};
+    /* this workgroup's run [u, u_end) of the list, and the sequence b that it starts in, `at` units in */
+    const int per = (A.B + 63) / 64; /* sequences of a lane */
+    int mine = 0;
+    for (int i = 0; i < per; ++i)
+        if (lane * per + i < A.B)
+            mine += kv4_seq<COLS>(A, lane * per + i).units;
+    int upto = mine;
+#pragma unroll
+    for (int k = 1; k < 64; k <<= 1) {
+        const int v = __shfl_up(upto, k, 64);
+        upto += lane >= k ? v : 0;
     }
+    const int total = __builtin_amdgcn_readlane(upto, 63);
+    const int share = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    if ((int64_t)blockIdx.x * share >= total)
+        return;
+    int u = blockIdx.x * share;
+    const int u_end = min(total - u, share) + u;
+    int b, at;
+    {
+        const int owner = __builtin_ctzll(__ballot(upto > u));
+        at = u - __builtin_amdgcn_readlane(upto - mine, owner);
+        b = owner * per;
+    }
+    Kv4Seq s = kv4_seq<COLS>(A, b);
+    auto skip = [&]() { /* to the sequence that `at` lies in */
+        while (at >= s.units) {
+            at -= s.units;
+            s = kv4_seq<COLS>(A, ++b);
+        }
+    };
+    skip();
 
-    /* this lane's rows: q as f16 operands, scaled to 2^14 .. 2^15 by a power of two that goes
-     * into the row's score factor */
-    Kv4Frag qf[NT][NB][2];
-    float factor[NT];
+    const uint32_t lane4 = (uint32_t)(lane & (KA_COPIES - 1)) * 4;
+    auto pair = [&](uint32_t word, int byte) { /* byte << 8 | lane4 */
+        return *(const uint32_t *)((const char *)lds + __builtin_amdgcn_perm(word, lane4, 0x0C0C0000u | ((4u + byte) << 8)));
+    };
+    float *sl = scales + wave * (2 * NB * KV4_PAGE);
+
+    for (bool first_group = true; u < u_end; first_group = false) {
+    const int group = at / s.rounds, begin = at % s.rounds;
+    const int h = kv4_uniform(group / s.blocks), rb = kv4_uniform(group % s.blocks);
+    const int nrounds = min(s.rounds - begin, u_end - u);
+    const int p0 = begin * KA_WAVES, p1 = A.part ? min((begin + nrounds) * KA_WAVES, s.npages) : s.npages;
+    const int rows = s.rows;
+
+    /* the group's loads first: this wave's first 64 pages, one a lane, and the lane's rows of q */
+    const int32_t *table = A.table + b * A.table_stride;
+    auto page_id = [&](int pg0) {
+        const int pg = pg0 + lane * KA_WAVES;
+        return pg < p1 ? table[pg] : -1;
+    };
+    int pid_mine = page_id(p0 + wave);
+    glint_u32x4 qw[NT][NB][2];
     int last[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
@@ -147,53 +195,25 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         const bool live = r < rows;
         last[n] = live ? s.len - s.nq + i : -1;
         const uint16_t *qr = A.q + (s.q0 + (live ? i : 0)) * A.q_st + (live ? hq : h * A.G) * A.q_sh;
-        glint_u32x4 w[NB][2];
-        uint32_t top = 0;
-#pragma unroll
-        for (int bb = 0; bb < NB; ++bb)
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                w[bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    top = max(top, max((w[bb][st][x] & 0x7FFFu) << 16, w[bb][st][x] & 0x7FFF0000u));
-            }
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const int ex = top >= 0x7F800000u ? 0 : (int)(top >> 23) - 127 - 14; /* 2^14 <= top 2^-ex < 2^15 */
 #pragma unroll
         for (int bb = 0; bb < NB; ++bb)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    qf[n][bb][st].f[2 * x] = (_Float16)ldexpf(glint_bf16lo(w[bb][st][x]), -ex);
-                    qf[n][bb][st].f[2 * x + 1] = (_Float16)ldexpf(glint_bf16hi(w[bb][st][x]), -ex);
-                }
-        factor[n] = ldexpf(A.scale * (1.44269504088896341f / KA_ALPHA), ex);
+                qw[n][bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
     }
-    __syncthreads();
-
-    glint_f32x4 o[NT][D / 16];
-    float m[NT], l[NT], vdown[NT][NB], vlimit[NT][NB];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        m[n] = -INFINITY;
-        l[n] = 0.f;
-#pragma unroll
-        for (int d = 0; d < D / 16; ++d)
-            o[n][d] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int bb = 0; bb < NB; ++bb) {
-            vdown[n][bb] = 0x1p126f;
-            vlimit[n][bb] = 0x1p-111f;
+    if (first_group) {
+        for (int i = threadIdx.x; i < 256 * KA_COPIES / 4; i += KA_T) {
+            const int byte = i / (KA_COPIES / 4);
+            union {
+                _Float16 f[2];
+                uint32_t u;
+            } e;
+            e.f[0] = (_Float16)(kKv4Parent[byte & 15] * KA_ALPHA);
+            e.f[1] = (_Float16)(kKv4Parent[byte >> 4] * KA_ALPHA);
+            ((glint_u32x4 *)lds)[byte * 16 + i % (KA_COPIES / 4)] = glint_u32x4{e.u, e.u, e.u, e.u};
         }
+        __syncthreads();
     }
-
-    const uint32_t lane4 = (uint32_t)(lane & (KA_COPIES - 1)) * 4;
-    auto pair = [&](uint32_t word, int byte) { /* byte << 8 | lane4 */
-        return *(const uint32_t *)((const char *)lds + __builtin_amdgcn_perm(word, lane4, 0x0C0C0000u | ((4u + byte) << 8)));
-    };
 
     /* A page's loads: this lane's 16-B pieces of the key rows and value columns, and one token's
      * scales, which go to the other lanes through LDS. */
@@ -219,28 +239,76 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         for (int p = 0; p < D / 32; ++p)
             vw[p] = *(const glint_u32x4 *)(vp + p * (16 * KV4_PAGE));
     };
-    float *sl = scales + wave * (2 * NB * KV4_PAGE);
-
-    for (int pg0 = p0 + wave; pg0 < p1; pg0 += 64 * KA_WAVES) {
-        /* this wave's next 64 pages, one a lane; those outside the pool drop out */
-        const int mine = pg0 + lane * KA_WAVES;
-        const int pid_mine = mine < p1 ? A.table[b * A.table_stride + mine] : -1;
-        uint64_t todo = __ballot(pid_mine >= 0 && pid_mine < A.pages);
-        if (todo == 0)
-            continue;
-        int at = __builtin_ctzll(todo);
+    /* the pages of the wave that lie in the pool, one bit a lane; the next one's place */
+    uint64_t todo = __ballot(pid_mine >= 0 && pid_mine < A.pages);
+    int lane_at = 0;
+    int64_t ph = 0;
+    auto take = [&]() {
+        lane_at = __builtin_ctzll(todo);
         todo &= todo - 1;
-        int64_t ph = (int64_t)__builtin_amdgcn_readlane(pid_mine, at) * A.H + h;
+        ph = (int64_t)__builtin_amdgcn_readlane(pid_mine, lane_at) * A.H + h;
+    };
+    auto start = [&]() {
+        if (todo == 0)
+            return false;
+        take();
         load_k(ph);
         load_v(ph);
-        for (bool more = true; more;) {
-        const int pg = pg0 + at * KA_WAVES;
-        more = todo != 0;
-        if (more) {
-            at = __builtin_ctzll(todo);
-            todo &= todo - 1;
-            ph = (int64_t)__builtin_amdgcn_readlane(pid_mine, at) * A.H + h;
+        return true;
+    };
+    bool have = start();
+
+    /* this lane's rows of q as f16 operands, scaled to 2^14 .. 2^15 by a power of two that goes
+     * into the row's score factor */
+    Kv4Frag qf[NT][NB][2];
+    float factor[NT];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        uint32_t top = 0;
+#pragma unroll
+        for (int bb = 0; bb < NB; ++bb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    top = max(top, max((qw[n][bb][st][x] & 0x7FFFu) << 16, qw[n][bb][st][x] & 0x7FFF0000u));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+        const int ex = top >= 0x7F800000u ? 0 : (int)(top >> 23) - 127 - 14; /* 2^14 <= top 2^-ex < 2^15 */
+#pragma unroll
+        for (int bb = 0; bb < NB; ++bb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    qf[n][bb][st].f[2 * x] = (_Float16)ldexpf(glint_bf16lo(qw[n][bb][st][x]), -ex);
+                    qf[n][bb][st].f[2 * x + 1] = (_Float16)ldexpf(glint_bf16hi(qw[n][bb][st][x]), -ex);
+                }
+        factor[n] = ldexpf(A.scale * (1.44269504088896341f / KA_ALPHA), ex);
+    }
+
+    glint_f32x4 o[NT][D / 16];
+    float m[NT], l[NT], vdown[NT][NB], vlimit[NT][NB];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+        m[n] = -INFINITY;
+        l[n] = 0.f;
+#pragma unroll
+        for (int d = 0; d < D / 16; ++d)
+            o[n][d] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int bb = 0; bb < NB; ++bb) {
+            vdown[n][bb] = 0x1p126f;
+            vlimit[n][bb] = 0x1p-111f;
         }
+    }
+
+    for (int pg0 = p0 + wave; pg0 < p1;) {
+        for (bool more = have; more;) {
+        const int pg = pg0 + lane_at * KA_WAVES;
+        more = todo != 0;
+        if (more)
+            take();
 #pragma unroll
         for (int x = 0; x < 2 * NB; ++x)
             sl[x * KV4_PAGE + lane] = sw[x];
@@ -378,23 +446,42 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         if (more)
             load_v(ph);
         }
+        pg0 += 64 * KA_WAVES; /* the next 64 pages */
+        pid_mine = page_id(pg0);
+        todo = __ballot(pid_mine >= 0 && pid_mine < A.pages);
+        have = start();
     }
 
-    /* the waves meet: each writes its rows' outputs, maximum and sum */
-    float *meet = (float *)lds;
+    /* The waves meet: each writes its rows' outputs, maximum and sum. A group that ends where it
+     * begins is done; else this workgroup's part goes to its slot 1, where it begins here, or 0,
+     * and the workgroup whose arrival completes the count adds all parts in order. */
+    const int u_begin = u - begin;
+    const bool whole_group = begin == 0 && nrounds == s.rounds;
+    const int w_first = u_begin / share, w_last = (u_begin + s.rounds - 1) / share;
+    float *parts = A.part + (int64_t)2 * w_first * COLS * ROW; /* of w_first; its slot 1, then slot 0 of each that follows */
+    auto part_of = [&](int w) { return parts + (int64_t)(2 * (w - w_first) + (w == w_first)) * COLS * ROW; };
+    auto store = [&](int r, int d, const float (&acc)[4], float total) {
+        const float inv = total == 0.f ? 0.f : 1.f / total;
+        uint16_t *dst = A.out + ((s.q0 + r / A.G) * A.Hq + h * A.G + r % A.G) * D + d;
+        glint_u32x2 two;
+        two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
+        two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
+        *(glint_u32x2 *)dst = two;
+    };
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
         float sum = l[n];
         sum += __shfl_xor(sum, 16, 64);
         sum += __shfl_xor(sum, 32, 64);
-        __syncthreads(); /* the table, or the previous rows, are read */
+        __syncthreads(); /* the previous rows are read */
         float *row = meet + (wave * 16 + col) * ROW;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
             glint_f32x4 v = o[n][d];
+            const float back = 1.f / vdown[n][d >> 2] * (1.f / KA_ALPHA); /* a power of two, inverted exactly */
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                v[i] = v[i] / vdown[n][d >> 2] * (1.f / KA_ALPHA);
+                v[i] *= back;
             *(glint_f32x4 *)(row + 16 * d + 4 * g) = v;
         }
         if (g == 0) {
@@ -412,7 +499,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             for (int w = 0; w < KA_WAVES; ++w)
                 mx = fmaxf(mx, meet[(w * 16 + c) * ROW + D]);
             const float base = mx == -INFINITY ? 0.f : mx;
-            glint_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
             float total = 0.f;
 #pragma unroll
             for (int w = 0; w < KA_WAVES; ++w) {
@@ -424,121 +511,137 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                 for (int i = 0; i < 4; ++i)
                     acc[i] = fmaf(f, v[i], acc[i]);
             }
-            if (A.nsplit > 1) {
-                float *dst = A.part + (((((int64_t)b * A.H + h) * A.nrb + rb) * A.nsplit + split) * COLS + 16 * n + c) * (D + 4);
-                *(glint_f32x4 *)(dst + d) = acc;
-                if (d == 0) {
-                    dst[D] = mx;
-                    dst[D + 1] = total;
-                }
+            if (whole_group) {
+                store(r, d, acc, total);
             } else {
-                const float inv = total == 0.f ? 0.f : 1.f / total;
-                uint16_t *dst = A.out + ((s.q0 + r / A.G) * A.Hq + h * A.G + r % A.G) * D + d;
-                glint_u32x2 two;
-                two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
-                two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
-                *(glint_u32x2 *)dst = two;
+                float *dst = part_of(blockIdx.x) + (16 * n + c) * ROW;
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    __hip_atomic_store(dst + d + i, acc[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                if (d == 0) {
+                    __hip_atomic_store(dst + D, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(dst + D + 1, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
             }
         }
     }
-}
-
-/* One thread per 4 dimensions of a row: the runs that hold pages of the sequence (the first
- * one always writes), in order. */
-template <int D, int NT>
-__global__ __launch_bounds__(256) void k_kv4_join(Kv4AttendArgs A) {
-    constexpr int COLS = 16 * NT, PER = D / 4;
-    const int h = blockIdx.y, b = blockIdx.z;
-    const Kv4Seq s = kv4_seq(A, b);
-    const int r = (int)((blockIdx.x * 256 + threadIdx.x) / PER), d = 4 * (int)(threadIdx.x % PER);
-    if (r >= A.G * min(s.nq, A.max_q))
-        return;
-    const int used = max(1, (s.npages + A.chunk - 1) / A.chunk);
-    const float *src = A.part + ((((int64_t)b * A.H + h) * A.nrb + r / COLS) * A.nsplit * COLS + r % COLS) * (D + 4);
-    const int64_t step = (int64_t)COLS * (D + 4);
-    float mx = -INFINITY;
-    for (int i = 0; i < used; ++i)
-        mx = fmaxf(mx, src[i * step + D]);
-    const float base = mx == -INFINITY ? 0.f : mx;
-    glint_f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-    float total = 0.f;
-    for (int i = 0; i < used; ++i) {
-        const float f = __builtin_amdgcn_exp2f(src[i * step + D] - base);
-        const glint_f32x4 v = *(const glint_f32x4 *)(src + i * step + d);
-        total = fmaf(f, src[i * step + D + 1], total);
+    if (!whole_group) {
+        __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+        __syncthreads();
+        if (threadIdx.x == 0)
+            s_last = __hip_atomic_fetch_add(&A.ctr[w_first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                     (unsigned)(w_last - w_first);
+        __syncthreads();
+        if (s_last) {
+            for (int t = threadIdx.x; t < COLS * (D / 4); t += KA_T) {
+                const int c = t / (D / 4), d = 4 * (t % (D / 4));
+                const int r = rb * COLS + c;
+                if (r >= rows)
+                    continue;
+                float mx = -INFINITY, total = 0.f;
+                float acc[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int w0 = w_first; w0 <= w_last; w0 += 4) { /* four parts' loads in flight */
+                    float v[4][6];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            acc[k] = fmaf(f, v[k], acc[k]);
+                    for (int k = 0; k < 4; ++k) {
+                        const float *src = part_of(min(w0 + k, w_last)) + c * ROW;
+#pragma unroll
+                        for (int i = 0; i < 6; ++i)
+                            v[k][i] = __hip_atomic_load(src + (i < 4 ? d + i : D + i - 4), __ATOMIC_RELAXED,
+                                                        __HIP_MEMORY_SCOPE_AGENT);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (w0 + k <= w_last) {
+                            const float to = fmaxf(mx, v[k][4]), base = to == -INFINITY ? 0.f : to;
+                            const float keep = __builtin_amdgcn_exp2f(mx - base), f = __builtin_amdgcn_exp2f(v[k][4] - base);
+                            mx = to;
+                            total = fmaf(total, keep, f * v[k][5]);
+#pragma unroll
+                            for (int i = 0; i < 4; ++i)
+                                acc[i] = fmaf(acc[i], keep, f * v[k][i]);
+                        }
+                }
+                store(r, d, acc, total);
+            }
+            if (threadIdx.x == 0)
+                __hip_atomic_store(&A.ctr[w_first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
     }
-    const float inv = total == 0.f ? 0.f : 1.f / total;
-    glint_u32x2 two;
-    two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
-    two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
-    *(glint_u32x2 *)(A.out + ((s.q0 + r / A.G) * A.Hq + h * A.G + r % A.G) * D + d) = two;
+    u += nrounds;
+    at += nrounds;
+    if (u < u_end)
+        skip();
+    }
 }
 
 /* Tiles of 16 rows a wave carries: two once a sequence's rows of a head fill more than one. */
 static int ka_tiles(int max_q, int G) { return (int64_t)max_q * G > 16 ? 2 : 1; }
 
-/* Runs of pages: enough workgroups for two per CU, none shorter than a page per wave. */
-static void ka_plan(int B, int max_q, int Hq, int H, int max_pages, int &nrb, int &nsplit, int &chunk) {
-    const int G = Hq / H, cols = 16 * ka_tiles(max_q, G);
-    nrb = (int)(((int64_t)max_q * G + cols - 1) / cols);
-    const int64_t groups = (int64_t)B * H * nrb, want = 2 * (int64_t)glint_cu_count();
-    const int64_t most = max(1, (max_pages + KA_WAVES - 1) / KA_WAVES);
-    const int64_t n = groups >= want ? 1 : std::min<int64_t>(most, (want + groups - 1) / groups);
-    const int64_t per = (most + n - 1) / n; /* rounds of KA_WAVES pages */
-    chunk = (int)(per * KA_WAVES);
-    nsplit = (int)((most + per - 1) / per);
-}
+#ifndef KA_LEAST
+#define KA_LEAST 2
+#endif
 
 static bool ka_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
-    return B >= 0 && B <= 65535 && max_q >= 1 && H >= 1 && H <= 65535 && Hq >= H && Hq % H == 0 &&
-           (D == 64 || D == 128) && max_pages >= 1 && max_pages <= (1 << 25) && (int64_t)max_q * (Hq / H) <= (1 << 20);
+    return B >= 0 && max_q >= 1 && H >= 1 && Hq >= H && Hq % H == 0 && (D == 64 || D == 128) && max_pages >= 1 &&
+           max_pages <= (1 << 25) && (int64_t)max_q * (Hq / H) <= (1 << 20);
 }
 
-GLINT_API int64_t glint_kv4_attend_part(int B, int max_q, int Hq, int H, int D, int max_pages) {
-    if (!ka_shape(B, max_q, Hq, H, D, max_pages))
-        return -2;
-    int nrb, nsplit, chunk;
-    ka_plan(B, max_q, Hq, H, max_pages, nrb, nsplit, chunk);
-    return nsplit <= 1 ? 0 : (int64_t)B * H * nrb * nsplit * 16 * ka_tiles(max_q, Hq / H) * (D + 4);
+/* Units of the longest list that the shape allows, or -1 where they leave 31 bits. */
+static int64_t ka_units(int B, int max_q, int H, int G, int max_pages) {
+    const int cols = 16 * ka_tiles(max_q, G);
+    const int64_t blocks = ((int64_t)max_q * G + cols - 1) / cols, rounds = (max_pages + KA_WAVES - 1) / KA_WAVES;
+    const double n = (double)B * H * (double)blocks * (double)rounds;
+    return n > (double)(1 << 30) ? -1 : (int64_t)B * H * blocks * rounds;
 }
 
 template <int D, int NT>
-static void ka_launch(const Kv4AttendArgs &a, hipStream_t stream) {
-    k_kv4_attend<D, NT><<<dim3(a.nsplit * a.nrb, a.H, a.B), KA_T, 0, stream>>>(a);
-    if (a.nsplit > 1) {
-        const int per = 256 / (D / 4); /* rows per workgroup */
-        k_kv4_join<D, NT><<<dim3((unsigned)((a.G * a.max_q + per - 1) / per), a.H, a.B), 256, 0, stream>>>(a);
-    }
+static void ka_launch(const Kv4AttendArgs &a, int64_t units, hipStream_t stream) {
+    const int64_t most = (units + a.least - 1) / a.least;
+    k_kv4_attend<D, NT><<<(unsigned)std::min<int64_t>(most, glint_cu_count()), KA_T, 0, stream>>>(a);
 }
+
+GLINT_API int glint_serve_workspace_reserve(struct ihipStream_t *stream) {
+    if (glint_stream_captures(stream))
+        return -1;
+    GlintSplitWs ws;
+    return glint_split_ws_stream(stream, ws) ? 0 : -1;
+}
+GLINT_API int glint_serve_workspace_release(struct ihipStream_t *stream) { return glint_split_ws_release(stream); }
 
 GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq,
                                const uint8_t *k_hole, const float *k_absmax, const uint8_t *v_hole,
                                const float *v_absmax, int64_t pages, const int32_t *table, int64_t table_stride,
                                int max_pages, const int32_t *lens, const int32_t *cu_q, int B, int max_q, int Hq, int H,
-                               int D, float scale, uint16_t *out, float *part, struct ihipStream_t *stream) {
+                               int D, float scale, uint16_t *out, struct ihipStream_t *stream) {
     if (!q || !k_hole || !k_absmax || !v_hole || !v_absmax || !table || !lens || !out)
         return -1;
     if (!ka_shape(B, max_q, Hq, H, D, max_pages) || Tq < 0 || pages < 1 || pages >= (int64_t)1 << 40 ||
         (!cu_q && Tq != (int64_t)B * max_q))
         return -2;
     if (!glint_aligned(q, 16) || !glint_aligned(out, 8) || !glint_aligned(k_hole, 16) || !glint_aligned(v_hole, 16) ||
-        !glint_aligned(k_absmax, 16) || !glint_aligned(v_absmax, 16) || !glint_aligned(part, 16) ||
-        ((q_stride_t | q_stride_h) & 7))
+        !glint_aligned(k_absmax, 16) || !glint_aligned(v_absmax, 16) || ((q_stride_t | q_stride_h) & 7))
         return -2;
     if (B == 0 || Tq == 0)
         return 0;
     Kv4AttendArgs a{q, q_stride_t, q_stride_h, Tq, k_hole, v_hole, k_absmax, v_absmax, pages, table, table_stride,
-                    max_pages, lens, cu_q, B, max_q, Hq, H, Hq / H, scale, out, part, 1, 1, 1};
-    ka_plan(B, max_q, Hq, H, max_pages, a.nrb, a.nsplit, a.chunk);
-    if (a.nsplit > 1 && !part)
-        return -1;
+                    max_pages, lens, cu_q, B, max_q, Hq, H, Hq / H, scale, out, nullptr, nullptr, 1};
+    int64_t units = ka_units(B, max_q, H, a.G, max_pages);
+    if (units < 0)
+        return -2;
     const bool two = ka_tiles(max_q, a.G) == 2;
+    GlintSplitWs ws;
+    if (max_pages > KA_WAVES && glint_split_ws_stream(stream, ws) && ws.nctr >= (size_t)glint_cu_count() &&
+        ws.part_floats >= (size_t)glint_cu_count() * 2 * 32 * (D + 4)) {
+        a.part = ws.part;
+        a.ctr = ws.ctr;
+        a.least = KA_LEAST;
+    } else {
+        units = ka_units(B, max_q, H, a.G, 1); /* whole groups */
+    }
     if (D == 64)
-        two ? ka_launch<64, 2>(a, stream) : ka_launch<64, 1>(a, stream);
+        two ? ka_launch<64, 2>(a, units, stream) : ka_launch<64, 1>(a, units, stream);
     else
-        two ? ka_launch<128, 2>(a, stream) : ka_launch<128, 1>(a, stream);
+        two ? ka_launch<128, 2>(a, units, stream) : ka_launch<128, 1>(a, units, stream);
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }

@@ -120,9 +120,10 @@ _P7_SIGS = {
 _SERVE_SIGS = {
     "glint_kv4_append": ([VP, VP, I32, I64, I64, I64, I64, VP, I64, I32, I32, VP, VP, VP, VP, I64, VP], I32),
     "glint_kv4_gather": ([VP, I64, I32, I32, VP, VP, VP, VP, I64, VP, VP, VP], I32),
-    "glint_kv4_attend_part": ([I32, I32, I32, I32, I32, I32], I64),
     "glint_kv4_attend": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32,
-                          _c.c_float, VP, VP, VP], I32),
+                          _c.c_float, VP, VP], I32),
+    "glint_serve_workspace_reserve": ([VP], I32),
+    "glint_serve_workspace_release": ([VP], I32),
     "glint_attend_prompt": ([VP, I64, I64, VP, I64, I64, VP, I64, I64, VP, VP, I64, I64, I32, I32, I32, I32, I32,
                              _c.c_float, VP, VP], I32),
     "glint_token_logprobs": ([VP, I32, I64, VP, I64, I64, I32, VP, VP, VP, VP, VP, VP], I32),
@@ -663,12 +664,9 @@ def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Opt
         return out
     if wide == 0:
         return out.zero_()
-    lib = serve_lib()
-    need = lib.glint_kv4_attend_part(B, max_q, hq, heads, dim, wide)
-    part = q.new_empty(need, dtype=torch.float32) if need > 0 else None
-    _check(lib.glint_kv4_attend(q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(), page_table.stride(0),
-                                wide, n, cu, B, max_q, hq, heads, dim, dim ** -0.5 if scale is None else scale,
-                                out.data_ptr(), None if part is None else part.data_ptr(), _sh(None)),
+    _check(serve_lib().glint_kv4_attend(q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(),
+                                        page_table.stride(0), wide, n, cu, B, max_q, hq, heads, dim,
+                                        dim ** -0.5 if scale is None else scale, out.data_ptr(), _sh(None)),
            "glint_kv4_attend")
     return out
 

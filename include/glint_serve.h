@@ -18,7 +18,8 @@
  * The place of a token is its slot, page * 64 + t.
  *
  * Return codes: 0 success, -1 null pointer, -2 shape, stride or alignment not supported,
- * -3 launch failure. All calls are asynchronous on `stream` and allocate nothing. D is 64 or
+ * -3 launch failure. All calls are asynchronous on `stream` and allocate nothing (but
+ * glint_kv4_attend a workspace, once per stream). D is 64 or
  * 128; strides count elements, a row's D elements are adjacent. */
 #ifndef GLINT_SERVE_H
 #define GLINT_SERVE_H
@@ -56,13 +57,23 @@ int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, const uint8_
  * BF16 out [Tq][Hq][D]; a row that sees nothing is zero. Rows outside every sequence's are
  * left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores, softmax and
  * sums are f32; PARENT and the softmax weights times the value scales enter the matrix
- * products in f16. part: f32 scratch of glint_kv4_attend_part(...) floats (NULL when 0). */
-int64_t glint_kv4_attend_part(int B, int max_q, int Hq, int H, int D, int max_pages);
+ * products in f16. B H max_q max_pages is bounded: -2 where the list of work passes 2^30.
+ * Sequences longer than 512 tokens are split over workgroups that meet in a workspace of the
+ * stream's (glint_serve_workspace_reserve): it is allocated by the first such call outside a
+ * capture and never grows. A capture on a stream that has none runs unsplit. */
 int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq, const uint8_t *k_hole,
                      const float *k_absmax, const uint8_t *v_hole, const float *v_absmax, int64_t pages,
                      const int32_t *table, int64_t table_stride, int max_pages, const int32_t *lens,
                      const int32_t *cu_q, int B, int max_q, int Hq, int H, int D, float scale, uint16_t *out,
-                     float *part, struct ihipStream_t *stream);
+                     struct ihipStream_t *stream);
+
+/* The stream's workspace, 128 MiB on 256 CUs: one for eager calls and, once the stream was
+ * captured, one for the graphs captured on it, whose replays must not overlap one another.
+ * reserve allocates the eager one ahead of time (0; -1: no memory, or the stream is being
+ * captured). release waits for the stream and frees both (0, or -1); graphs captured before
+ * must not be replayed after it. */
+int glint_serve_workspace_reserve(struct ihipStream_t *stream);
+int glint_serve_workspace_release(struct ihipStream_t *stream);
 
 /* Causal attention of B packed sequences. Sequence b has queries cu_q[b] .. cu_q[b + 1] of
  * q [Tq] (at most max_q) and keys cu_k[b] .. cu_k[b + 1] of k, v [Tk]; the last query sees

@@ -43,7 +43,7 @@ def append(lib, **kw):
 
 def attend(lib, **kw):
     a = dict(q=P, qt=1024, qh=128, Tq=2, kh=P, ka=P, vh=P, va=P, pages=2, table=P, ts=4, wide=4, lens=P, cu=None, B=2,
-             max_q=1, Hq=8, H=2, D=128, scale=1.0, out=P, part=P, stream=None)
+             max_q=1, Hq=8, H=2, D=128, scale=1.0, out=P, stream=None)
     a.update(kw)
     return lib.glint_kv4_attend(*a.values())
 
@@ -66,7 +66,7 @@ def scores(lib, **kw):
               ("vsh", 129, -2), ("k", ctypes.c_void_p(68), -2), ("H", 0, -2), ("T", -1, -2), ("pages", 0, -2),
               ("T", 1 << 41, -2)]),
     (attend, [("q", None, -1), ("lens", None, -1), ("out", None, -1), ("D", 256, -2), ("H", 3, -2), ("Tq", 3, -2),
-              ("qt", 1020, -2), ("q", ctypes.c_void_p(72), -2), ("wide", 0, -2), ("max_q", 0, -2), ("B", 65536, -2),
+              ("qt", 1020, -2), ("q", ctypes.c_void_p(72), -2), ("wide", 0, -2), ("max_q", 0, -2), ("B", -1, -2), ("wide", (1 << 25) + 1, -2),
               ("pages", 0, -2)]),
     (prompt, [("v", None, -1), ("cq", None, -1), ("out", None, -1), ("D", 80, -2), ("H", 3, -2), ("kt", 252, -2),
               ("v", ctypes.c_void_p(72), -2), ("B", -1, -2), ("max_q", -1, -2), ("Tk", -1, -2)]),
@@ -88,7 +88,6 @@ def test_empty_calls_do_nothing():
     assert lib.glint_kv4_gather(P, 0, 8, 128, P, P, P, P, 2, P, P, None) == 0
     assert lib.glint_kv4_gather(P, 1, 8, 128, P, P, P, P, 2, None, P, None) == -1
     assert lib.glint_kv4_gather(P, 1, 8, 100, P, P, P, P, 2, P, P, None) == -2
-    assert lib.glint_kv4_attend_part(2, 1, 8, 3, 128, 4) == -2
 
 
 def test_helpers_refuse():
