@@ -47,6 +47,7 @@ typedef _Float16 kv4_f16x8 __attribute__((ext_vector_type(8)));
 #define KA_ALPHA 1.458935f
 #define KA_VMAX 15 /* a scaled weight stays below 2^KA_VMAX */
 #define KA_VSTART 10
+#define KA_FAR (1 << 24) /* a page number past every sequence's: tables hold no more pages */
 
 union Kv4Frag {
     uint32_t u[4];
@@ -77,6 +78,7 @@ struct Kv4Seq {
     int nq, rows, len, npages;
     int rounds; /* of a group; one at least: a group without pages writes zeros */
     int blocks; /* row blocks */
+    int each;   /* units of a group: its rounds, or 1 where groups are not split */
     int units;  /* of the list that the sequence takes */
 };
 template <int COLS>
@@ -88,9 +90,10 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttendArgs &a, int b) {
     s.rows = a.G * min(s.nq, a.max_q);
     s.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * KV4_PAGE);
     s.npages = (s.len + KV4_PAGE - 1) / KV4_PAGE;
-    s.rounds = a.part ? max(1, (s.npages + KA_WAVES - 1) / KA_WAVES) : 1;
+    s.rounds = max(1, (s.npages + KA_WAVES - 1) / KA_WAVES);
     s.blocks = (s.rows + COLS - 1) / COLS;
-    s.units = s.rounds * s.blocks * a.H;
+    s.each = a.part ? s.rounds : 1;
+    s.units = s.each * s.blocks * a.H;
     return s;
 }
 __device__ __forceinline__ int kv4_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -121,6 +124,20 @@ __device__ __forceinline__ void kv4_new_power(const glint_f32x4 (&vscale)[4], fl
     limit = ldexpf(1.f, e + KA_VMAX);
 }
 
+/* A group, or the part of it that this workgroup's run holds. */
+struct Kv4Group {
+    Kv4Seq s;
+    int b, at;       /* the sequence, and where in it the part begins */
+    int h, rb;       /* key head, row block */
+    int u, units;    /* place in the list, units */
+    int begin, n;    /* first round, rounds */
+};
+/* A part that other workgroups share: what the one that joins them has to know. */
+struct Kv4Join {
+    int on, w_first, w_last, rows, rb, h;
+    int64_t q0;
+};
+
 template <int D, int NT>
 __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     constexpr int NB = D / 64, COLS = 16 * NT;
@@ -128,12 +145,12 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     __shared__ __attribute__((aligned(16))) uint32_t lds[KA_TABLE_WORDS];
     __shared__ __attribute__((aligned(16))) float meet[KA_WAVES * 16 * ROW];
     __shared__ __attribute__((aligned(16))) float scales[KA_WAVES * 2 * NB * KV4_PAGE];
-    __shared__ unsigned s_last;
+    __shared__ unsigned s_last[2];
 
     const int lane = threadIdx.x & 63, wave = kv4_uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
 
-    /* this workgroup's run [u, u_end) of the list, and the sequence b that it starts in, `at` units in */
+    /* this workgroup's run [u, u_end) of the list, and where it begins */
     const int per = (A.B + 63) / 64; /* sequences of a lane */
     int mine = 0;
     for (int i = 0; i < per; ++i)
@@ -149,22 +166,29 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     const int share = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
     if ((int64_t)blockIdx.x * share >= total)
         return;
-    int u = blockIdx.x * share;
-    const int u_end = min(total - u, share) + u;
-    int b, at;
-    {
-        const int owner = __builtin_ctzll(__ballot(upto > u));
-        at = u - __builtin_amdgcn_readlane(upto - mine, owner);
-        b = owner * per;
-    }
-    Kv4Seq s = kv4_seq<COLS>(A, b);
-    auto skip = [&]() { /* to the sequence that `at` lies in */
-        while (at >= s.units) {
-            at -= s.units;
-            s = kv4_seq<COLS>(A, ++b);
+    const int u_end = min(total - (int)blockIdx.x * share, share) + blockIdx.x * share;
+    /* completes a group whose sequence, place in it and place in the list are set */
+    auto place = [&](Kv4Group &G) {
+        while (G.at >= G.s.units) { /* on to the sequence that it lies in */
+            G.at -= G.s.units;
+            G.s = kv4_seq<COLS>(A, ++G.b);
         }
+        const int group = G.at / G.s.each;
+        G.begin = G.at % G.s.each;
+        G.h = kv4_uniform(group / G.s.blocks);
+        G.rb = kv4_uniform(group % G.s.blocks);
+        G.units = min(G.s.each - G.begin, u_end - G.u);
+        G.n = A.part ? G.units : G.s.rounds;
     };
-    skip();
+    Kv4Group G;
+    {
+        G.u = blockIdx.x * share;
+        const int owner = __builtin_ctzll(__ballot(upto > G.u));
+        G.at = G.u - __builtin_amdgcn_readlane(upto - mine, owner);
+        G.b = owner * per;
+        G.s = kv4_seq<COLS>(A, G.b);
+        place(G);
+    }
 
     const uint32_t lane4 = (uint32_t)(lane & (KA_COPIES - 1)) * 4;
     auto pair = [&](uint32_t word, int byte) { /* byte << 8 | lane4 */
@@ -172,55 +196,36 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     };
     float *sl = scales + wave * (2 * NB * KV4_PAGE);
 
-    for (bool first_group = true; u < u_end; first_group = false) {
-    const int group = at / s.rounds, begin = at % s.rounds;
-    const int h = kv4_uniform(group / s.blocks), rb = kv4_uniform(group % s.blocks);
-    const int nrounds = min(s.rounds - begin, u_end - u);
-    const int p0 = begin * KA_WAVES, p1 = A.part ? min((begin + nrounds) * KA_WAVES, s.npages) : s.npages;
-    const int rows = s.rows;
-
-    /* the group's loads first: this wave's first 64 pages, one a lane, and the lane's rows of q */
-    const int32_t *table = A.table + b * A.table_stride;
-    auto page_id = [&](int pg0) {
-        const int pg = pg0 + lane * KA_WAVES;
-        return pg < p1 ? table[pg] : -1;
+    /* This wave's pages of a group's part from its i-th round on, 64 of them, one a lane. A page
+     * that is not there, past the sequence's end or not in the pool, is read as the pool's first
+     * page and seen by nobody: its lane holds -1. */
+    auto page_ids = [&](const Kv4Group &X, int i) {
+        const int pg = (X.begin + i + lane) * KA_WAVES + wave;
+        const int pid = i + lane < X.n && pg < X.s.npages ? A.table[X.b * A.table_stride + pg] : -1;
+        return pid < A.pages ? pid : -1;
     };
-    int pid_mine = page_id(p0 + wave);
+    /* The lane's rows of q. */
     glint_u32x4 qw[NT][NB][2];
-    int last[NT];
+    auto load_q = [&](const Kv4Group &X) {
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = rb * COLS + 16 * n + col;
-        const int i = r / A.G, hq = h * A.G + r % A.G;
-        const bool live = r < rows;
-        last[n] = live ? s.len - s.nq + i : -1;
-        const uint16_t *qr = A.q + (s.q0 + (live ? i : 0)) * A.q_st + (live ? hq : h * A.G) * A.q_sh;
+        for (int n = 0; n < NT; ++n) {
+            const int r = X.rb * COLS + 16 * n + col;
+            const bool live = r < X.s.rows;
+            const uint16_t *qr = A.q + (X.s.q0 + (live ? r / A.G : 0)) * A.q_st + (X.h * A.G + (live ? r % A.G : 0)) * A.q_sh;
 #pragma unroll
-        for (int bb = 0; bb < NB; ++bb)
+            for (int bb = 0; bb < NB; ++bb)
 #pragma unroll
-            for (int st = 0; st < 2; ++st)
-                qw[n][bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
-    }
-    if (first_group) {
-        for (int i = threadIdx.x; i < 256 * KA_COPIES / 4; i += KA_T) {
-            const int byte = i / (KA_COPIES / 4);
-            union {
-                _Float16 f[2];
-                uint32_t u;
-            } e;
-            e.f[0] = (_Float16)(kKv4Parent[byte & 15] * KA_ALPHA);
-            e.f[1] = (_Float16)(kKv4Parent[byte >> 4] * KA_ALPHA);
-            ((glint_u32x4 *)lds)[byte * 16 + i % (KA_COPIES / 4)] = glint_u32x4{e.u, e.u, e.u, e.u};
+                for (int st = 0; st < 2; ++st)
+                    qw[n][bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
         }
-        __syncthreads();
-    }
-
+    };
     /* A page's loads: this lane's 16-B pieces of the key rows and value columns, and one token's
-     * scales, which go to the other lanes through LDS. */
+     * scales, which go to the other lanes through LDS. `ph` is the page's place times the heads. */
     uint32_t kw[4][2 * NB];
     glint_u32x4 vw[D / 32];
     float sw[2 * NB];
-    auto load_k = [&](int64_t ph) {
+    int64_t ph = 0;
+    auto load_k = [&]() {
         const uint8_t *kp = A.k_hole + ph * (KV4_PAGE * D / 2) + (16 * (col >> 2) + (col & 3)) * (D / 2) + g * (8 * NB);
 #pragma unroll
         for (int a = 0; a < 4; ++a)
@@ -233,37 +238,57 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             sw[NB + bb] = A.v_absmax[ph * (NB * KV4_PAGE) + bb * KV4_PAGE + lane];
         }
     };
-    auto load_v = [&](int64_t ph) {
+    auto load_v = [&]() {
         const uint8_t *vp = A.v_hole + ph * (KV4_PAGE * D / 2) + col * KV4_PAGE + 16 * g;
 #pragma unroll
         for (int p = 0; p < D / 32; ++p)
             vw[p] = *(const glint_u32x4 *)(vp + p * (16 * KV4_PAGE));
     };
-    /* the pages of the wave that lie in the pool, one bit a lane; the next one's place */
-    uint64_t todo = __ballot(pid_mine >= 0 && pid_mine < A.pages);
-    int lane_at = 0;
-    int64_t ph = 0;
-    auto take = [&]() {
-        lane_at = __builtin_ctzll(todo);
-        todo &= todo - 1;
-        ph = (int64_t)__builtin_amdgcn_readlane(pid_mine, lane_at) * A.H + h;
+    int pids = page_ids(G, 0);
+    auto page = [&](const Kv4Group &X, int i) { /* of round i; whether it is there */
+        const int pid = __builtin_amdgcn_readlane(pids, i & 63);
+        ph = (int64_t)max(pid, 0) * A.H + X.h;
+        return pid >= 0;
     };
-    auto start = [&]() {
-        if (todo == 0)
-            return false;
-        take();
-        load_k(ph);
-        load_v(ph);
-        return true;
-    };
-    bool have = start();
+    load_q(G);
+    for (int i = threadIdx.x; i < 256 * KA_COPIES / 4; i += KA_T) {
+        const int byte = i / (KA_COPIES / 4);
+        union {
+            _Float16 f[2];
+            uint32_t u;
+        } e;
+        e.f[0] = (_Float16)(kKv4Parent[byte & 15] * KA_ALPHA);
+        e.f[1] = (_Float16)(kKv4Parent[byte >> 4] * KA_ALPHA);
+        ((glint_u32x4 *)lds)[byte * 16 + i % (KA_COPIES / 4)] = glint_u32x4{e.u, e.u, e.u, e.u};
+    }
+    __syncthreads();
+    bool there = page(G, 0);
+    load_k();
+    load_v();
+
+    Kv4Join join0{0}, join1{0}; /* of this workgroup's slot 0 and slot 1 */
+    while (true) {
+    const Kv4Seq &s = G.s;
+    /* the group after this one; its pages' numbers are on their way while this one's are read */
+    Kv4Group N = G;
+    N.u = G.u + G.units;
+    N.at = G.at + G.units;
+    const bool more_groups = N.u < u_end;
+    int pids_next = -1;
+    if (more_groups) {
+        place(N);
+        pids_next = page_ids(N, 0);
+    }
 
     /* this lane's rows of q as f16 operands, scaled to 2^14 .. 2^15 by a power of two that goes
      * into the row's score factor */
     Kv4Frag qf[NT][NB][2];
     float factor[NT];
+    int last[NT];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
+        const int r = G.rb * COLS + 16 * n + col;
+        last[n] = r < s.rows ? s.len - s.nq + r / A.G : -1;
         uint32_t top = 0;
 #pragma unroll
         for (int bb = 0; bb < NB; ++bb)
@@ -303,12 +328,23 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         }
     }
 
-    for (int pg0 = p0 + wave; pg0 < p1;) {
-        for (bool more = have; more;) {
-        const int pg = pg0 + lane_at * KA_WAVES;
-        more = todo != 0;
-        if (more)
-            take();
+    for (int i = 0; i < G.n; ++i) {
+        /* a page that nobody sees lies past every row's last position */
+        const int pg = there ? (G.begin + i) * KA_WAVES + wave : KA_FAR;
+        /* the run's last page is loaded again: without a branch around them the next page's
+         * loads can be counted, and this page's waits leave them in flight */
+        if (i + 1 < G.n) {
+            /* waited for here, lest every page waits for its values where the branch joins */
+            if (((i + 1) & 63) == 0) {
+                pids = page_ids(G, i + 1);
+                __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+            }
+            there = page(G, i + 1);
+        } else if (more_groups) {
+            __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+            pids = pids_next;
+            there = page(N, 0);
+        }
 #pragma unroll
         for (int x = 0; x < 2 * NB; ++x)
             sl[x * KV4_PAGE + lane] = sw[x];
@@ -348,8 +384,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                     sc[n][a][i] = x * factor[n];
                 }
         }
-        if (more)
-            load_k(ph);
+        load_k();
         /* what the row does not see; a whole page below every row's last position needs no look */
         const int t0 = pg * KV4_PAGE + 16 * g;
         const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
@@ -443,26 +478,19 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                 }
             }
         }
-        if (more)
-            load_v(ph);
-        }
-        pg0 += 64 * KA_WAVES; /* the next 64 pages */
-        pid_mine = page_id(pg0);
-        todo = __ballot(pid_mine >= 0 && pid_mine < A.pages);
-        have = start();
+        load_v();
     }
+    if (more_groups)
+        load_q(N);
 
-    /* The waves meet: each writes its rows' outputs, maximum and sum. A group that ends where it
-     * begins is done; else this workgroup's part goes to its slot 1, where it begins here, or 0,
-     * and the workgroup whose arrival completes the count adds all parts in order. */
-    const int u_begin = u - begin;
-    const bool whole_group = begin == 0 && nrounds == s.rounds;
-    const int w_first = u_begin / share, w_last = (u_begin + s.rounds - 1) / share;
-    float *parts = A.part + (int64_t)2 * w_first * COLS * ROW; /* of w_first; its slot 1, then slot 0 of each that follows */
-    auto part_of = [&](int w) { return parts + (int64_t)(2 * (w - w_first) + (w == w_first)) * COLS * ROW; };
-    auto store = [&](int r, int d, const float (&acc)[4], float total) {
+    /* The waves meet: each writes its rows' outputs, maximum and sum. A group that lies whole in
+     * this workgroup's run is done; of one that does not, this workgroup's part goes to its slot
+     * 1, where the group begins here, or 0. */
+    const bool whole_group = G.n == s.rounds;
+    const int slot = G.begin == 0;
+    auto store = [&](int64_t q0, int h, int r, int d, const float (&acc)[4], float total) {
         const float inv = total == 0.f ? 0.f : 1.f / total;
-        uint16_t *dst = A.out + ((s.q0 + r / A.G) * A.Hq + h * A.G + r % A.G) * D + d;
+        uint16_t *dst = A.out + ((q0 + r / A.G) * A.Hq + h * A.G + r % A.G) * D + d;
         glint_u32x2 two;
         two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
         two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
@@ -491,8 +519,8 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         __syncthreads();
         for (int t = threadIdx.x; t < 16 * (D / 4); t += KA_T) {
             const int c = t / (D / 4), d = 4 * (t % (D / 4));
-            const int r = rb * COLS + 16 * n + c;
-            if (r >= rows)
+            const int r = G.rb * COLS + 16 * n + c;
+            if (r >= s.rows)
                 continue;
             float mx = -INFINITY;
 #pragma unroll
@@ -512,9 +540,9 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                     acc[i] = fmaf(f, v[i], acc[i]);
             }
             if (whole_group) {
-                store(r, d, acc, total);
+                store(s.q0, G.h, r, d, acc, total);
             } else {
-                float *dst = part_of(blockIdx.x) + (16 * n + c) * ROW;
+                float *dst = A.part + ((int64_t)(2 * blockIdx.x + slot) * COLS + 16 * n + c) * ROW;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     __hip_atomic_store(dst + d + i, acc[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -526,52 +554,75 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         }
     }
     if (!whole_group) {
-        __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
-        __syncthreads();
-        if (threadIdx.x == 0)
-            s_last = __hip_atomic_fetch_add(&A.ctr[w_first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
-                     (unsigned)(w_last - w_first);
-        __syncthreads();
-        if (s_last) {
-            for (int t = threadIdx.x; t < COLS * (D / 4); t += KA_T) {
-                const int c = t / (D / 4), d = 4 * (t % (D / 4));
-                const int r = rb * COLS + c;
-                if (r >= rows)
-                    continue;
-                float mx = -INFINITY, total = 0.f;
-                float acc[4] = {0.f, 0.f, 0.f, 0.f};
-                for (int w0 = w_first; w0 <= w_last; w0 += 4) { /* four parts' loads in flight */
-                    float v[4][6];
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const float *src = part_of(min(w0 + k, w_last)) + c * ROW;
-#pragma unroll
-                        for (int i = 0; i < 6; ++i)
-                            v[k][i] = __hip_atomic_load(src + (i < 4 ? d + i : D + i - 4), __ATOMIC_RELAXED,
-                                                        __HIP_MEMORY_SCOPE_AGENT);
-                    }
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (w0 + k <= w_last) {
-                            const float to = fmaxf(mx, v[k][4]), base = to == -INFINITY ? 0.f : to;
-                            const float keep = __builtin_amdgcn_exp2f(mx - base), f = __builtin_amdgcn_exp2f(v[k][4] - base);
-                            mx = to;
-                            total = fmaf(total, keep, f * v[k][5]);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                acc[i] = fmaf(acc[i], keep, f * v[k][i]);
-                        }
-                }
-                store(r, d, acc, total);
-            }
-            if (threadIdx.x == 0)
-                __hip_atomic_store(&A.ctr[w_first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        }
+        const int u_begin = G.u - G.begin;
+        const Kv4Join J{1, u_begin / share, (u_begin + s.rounds - 1) / share, s.rows, G.rb, G.h, s.q0};
+        if (slot)
+            join1 = J;
+        else
+            join0 = J;
     }
-    u += nrounds;
-    at += nrounds;
-    if (u < u_end)
-        skip();
+    if (!more_groups)
+        break;
+    G = N;
+    }
+
+    /* The workgroups that share a group meet in the last of them to arrive: workgroup w_first has
+     * its part in slot 1, those up to w_last in slot 0, and w_first's counter is theirs. */
+    if (!join0.on && !join1.on)
+        return;
+    __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+    __syncthreads();
+    auto arrive = [&](const Kv4Join &J) {
+        return J.on && __hip_atomic_fetch_add(&A.ctr[J.w_first], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                           (unsigned)(J.w_last - J.w_first);
+    };
+    if (threadIdx.x == 0) {
+        s_last[0] = arrive(join0);
+        s_last[1] = arrive(join1);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const Kv4Join &J = j ? join1 : join0;
+        if (!s_last[j])
+            continue;
+        for (int t = threadIdx.x; t < COLS * (D / 4); t += KA_T) {
+            const int c = t / (D / 4), d = 4 * (t % (D / 4));
+            const int r = J.rb * COLS + c;
+            if (r >= J.rows)
+                continue;
+            float mx = -INFINITY, total = 0.f;
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int w0 = J.w_first; w0 <= J.w_last; w0 += 4) { /* four parts' loads in flight */
+                float v[4][6];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const int w = min(w0 + k, J.w_last);
+                    const float *src = A.part + ((int64_t)(2 * w + (w == J.w_first)) * COLS + c) * ROW;
+#pragma unroll
+                    for (int i = 0; i < 6; ++i)
+                        v[k][i] = __hip_atomic_load(src + (i < 4 ? d + i : D + i - 4), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    if (w0 + k <= J.w_last) {
+                        const float to = fmaxf(mx, v[k][4]), base = to == -INFINITY ? 0.f : to;
+                        const float keep = __builtin_amdgcn_exp2f(mx - base), f = __builtin_amdgcn_exp2f(v[k][4] - base);
+                        mx = to;
+                        total = fmaf(total, keep, f * v[k][5]);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            acc[i] = fmaf(acc[i], keep, f * v[k][i]);
+                    }
+            }
+            const float inv = total == 0.f ? 0.f : 1.f / total;
+            glint_u32x2 two;
+            two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
+            two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
+            *(glint_u32x2 *)(A.out + ((J.q0 + r / A.G) * A.Hq + J.h * A.G + r % A.G) * D + d) = two;
+        }
+        if (threadIdx.x == 0)
+            __hip_atomic_store(&A.ctr[J.w_first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
@@ -584,7 +635,7 @@ static int ka_tiles(int max_q, int G) { return (int64_t)max_q * G > 16 ? 2 : 1; 
 
 static bool ka_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
     return B >= 0 && max_q >= 1 && H >= 1 && Hq >= H && Hq % H == 0 && (D == 64 || D == 128) && max_pages >= 1 &&
-           max_pages <= (1 << 25) && (int64_t)max_q * (Hq / H) <= (1 << 20);
+           max_pages <= KA_FAR && (int64_t)max_q * (Hq / H) <= (1 << 20);
 }
 
 /* Units of the longest list that the shape allows, or -1 where they leave 31 bits. */

@@ -66,7 +66,7 @@ def scores(lib, **kw):
               ("vsh", 129, -2), ("k", ctypes.c_void_p(68), -2), ("H", 0, -2), ("T", -1, -2), ("pages", 0, -2),
               ("T", 1 << 41, -2)]),
     (attend, [("q", None, -1), ("lens", None, -1), ("out", None, -1), ("D", 256, -2), ("H", 3, -2), ("Tq", 3, -2),
-              ("qt", 1020, -2), ("q", ctypes.c_void_p(72), -2), ("wide", 0, -2), ("max_q", 0, -2), ("B", -1, -2), ("wide", (1 << 25) + 1, -2),
+              ("qt", 1020, -2), ("q", ctypes.c_void_p(72), -2), ("wide", 0, -2), ("max_q", 0, -2), ("B", -1, -2), ("wide", (1 << 24) + 1, -2),
               ("pages", 0, -2)]),
     (prompt, [("v", None, -1), ("cq", None, -1), ("out", None, -1), ("D", 80, -2), ("H", 3, -2), ("kt", 252, -2),
               ("v", ctypes.c_void_p(72), -2), ("B", -1, -2), ("max_q", -1, -2), ("Tk", -1, -2)]),
