@@ -70,17 +70,6 @@ struct ApRows {
     uint32_t vat[D / 32];
 };
 
-__device__ __forceinline__ uint32_t ap_pack(float a, float b) { /* two BF16, round to nearest even */
-    typedef float f32x2 __attribute__((ext_vector_type(2)));
-    typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-    union {
-        bf16x2 b;
-        uint32_t u;
-    } r;
-    r.b = __builtin_convertvector((f32x2{a, b}), bf16x2);
-    return r.u;
-}
-
 /* One tile of keys. */
 template <int D>
 __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int t, ApRows<D> &w, float scale2, bool masked,
@@ -138,7 +127,7 @@ __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int 
                 sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], scale2, -base));
                 sum += sc[a][x];
             }
-            pf[2 * a + (i >> 3)].u[(i & 7) >> 1] = ap_pack(sc[a][i], sc[a][i + 1]);
+            pf[2 * a + (i >> 3)].u[(i & 7) >> 1] = glint_cvt_bf16x2(sc[a][i], sc[a][i + 1]);
         }
     w.l += sum;
     /* Step s multiplies the keys that pf[s] holds: 16 s + 4 half + 0..3, and 8 on. */
@@ -159,7 +148,7 @@ __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int 
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int i = 8 * (s & 1) + 2 * x;
-                rest.u[x] = ap_pack(sc[s >> 1][i] - glint_bf16lo(pf[s].u[x]), sc[s >> 1][i + 1] - glint_bf16hi(pf[s].u[x]));
+                rest.u[x] = glint_cvt_bf16x2(sc[s >> 1][i] - glint_bf16lo(pf[s].u[x]), sc[s >> 1][i + 1] - glint_bf16hi(pf[s].u[x]));
             }
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -313,8 +302,8 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
 #pragma unroll
         for (int i = 0; i < 16; i += 4) {
             glint_u32x2 two;
-            two.x = ap_pack(w.o[d][i] * inv, w.o[d][i + 1] * inv);
-            two.y = ap_pack(w.o[d][i + 2] * inv, w.o[d][i + 3] * inv);
+            two.x = glint_cvt_bf16x2(w.o[d][i] * inv, w.o[d][i + 1] * inv);
+            two.y = glint_cvt_bf16x2(w.o[d][i + 2] * inv, w.o[d][i + 3] * inv);
             *(glint_u32x2 *)(dst + 32 * d + 2 * i + 4 * half) = two;
         }
 }

@@ -223,6 +223,14 @@ __device__ __forceinline__ uint32_t glint_pack_bf16x2(float lo, float hi) {
     return __builtin_amdgcn_perm(glint_rne_hi(hi), glint_rne_hi(lo), 0x07060302u);
 }
 
+typedef __bf16 glint_bf16x2 __attribute__((ext_vector_type(2)));
+typedef float glint_f32x2 __attribute__((ext_vector_type(2)));
+
+/* Two f32 to BF16 (round to nearest even; v_cvt_pk_bf16_f32), lo in the low half. */
+__device__ __forceinline__ uint32_t glint_cvt_bf16x2(float lo, float hi) {
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(glint_f32x2{lo, hi}, glint_bf16x2));
+}
+
 /* DPP lane moves (gfx9 encodings). */
 #define GLINT_DPP_QUAD_1032 0xB1  /* quad_perm [1,0,3,2] */
 #define GLINT_DPP_QUAD_2301 0x4E  /* quad_perm [2,3,0,1] */
@@ -272,6 +280,25 @@ __device__ __forceinline__ float glint_wave_max(float v) {
         v = fmaxf(v, __shfl_xor(v, o, 64));
     return v;
 }
+
+/* v of this lane and of the lane 32 (16) away: the two halves (rows of 16) of the wave exchanged
+ * by a vector instruction, not through LDS. op is symmetric. */
+template <class F>
+__device__ __forceinline__ float glint_xor32(float v, F op) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <class F>
+__device__ __forceinline__ float glint_xor16(float v, F op) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return op(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+struct GlintMax {
+    __device__ float operator()(float a, float b) const { return fmaxf(a, b); }
+};
+struct GlintAdd {
+    __device__ float operator()(float a, float b) const { return a + b; }
+};
 
 /* ------------------------------------------------------------- host helpers */
 #include <mutex>

@@ -1,7 +1,7 @@
 /* Attention over the 4-bit cache (include/glint_serve.h).
  *
  * k_kv4_attend — the work is a list of rounds: a group is one sequence, key head and block of
- *   up to 16 NT query rows (the heads that share the key head, times the new tokens), and a
+ *   up to 16 query rows (the heads that share the key head, times the new tokens), and a
  *   round is KA_WAVES pages of a group, one a wave. Every workgroup takes an equal run of the
  *   list, whatever the lengths, so that a batch of short and long sequences fills the device
  *   evenly and the table below is filled once per workgroup. A wave keeps a running maximum,
@@ -28,14 +28,23 @@
  *   seen, so that they stay inside f16's range whatever the scales' size.
  */
 #include <algorithm>
+#include <cfloat>
+#include <cmath>
 
 #include "kv4.h"
 #include "tile_mfma.h"
 
 typedef _Float16 kv4_f16x8 __attribute__((ext_vector_type(8)));
+/* the value scales' place in LDS holds f16 or f32 */
+typedef _Float16 kv4_lds_f16 __attribute__((may_alias));
+typedef kv4_f16x8 kv4_lds_f16x8 __attribute__((may_alias));
+typedef float kv4_lds_f32 __attribute__((may_alias));
+typedef glint_f32x4 kv4_lds_f32x4 __attribute__((may_alias));
 
 #define KA_WAVES 8
 #define KA_T (64 * KA_WAVES)
+#define KA_ROWS 16 /* of q in a group */
+#define KA_SWITCH 8 /* what turning to a group costs, in pages */
 #define KA_COPIES 32 /* of an entry; entries are 64 words apart, so that an address is one byte permute */
 #define KA_TABLE_WORDS (256 * 64)
 /* The table holds PARENT * KA_ALPHA, whose f16 roundings are smaller and cancel: over the code
@@ -65,82 +74,114 @@ struct Kv4AttendArgs {
     int max_pages;
     const int32_t *lens, *cu_q;
     int B, max_q, Hq, H, G;
-    float scale;
+    float scale2;    /* |scale| log2 e / KA_ALPHA, above 0 */
+    uint32_t q_sign; /* 0x80008000 where the scale is negative */
     uint16_t *out;
     float *part; /* two partials per workgroup; NULL: groups are not split */
     unsigned *ctr;
-    int least; /* fewest rounds of a workgroup's run */
 };
 
-/* The sequence's rows and length, with every device value bounded. */
-struct Kv4Seq {
-    int64_t q0;
-    int nq, rows, len, npages;
-    int rounds; /* of a group; one at least: a group without pages writes zeros */
-    int blocks; /* row blocks */
-    int each;   /* units of a group: its rounds, or 1 where groups are not split */
-    int units;  /* of the list that the sequence takes */
+/* A sequence's rows and length, with every device value bounded. */
+struct Kv4Raw {
+    int q0, nq, len;
 };
-template <int COLS>
-__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttendArgs &a, int b) {
+__device__ __forceinline__ Kv4Raw kv4_raw(const Kv4AttendArgs &a, int b) {
+    Kv4Raw s{0, 0, 0};
+    if (b < a.B) {
+        const int64_t q0 = a.cu_q ? a.cu_q[b] : (int64_t)b * a.max_q, q1 = a.cu_q ? a.cu_q[b + 1] : q0 + a.max_q;
+        const int len = a.lens[b];
+        if (q0 >= 0 && q1 > q0 && q1 <= a.Tq) {
+            s.q0 = (int)q0;
+            s.nq = (int)(q1 - q0);
+        }
+        s.len = (int)min((int64_t)max(len, 0), (int64_t)a.max_pages * KV4_PAGE);
+    }
+    return s;
+}
+struct Kv4Seq : Kv4Raw {
+    int rows, npages;
+    int rounds; /* of a group */
+    int blocks; /* row blocks */
+    int all;    /* rounds of all its groups */
+    int cost;   /* of a group: KA_WAVES a round, and KA_SWITCH for turning to it */
+};
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttendArgs &a, const Kv4Raw &r) {
     Kv4Seq s;
-    s.q0 = a.cu_q ? a.cu_q[b] : (int64_t)b * a.max_q;
-    const int64_t q1 = a.cu_q ? a.cu_q[b + 1] : s.q0 + a.max_q;
-    s.nq = s.q0 >= 0 && q1 > s.q0 && q1 <= a.Tq ? (int)(q1 - s.q0) : 0;
+    s.q0 = r.q0;
+    s.nq = r.nq;
+    s.len = r.len;
     s.rows = a.G * min(s.nq, a.max_q);
-    s.len = (int)min((int64_t)max(a.lens[b], 0), (int64_t)a.max_pages * KV4_PAGE);
     s.npages = (s.len + KV4_PAGE - 1) / KV4_PAGE;
-    s.rounds = max(1, (s.npages + KA_WAVES - 1) / KA_WAVES);
-    s.blocks = (s.rows + COLS - 1) / COLS;
-    s.each = a.part ? s.rounds : 1;
-    s.units = s.each * s.blocks * a.H;
+    s.rounds = (s.npages + KA_WAVES - 1) / KA_WAVES;
+    s.blocks = (s.rows + KA_ROWS - 1) / KA_ROWS;
+    s.all = s.rounds * s.blocks * a.H;
+    s.cost = s.rounds > 0 ? s.rounds * KA_WAVES + KA_SWITCH : 0;
     return s;
 }
 __device__ __forceinline__ int kv4_uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
-/* Some row's value scales leave f16's range: rows whose largest finite one does take a power
- * of two that puts it at 2^KA_VSTART and carry their outputs over. An infinite scale stays
- * infinite under any power and must not push the others out of range. */
-template <int TILES>
-__device__ __forceinline__ void kv4_new_power(const glint_f32x4 (&vscale)[4], float &down, float &limit, glint_f32x4 *o) {
-    float top = 0.f;
-#pragma unroll
-    for (int a = 0; a < 4; ++a)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            top = fmaxf(top, vscale[a][i] < INFINITY ? vscale[a][i] : 0.f);
-    top = fmaxf(top, __shfl_xor(top, 16, 64));
-    top = fmaxf(top, __shfl_xor(top, 32, 64));
-    if (top < limit)
-        return;
+/* Over the four lane groups that hold one row. */
+template <class F>
+__device__ __forceinline__ float kv4_over_row(float v, F op) { return glint_xor32(glint_xor16(v, op), op); }
+
+/* A power of two for value scales up to `top` (finite): 2^KA_VSTART in place of the largest. The
+ * outputs so far are carried over by the factor returned. An infinite scale stays infinite under
+ * any power and must not push the others out of range: it is left out of `top`. */
+__device__ __forceinline__ float kv4_new_power(float top, float &down, float &limit) {
     const int e = max(-126, (int)(__float_as_uint(top) >> 23) - 127 - KA_VSTART);
     const float to = ldexpf(1.f, -e), by = to / down; /* by >= 2^-252: 0 where it underflows */
-#pragma unroll
-    for (int d = 0; d < TILES; ++d)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            o[d][i] *= by;
     down = to;
     limit = ldexpf(1.f, e + KA_VMAX);
+    return by;
 }
 
 /* A group, or the part of it that this workgroup's run holds. */
 struct Kv4Group {
     Kv4Seq s;
-    int b, at;       /* the sequence, and where in it the part begins */
-    int h, rb;       /* key head, row block */
-    int u, units;    /* place in the list, units */
-    int begin, n;    /* first round, rounds */
+    int b, at;    /* the sequence, and where in its rounds the part begins */
+    int ahead;    /* cost of the sequences before it */
+    int h, rb;    /* key head, row block */
+    int k;        /* rounds of the run ahead of it */
+    int begin, n; /* first round of the group, rounds */
 };
 /* A part that other workgroups share: what the one that joins them has to know. */
 struct Kv4Join {
-    int on, w_first, w_last, rows, rb, h;
-    int64_t q0;
+    int on, w_first, w_last, rows, rb, h, q0;
 };
 
-template <int D, int NT>
+/* A row's outputs (4 dimensions), maximum and sum, added up from parts. */
+struct Kv4Sum {
+    glint_f32x4 o = {0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    __device__ void add(const glint_f32x4 v, float vm, float vl) {
+        const float to = fmaxf(m, vm), base = to == -INFINITY ? 0.f : to;
+        const float keep = __builtin_amdgcn_exp2f(m - base), f = __builtin_amdgcn_exp2f(vm - base);
+        m = to;
+        l = fmaf(l, keep, f * vl);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            o[x] = fmaf(o[x], keep, f * v[x]);
+    }
+    __device__ void add_below(const glint_f32x4 v, float vm, float vl) { /* vm <= m */
+        const float f = __builtin_amdgcn_exp2f(vm - (m == -INFINITY ? 0.f : m));
+        l = fmaf(f, vl, l);
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+            o[x] = fmaf(f, v[x], o[x]);
+    }
+    __device__ void store(uint16_t *dst) const { /* a row that saw nothing is zero */
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        *(glint_u32x2 *)dst = glint_u32x2{glint_cvt_bf16x2(o[0] * inv, o[1] * inv), glint_cvt_bf16x2(o[2] * inv, o[3] * inv)};
+    }
+};
+template <int D>
+__device__ __forceinline__ uint16_t *kv4_out(const Kv4AttendArgs &a, int q0, int h, int r) {
+    return a.out + ((int64_t)(q0 + r / a.G) * a.Hq + h * a.G + r % a.G) * D;
+}
+
+template <int D>
 __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
-    constexpr int NB = D / 64, COLS = 16 * NT;
+    constexpr int NB = D / 64;
     constexpr int ROW = D + 4; /* a row's output, then its maximum and sum */
     __shared__ __attribute__((aligned(16))) uint32_t lds[KA_TABLE_WORDS];
     __shared__ __attribute__((aligned(16))) float meet[KA_WAVES * 16 * ROW];
@@ -150,45 +191,156 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     const int lane = threadIdx.x & 63, wave = kv4_uniform((int)threadIdx.x >> 6);
     const int col = lane & 15, g = lane >> 4;
 
-    /* this workgroup's run [u, u_end) of the list, and where it begins */
-    const int per = (A.B + 63) / 64; /* sequences of a lane */
-    int mine = 0;
-    for (int i = 0; i < per; ++i)
-        if (lane * per + i < A.B)
-            mine += kv4_seq<COLS>(A, lane * per + i).units;
-    int upto = mine;
+    /* 64 sequences, one a lane, from `chunk` on: what follows finds its way in registers */
+    int chunk = 0;
+    Kv4Raw raw = kv4_raw(A, lane);
+    /* The table, while they are on their way: thread t writes four copies of the entries t / 8 + 64 i. */
+    static_assert(KA_T == 512 && KA_COPIES == 32, "the table's shares");
+    {
+        const float lo = kKv4Parent[(threadIdx.x >> 3) & 15] * KA_ALPHA;
 #pragma unroll
-    for (int k = 1; k < 64; k <<= 1) {
-        const int v = __shfl_up(upto, k, 64);
-        upto += lane >= k ? v : 0;
+        for (int i = 0; i < 4; ++i) {
+            union {
+                _Float16 f[2];
+                uint32_t u;
+            } e;
+            e.f[0] = (_Float16)lo;
+            e.f[1] = (_Float16)(kKv4Parent[(wave >> 1) + 4 * i] * KA_ALPHA);
+            ((glint_u32x4 *)lds)[((threadIdx.x >> 3) + 64 * i) * 16 + (threadIdx.x & 7)] = glint_u32x4{e.u, e.u, e.u, e.u};
+        }
     }
-    const int total = __builtin_amdgcn_readlane(upto, 63);
-    const int share = max(A.least, (total + (int)gridDim.x - 1) / (int)gridDim.x);
+    auto to_chunk = [&](int b) {
+        chunk = b;
+        raw = kv4_raw(A, b + lane);
+    };
+    auto sequence = [&](int b) { /* uniform; in the chunk */
+        Kv4Raw r;
+        r.q0 = __builtin_amdgcn_readlane(raw.q0, b - chunk);
+        r.nq = __builtin_amdgcn_readlane(raw.nq, b - chunk);
+        r.len = __builtin_amdgcn_readlane(raw.len, b - chunk);
+        return kv4_seq(A, r);
+    };
+    auto scan = [](int v) { /* of the lanes up to this one: row_shr 1, 2, 4, 8, row_bcast 15, 31 */
+        v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);
+        v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);
+        return v;
+    };
+    /* Rows of sequences without a token are zero: sequence b is workgroup b mod grid's to fill. */
+    const int per = (A.B + 63) / 64; /* sequences of a lane */
+    for (int c = 0; c < per; ++c) {
+        const Kv4Raw r = c ? kv4_raw(A, 64 * c + lane) : raw;
+        uint64_t empty = __ballot(r.len == 0 && r.nq > 0 && (64 * c + lane) % (int)gridDim.x == (int)blockIdx.x);
+        for (; empty; empty &= empty - 1) {
+            const int j = __builtin_ctzll(empty);
+            const int q0 = __builtin_amdgcn_readlane(r.q0, j), nq = min(__builtin_amdgcn_readlane(r.nq, j), A.max_q);
+            glint_u32x2 *dst = (glint_u32x2 *)(A.out + (int64_t)q0 * A.Hq * D);
+            for (int64_t i = threadIdx.x; i < (int64_t)nq * A.Hq * (D / 4); i += KA_T)
+                dst[i] = glint_u32x2{0, 0};
+        }
+    }
+    /* The list in units of cost: a group is KA_SWITCH units and KA_WAVES per round; its round j belongs to
+     * the workgroup whose run holds its unit KA_SWITCH + KA_WAVES j. A workgroup takes `share` units
+     * (KA_WAVES at least, so that each run inside a group holds a round of it), or, where groups are
+     * not split, one group. */
+    auto weight = [&](const Kv4Seq &s) { return (A.part ? s.cost : s.cost > 0 ? 1 : 0) * s.blocks * A.H; };
+    int mine = 0, mine_rounds = 0;
+    for (int i = 0; i < per; ++i) {
+        const Kv4Seq s = kv4_seq(A, per == 1 ? raw : kv4_raw(A, lane * per + i));
+        mine += weight(s);
+        mine_rounds += s.all;
+    }
+    const int upto = scan(mine), total = __builtin_amdgcn_readlane(upto, 63);
+    const int share = A.part ? max(KA_WAVES, (total + (int)gridDim.x - 1) / (int)gridDim.x) : 1;
     if ((int64_t)blockIdx.x * share >= total)
         return;
-    const int u_end = min(total - (int)blockIdx.x * share, share) + blockIdx.x * share;
-    /* completes a group whose sequence, place in it and place in the list are set */
-    auto place = [&](Kv4Group &G) {
-        while (G.at >= G.s.units) { /* on to the sequence that it lies in */
-            G.at -= G.s.units;
-            G.s = kv4_seq<COLS>(A, ++G.b);
+    const int upto_rounds = scan(mine_rounds);
+    const int u0 = blockIdx.x * share, u1 = min(total - u0, share) + u0;
+    /* the sequence that unit u lies in, the rounds before u in it, and in the sequences before it */
+    auto locate = [&](int u, int &b, int &at, int &ahead, int &rounds_ahead) {
+        const int owner = __builtin_ctzll(__ballot(upto > u));
+        ahead = __builtin_amdgcn_readlane(upto - mine, owner);
+        rounds_ahead = __builtin_amdgcn_readlane(upto_rounds - mine_rounds, owner);
+        b = owner * per;
+        while (true) {
+            if (b < chunk || b - chunk >= 64)
+                to_chunk(b);
+            const Kv4Seq s = sequence(b);
+            const int w = weight(s);
+            if (u - ahead < w) {
+                const int e = A.part ? (u - ahead) % s.cost - KA_SWITCH : 0;
+                at = (A.part ? (u - ahead) / s.cost : u - ahead) * s.rounds + (max(e, 0) + KA_WAVES - 1) / KA_WAVES;
+                return;
+            }
+            ahead += w;
+            rounds_ahead += s.all;
+            ++b;
         }
-        const int group = G.at / G.s.each;
-        G.begin = G.at % G.s.each;
-        G.h = kv4_uniform(group / G.s.blocks);
-        G.rb = kv4_uniform(group % G.s.blocks);
-        G.units = min(G.s.each - G.begin, u_end - G.u);
-        G.n = A.part ? G.units : G.s.rounds;
     };
     Kv4Group G;
+    int run; /* rounds */
     {
-        G.u = blockIdx.x * share;
-        const int owner = __builtin_ctzll(__ballot(upto > G.u));
-        G.at = G.u - __builtin_amdgcn_readlane(upto - mine, owner);
-        G.b = owner * per;
-        G.s = kv4_seq<COLS>(A, G.b);
-        place(G);
+        int before, after, b1, at1, ahead1;
+        if (u1 < total)
+            locate(u1, b1, at1, ahead1, after);
+        else {
+            after = __builtin_amdgcn_readlane(upto_rounds, 63);
+            at1 = 0;
+        }
+        locate(u0, G.b, G.at, G.ahead, before);
+        run = after + at1 - before - G.at;
+        G.k = 0;
     }
+    if (run == 0)
+        return;
+    /* completes a group whose b, at, ahead and k are set */
+    auto place = [&](Kv4Group &X) {
+        if (X.b < chunk || X.b - chunk >= 64)
+            to_chunk(X.b);
+        X.s = sequence(X.b);
+        while (X.at >= X.s.all) { /* on to the sequence that it lies in */
+            X.at -= X.s.all;
+            X.ahead += X.s.cost * X.s.blocks * A.H;
+            if (++X.b - chunk == 64)
+                to_chunk(X.b);
+            X.s = sequence(X.b);
+        }
+        const int group = X.at / X.s.rounds;
+        X.begin = X.at % X.s.rounds;
+        X.h = kv4_uniform(group / X.s.blocks);
+        X.rb = kv4_uniform(group % X.s.blocks);
+        X.n = min(X.s.rounds - X.begin, run - X.k);
+    };
+    place(G);
+    /* This wave's pages of the run's next rounds, from group X's first on, one a lane: as many as the
+     * chunk's sequences hold, 64 at most. A page that is not there, past the sequence's end or not in
+     * the pool, is read as the pool's first page and seen by nobody: its lane holds -1. */
+    int pids, window, window_n; /* the window's first round in the run, its length */
+    auto open_window = [&](int b, int at, int k) {
+        if (b < chunk || b - chunk >= 48)
+            to_chunk(b);
+        const int all = lane >= b - chunk ? kv4_seq(A, raw).all : 0;
+        const int sum = scan(all) - at; /* rounds from here to the lane's sequence's end */
+        int j = 0;                        /* the lane whose sequence holds this lane's round */
+#pragma unroll
+        for (int step = 32; step; step >>= 1)
+            j += __shfl(sum, j + step - 1, 64) <= lane ? step : 0;
+        /* every lane reads the others before any condition on its own */
+        const int sum_j = __shfl(sum, j, 64);
+        const Kv4Raw r{0, __shfl(raw.nq, j, 64), __shfl(raw.len, j, 64)};
+        const bool in = lane < run - k && lane < sum_j;
+        const Kv4Seq s = kv4_seq(A, r);
+        const int in_seq = lane - (sum_j - s.all);
+        const int pg = in_seq % max(s.rounds, 1) * KA_WAVES + wave;
+        pids = in && pg < s.npages ? A.table[(int64_t)(chunk + j) * A.table_stride + pg] : -1;
+        pids = pids < A.pages ? pids : -1;
+        window = k;
+        window_n = __builtin_popcountll(__ballot(in));
+    };
+    open_window(G.b, G.at, 0);
 
     const uint32_t lane4 = (uint32_t)(lane & (KA_COPIES - 1)) * 4;
     auto pair = [&](uint32_t word, int byte) { /* byte << 8 | lane4 */
@@ -196,28 +348,17 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     };
     float *sl = scales + wave * (2 * NB * KV4_PAGE);
 
-    /* This wave's pages of a group's part from its i-th round on, 64 of them, one a lane. A page
-     * that is not there, past the sequence's end or not in the pool, is read as the pool's first
-     * page and seen by nobody: its lane holds -1. */
-    auto page_ids = [&](const Kv4Group &X, int i) {
-        const int pg = (X.begin + i + lane) * KA_WAVES + wave;
-        const int pid = i + lane < X.n && pg < X.s.npages ? A.table[X.b * A.table_stride + pg] : -1;
-        return pid < A.pages ? pid : -1;
-    };
     /* The lane's rows of q. */
-    glint_u32x4 qw[NT][NB][2];
+    glint_u32x4 qw[NB][2];
     auto load_q = [&](const Kv4Group &X) {
+        const int r = X.rb * KA_ROWS + col;
+        const bool live = r < X.s.rows;
+        const uint16_t *qr = A.q + (int64_t)(X.s.q0 + (live ? r / A.G : 0)) * A.q_st + (X.h * A.G + (live ? r % A.G : 0)) * A.q_sh;
 #pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            const int r = X.rb * COLS + 16 * n + col;
-            const bool live = r < X.s.rows;
-            const uint16_t *qr = A.q + (X.s.q0 + (live ? r / A.G : 0)) * A.q_st + (X.h * A.G + (live ? r % A.G : 0)) * A.q_sh;
+        for (int bb = 0; bb < NB; ++bb)
 #pragma unroll
-            for (int bb = 0; bb < NB; ++bb)
-#pragma unroll
-                for (int st = 0; st < 2; ++st)
-                    qw[n][bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
-        }
+            for (int st = 0; st < 2; ++st)
+                qw[bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
     };
     /* A page's loads: this lane's 16-B pieces of the key rows and value columns, and one token's
      * scales, which go to the other lanes through LDS. `ph` is the page's place times the heads. */
@@ -244,326 +385,288 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         for (int p = 0; p < D / 32; ++p)
             vw[p] = *(const glint_u32x4 *)(vp + p * (16 * KV4_PAGE));
     };
-    int pids = page_ids(G, 0);
-    auto page = [&](const Kv4Group &X, int i) { /* of round i; whether it is there */
-        const int pid = __builtin_amdgcn_readlane(pids, i & 63);
-        ph = (int64_t)max(pid, 0) * A.H + X.h;
+    auto page = [&](int k, int h) { /* of the run's round k; whether it is there */
+        const int pid = __builtin_amdgcn_readlane(pids, k - window);
+        ph = (int64_t)max(pid, 0) * A.H + h;
         return pid >= 0;
     };
     load_q(G);
-    for (int i = threadIdx.x; i < 256 * KA_COPIES / 4; i += KA_T) {
-        const int byte = i / (KA_COPIES / 4);
-        union {
-            _Float16 f[2];
-            uint32_t u;
-        } e;
-        e.f[0] = (_Float16)(kKv4Parent[byte & 15] * KA_ALPHA);
-        e.f[1] = (_Float16)(kKv4Parent[byte >> 4] * KA_ALPHA);
-        ((glint_u32x4 *)lds)[byte * 16 + i % (KA_COPIES / 4)] = glint_u32x4{e.u, e.u, e.u, e.u};
-    }
-    __syncthreads();
-    bool there = page(G, 0);
+    __syncthreads(); /* the table is written */
+    bool there = page(0, G.h);
     load_k();
     load_v();
 
     Kv4Join join0{0}, join1{0}; /* of this workgroup's slot 0 and slot 1 */
-    while (true) {
-    const Kv4Seq &s = G.s;
-    /* the group after this one; its pages' numbers are on their way while this one's are read */
-    Kv4Group N = G;
-    N.u = G.u + G.units;
-    N.at = G.at + G.units;
-    const bool more_groups = N.u < u_end;
-    int pids_next = -1;
-    if (more_groups) {
-        place(N);
-        pids_next = page_ids(N, 0);
-    }
+    for (;;) {
+        const Kv4Seq &s = G.s;
+        Kv4Group N = G; /* the group after this one */
+        N.k = G.k + G.n;
+        N.at = G.at + G.n;
+        const bool more_groups = N.k < run;
+        if (more_groups)
+            place(N);
 
-    /* this lane's rows of q as f16 operands, scaled to 2^14 .. 2^15 by a power of two that goes
-     * into the row's score factor */
-    Kv4Frag qf[NT][NB][2];
-    float factor[NT];
-    int last[NT];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        const int r = G.rb * COLS + 16 * n + col;
-        last[n] = r < s.rows ? s.len - s.nq + r / A.G : -1;
-        uint32_t top = 0;
+        /* this lane's row of q as f16 operands, scaled to 2^14 .. 2^15 by a power of two that goes
+         * into the row's score factor */
+        Kv4Frag qf[NB][2];
+        const int my_row = G.rb * KA_ROWS + col;
+        const int last = my_row < s.rows ? s.len - s.nq + my_row / A.G : -1; /* the last position that it sees */
+        uint32_t high = 0;
 #pragma unroll
         for (int bb = 0; bb < NB; ++bb)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    top = max(top, max((qw[n][bb][st][x] & 0x7FFFu) << 16, qw[n][bb][st][x] & 0x7FFF0000u));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-        top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-        const int ex = top >= 0x7F800000u ? 0 : (int)(top >> 23) - 127 - 14; /* 2^14 <= top 2^-ex < 2^15 */
+                    high = max(high, max((qw[bb][st][x] & 0x7FFFu) << 16, qw[bb][st][x] & 0x7FFF0000u));
+        high = __float_as_uint(kv4_over_row(__uint_as_float(min(high, 0x7F800000u)), GlintMax())); /* inf for NaN */
+        const int ex = high >= 0x7F800000u ? 0 : (int)(high >> 23) - 127 - 14;
 #pragma unroll
         for (int bb = 0; bb < NB; ++bb)
 #pragma unroll
             for (int st = 0; st < 2; ++st)
 #pragma unroll
                 for (int x = 0; x < 4; ++x) {
-                    qf[n][bb][st].f[2 * x] = (_Float16)ldexpf(glint_bf16lo(qw[n][bb][st][x]), -ex);
-                    qf[n][bb][st].f[2 * x + 1] = (_Float16)ldexpf(glint_bf16hi(qw[n][bb][st][x]), -ex);
+                    const uint32_t w = qw[bb][st][x] ^ A.q_sign;
+                    qf[bb][st].f[2 * x] = (_Float16)ldexpf(glint_bf16lo(w), -ex);
+                    qf[bb][st].f[2 * x + 1] = (_Float16)ldexpf(glint_bf16hi(w), -ex);
                 }
-        factor[n] = ldexpf(A.scale * (1.44269504088896341f / KA_ALPHA), ex);
-    }
+        const float factor = fmaxf(ldexpf(A.scale2, ex), FLT_MIN); /* above 0: -inf stays -inf */
 
-    glint_f32x4 o[NT][D / 16];
-    float m[NT], l[NT], vdown[NT][NB], vlimit[NT][NB];
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        m[n] = -INFINITY;
-        l[n] = 0.f;
+        glint_f32x4 o[D / 16];
+        float m = -INFINITY, l = 0.f, vdown[NB], vlimit[NB];
 #pragma unroll
         for (int d = 0; d < D / 16; ++d)
-            o[n][d] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
+            o[d] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int bb = 0; bb < NB; ++bb) {
-            vdown[n][bb] = 0x1p126f;
-            vlimit[n][bb] = 0x1p-111f;
+            vdown[bb] = 0x1p126f;
+            vlimit[bb] = 0x1p-111f;
         }
-    }
+        auto carry = [&](int bb, float by) { /* block bb's outputs, to another power */
+#pragma unroll
+            for (int d = 4 * bb; d < 4 * bb + 4; ++d)
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    o[d][x] *= by;
+        };
 
-    for (int i = 0; i < G.n; ++i) {
-        /* a page that nobody sees lies past every row's last position */
-        const int pg = there ? (G.begin + i) * KA_WAVES + wave : KA_FAR;
-        /* the run's last page is loaded again: without a branch around them the next page's
-         * loads can be counted, and this page's waits leave them in flight */
-        if (i + 1 < G.n) {
-            /* waited for here, lest every page waits for its values where the branch joins */
-            if (((i + 1) & 63) == 0) {
-                pids = page_ids(G, i + 1);
-                __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+        for (int i = 0; i < G.n; ++i) {
+            /* a page that nobody sees lies past every row's last position */
+            const int pg = there ? (G.begin + i) * KA_WAVES + wave : KA_FAR;
+            /* The run's last page is loaded again: without a branch around them the next page's
+             * loads can be counted, and this page's waits leave them in flight. */
+            const int k = G.k + i + 1;
+            if (k < run) {
+                if (k - window == window_n) {
+                    open_window(i + 1 < G.n ? G.b : N.b, i + 1 < G.n ? G.at + i + 1 : N.at, k);
+                    __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0); /* here, not where the branch joins */
+                }
+                there = page(k, i + 1 < G.n ? G.h : N.h);
             }
-            there = page(G, i + 1);
-        } else if (more_groups) {
-            __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
-            pids = pids_next;
-            there = page(N, 0);
-        }
-#pragma unroll
-        for (int x = 0; x < 2 * NB; ++x)
-            sl[x * KV4_PAGE + lane] = sw[x];
-
-        /* scores */
-        glint_f32x4 sc[NT][4];
-#pragma unroll
-        for (int a = 0; a < 4; ++a) {
-            glint_f32x4 c[NT][NB];
+            /* A whole page lies below every row's last position: nothing of it is masked, and the
+             * rows have one power for its value scales, which go to LDS scaled and rounded to f16.
+             * Of another page they go there as they are. */
+            const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
 #pragma unroll
             for (int bb = 0; bb < NB; ++bb) {
-#pragma unroll
-                for (int n = 0; n < NT; ++n)
-                    c[n][bb] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    Kv4Frag f;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        f.u[x] = pair(kw[a][2 * bb + st], x);
-#pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        c[n][bb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.f, qf[n][bb][st].f, c[n][bb], 0, 0, 0);
+                sl[bb * KV4_PAGE + lane] = sw[bb];
+                const float v = sw[NB + bb];
+                if (whole) {
+                    if (__any(v >= vlimit[bb])) {
+                        const float top = glint_wave_max(v < INFINITY ? v : 0.f);
+                        if (top >= vlimit[bb])
+                            carry(bb, kv4_new_power(top, vdown[bb], vlimit[bb]));
+                    }
+                    ((kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE))[lane] = (_Float16)(v * vdown[bb]);
+                } else {
+                    ((kv4_lds_f32 *)sl)[(NB + bb) * KV4_PAGE + lane] = v;
                 }
             }
-            glint_f32x4 kscale[NB];
+
+            /* scores, without the row's factor */
+            glint_f32x4 sc[4];
 #pragma unroll
-            for (int bb = 0; bb < NB; ++bb)
-                kscale[bb] = *(const glint_f32x4 *)(sl + bb * KV4_PAGE + 16 * g + 4 * a);
+            for (int a = 0; a < 4; ++a) {
+                glint_f32x4 c[NB];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int bb = 0; bb < NB; ++bb) {
+                    c[bb] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float x = c[n][0][i] * kscale[0][i];
-                    if (NB == 2)
-                        x = fmaf(c[n][NB - 1][i], kscale[NB - 1][i], x);
-                    sc[n][a][i] = x * factor[n];
+                    for (int st = 0; st < 2; ++st) {
+                        Kv4Frag f;
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            f.u[x] = pair(kw[a][2 * bb + st], x);
+                        c[bb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.f, qf[bb][st].f, c[bb], 0, 0, 0);
+                    }
                 }
-        }
-        load_k();
-        /* what the row does not see; a whole page below every row's last position needs no look */
-        const int t0 = pg * KV4_PAGE + 16 * g;
-        const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
-        if (!whole) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+                for (int bb = 0; bb < NB; ++bb) {
+                    const glint_f32x4 kscale = *(const glint_f32x4 *)(sl + bb * KV4_PAGE + 16 * g + 4 * a);
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        sc[a][x] = bb ? fmaf(c[bb][x], kscale[x], sc[a][x]) : c[bb][x] * kscale[x];
+                }
+            }
+            load_k();
+            const int t0 = pg * KV4_PAGE + 16 * g;
+            if (!whole) { /* what the row does not see */
 #pragma unroll
                 for (int a = 0; a < 4; ++a)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        sc[n][a][i] = t0 + 4 * a + i <= last[n] ? sc[n][a][i] : -INFINITY;
-        }
+                    for (int x = 0; x < 4; ++x)
+                        sc[a][x] = t0 + 4 * a + x <= last ? sc[a][x] : -INFINITY;
+            }
 
-        /* softmax weights, times the value scales, as f16 */
-        Kv4Frag pf[NT][NB][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n) {
-            float top = sc[n][0][0];
+            /* softmax weights */
+            float top = -INFINITY;
 #pragma unroll
             for (int a = 0; a < 4; ++a)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    top = fmaxf(top, sc[n][a][i]);
-            top = fmaxf(top, __shfl_xor(top, 16, 64));
-            top = fmaxf(top, __shfl_xor(top, 32, 64));
-            if (__any(top > m[n])) {
-                const float mn = fmaxf(m[n], top);
-                const float keep = __builtin_amdgcn_exp2f(m[n] - (mn == -INFINITY ? 0.f : mn));
-                m[n] = mn;
-                l[n] *= keep;
+                for (int x = 0; x < 4; ++x)
+                    top = fmaxf(top, sc[a][x]);
+            top = kv4_over_row(top, GlintMax()) * factor;
+            if (__any(top > m)) {
+                const float mn = fmaxf(m, top);
+                const float keep = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                m = mn;
+                l *= keep;
 #pragma unroll
-                for (int d = 0; d < D / 16; ++d)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        o[n][d][i] *= keep;
+                for (int bb = 0; bb < NB; ++bb)
+                    carry(bb, keep);
             }
-            const float base = m[n] == -INFINITY ? 0.f : m[n];
+            const float base = m == -INFINITY ? 0.f : m;
             float sum = 0.f;
 #pragma unroll
             for (int a = 0; a < 4; ++a)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    sc[n][a][i] = __builtin_amdgcn_exp2f(sc[n][a][i] - base);
-                    sum += sc[n][a][i];
+                for (int x = 0; x < 4; ++x) {
+                    sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], factor, -base));
+                    sum += sc[a][x];
                 }
-            l[n] += sum;
+            l += sum;
+
+            /* times the value scales, as f16 */
+            Kv4Frag pf[NB][2];
+            if (whole) {
 #pragma unroll
-            for (int bb = 0; bb < NB; ++bb) {
-                glint_f32x4 vscale[4];
-                float vtop = 0.f;
+                for (int st = 0; st < 2; ++st) {
+                    kv4_f16x8 w;
 #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    vscale[a] = *(const glint_f32x4 *)(sl + (NB + bb) * KV4_PAGE + 16 * g + 4 * a);
-                    if (!whole) { /* an unseen place counts as 0, whatever it holds */
+                    for (int x = 0; x < 8; ++x)
+                        w[x] = (_Float16)sc[2 * st + (x >> 2)][x & 3];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            vscale[a][i] = t0 + 4 * a + i <= last[n] ? vscale[a][i] : 0.f;
+                    for (int bb = 0; bb < NB; ++bb)
+                        pf[bb][st].f =
+                            w * *(const kv4_lds_f16x8 *)((const kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE) + 16 * g + 8 * st);
+                }
+            } else {
+#pragma unroll
+                for (int bb = 0; bb < NB; ++bb) {
+                    glint_f32x4 vscale[4];
+                    float any = 0.f, finite = 0.f;
+#pragma unroll
+                    for (int a = 0; a < 4; ++a) {
+                        vscale[a] = *(const kv4_lds_f32x4 *)(sl + (NB + bb) * KV4_PAGE + 16 * g + 4 * a);
+#pragma unroll
+                        for (int x = 0; x < 4; ++x) { /* an unseen place counts as 0, whatever it holds */
+                            const float v = t0 + 4 * a + x <= last ? vscale[a][x] : 0.f;
+                            vscale[a][x] = v;
+                            any = fmaxf(any, v);
+                            finite = fmaxf(finite, v < INFINITY ? v : 0.f);
+                        }
+                    }
+                    if (__any(any >= vlimit[bb])) { /* outside f16's range under some row's power */
+                        finite = kv4_over_row(finite, GlintMax());
+                        if (finite >= vlimit[bb])
+                            carry(bb, kv4_new_power(finite, vdown[bb], vlimit[bb]));
                     }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        vtop = fmaxf(vtop, vscale[a][i]);
-                }
-                if (__any(vtop >= vlimit[n][bb])) /* outside f16's range under some row's power */
-                    kv4_new_power<D / (16 * NB)>(vscale, vdown[n][bb], vlimit[n][bb], &o[n][4 * bb]);
+                    for (int a = 0; a < 4; ++a)
 #pragma unroll
-                for (int a = 0; a < 4; ++a)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        pf[n][bb][a >> 1].f[4 * (a & 1) + i] = (_Float16)(sc[n][a][i] * (vscale[a][i] * vdown[n][bb]));
-            }
-        }
-
-        /* outputs */
-#pragma unroll
-        for (int p = 0; p < D / 32; ++p) {
-#pragma unroll
-            for (int st = 0; st < 2; ++st) {
-                Kv4Frag lo, hi;
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t w = vw[p][2 * st + (x >> 1)];
-                    const uint32_t e0 = pair(w, 2 * (x & 1)), e1 = pair(w, 2 * (x & 1) + 1);
-                    lo.u[x] = __builtin_amdgcn_perm(e1, e0, 0x05040100u);
-                    hi.u[x] = __builtin_amdgcn_perm(e1, e0, 0x07060302u);
-                }
-#pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    o[n][2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.f, pf[n][p >> 1][st].f, o[n][2 * p], 0, 0, 0);
-                    o[n][2 * p + 1] =
-                        __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.f, pf[n][p >> 1][st].f, o[n][2 * p + 1], 0, 0, 0);
+                        for (int x = 0; x < 4; ++x)
+                            pf[bb][a >> 1].f[4 * (a & 1) + x] = (_Float16)(sc[a][x] * (vscale[a][x] * vdown[bb]));
                 }
             }
-        }
-        load_v();
-    }
-    if (more_groups)
-        load_q(N);
 
-    /* The waves meet: each writes its rows' outputs, maximum and sum. A group that lies whole in
-     * this workgroup's run is done; of one that does not, this workgroup's part goes to its slot
-     * 1, where the group begins here, or 0. */
-    const bool whole_group = G.n == s.rounds;
-    const int slot = G.begin == 0;
-    auto store = [&](int64_t q0, int h, int r, int d, const float (&acc)[4], float total) {
-        const float inv = total == 0.f ? 0.f : 1.f / total;
-        uint16_t *dst = A.out + ((q0 + r / A.G) * A.Hq + h * A.G + r % A.G) * D + d;
-        glint_u32x2 two;
-        two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
-        two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
-        *(glint_u32x2 *)dst = two;
-    };
+            /* outputs */
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-        float sum = l[n];
-        sum += __shfl_xor(sum, 16, 64);
-        sum += __shfl_xor(sum, 32, 64);
-        __syncthreads(); /* the previous rows are read */
-        float *row = meet + (wave * 16 + col) * ROW;
+            for (int p = 0; p < D / 32; ++p)
+#pragma unroll
+                for (int st = 0; st < 2; ++st) {
+                    Kv4Frag lo, hi;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        const uint32_t w = vw[p][2 * st + (x >> 1)];
+                        const uint32_t e0 = pair(w, 2 * (x & 1)), e1 = pair(w, 2 * (x & 1) + 1);
+                        lo.u[x] = __builtin_amdgcn_perm(e1, e0, 0x05040100u);
+                        hi.u[x] = __builtin_amdgcn_perm(e1, e0, 0x07060302u);
+                    }
+                    o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.f, pf[p >> 1][st].f, o[2 * p], 0, 0, 0);
+                    o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.f, pf[p >> 1][st].f, o[2 * p + 1], 0, 0, 0);
+                }
+            load_v();
+        }
+        if (more_groups)
+            load_q(N);
+
+        /* The waves meet: each writes its rows' outputs, maximum and sum. A group that lies whole in
+         * this workgroup's run is done; of one that does not, this workgroup's part goes to its slot
+         * 1, where the group begins here, or 0. */
+        const bool whole_group = G.n == s.rounds;
+        const int slot = G.begin == 0;
+        const float sum = kv4_over_row(l, GlintAdd());
+        __syncthreads(); /* the previous group's rows are read */
+        float *row = meet + (wave * KA_ROWS + col) * ROW;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            glint_f32x4 v = o[n][d];
-            const float back = 1.f / vdown[n][d >> 2] * (1.f / KA_ALPHA); /* a power of two, inverted exactly */
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                v[i] *= back;
-            *(glint_f32x4 *)(row + 16 * d + 4 * g) = v;
+            const float back = 1.f / vdown[d >> 2] * (1.f / KA_ALPHA); /* a power of two, inverted exactly */
+            *(glint_f32x4 *)(row + 16 * d + 4 * g) = glint_f32x4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
         }
         if (g == 0) {
-            row[D] = m[n];
+            row[D] = m;
             row[D + 1] = sum;
         }
         __syncthreads();
-        for (int t = threadIdx.x; t < 16 * (D / 4); t += KA_T) {
+        for (int t = threadIdx.x; t < KA_ROWS * (D / 4); t += KA_T) {
             const int c = t / (D / 4), d = 4 * (t % (D / 4));
-            const int r = G.rb * COLS + 16 * n + c;
+            const int r = G.rb * KA_ROWS + c;
             if (r >= s.rows)
                 continue;
-            float mx = -INFINITY;
+            Kv4Sum z;
 #pragma unroll
             for (int w = 0; w < KA_WAVES; ++w)
-                mx = fmaxf(mx, meet[(w * 16 + c) * ROW + D]);
-            const float base = mx == -INFINITY ? 0.f : mx;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            float total = 0.f;
+                z.m = fmaxf(z.m, meet[(w * KA_ROWS + c) * ROW + D]);
 #pragma unroll
             for (int w = 0; w < KA_WAVES; ++w) {
-                const float *wr = meet + (w * 16 + c) * ROW;
-                const float f = __builtin_amdgcn_exp2f(wr[D] - base);
-                const glint_f32x4 v = *(const glint_f32x4 *)(wr + d);
-                total = fmaf(f, wr[D + 1], total);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    acc[i] = fmaf(f, v[i], acc[i]);
+                const float *wr = meet + (w * KA_ROWS + c) * ROW;
+                z.add_below(*(const glint_f32x4 *)(wr + d), wr[D], wr[D + 1]);
             }
             if (whole_group) {
-                store(s.q0, G.h, r, d, acc, total);
+                z.store(kv4_out<D>(A, s.q0, G.h, r) + d);
             } else {
-                float *dst = A.part + ((int64_t)(2 * blockIdx.x + slot) * COLS + 16 * n + c) * ROW;
+                float *dst = A.part + ((int64_t)(2 * blockIdx.x + slot) * KA_ROWS + c) * ROW;
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    __hip_atomic_store(dst + d + i, acc[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                for (int x = 0; x < 4; ++x)
+                    __hip_atomic_store(dst + d + x, z.o[x], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 if (d == 0) {
-                    __hip_atomic_store(dst + D, mx, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                    __hip_atomic_store(dst + D + 1, total, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(dst + D, z.m, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    __hip_atomic_store(dst + D + 1, z.l, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
             }
         }
-    }
-    if (!whole_group) {
-        const int u_begin = G.u - G.begin;
-        const Kv4Join J{1, u_begin / share, (u_begin + s.rounds - 1) / share, s.rows, G.rb, G.h, s.q0};
-        if (slot)
-            join1 = J;
-        else
-            join0 = J;
-    }
-    if (!more_groups)
-        break;
-    G = N;
+        if (!whole_group) {
+            const int first = G.ahead + (G.h * s.blocks + G.rb) * s.cost + KA_SWITCH; /* the unit of its round 0 */
+            const Kv4Join J{1, first / share, (first + KA_WAVES * (s.rounds - 1)) / share, s.rows, G.rb, G.h, s.q0};
+            if (slot)
+                join1 = J;
+            else
+                join0 = J;
+        }
+        if (!more_groups)
+            break;
+        G = N;
     }
 
     /* The workgroups that share a group meet in the last of them to arrive: workgroup w_first has
@@ -586,70 +689,69 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         const Kv4Join &J = j ? join1 : join0;
         if (!s_last[j])
             continue;
-        for (int t = threadIdx.x; t < COLS * (D / 4); t += KA_T) {
-            const int c = t / (D / 4), d = 4 * (t % (D / 4));
-            const int r = J.rb * COLS + c;
-            if (r >= J.rows)
-                continue;
-            float mx = -INFINITY, total = 0.f;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int w0 = J.w_first; w0 <= J.w_last; w0 += 4) { /* four parts' loads in flight */
+        /* teams of threads, one thread per 4 dimensions of a row, take the parts in turn, four loads
+         * of each in flight, and meet in LDS; up to four parts are one team's */
+        const int rows = min(KA_ROWS, J.rows - J.rb * KA_ROWS), items = rows * (D / 4);
+        const int teams = min(KA_T / items, (J.w_last - J.w_first + 4) >> 2);
+        const int team = (int)threadIdx.x / items, item = (int)threadIdx.x % items;
+        const int c = item / (D / 4), d = 4 * (item % (D / 4));
+        float *mine = meet + (team * rows + c) * ROW;
+        if (team < teams) {
+            Kv4Sum z;
+            for (int w0 = J.w_first + team; w0 <= J.w_last; w0 += 4 * teams) {
                 float v[4][6];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const int w = min(w0 + k, J.w_last);
-                    const float *src = A.part + ((int64_t)(2 * w + (w == J.w_first)) * COLS + c) * ROW;
+                    const int w = min(w0 + k * teams, J.w_last);
+                    const float *src = A.part + ((int64_t)(2 * w + (w == J.w_first)) * KA_ROWS + c) * ROW;
 #pragma unroll
-                    for (int i = 0; i < 6; ++i)
-                        v[k][i] = __hip_atomic_load(src + (i < 4 ? d + i : D + i - 4), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    for (int x = 0; x < 6; ++x)
+                        v[k][x] = __hip_atomic_load(src + (x < 4 ? d + x : D + x - 4), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (w0 + k <= J.w_last) {
-                        const float to = fmaxf(mx, v[k][4]), base = to == -INFINITY ? 0.f : to;
-                        const float keep = __builtin_amdgcn_exp2f(mx - base), f = __builtin_amdgcn_exp2f(v[k][4] - base);
-                        mx = to;
-                        total = fmaf(total, keep, f * v[k][5]);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            acc[i] = fmaf(acc[i], keep, f * v[k][i]);
-                    }
+                    if (w0 + k * teams <= J.w_last)
+                        z.add(glint_f32x4{v[k][0], v[k][1], v[k][2], v[k][3]}, v[k][4], v[k][5]);
             }
-            const float inv = total == 0.f ? 0.f : 1.f / total;
-            glint_u32x2 two;
-            two.x = glint_f32_to_bf16(acc[0] * inv) | (uint32_t)glint_f32_to_bf16(acc[1] * inv) << 16;
-            two.y = glint_f32_to_bf16(acc[2] * inv) | (uint32_t)glint_f32_to_bf16(acc[3] * inv) << 16;
-            *(glint_u32x2 *)(A.out + ((J.q0 + r / A.G) * A.Hq + J.h * A.G + r % A.G) * D + d) = two;
+            if (teams == 1) {
+                z.store(kv4_out<D>(A, J.q0, J.h, J.rb * KA_ROWS + c) + d);
+            } else {
+                *(glint_f32x4 *)(mine + d) = z.o;
+                if (d == 0) {
+                    mine[D] = z.m;
+                    mine[D + 1] = z.l;
+                }
+            }
+        }
+        if (teams > 1) {
+            __syncthreads();
+            if (team == 0) {
+                Kv4Sum z;
+                for (int t = 0; t < teams; ++t)
+                    z.m = fmaxf(z.m, meet[(t * rows + c) * ROW + D]);
+                for (int t = 0; t < teams; ++t) {
+                    const float *from = meet + (t * rows + c) * ROW;
+                    z.add_below(*(const glint_f32x4 *)(from + d), from[D], from[D + 1]);
+                }
+                z.store(kv4_out<D>(A, J.q0, J.h, J.rb * KA_ROWS + c) + d);
+            }
+            __syncthreads(); /* before the other group's teams write */
         }
         if (threadIdx.x == 0)
             __hip_atomic_store(&A.ctr[J.w_first], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
 }
 
-/* Tiles of 16 rows a wave carries: two once a sequence's rows of a head fill more than one. */
-static int ka_tiles(int max_q, int G) { return (int64_t)max_q * G > 16 ? 2 : 1; }
-
-#ifndef KA_LEAST
-#define KA_LEAST 2
-#endif
-
 static bool ka_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
     return B >= 0 && max_q >= 1 && H >= 1 && Hq >= H && Hq % H == 0 && (D == 64 || D == 128) && max_pages >= 1 &&
            max_pages <= KA_FAR && (int64_t)max_q * (Hq / H) <= (1 << 20);
 }
 
-/* Units of the longest list that the shape allows, or -1 where they leave 31 bits. */
-static int64_t ka_units(int B, int max_q, int H, int G, int max_pages) {
-    const int cols = 16 * ka_tiles(max_q, G);
-    const int64_t blocks = ((int64_t)max_q * G + cols - 1) / cols, rounds = (max_pages + KA_WAVES - 1) / KA_WAVES;
-    const double n = (double)B * H * (double)blocks * (double)rounds;
-    return n > (double)(1 << 30) ? -1 : (int64_t)B * H * blocks * rounds;
-}
-
-template <int D, int NT>
-static void ka_launch(const Kv4AttendArgs &a, int64_t units, hipStream_t stream) {
-    const int64_t most = (units + a.least - 1) / a.least;
-    k_kv4_attend<D, NT><<<(unsigned)std::min<int64_t>(most, glint_cu_count()), KA_T, 0, stream>>>(a);
+/* Groups that the shape allows, or -1 where their units of cost leave 30 bits. */
+static int64_t ka_groups(int B, int max_q, int H, int G, int max_pages) {
+    const int64_t blocks = ((int64_t)max_q * G + KA_ROWS - 1) / KA_ROWS;
+    const double n = (double)B * H * (double)blocks * ((double)max_pages + KA_WAVES + KA_SWITCH);
+    return n > (double)(1 << 30) ? -1 : (int64_t)B * H * blocks;
 }
 
 GLINT_API int glint_serve_workspace_reserve(struct ihipStream_t *stream) {
@@ -667,7 +769,7 @@ GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_
                                int D, float scale, uint16_t *out, struct ihipStream_t *stream) {
     if (!q || !k_hole || !k_absmax || !v_hole || !v_absmax || !table || !lens || !out)
         return -1;
-    if (!ka_shape(B, max_q, Hq, H, D, max_pages) || Tq < 0 || pages < 1 || pages >= (int64_t)1 << 40 ||
+    if (!ka_shape(B, max_q, Hq, H, D, max_pages) || Tq < 0 || Tq > INT32_MAX || pages < 1 || pages >= (int64_t)1 << 40 ||
         (!cu_q && Tq != (int64_t)B * max_q))
         return -2;
     if (!glint_aligned(q, 16) || !glint_aligned(out, 8) || !glint_aligned(k_hole, 16) || !glint_aligned(v_hole, 16) ||
@@ -675,24 +777,26 @@ GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_
         return -2;
     if (B == 0 || Tq == 0)
         return 0;
+    const float scale2 = fabsf(scale) * (1.44269504088896341f / KA_ALPHA);
     Kv4AttendArgs a{q, q_stride_t, q_stride_h, Tq, k_hole, v_hole, k_absmax, v_absmax, pages, table, table_stride,
-                    max_pages, lens, cu_q, B, max_q, Hq, H, Hq / H, scale, out, nullptr, nullptr, 1};
-    int64_t units = ka_units(B, max_q, H, a.G, max_pages);
-    if (units < 0)
+                    max_pages, lens, cu_q, B, max_q, Hq, H, Hq / H, scale2 < FLT_MIN ? FLT_MIN : scale2,
+                    scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr};
+    int64_t grid = ka_groups(B, max_q, H, a.G, max_pages);
+    if (grid < 0)
         return -2;
-    const bool two = ka_tiles(max_q, a.G) == 2;
+    const int64_t cus = glint_cu_count();
     GlintSplitWs ws;
-    if (max_pages > KA_WAVES && glint_split_ws_stream(stream, ws) && ws.nctr >= (size_t)glint_cu_count() &&
-        ws.part_floats >= (size_t)glint_cu_count() * 2 * 32 * (D + 4)) {
+    if (glint_split_ws_stream(stream, ws) && ws.nctr >= (size_t)cus &&
+        ws.part_floats >= (size_t)cus * 2 * KA_ROWS * (D + 4)) {
         a.part = ws.part;
         a.ctr = ws.ctr;
-        a.least = KA_LEAST;
-    } else {
-        units = ka_units(B, max_q, H, a.G, 1); /* whole groups */
+        grid = std::min<int64_t>((grid * (max_pages + KA_WAVES + KA_SWITCH) + KA_WAVES - 1) / KA_WAVES, cus);
+    } else if (grid > INT32_MAX / KA_T) { /* a workgroup per group */
+        return -2;
     }
     if (D == 64)
-        two ? ka_launch<64, 2>(a, units, stream) : ka_launch<64, 1>(a, units, stream);
+        k_kv4_attend<64><<<(unsigned)grid, KA_T, 0, stream>>>(a);
     else
-        two ? ka_launch<128, 2>(a, units, stream) : ka_launch<128, 1>(a, units, stream);
+        k_kv4_attend<128><<<(unsigned)grid, KA_T, 0, stream>>>(a);
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }

@@ -39,14 +39,6 @@
 #include <algorithm>
 
 typedef __bf16 glint_bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 glint_bf16x2 __attribute__((ext_vector_type(2)));
-typedef float glint_f32x2 __attribute__((ext_vector_type(2)));
-
-/* Two f32 to BF16 (round to nearest even; v_cvt_pk_bf16_f32), lo in the low half. */
-__device__ __forceinline__ uint32_t glint_cvt_bf16x2(float lo, float hi) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(glint_f32x2{lo, hi}, glint_bf16x2));
-}
-
 /* 128-byte LDS rows (64 BF16), 16-byte chunk c of row r stored at chunk c ^ f(r) with
  * f(r) = ((r >> 1) ^ ((r & 1) << 2)) & 7: the 16 rows of a fragment read (one chunk) then
  * hit distinct banks in every group of 8 lanes and in every group of 16. (Measured no

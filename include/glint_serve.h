@@ -58,7 +58,7 @@ int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, const uint8_
  * left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores, softmax and
  * sums are f32; PARENT and the softmax weights times the value scales enter the matrix
  * products in f16. B H max_q max_pages is bounded: -2 where the list of work passes 2^30.
- * Sequences longer than 512 tokens are split over workgroups that meet in a workspace of the
+ * Long sequences are split over workgroups that meet in a workspace of the
  * stream's (glint_serve_workspace_reserve): it is allocated by the first such call outside a
  * capture and never grows. A capture on a stream that has none runs unsplit. */
 int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq, const uint8_t *k_hole,
