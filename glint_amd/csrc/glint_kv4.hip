@@ -134,6 +134,211 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_gather(const int64_t *__restrict_
     }
 }
 
+/* ------------------------------------------------------------------ tiles
+ * 64 tokens of one head a workgroup. A value column lies a byte a token, 64 B apart, so values
+ * pass through LDS: columns there are shifted by the first token's place modulo 4, so that four
+ * tokens whose slots follow each other, as a prompt's do, are one aligned word on both sides;
+ * other tokens go byte by byte. */
+#define KT_TOKENS 64
+#define KT_COLS (KT_TOKENS + 4) /* the shift */
+#define KT_GROUPS (KT_COLS / 4)
+
+/* The slots of a tile, by shifted column; -1 where there is no token. */
+__device__ __forceinline__ int kt_slots(const int64_t *slots, int64_t t0, int64_t T, int64_t nslots, int64_t *place) {
+    const int64_t first = slots[t0];
+    const int shift = first >= 0 && first < nslots ? (int)(first & 3) : 0;
+    for (int c = threadIdx.x; c < KT_COLS; c += KV4_T) {
+        const int64_t t = t0 + c - shift;
+        const int64_t s = c >= shift && c - shift < KT_TOKENS && t < T ? slots[t] : -1;
+        place[c] = s < nslots ? s : -1;
+    }
+    return shift;
+}
+/* Whether columns c .. c + 3 are four slots in a row, the first a multiple of 4: its place, or -1. */
+__device__ __forceinline__ int64_t kt_word(const int64_t *place, int c) {
+    const int64_t s = place[c];
+    return s >= 0 && (s & 3) == 0 && place[c + 1] == s + 1 && place[c + 2] == s + 2 && place[c + 3] == s + 3 ? s : -1;
+}
+
+template <int D>
+__device__ __forceinline__ void kt_load8(const uint16_t *p, float (&w)[8]) {
+    const glint_u32x4 u = *(const glint_u32x4 *)p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        w[2 * i] = glint_bf16lo(u[i]);
+        w[2 * i + 1] = glint_bf16hi(u[i]);
+    }
+}
+template <int D>
+__device__ __forceinline__ void kt_load8(const float *p, float (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const glint_f32x4 u = ((const glint_f32x4 *)p)[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            w[4 * i + k] = u[k];
+    }
+}
+
+/* A row of 8 lanes encodes a 64-block, 8 dimensions a lane: their quotients by one multiply where the
+ * input is BF16 and the absmax ordinary (no code differs from the divide's, see
+ * tests/native/check_encode_quotient.c), by the divide elsewhere. */
+template <class E, int D>
+__global__ __launch_bounds__(KV4_T) void k_kv4_append_tile(const E *__restrict__ k, const E *__restrict__ v, int64_t k_st,
+                                                           int64_t k_sh, int64_t v_st, int64_t v_sh,
+                                                           const int64_t *__restrict__ slots, int64_t T, int H,
+                                                           uint8_t *__restrict__ k_hole, float *__restrict__ k_absmax,
+                                                           uint8_t *__restrict__ v_hole, float *__restrict__ v_absmax,
+                                                           int64_t nslots) {
+    constexpr int NB = D / 64, ROWS = KV4_T / 8, PASSES = KT_TOKENS * NB / ROWS;
+    __shared__ Kv4Bucket buckets[KV4_BUCKETS];
+    __shared__ int64_t place[KT_COLS];
+    __shared__ __attribute__((aligned(16))) uint8_t vt[(D / 2) * KT_COLS];
+    __shared__ float scale[2][NB][KT_COLS];
+    const int64_t t0 = (int64_t)blockIdx.x * KT_TOKENS;
+    const int h = blockIdx.y, e = threadIdx.x & 7, r = threadIdx.x >> 3;
+    kv4_fill_buckets(buckets);
+    const int shift = kt_slots(slots, t0, T, nslots, place);
+    __syncthreads();
+#pragma unroll
+    for (int is_v = 0; is_v < 2; ++is_v) {
+        float w[PASSES][8];
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) { /* every load first */
+            const int item = r + i * ROWS, j = item / NB, b = item % NB;
+            const int64_t t = min(t0 + j, T - 1);
+            kt_load8<D>((is_v ? v + t * v_st + h * v_sh : k + t * k_st + h * k_sh) + 64 * b + 8 * e, w[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < PASSES; ++i) {
+            const int item = r + i * ROWS, j = item / NB, b = item % NB, c = j + shift;
+            float s = 0.f; /* fmaxf leaves NaN out */
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                s = fmaxf(s, fabsf(w[i][x]));
+            s = kv4_max_dpp<GLINT_DPP_QUAD_1032>(s);
+            s = kv4_max_dpp<GLINT_DPP_QUAD_2301>(s);
+            s = kv4_max_dpp<GLINT_DPP_ROW_HALF_MIRROR>(s);
+            uint32_t code = 0; /* 8 nibbles */
+            if (sizeof(E) == 2 && s >= 0x1p-90f && s < 0x1p90f) {
+                const float inv = 1.f / s;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) /* NaN among them: an absmax that leaves it out is no bound for it */
+                    code |= kv4_code(buckets, w[i][x] * inv) << (4 * x);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    code |= kv4_code(buckets, s == 0.f ? 0.f : w[i][x] / s) << (4 * x);
+            }
+            const int64_t slot = place[c];
+            if (e == 0)
+                scale[is_v][b][c] = s;
+            if (!is_v) {
+                if (slot >= 0)
+                    *(uint32_t *)(k_hole + (((slot >> 6) * H + h) * KV4_PAGE + (slot & 63)) * (D / 2) +
+                                  kv4_k_byte<NB>(64 * b + 8 * e)) = code;
+            } else {
+                /* dimensions 16 on are two lanes on; this lane writes four of the pair's rows */
+                const uint32_t other = (uint32_t)glint_dpp<GLINT_DPP_QUAD_2301>((int)code);
+                const int up = e & 2 ? 16 : 0;
+                const uint32_t lo = (e & 2 ? other : code) >> up, hi = (e & 2 ? code : other) >> up;
+                uint8_t *row = vt + (kv4_v_row(64 * b + 8 * (e & ~2)) + (e & 2 ? 4 : 0)) * KT_COLS + c;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    row[x * KT_COLS] = (uint8_t)(((lo >> (4 * x)) & 15u) | ((hi >> (4 * x)) & 15u) << 4);
+            }
+        }
+    }
+    __syncthreads();
+    for (int u = threadIdx.x; u < (D / 2) * KT_GROUPS; u += KV4_T) {
+        const int row = u / KT_GROUPS, c = 4 * (u % KT_GROUPS);
+        const uint32_t word = *(const uint32_t *)(vt + row * KT_COLS + c);
+        const int64_t s = kt_word(place, c);
+        if (s >= 0) {
+            *(uint32_t *)(v_hole + (((s >> 6) * H + h) * (D / 2) + row) * KV4_PAGE + (s & 63)) = word;
+        } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int64_t p = place[c + x];
+                if (p >= 0)
+                    v_hole[(((p >> 6) * H + h) * (D / 2) + row) * KV4_PAGE + (p & 63)] = (uint8_t)(word >> (8 * x));
+            }
+        }
+    }
+    for (int u = threadIdx.x; u < 2 * NB * KT_COLS; u += KV4_T) {
+        const int c = u % KT_COLS, b = u / KT_COLS % NB, is_v = u / (KT_COLS * NB);
+        const int64_t p = place[c];
+        if (p >= 0)
+            (is_v ? v_absmax : k_absmax)[(((p >> 6) * H + h) * NB + b) * KV4_PAGE + (p & 63)] = scale[is_v][b][c];
+    }
+}
+
+/* A thread writes 8 dimensions of a token: keys from their 4 bytes, values from LDS. */
+template <int D>
+__global__ __launch_bounds__(KV4_T) void k_kv4_gather_tile(const int64_t *__restrict__ slots, int64_t T, int H,
+                                                           const uint8_t *__restrict__ k_hole,
+                                                           const float *__restrict__ k_absmax,
+                                                           const uint8_t *__restrict__ v_hole,
+                                                           const float *__restrict__ v_absmax, int64_t nslots,
+                                                           uint16_t *__restrict__ k, uint16_t *__restrict__ v) {
+    constexpr int NB = D / 64, CH = D / 8;
+    __shared__ int64_t place[KT_COLS];
+    __shared__ __attribute__((aligned(16))) uint8_t vt[(D / 2) * KT_COLS];
+    __shared__ float par[16 * 32]; /* 32 copies, one a bank */
+    const int64_t t0 = (int64_t)blockIdx.x * KT_TOKENS;
+    const int h = blockIdx.y;
+    for (int i = threadIdx.x; i < 16 * 32; i += KV4_T)
+        par[i] = kKv4Parent[i >> 5];
+    const int shift = kt_slots(slots, t0, T, nslots, place);
+    __syncthreads();
+    const float *mine = par + (threadIdx.x & 31);
+    for (int u = threadIdx.x; u < (D / 2) * KT_GROUPS; u += KV4_T) {
+        const int row = u / KT_GROUPS, c = 4 * (u % KT_GROUPS);
+        uint32_t word = 0;
+        const int64_t s = kt_word(place, c);
+        if (s >= 0) {
+            word = *(const uint32_t *)(v_hole + (((s >> 6) * H + h) * (D / 2) + row) * KV4_PAGE + (s & 63));
+        } else {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const int64_t p = place[c + x];
+                if (p >= 0)
+                    word |= (uint32_t)v_hole[(((p >> 6) * H + h) * (D / 2) + row) * KV4_PAGE + (p & 63)] << (8 * x);
+            }
+        }
+        *(uint32_t *)(vt + row * KT_COLS + c) = word;
+    }
+    __syncthreads();
+#pragma unroll 4
+    for (int u = threadIdx.x; u < KT_TOKENS * CH; u += KV4_T) {
+        const int j = u / CH, d = 8 * (u % CH), c = j + shift, b = d >> 6;
+        const int64_t t = t0 + j, p = place[c];
+        if (t >= T)
+            break;
+        const int64_t ph = max(p, (int64_t)0) / KV4_PAGE * H + h;
+        const int at = (int)(max(p, (int64_t)0) & 63);
+        const uint32_t kw = *(const uint32_t *)(k_hole + (ph * KV4_PAGE + at) * (D / 2) + kv4_k_byte<NB>(d));
+        const float ks = k_absmax[(ph * NB + b) * KV4_PAGE + at], vs = v_absmax[(ph * NB + b) * KV4_PAGE + at];
+        const uint8_t *vr = vt + kv4_v_row(d) * KT_COLS + c;
+        const int up = d & 16 ? 4 : 0;
+        glint_u32x4 ko = {0, 0, 0, 0}, vo = {0, 0, 0, 0};
+        if (p >= 0) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                ko[x] = glint_cvt_bf16x2(mine[((kw >> (8 * x)) & 15u) * 32] * ks, mine[((kw >> (8 * x + 4)) & 15u) * 32] * ks);
+                const uint32_t a = (uint32_t)vr[2 * x * KT_COLS] >> up, z = (uint32_t)vr[(2 * x + 1) * KT_COLS] >> up;
+                vo[x] = glint_cvt_bf16x2(mine[(a & 15u) * 32] * vs, mine[(z & 15u) * 32] * vs);
+            }
+        }
+        *(glint_u32x4 *)(k + (t * H + h) * D + d) = ko;
+        *(glint_u32x4 *)(v + (t * H + h) * D + d) = vo;
+    }
+}
+
+#ifndef KV4_TILE_T
+#define KV4_TILE_T 32 /* tokens from which on the tiles are taken */
+#endif
+
 /* Workgroups of KV4_T threads for n threads' work, or 0 where a grid cannot hold them. */
 static unsigned kv4_grid(int64_t T, int64_t per_token) {
     if (T > ((int64_t)1 << 40) / per_token)
@@ -144,6 +349,19 @@ static unsigned kv4_grid(int64_t T, int64_t per_token) {
 
 static bool kv4_shape(int64_t T, int H, int D, int64_t pages) {
     return T >= 0 && H >= 1 && H <= 65535 && (D == 64 || D == 128) && pages >= 1 && pages < (int64_t)1 << 40;
+}
+
+template <class E>
+static void kv4_append_tiles(const void *k, const void *v, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                             const int64_t *slots, int64_t T, int H, int D, uint8_t *k_hole, float *k_absmax,
+                             uint8_t *v_hole, float *v_absmax, int64_t pages, hipStream_t stream) {
+    const dim3 g((unsigned)((T + KT_TOKENS - 1) / KT_TOKENS), H);
+    if (D == 64)
+        k_kv4_append_tile<E, 64><<<g, KV4_T, 0, stream>>>((const E *)k, (const E *)v, k_st, k_sh, v_st, v_sh, slots, T, H,
+                                                          k_hole, k_absmax, v_hole, v_absmax, pages * 64);
+    else
+        k_kv4_append_tile<E, 128><<<g, KV4_T, 0, stream>>>((const E *)k, (const E *)v, k_st, k_sh, v_st, v_sh, slots, T, H,
+                                                           k_hole, k_absmax, v_hole, v_absmax, pages * 64);
 }
 
 template <class E>
@@ -175,7 +393,16 @@ GLINT_API int glint_kv4_append(const void *k, const void *v, int elt, int64_t k_
     const unsigned g = kv4_grid(T, (int64_t)H * (D / 64) * 16);
     if (!g)
         return -2;
-    if (elt == GLINT_KV_BF16)
+    /* the tiles load 8 elements at once */
+    const bool tiles = T >= KV4_TILE_T && glint_aligned(k, 16) && glint_aligned(v, 16) &&
+                       !((k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7);
+    if (tiles && elt == GLINT_KV_BF16)
+        kv4_append_tiles<uint16_t>(k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, T, H, D, k_hole, k_absmax,
+                                   v_hole, v_absmax, pages, stream);
+    else if (tiles)
+        kv4_append_tiles<float>(k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, T, H, D, k_hole, k_absmax,
+                                v_hole, v_absmax, pages, stream);
+    else if (elt == GLINT_KV_BF16)
         kv4_append_launch<uint16_t>(g, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, T, H, D, k_hole,
                                     k_absmax, v_hole, v_absmax, pages, stream);
     else
@@ -196,7 +423,13 @@ GLINT_API int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, co
     const unsigned g = kv4_grid(T, (int64_t)H * (D / 2));
     if (!g)
         return -2;
-    if (D == 64)
+    const dim3 tiles((unsigned)((T + KT_TOKENS - 1) / KT_TOKENS), H);
+    if (T >= KV4_TILE_T && glint_aligned(k, 16) && glint_aligned(v, 16)) {
+        if (D == 64)
+            k_kv4_gather_tile<64><<<tiles, KV4_T, 0, stream>>>(slots, T, H, k_hole, k_absmax, v_hole, v_absmax, pages * 64, k, v);
+        else
+            k_kv4_gather_tile<128><<<tiles, KV4_T, 0, stream>>>(slots, T, H, k_hole, k_absmax, v_hole, v_absmax, pages * 64, k, v);
+    } else if (D == 64)
         k_kv4_gather<64><<<dim3(g, 2), KV4_T, 0, stream>>>(slots, T, H, k_hole, k_absmax, v_hole, v_absmax, pages * 64,
                                                            k, v);
     else

@@ -25,6 +25,39 @@ __device__ __forceinline__ uint32_t kv4_code(float v) {
     return c;
 }
 
+/* The same by a table of buckets a sixteenth wide, of which each holds one edge at most (they lie
+ * 0.08 apart): hole = base + (v > edge). fmaf(v, 16, 2^23 + 16) is an integer in [2^23, 2^23 + 32]
+ * for v in [-1, 1]. */
+#define KV4_BUCKETS 33
+#define KV4_MAGIC 8388624.f       /* 2^23 + 16 */
+#define KV4_MAGIC_BITS 0x4B000000u /* 2^23 */
+struct Kv4Bucket {
+    float edge;
+    uint32_t base;
+};
+__device__ __forceinline__ void kv4_fill_buckets(Kv4Bucket *t) { /* a barrier follows */
+    constexpr float edge[15] = KV4_EDGES;
+    const int i = threadIdx.x;
+    if (i < KV4_BUCKETS) {
+        /* values that round to the bucket's integer: half a bucket on either side */
+        const float low = (i - 16 - 0.5f) * 0.0625f;
+        uint32_t base = 0;
+        float e = INFINITY;
+#pragma unroll
+        for (int k = 14; k >= 0; --k) {
+            if (edge[k] >= low)
+                e = edge[k];
+            else
+                ++base;
+        }
+        t[i] = Kv4Bucket{e, base};
+    }
+}
+__device__ __forceinline__ uint32_t kv4_code(const Kv4Bucket *t, float v) { /* |v| <= 1, or NaN: 0 */
+    const Kv4Bucket e = t[__float_as_uint(fmaf(fmaxf(v, -1.f), 16.f, KV4_MAGIC)) - KV4_MAGIC_BITS];
+    return e.base + (v > e.edge ? 1u : 0u);
+}
+
 /* Byte of dimension pair (d, d + 1), d even, in a key row of NB blocks. */
 template <int NB>
 __host__ __device__ __forceinline__ int kv4_k_byte(int d) {

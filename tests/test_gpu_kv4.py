@@ -91,6 +91,26 @@ def test_append_in_a_row_fills_whole_pages():
         assert got.tobytes() == w.tobytes()
 
 
+@pytest.mark.parametrize("T", [8, 64])
+def test_append_at_the_edges(T):
+    """Quotients at and one float beside every edge between two codes, under an absmax of 1 (T = 8 and 64
+    take the two launches)."""
+    torch_cuda()
+    edges = ((S.PARENT[1:].astype(np.float64) + S.PARENT[:-1]) / 2).astype(np.float32)
+    near = (edges.view(np.int32)[:, None] + np.arange(-2, 3)).astype(np.int32).view(np.float32).ravel()
+    rows = np.concatenate([near, S.PARENT, [0.0, -0.0, 0.5 / 16, 1.5 / 16, -2.5 / 16]]).astype(np.float32)
+    rows = np.resize(rows, T * 2 * 63).reshape(T, 2, 63)
+    k = np.concatenate([rows, np.ones((T, 2, 1), np.float32)], -1)
+    v = np.concatenate([-np.ones((T, 2, 1), np.float32), rows[::-1]], -1)
+    want = S.empty_planes(2, 2, 64)
+    cache = tuple(gpu(p) for p in want)
+    for t in range(T):
+        S.put(want, t + 3, k[t], v[t])
+    H.kv4_append(gpu(k), gpu(v), gpu(np.arange(T, dtype=np.int64) + 3), cache)
+    for got, w, name in zip(planes_of(cache), want, ("k_hole", "k_absmax", "v_hole", "v_absmax")):
+        assert got.tobytes() == w.tobytes(), name
+
+
 def test_append_takes_strided_rows():
     """k and v as slices of one projection's output, an odd offset among them, and one head for all."""
     torch = torch_cuda()
