@@ -32,6 +32,7 @@
 #include <cmath>
 
 #include "kv4.h"
+#include "serve_ws.h"
 #include "tile_mfma.h"
 
 typedef _Float16 kv4_f16x8 __attribute__((ext_vector_type(8)));
@@ -754,11 +755,13 @@ static int64_t ka_groups(int B, int max_q, int H, int G, int max_pages) {
     return n > (double)(1 << 30) ? -1 : (int64_t)B * H * blocks;
 }
 
+bool glint_serve_ws(hipStream_t stream, GlintSplitWs &ws) { return glint_split_ws_stream(stream, ws); }
+
 GLINT_API int glint_serve_workspace_reserve(struct ihipStream_t *stream) {
     if (glint_stream_captures(stream))
         return -1;
     GlintSplitWs ws;
-    return glint_split_ws_stream(stream, ws) ? 0 : -1;
+    return glint_serve_ws(stream, ws) ? 0 : -1;
 }
 GLINT_API int glint_serve_workspace_release(struct ihipStream_t *stream) { return glint_split_ws_release(stream); }
 
@@ -786,7 +789,7 @@ GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_
         return -2;
     const int64_t cus = glint_cu_count();
     GlintSplitWs ws;
-    if (glint_split_ws_stream(stream, ws) && ws.nctr >= (size_t)cus &&
+    if (glint_serve_ws(stream, ws) && ws.nctr >= (size_t)cus &&
         ws.part_floats >= (size_t)cus * 2 * KA_ROWS * (D + 4)) {
         a.part = ws.part;
         a.ctr = ws.ctr;

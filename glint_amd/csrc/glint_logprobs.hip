@@ -8,15 +8,21 @@
  *   own maxima, every entry of the list is at least T and sits in one of the `top` threads
  *   whose maximum is at least T, so those threads look at their elements again and put
  *   what reaches T into LDS, at most top * (elements of a thread). Entries are compared as
- *   one 64-bit key, the value's order over the inverted index, so ties need no rule. */
+ *   one 64-bit key, the value's order over the inverted index, so ties need no rule.
+ *   Few long rows are split over workgroups, whose sums and lists meet in the last to arrive. */
+#include <algorithm>
+
 #include "glint_common.h"
 #include "glint_serve.h"
+#include "serve_ws.h"
 
 #define LP_T 1024
 #define LP_WAVES (LP_T / 64)
 #define LP_TOP 20
 #define LP_T_MAX 0x3FFFFF /* rows of one launch */
 #define LP_V_TOP 262144 /* longest row with a top list: its candidates fit LDS */
+#define LP_SPLIT 32 /* most parts of a row */
+#define LP_PART (4 + 2 * LP_TOP) /* words of a part: three sums, the count, the list */
 /* a thread's 16-B loads hold at most LP_V_TOP / LP_T elements, rounded up to a load, and it
  * may own one element before and one after the aligned part */
 #define LP_CAND (LP_TOP * (LP_V_TOP / LP_T + 8 + 2))
@@ -172,6 +178,68 @@ __device__ __forceinline__ uint64_t lp_wave_max(uint64_t v) {
     return (uint64_t)hi << 32 | lo;
 }
 
+/* A row's or a part's sums, and how many of its entries come before the token. */
+struct LpPart {
+    LpSum z;
+    int n;
+};
+/* A row's outputs from its sums; `ref` and `ls` are what its top list needs. */
+__device__ __forceinline__ void lp_write(const LpPart &p, int64_t tok, bool is_tok, float xt, bool writes, float *logprob,
+                                         float *entropy, int32_t *rank, float &ref, float &log_sum) {
+    const float s = p.z.m == -INFINITY ? NAN : p.z.s; /* nothing is possible */
+    const float ls = log2f(s);
+    if (writes) { /* x - lse, in powers of two up to the last product */
+        *logprob = tok < 0 ? 0.f : is_tok ? (fmaf(xt, LP_LOG2E, -p.z.m) - ls) * LP_LN2 : NAN;
+        if (entropy)
+            *entropy = (ls - p.z.t / s) * LP_LN2;
+        if (rank)
+            *rank = is_tok ? p.n : -1;
+        ref = p.z.m;
+        log_sum = ls;
+    }
+}
+/* How many of n keys are larger. */
+__device__ __forceinline__ int lp_place(const uint64_t *keys, int n, uint64_t key) {
+    int place = 0;
+#pragma unroll 8
+    for (int i = 0; i < n; ++i)
+        place += keys[i] > key ? 1 : 0;
+    return place;
+}
+/* The elements that reach `least` of every thread whose maximum does: a load per lane of its wave,
+ * 64 rounds at most (V <= LP_V_TOP). */
+template <class E>
+__device__ __forceinline__ void lp_candidates(const LpRow<E> &r, int v0, int nvec, const int64_t (&ends)[2], uint64_t mine,
+                                              uint64_t least, uint64_t *cand, int *ncand) {
+    constexpr int PER = LpRow<E>::PER;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (uint64_t who = __ballot(mine != 0 && mine >= least); who; who &= who - 1) {
+        const int vec = wave * 64 + __builtin_ctzll(who) + lane * LP_T;
+        if (vec < nvec) {
+            float w[PER];
+            r.unpack(r.raw(v0 + vec), w);
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const uint64_t key = lp_key(w[i], r.head + (int64_t)(v0 + vec) * PER + i);
+                if (key >= least)
+                    cand[atomicAdd(ncand, 1)] = key;
+            }
+        }
+    }
+    if (mine != 0 && mine >= least) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            if (ends[k] >= 0) {
+                const uint64_t key = lp_key(r.at(ends[k]), ends[k]);
+                if (key >= least)
+                    cand[atomicAdd(ncand, 1)] = key;
+            }
+    }
+}
+
+#ifndef LP_LOADS
+#define LP_LOADS 1
+#endif
 #define LP_U 4 /* 16-B loads of a thread in flight, twice */
 
 template <class E>
@@ -179,25 +247,32 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
                                                             const int64_t *__restrict__ tokens, int64_t V, int top,
                                                             float *__restrict__ logprob, float *__restrict__ entropy,
                                                             int32_t *__restrict__ rank, float *__restrict__ top_logprob,
-                                                            int32_t *__restrict__ top_index) {
+                                                            int32_t *__restrict__ top_index, int nsplit, float *part,
+                                                            unsigned *ctr) {
     constexpr int PER = LpRow<E>::PER;
     __shared__ float sm[LP_WAVES], ss[LP_WAVES], st[LP_WAVES];
     __shared__ int sr[LP_WAVES];
-    __shared__ uint64_t best[LP_WAVES * LP_TOP], cand[LP_CAND];
+    __shared__ uint32_t wave_reach[LP_WAVES];
+    __shared__ uint64_t cand[LP_CAND];
     __shared__ uint64_t floor_key;
     __shared__ int ncand;
     __shared__ float s_ref, s_ls;
-    const int64_t row = blockIdx.x;
+    __shared__ LpPart whole;
+    __shared__ unsigned s_last;
+    const int64_t row = blockIdx.x / nsplit;
+    const int split = blockIdx.x % nsplit;
     const LpRow<E> r(logits + row * stride, V);
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 
-    /* vectors threadIdx.x + k LP_T; one past the end repeats the last and counts as -inf */
-    const int nvec = (int)r.nvec, rounds = (nvec + LP_T - 1) / LP_T;
+    /* this workgroup's 16-B loads, v0 + threadIdx.x + k LP_T; one past the end repeats the last and
+     * does not count */
+    const int per = ((int)r.nvec + nsplit - 1) / nsplit, v0 = min(split * per, (int)r.nvec);
+    const int nvec = min(per, (int)r.nvec - v0), rounds = (nvec + LP_T - 1) / LP_T;
     glint_u32x4 now[LP_U], next[LP_U];
     auto fetch = [&](int k0, glint_u32x4 (&w)[LP_U]) {
 #pragma unroll
         for (int u = 0; u < LP_U; ++u)
-            w[u] = r.raw(min((int)threadIdx.x + (k0 + u) * LP_T, nvec - 1));
+            w[u] = r.raw(v0 + min((int)threadIdx.x + (k0 + u) * LP_T, nvec - 1));
     };
     if (rounds > 0)
         fetch(0, now);
@@ -251,14 +326,14 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         for (int u = 0; u < LP_U; ++u) {
             const int vec = (int)threadIdx.x + (k0 + u) * LP_T;
             if (vec < nvec)
-                take(vec, now[u]);
+                take(v0 + vec, now[u]);
         }
 #pragma unroll
         for (int u = 0; u < LP_U; ++u)
             now[u] = next[u];
     }
     uint64_t mine = 0;
-    const int64_t ends[2] = {r.before(), r.after()};
+    const int64_t ends[2] = {split == 0 ? r.before() : -1, split == nsplit - 1 ? r.after() : -1};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         if (ends[k] >= 0) {
@@ -293,17 +368,22 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         st[wave] = wt;
         sr[wave] = wr;
     }
-    /* this wave's `top` largest thread maxima, in order */
-    uint64_t rest = mine;
-    for (int i = 0; i < top; ++i) {
-        const uint64_t k = lp_wave_max(rest);
+    /* The top-th largest thread maximum: the largest value that `top` lanes of one wave reach is
+     * below it in no wave, so the maxima that reach the waves' largest such value hold it; each of
+     * them counts those before it. */
+    if (top > 0) {
+        const uint32_t value = (uint32_t)(mine >> 32);
+        uint32_t reach = 0; /* bit by bit */
+        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
+            if (__builtin_popcountll(__ballot(value >= (reach | bit))) >= top)
+                reach |= bit;
         if (lane == 0)
-            best[wave * LP_TOP + i] = k;
-        if (rest == k)
-            rest = 0; /* keys differ, but for 0 */
+            wave_reach[wave] = reach;
     }
-    if (threadIdx.x == 0)
+    if (threadIdx.x == 0) {
         ncand = 0;
+        floor_key = 0; /* fewer threads than `top` have an element: every element counts */
+    }
     __syncthreads();
     if (wave == 0) {
         static_assert(LP_WAVES == 16, "one row of lanes holds every wave's sums");
@@ -312,78 +392,109 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         lp_refer(z, lp_row16(z.m, LpMax()));
         z.s = lp_row16(z.s, LpAdd());
         z.t = lp_row16(z.t, LpAdd());
-        if (z.m == -INFINITY)
-            z.s = NAN; /* nothing is possible */
-        const float ls = log2f(z.s);
-        if (lane == 0) {
-            /* x - lse, in powers of two up to the last product */
-            logprob[row] = tok < 0 ? 0.f : is_tok ? (fmaf(xt, LP_LOG2E, -z.m) - ls) * LP_LN2 : NAN;
-            if (entropy)
-                entropy[row] = (ls - z.t / z.s) * LP_LN2;
-            if (rank)
-                rank[row] = is_tok ? n : -1;
-            s_ref = z.m;
-            s_ls = ls;
-        }
-        /* the top-th largest over the waves */
-        constexpr int LISTS = (LP_WAVES * LP_TOP + 63) / 64;
-        uint64_t v[LISTS];
-#pragma unroll
-        for (int i = 0; i < LISTS; ++i) {
-            const int k = lane + 64 * i;
-            v[i] = k < LP_WAVES * LP_TOP && k % LP_TOP < top ? best[k] : 0;
-        }
-        uint64_t k = 0;
-        for (int i = 0; i < top; ++i) {
-            k = 0;
-#pragma unroll
-            for (int u = 0; u < LISTS; ++u)
-                k = v[u] > k ? v[u] : k;
-            k = lp_wave_max(k);
-#pragma unroll
-            for (int u = 0; u < LISTS; ++u)
-                v[u] = v[u] == k ? 0 : v[u];
-        }
         if (lane == 0)
-            floor_key = k;
+            whole = LpPart{z, n};
+    }
+    if (top > 0) {
+        uint32_t reach = wave_reach[0];
+#pragma unroll
+        for (int i = 1; i < LP_WAVES; ++i)
+            reach = max(reach, wave_reach[i]);
+        if (mine != 0 && (uint32_t)(mine >> 32) >= reach)
+            cand[atomicAdd(&ncand, 1)] = mine;
+        __syncthreads();
+        const int n = ncand;
+        for (int c = threadIdx.x; c < n; c += LP_T)
+            if (lp_place(cand, n, cand[c]) == top - 1)
+                floor_key = cand[c];
+        __syncthreads();
+        if (threadIdx.x == 0)
+            ncand = 0;
+    }
+    __syncthreads();
+    if (nsplit == 1 && wave == 0)
+        lp_write(whole, tok, is_tok, xt, lane == 0, logprob + row, entropy ? entropy + row : nullptr, rank ? rank + row : nullptr,
+                 s_ref, s_ls);
+    if (top > 0) {
+        const uint64_t least = floor_key;
+        lp_candidates(r, v0, nvec, ends, mine, least, cand, &ncand);
+    }
+    __syncthreads();
+    if (nsplit > 1) {
+        /* This part's sums and list go to the workspace; the part that arrives last takes all of
+         * them as it took its threads': the largest of the lists' last entries is a floor. */
+        uint32_t *mine_part = (uint32_t *)part + (row * nsplit + split) * LP_PART;
+        if (threadIdx.x == 0) {
+            const uint32_t v[4] = {__float_as_uint(whole.z.m), __float_as_uint(whole.z.s), __float_as_uint(whole.z.t),
+                                   (uint32_t)whole.n};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                __hip_atomic_store(mine_part + i, v[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+        auto put = [&](int place, uint64_t key) {
+            __hip_atomic_store(mine_part + 4 + 2 * place, (uint32_t)key, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_store(mine_part + 5 + 2 * place, (uint32_t)(key >> 32), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        };
+        const int n = top > 0 ? ncand : 0;
+        for (int c = threadIdx.x; c < n; c += LP_T) {
+            const int place = lp_place(cand, n, cand[c]);
+            if (place < top)
+                put(place, cand[c]);
+        }
+        if ((int)threadIdx.x < top && (int)threadIdx.x >= n)
+            put(threadIdx.x, 0); /* a part shorter than the list */
+        __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            s_last = __hip_atomic_fetch_add(ctr + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)nsplit - 1u;
+            ncand = 0;
+            floor_key = 0;
+        }
+        __syncthreads();
+        if (!s_last)
+            return;
+        const uint32_t *parts = (const uint32_t *)part + row * nsplit * LP_PART;
+        auto get = [&](int i) { return __hip_atomic_load(parts + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); };
+        auto key_of = [&](int p, int place) {
+            return (uint64_t)get(p * LP_PART + 5 + 2 * place) << 32 | get(p * LP_PART + 4 + 2 * place);
+        };
+        const int p = (int)threadIdx.x / LP_TOP, place = (int)threadIdx.x % LP_TOP;
+        const uint64_t key = p < nsplit && place < top ? key_of(p, place) : 0;
+        if (wave == 0) {
+            static_assert(LP_SPLIT <= 64, "a part a lane");
+            LpPart z{{-INFINITY, 0.f, 0.f}, 0};
+            uint64_t floor = 0;
+            if (lane < nsplit) {
+                z.z.m = __uint_as_float(get(lane * LP_PART));
+                z.z.s = __uint_as_float(get(lane * LP_PART + 1));
+                z.z.t = __uint_as_float(get(lane * LP_PART + 2));
+                z.n = (int)get(lane * LP_PART + 3);
+                floor = top > 0 ? key_of(lane, top - 1) : 0;
+            }
+            lp_refer(z.z, lp_wave(z.z.m, LpMax()));
+            z.z.s = lp_wave(z.z.s, LpAdd());
+            z.z.t = lp_wave(z.z.t, LpAdd());
+            z.n = lp_wave_sum(z.n);
+            lp_write(z, tok, is_tok, xt, lane == 0, logprob + row, entropy ? entropy + row : nullptr,
+                     rank ? rank + row : nullptr, s_ref, s_ls);
+            floor = lp_wave_max(floor);
+            if (lane == 0) {
+                floor_key = floor;
+                __hip_atomic_store(ctr + row, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
+        }
+        __syncthreads();
+        if (key != 0 && key >= floor_key)
+            cand[atomicAdd(&ncand, 1)] = key;
+        __syncthreads();
     }
     if (top == 0)
         return;
-    __syncthreads();
-    const uint64_t least = floor_key;
-    /* the elements of each thread whose maximum counts, a load per lane of its wave */
-    for (uint64_t who = __ballot(mine != 0 && mine >= least); who; who &= who - 1) {
-        const int owner = wave * 64 + __builtin_ctzll(who);
-        const int vec = owner + lane * LP_T;
-        if (vec < nvec) { /* at most 64 rounds: V <= LP_V_TOP */
-            float w[PER];
-            r.unpack(r.raw(vec), w);
-#pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const uint64_t key = lp_key(w[i], r.head + (int64_t)vec * PER + i);
-                if (key >= least)
-                    cand[atomicAdd(&ncand, 1)] = key;
-            }
-        }
-    }
-    if (mine != 0 && mine >= least) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-            if (ends[k] >= 0) {
-                const uint64_t key = lp_key(r.at(ends[k]), ends[k]);
-                if (key >= least)
-                    cand[atomicAdd(&ncand, 1)] = key;
-            }
-    }
-    __syncthreads();
     const int n = ncand;
     const float m = s_ref, ls = s_ls;
     for (int c = threadIdx.x; c < n; c += LP_T) {
         const uint64_t key = cand[c];
-        int place = 0;
-#pragma unroll 8
-        for (int i = 0; i < n; ++i)
-            place += cand[i] > key ? 1 : 0;
+        const int place = lp_place(cand, n, key);
         if (place < top) {
             top_logprob[row * top + place] = (fmaf(lp_key_value(key), LP_LOG2E, -m) - ls) * LP_LN2;
             top_index[row * top + place] = (int32_t)lp_key_index(key);
@@ -401,11 +512,20 @@ GLINT_API int glint_token_logprobs(const void *logits, int elt, int64_t stride, 
         return -2;
     if (T == 0)
         return 0;
+    /* Few rows are split, so that some 256 workgroups share the reading, none with less than two loads
+     * of every thread: 8 rows of 128256 BF16 LP_T_SPLIT us, LP_T_WHOLE in one workgroup each. */
+    const int64_t loads = V / (elt == GLINT_KV_BF16 ? 8 : 4) / (LP_LOADS * LP_T);
+    int nsplit = (int)std::min<int64_t>(std::min<int64_t>(LP_SPLIT, loads), glint_cu_count() / T);
+    GlintSplitWs ws{nullptr, nullptr, 0, 0};
+    if (nsplit < 2 || !glint_serve_ws(stream, ws) || ws.nctr < (size_t)T ||
+        ws.part_floats < (size_t)T * nsplit * LP_PART)
+        nsplit = 1;
+    const unsigned grid = (unsigned)T * nsplit;
     if (elt == GLINT_KV_BF16)
-        k_token_logprobs<uint16_t><<<(unsigned)T, LP_T, 0, stream>>>((const uint16_t *)logits, stride, tokens, V, top,
-                                                                     logprob, entropy, rank, top_logprob, top_index);
+        k_token_logprobs<uint16_t><<<grid, LP_T, 0, stream>>>((const uint16_t *)logits, stride, tokens, V, top, logprob,
+                                                              entropy, rank, top_logprob, top_index, nsplit, ws.part, ws.ctr);
     else
-        k_token_logprobs<float><<<(unsigned)T, LP_T, 0, stream>>>((const float *)logits, stride, tokens, V, top,
-                                                                  logprob, entropy, rank, top_logprob, top_index);
+        k_token_logprobs<float><<<grid, LP_T, 0, stream>>>((const float *)logits, stride, tokens, V, top, logprob, entropy,
+                                                           rank, top_logprob, top_index, nsplit, ws.part, ws.ctr);
     return hipGetLastError() == hipSuccess ? 0 : -3;
 }

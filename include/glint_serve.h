@@ -19,7 +19,7 @@
  *
  * Return codes: 0 success, -1 null pointer, -2 shape, stride or alignment not supported,
  * -3 launch failure. All calls are asynchronous on `stream` and allocate nothing (but
- * glint_kv4_attend a workspace, once per stream). D is 64 or
+ * a workspace, once per stream: see glint_serve_workspace_reserve). D is 64 or
  * 128; strides count elements, a row's D elements are adjacent. */
 #ifndef GLINT_SERVE_H
 #define GLINT_SERVE_H
@@ -94,7 +94,8 @@ int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_
  * A token below 0 (a place without one) gives logprob 0 and rank -1, one of V or above NaN
  * and -1. A row with a NaN or +inf, or with -inf alone, gives NaN log probabilities and
  * entropy; in the top list NaN takes the place of -inf, and rank counts no NaN. T < 4194304,
- * 0 <= top <= min(20, V), and V <= 262144 where top > 0. entropy, rank and, for top == 0, the top_ pointers may be NULL. */
+ * 0 <= top <= min(20, V), and V <= 262144 where top > 0. A few long rows are split
+ * over workgroups as glint_kv4_attend's sequences are. entropy, rank and, for top == 0, the top_ pointers may be NULL. */
 int glint_token_logprobs(const void *logits, int elt, int64_t stride, const int64_t *tokens, int64_t T, int64_t V,
                          int top, float *logprob, float *entropy, int32_t *rank, float *top_logprob,
                          int32_t *top_index, struct ihipStream_t *stream);
