@@ -103,9 +103,10 @@ __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int 
 #pragma unroll
         for (int i = 0; i < 16; ++i)
             top = fmaxf(top, sc[a][i]);
-    top = fmaxf(top, __shfl_xor(top, 32, 64)) * scale2;
-    if (__any(top > w.m + AP_SLACK)) {
-        const float mn = fmaxf(w.m, top);
+    top = glint_xor32(top, GlintMax()) * scale2;
+    const bool more = top > w.m + AP_SLACK; /* a row's own test, here and below: its bits depend on no other row */
+    if (__any(more)) {
+        const float mn = more ? top : w.m;
         const float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
         w.m = mn;
         w.l *= keep;
@@ -139,16 +140,18 @@ __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int 
         return f;
     };
     /* A weight's bf16 rounding (2^-8) averages out over many keys and does not where few hold
-     * the sum: a tile with a weight above 1 / 16 of some row's sum so far is multiplied by
-     * what the rounding left as well. */
-    if (__any(__builtin_amdgcn_exp2f(top - base) * 16.f > w.l + __shfl_xor(w.l, 32, 64))) {
+     * the sum: rows with a weight above 1 / 16 of their sum so far add what the rounding left. */
+    const bool few = __builtin_amdgcn_exp2f(top - base) * 16.f > glint_xor32(w.l, GlintAdd());
+    if (__any(few)) {
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
             ApFrag rest;
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 const int i = 8 * (s & 1) + 2 * x;
-                rest.u[x] = glint_cvt_bf16x2(sc[s >> 1][i] - glint_bf16lo(pf[s].u[x]), sc[s >> 1][i + 1] - glint_bf16hi(pf[s].u[x]));
+                const uint32_t left =
+                    glint_cvt_bf16x2(sc[s >> 1][i] - glint_bf16lo(pf[s].u[x]), sc[s >> 1][i + 1] - glint_bf16hi(pf[s].u[x]));
+                rest.u[x] = few ? left : 0u;
             }
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -170,6 +173,7 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
     constexpr int TILE = AP_KEYS * D * 2;      /* bytes */
     /* two tiles of each; arrays of their own, so that reads of one do not wait for loads into the other */
     __shared__ __attribute__((aligned(16))) char k0t[TILE], k1t[TILE], v0t[TILE], v1t[TILE];
+    __shared__ uint32_t apart; /* a value that is not finite was taken out */
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
     /* Work items are the row blocks of a group's heads, a group being one sequence and key head;
@@ -276,14 +280,40 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
         }
     };
 
+    /* Of a tile that some row does not see whole, every thread looks through the values it loaded:
+     * an infinite or NaN one, of which a weight of 0 would make NaN, becomes 0 until the
+     * end. */
+    const int t_part = (int)max((int64_t)0, r0 + gap + 1) / AP_KEYS;
     auto step = [&](int t, ap_lds *kt, ap_lds *vt, ap_lds *kn, ap_lds *vn) {
         __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0); /* this wave's part of tile t */
         __syncthreads();
         if (t + 1 < ntiles)
             fetch(t + 1, kn, vn); /* over tile t - 1, which every wave has left */
+        if (t >= t_part) {
+            typedef __attribute__((address_space(3))) glint_u32x4 lds_u32x4;
+#pragma unroll
+            for (int i = 0; i < LOADS; ++i) {
+                lds_u32x4 *at = (lds_u32x4 *)(vt + (threadIdx.x + i * AP_T) * 16);
+                glint_u32x4 x = *at;
+                bool odd = false;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const bool lo = (x[j] & 0x7F80u) == 0x7F80u, hi = (x[j] & 0x7F800000u) == 0x7F800000u;
+                    x[j] &= (lo ? 0xFFFF0000u : ~0u) & (hi ? 0xFFFFu : ~0u);
+                    odd |= lo || hi;
+                }
+                if (odd) {
+                    *at = x;
+                    apart = 1;
+                }
+            }
+            __syncthreads();
+        }
         if (t * AP_KEYS <= wave_high)
             ap_tile<D>(kt, vt, t, w, A.scale2, t * AP_KEYS + AP_KEYS - 1 > wave_low, half);
     };
+    if (threadIdx.x == 0)
+        apart = 0;
     if (ntiles > 0)
         fetch(0, (ap_lds *)k0t, (ap_lds *)v0t);
     for (int t = 0; t < ntiles; t += 2) {
@@ -291,8 +321,35 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
         if (t + 1 < ntiles)
             step(t + 1, (ap_lds *)k1t, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t);
     }
-    float l = w.l;
-    l += __shfl_xor(l, 32, 64);
+    const float l = glint_xor32(w.l, GlintAdd());
+    /* A value that is not finite leaves itself or NaN in its dimension of the rows that see it,
+     * whatever its weight: the products above made NaN of some infinities, by what a weight's rounding
+     * left (0, or negative), so the dimensions they spoilt are walked again for such values alone. */
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d) {
+        bool spoilt = false;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            spoilt |= !(fabsf(w.o[d][i]) <= FLT_MAX);
+        if (!__any(spoilt && l <= FLT_MAX) && !__builtin_amdgcn_readfirstlane((int)apart))
+            continue;
+        ap_f32x16 odd;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            odd[i] = 0.f;
+        for (int key = 0; key <= wave_high; ++key) {
+            const uint16_t *from = vb + key * A.v_st + 32 * d + 4 * half;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t v = from[8 * (i >> 2) + (i & 3)];
+                if ((v & 0x7F80u) == 0x7F80u && key <= w.last)
+                    odd[i] += __uint_as_float(v << 16);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            w.o[d][i] = odd[i] == 0.f ? w.o[d][i] : odd[i];
+    }
     if (row >= nq)
         return;
     const float inv = l == 0.f ? 0.f : 1.f / l;

@@ -13,7 +13,6 @@ A missing library raises RuntimeError: there is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 from pathlib import Path
 from typing import NamedTuple, Optional, Tuple
@@ -514,21 +513,11 @@ def int8_gemm_scaled_bf16(A, B, sa, sb, out=None, stream=None):
 # Every helper here takes stream= (default: the current stream).
 KV_PAGE = 64
 
-
-def _on_stream(f):
-    """With a stream given, the whole call (its outputs, scratch and copies too) belongs to it."""
-    @functools.wraps(f)
-    def call(*args, stream=None, **kw):
-        if stream is None:
-            return f(*args, **kw)
-        with _torch().cuda.stream(stream):
-            return f(*args, **kw)
-    return call
+# With a stream given, a helper's whole call (its outputs, scratch and copies too) belongs to it.
 
 
-def _on_gpu(*tensors) -> None:
-    if not all(t.is_cuda for t in tensors):
-        raise ValueError(f"tensors on {', '.join(str(t.device) for t in tensors)}: all must be on the GPU")
+def _refuse_devices(*tensors) -> None:
+    raise ValueError(f"tensors on {', '.join(str(t.device) for t in tensors)}: all must be on the GPU")
 
 
 class Kv4Cache(NamedTuple):
@@ -552,7 +541,8 @@ def kv4_cache(pages: int, heads: int, dim: int, device="cuda") -> Kv4Cache:
 def _planes(cache):
     """(pages, H, D, the four data pointers) of a cache whose planes agree."""
     kh, ka, vh, va = cache
-    _on_gpu(kh, ka, vh, va)
+    if not (kh.is_cuda and ka.is_cuda and vh.is_cuda and va.is_cuda):
+        _refuse_devices(kh, ka, vh, va)
     torch = _TORCH or _torch()
     pages, heads, page, half = kh.shape
     scales = (pages, heads, half // 32, page)
@@ -595,17 +585,20 @@ def _ints(t, dtype, n: int, what: str):
     return t.data_ptr()
 
 
-@_on_stream
-def kv4_append(k, v, slots, cache) -> None:
+def kv4_append(k, v, slots, cache, stream=None) -> None:
     """Encode keys and values [T, H, D] (bf16 or f32) into the cache at slots [T] (int64: page * 64
     + place; negative ones are skipped)."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return kv4_append(k, v, slots, cache)
     torch = _TORCH or _torch()
     pages, heads, dim, *planes = _planes(cache)
     T = k.shape[0]
     if k.shape != (T, heads, dim) or v.shape != k.shape or v.dtype is not k.dtype:
         raise ValueError(f"k {tuple(k.shape)} {k.dtype}, v {tuple(v.shape)} {v.dtype}, cache of {heads} heads of {dim}")
     elt = _kv_elt(k)
-    _on_gpu(k, v, slots)
+    if not (k.is_cuda and v.is_cuda and slots.is_cuda):
+        _refuse_devices(k, v, slots)
     k, kt, kh = _rows(k, 4)
     v, vt, vh = _rows(v, 4)
     at = _ints(slots, torch.int64, T, "slots")
@@ -615,13 +608,16 @@ def kv4_append(k, v, slots, cache) -> None:
                                         pages, _sh(None)), "glint_kv4_append")
 
 
-@_on_stream
-def kv4_gather(slots, cache, out=None):
+def kv4_gather(slots, cache, out=None, stream=None):
     """The cache's tokens at slots [T] (int64) as bf16 (k, v), each [T, H, D]; zeros for negative slots."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return kv4_gather(slots, cache, out)
     torch = _TORCH or _torch()
     pages, heads, dim, *planes = _planes(cache)
     T = slots.numel()
-    _on_gpu(slots)
+    if not slots.is_cuda:
+        _refuse_devices(slots)
     at = _ints(slots, torch.int64, T, "slots")
     if out is None:
         k = slots.new_empty((T, heads, dim), dtype=torch.bfloat16)
@@ -636,18 +632,22 @@ def kv4_gather(slots, cache, out=None):
     return k, v
 
 
-@_on_stream
-def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Optional[float] = None, out=None):
+def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Optional[float] = None, out=None,
+               stream=None):
     """Attention of the newest tokens over the cache: q bf16 [rows, Hq, D] -> bf16 [rows, Hq, D].
 
     page_table int32 [B, max_pages] and lens int32 [B] (tokens in the cache, the new ones
     included) say what each sequence sees; its rows are cu_q[b] .. cu_q[b + 1] (int32, at most
     max_q each), or max_q each where cu_q is None. A row sees the positions up to its own."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return kv4_attend(q, cache, page_table, lens, cu_q, max_q, scale, out)
     torch = _TORCH or _torch()
     pages, heads, dim, *planes = _planes(cache)
     rows, hq, d = q.shape
     B, wide = page_table.shape
-    _on_gpu(q, page_table, lens, *(() if cu_q is None else (cu_q,)))
+    if not (q.is_cuda and page_table.is_cuda and lens.is_cuda and (cu_q is None or cu_q.is_cuda)):
+        _refuse_devices(q, page_table, lens, lens if cu_q is None else cu_q)
     if d != dim or hq % heads:
         raise ValueError(f"q {tuple(q.shape)}, cache of {heads} heads of {dim}")
     if q.dtype is not torch.bfloat16:
@@ -679,17 +679,21 @@ def _attend_out(out, q, rows: int, hq: int, dim: int):
     return out
 
 
-@_on_stream
-def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: Optional[float] = None, out=None):
+def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: Optional[float] = None, out=None,
+                  stream=None):
     """Causal attention over packed sequences: q bf16 [Tq, Hq, D], k and v bf16 [Tk, H, D] -> bf16 [Tq, Hq, D].
 
     cu_q, cu_k int32 [B + 1]: where each sequence's queries and keys start (cu_k is cu_q where
     None); a sequence's last query sees its last key. max_q: no sequence has more queries
     (Tq where None)."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return attend_prompt(q, k, v, cu_q, cu_k, max_q, scale, out)
     torch = _TORCH or _torch()
     Tq, hq, dim = q.shape
     Tk, heads, _ = k.shape
-    _on_gpu(q, k, v, cu_q, *(() if cu_k is None else (cu_k,)))
+    if not (q.is_cuda and k.is_cuda and v.is_cuda and cu_q.is_cuda and (cu_k is None or cu_k.is_cuda)):
+        _refuse_devices(q, k, v, cu_q, cu_q if cu_k is None else cu_k)
     if k.shape != v.shape or k.shape[2] != dim or heads == 0 or hq % heads:
         raise ValueError(f"q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}")
     if any(t.dtype is not torch.bfloat16 for t in (q, k, v)):
@@ -712,27 +716,33 @@ def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: 
     return out
 
 
-@_on_stream
-def token_logprobs(logits, tokens, top: int = 0) -> dict:
+def token_logprobs(logits, tokens, top: int = 0, stream=None) -> dict:
     """Scores of tokens [T] (int64) under logits [T, V] (bf16 or f32): f32 "logprob" and "entropy"
     [T], int32 "rank" [T] (entries ahead of the token; 0 where it is the likeliest), and the
     `top` likeliest entries, "top_logprob" f32 and "top_index" int32 [T, top], equal ones by
     index. A negative token gives logprob 0 and rank -1."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return token_logprobs(logits, tokens, top)
     torch = _TORCH or _torch()
     T, V = logits.shape
     elt = _kv_elt(logits)
-    _on_gpu(logits, tokens)
+    if not (logits.is_cuda and tokens.is_cuda):
+        _refuse_devices(logits, tokens)
     if logits.stride(1) != 1 and V > 1:
         logits = logits.contiguous()
     at = _ints(tokens, torch.int64, T, "tokens")
-    new = lambda dtype, *s: logits.new_empty(s, dtype=dtype)
-    r = {"logprob": new(torch.float32, T), "entropy": new(torch.float32, T), "rank": new(torch.int32, T),
-         "top_logprob": new(torch.float32, T, top), "top_index": new(torch.int32, T, top)}
+    logprob = logits.new_empty(T, dtype=torch.float32)
+    entropy = torch.empty_like(logprob)
+    rank = logits.new_empty(T, dtype=torch.int32)
+    top_logprob = logits.new_empty((T, top), dtype=torch.float32)
+    top_index = logits.new_empty((T, top), dtype=torch.int32)
     if T:
         _check(serve_lib().glint_token_logprobs(logits.data_ptr(), elt, logits.stride(0), at, T, V, top,
-                                                *(t.data_ptr() for t in r.values()), _sh(None)),
+                                                logprob.data_ptr(), entropy.data_ptr(), rank.data_ptr(),
+                                                top_logprob.data_ptr(), top_index.data_ptr(), _sh(None)),
                "glint_token_logprobs")
-    return r
+    return {"logprob": logprob, "entropy": entropy, "rank": rank, "top_logprob": top_logprob, "top_index": top_index}
 
 
 # ------------------------------------------------------------- host-pointer wrappers

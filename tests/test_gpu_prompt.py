@@ -88,6 +88,35 @@ def test_strides_and_streams():
     assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("D", [64, 128])
+def test_what_a_row_does_not_see(D):
+    """NaN and infinities in keys and values past a row's last change nothing for it; a row that sees
+    an infinite or NaN value shows it in that dimension alone."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(9)
+    n = 200
+    q, k, v = (bf16(rng.normal(0, 1, (n, 2, D)).astype(np.float32)) for _ in range(3))
+    cu = gpu(np.array([0, n], np.int32))
+    clean = values(H.attend_prompt(q, k, v, cu))
+    for at in (199, 150, 64, 63, 5):
+        for value in (float("nan"), float("inf"), float("-inf")):
+            v2, k2 = v.clone(), k.clone()
+            v2[at, 1, 37] = value
+            v2[at, 1, D - 1] = value
+            got = values(H.attend_prompt(q, k, v2, cu))
+            same = np.ones_like(got, bool)
+            same[at:, 1, 37] = same[at:, 1, D - 1] = False
+            assert np.array_equal(got[same], clean[same]), (at, value)
+            assert not np.isfinite(got[~same]).any()
+            if value != value:
+                assert np.isnan(got[~same]).all()
+            else:
+                assert (got[~same] == value).all(), (at, value)
+            k2[at, 0, 3] = value
+            got = values(H.attend_prompt(q, k2, v, cu))
+            assert np.array_equal(got[:at], clean[:at]) and np.array_equal(got[:, 1], clean[:, 1]), (at, value)
+
+
 def test_rows_outside_the_sequences_stay():
     torch = torch_cuda()
     rng = np.random.default_rng(8)
