@@ -1,9 +1,15 @@
 /* The 4-bit key/value cache: append and gather (include/glint_serve.h).
  *
+ * Both move bytes: a token and head of D dimensions is 4 D bytes in BF16 (8 D in FP32) on one side and
+ * D + 8 D / 64 on the other. Calls of few tokens are a launch and one load's latency after another.
+ *
  * k_kv4_append — a row of 16 lanes encodes one 64-block of one token's key or value, four
- *   elements a lane.
+ *   elements a lane; 8 tokens of 8 heads in 3.5 us.
  * k_kv4_gather — a thread reads one byte of a key row (two adjacent dimensions) or of a value
- *   column (dimensions 16 apart) and writes its two BF16. */
+ *   column (dimensions 16 apart) and writes its two BF16; 8 tokens in 2.8 us.
+ * k_kv4_append_tile, k_kv4_gather_tile — 64 tokens of one head a workgroup, for prompts: without
+ *   them a value's bytes are written and read one by one, 64 B apart. 4096 tokens of 8 heads of
+ *   128: append 12.2 us (1.8 TB/s; 24 element-wise), gather 14.3 us (1.5 TB/s; 18). */
 #include "kv4.h"
 
 #define KV4_T 256
@@ -335,9 +341,17 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_gather_tile(const int64_t *__rest
     }
 }
 
-#ifndef KV4_TILE_T
-#define KV4_TILE_T 32 /* tokens from which on the tiles are taken */
-#endif
+/* When tiles are taken. A workgroup of them runs 7 to 10 us however little it has, so they want the
+ * device's workgroups, and half their tokens. us, BF16, 128 dimensions, element-wise against tiles:
+ *   tokens x heads   1024 x 8      1250 x 8      1536 x 8       2048 x 8       4096 x 8
+ *   append           8.6, 9.7      9.8, 10.0     11.4, 10.1     14.5, 10.4     23.6, 12.2
+ *   gather           6.6, 10.6     7.3, 11.1     8.5, 10.0      10.4, 10.3     18.0, 14.3
+ *   tokens x heads   16 x 1024     32 x 512
+ *   append           13.4, 15.2    12.9, 11.1 */
+#define KV4_TILE_APPEND 10240 /* tokens of one head */
+#define KV4_TILE_GATHER 16384
+#define KV4_TILE_T 32
+static bool kv4_tiles(int64_t T, int H, int64_t from) { return T >= KV4_TILE_T && T * H >= from; }
 
 /* Workgroups of KV4_T threads for n threads' work, or 0 where a grid cannot hold them. */
 static unsigned kv4_grid(int64_t T, int64_t per_token) {
@@ -394,7 +408,7 @@ GLINT_API int glint_kv4_append(const void *k, const void *v, int elt, int64_t k_
     if (!g)
         return -2;
     /* the tiles load 8 elements at once */
-    const bool tiles = T >= KV4_TILE_T && glint_aligned(k, 16) && glint_aligned(v, 16) &&
+    const bool tiles = kv4_tiles(T, H, KV4_TILE_APPEND) && glint_aligned(k, 16) && glint_aligned(v, 16) &&
                        !((k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7);
     if (tiles && elt == GLINT_KV_BF16)
         kv4_append_tiles<uint16_t>(k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, slots, T, H, D, k_hole, k_absmax,
@@ -424,7 +438,7 @@ GLINT_API int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, co
     if (!g)
         return -2;
     const dim3 tiles((unsigned)((T + KT_TOKENS - 1) / KT_TOKENS), H);
-    if (T >= KV4_TILE_T && glint_aligned(k, 16) && glint_aligned(v, 16)) {
+    if (kv4_tiles(T, H, KV4_TILE_GATHER) && glint_aligned(k, 16) && glint_aligned(v, 16)) {
         if (D == 64)
             k_kv4_gather_tile<64><<<tiles, KV4_T, 0, stream>>>(slots, T, H, k_hole, k_absmax, v_hole, v_absmax, pages * 64, k, v);
         else

@@ -51,6 +51,20 @@ def put(planes, slot, k, v):
         vh[page, :, r, t] = (vh[page, :, r, t] & (0xF0 >> sh)) | (cv[:, d] << sh)
 
 
+def put_all(planes, slots, k, v):
+    """put() for tokens [T, H, D] in different slots, all at once."""
+    kh, ka, vh, va = planes
+    page, t = np.divmod(np.asarray(slots, np.int64), PAGE)
+    D = k.shape[-1]
+    (ck, sk), (cv, sv) = hole_codes(k), hole_codes(v)
+    ka[page, :, :, t], va[page, :, :, t] = sk, sv
+    for d in range(D):
+        b, sh = _k_at(d, D // 64)
+        kh[page, :, t, b] = (kh[page, :, t, b] & (0xF0 >> sh)) | (ck[..., d] << sh)
+        r, sh = _v_at(d)
+        vh[page, :, r, t] = (vh[page, :, r, t] & (0xF0 >> sh)) | (cv[..., d] << sh)
+
+
 def held(planes, slots):
     """f64 (k, v) [tokens, H, D] of the slots."""
     kh, ka, vh, va = planes

@@ -91,10 +91,48 @@ def test_append_in_a_row_fills_whole_pages():
         assert got.tobytes() == w.tobytes()
 
 
-@pytest.mark.parametrize("T", [8, 64])
+@pytest.mark.parametrize("T,heads,D,dtype", [(33, 311, 64, "f32"), (64, 256, 128, "bf16"), (130, 127, 64, "bf16"), (700, 24, 128, "f32")])
+def test_append_and_gather_in_tiles(T, heads, D, dtype):
+    """Enough tokens of one head for the launches by tiles: runs of slots that start at every place modulo 4,
+    single slots, tokens that are skipped, tiles that are not whole, special values."""
+    torch_cuda()
+    print(f"append T={T} H={heads} D={D} {dtype}", flush=True)
+    rng = np.random.default_rng(T)
+    k, v = rng.normal(0, 1, (2, T, heads, D)).astype(np.float32)
+    k[0, 0, :64] = 0
+    v[-1, -1, 3], v[-1, -1, 7], k[T // 2, 0, 5] = np.nan, -np.nan, np.inf
+    v[T // 2, 0, :64] = 1e-41
+    v[T // 2, 1] *= 1e30
+    if dtype == "bf16":
+        kb, vb = bf16(k), bf16(v)
+        k, v = S.bf16_values(host(kb)).reshape(k.shape), S.bf16_values(host(vb)).reshape(v.shape)
+    else:
+        kb, vb = gpu(k), gpu(v)
+    pages = T // 64 + 3
+    for first in (0, 1, 3, 64, 66):
+        slots = np.arange(T, dtype=np.int64) + first
+        slots[T // 3:T // 3 + 9] = rng.permutation(slots[T // 3:T // 3 + 9])
+        slots[T // 2], slots[T // 4] = -1, pages * 64
+        want = S.empty_planes(pages, heads, D, fill=0x5A)
+        cache = tuple(gpu(p) for p in want)
+        ok = (slots >= 0) & (slots < pages * 64)
+        S.put_all(want, slots[ok], k[ok], v[ok])
+        H.kv4_append(kb, vb, gpu(slots), cache)
+        for got, w, name in zip(planes_of(cache), want, ("k_hole", "k_absmax", "v_hole", "v_absmax")):
+            assert got.tobytes() == w.tobytes(), (name, first)
+        some = np.concatenate([slots, rng.permutation(slots)[:17], [pages * 64 - 1]])
+        ok = (some >= 0) & (some < pages * 64)
+        with np.errstate(all="ignore"):
+            for got, w in zip(H.kv4_gather(gpu(some), cache), S.held(want, np.where(ok, some, 0))):
+                w = np.where(ok[:, None, None], w, 0).astype(np.float32)
+                assert np.array_equal(S.bf16_values(host(got)).reshape(w.shape),
+                                      S.bf16_values(bf16_bits(w)).reshape(w.shape), equal_nan=True), first
+
+
+@pytest.mark.parametrize("T", [8, 64, 5120])
 def test_append_at_the_edges(T):
-    """Quotients at and one float beside every edge between two codes, under an absmax of 1 (T = 8 and 64
-    take the two launches)."""
+    """Quotients at and one float beside every edge between two codes, under an absmax of 1 (5120 tokens of
+    2 heads are appended by tiles)."""
     torch_cuda()
     edges = ((S.PARENT[1:].astype(np.float64) + S.PARENT[:-1]) / 2).astype(np.float32)
     near = (edges.view(np.int32)[:, None] + np.arange(-2, 3)).astype(np.int32).view(np.float32).ravel()
@@ -102,10 +140,9 @@ def test_append_at_the_edges(T):
     rows = np.resize(rows, T * 2 * 63).reshape(T, 2, 63)
     k = np.concatenate([rows, np.ones((T, 2, 1), np.float32)], -1)
     v = np.concatenate([-np.ones((T, 2, 1), np.float32), rows[::-1]], -1)
-    want = S.empty_planes(2, 2, 64)
+    want = S.empty_planes(T // 64 + 2, 2, 64)
     cache = tuple(gpu(p) for p in want)
-    for t in range(T):
-        S.put(want, t + 3, k[t], v[t])
+    S.put_all(want, np.arange(T) + 3, k, v)
     H.kv4_append(gpu(k), gpu(v), gpu(np.arange(T, dtype=np.int64) + 3), cache)
     for got, w, name in zip(planes_of(cache), want, ("k_hole", "k_absmax", "v_hole", "v_absmax")):
         assert got.tobytes() == w.tobytes(), name
