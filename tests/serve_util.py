@@ -108,7 +108,8 @@ def kv4_bound(out, mass, size):
 
 
 def prompt_bound(out, mass, size):
-    """bf16 output and bf16 weights (2^-9 each, the first doubled for a rounded sum); f32 scores."""
+    """The output's bf16 rounding (2^-8); 2^-9 for the weights, half of what they would be off if bf16 rounded
+    all of them the same way: many average out, and where few count their rest is added back; f32 scores."""
     return 2.0 ** -8 * np.abs(out) + mass * (2.0 ** -9 + np.expm1(2.0 ** -16 * size)[:, None] + 2.0 ** -16)
 
 
