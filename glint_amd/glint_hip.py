@@ -624,8 +624,9 @@ def kv4_gather(slots, cache, out=None, stream=None):
         v = torch.empty_like(k)
     else:
         k, v = out
-        if any(t.shape != (T, heads, dim) or t.dtype is not torch.bfloat16 or not t.is_contiguous() for t in (k, v)):
-            raise ValueError(f"out: two contiguous bfloat16 tensors of {(T, heads, dim)}")
+        if any(t.shape != (T, heads, dim) or t.dtype is not torch.bfloat16 or not t.is_contiguous() or not t.is_cuda
+               for t in (k, v)):
+            raise ValueError(f"out: two contiguous bfloat16 tensors of {(T, heads, dim)} on the GPU")
     if T:
         _check(serve_lib().glint_kv4_gather(at, T, heads, dim, *planes, pages, k.data_ptr(), v.data_ptr(), _sh(None)),
                "glint_kv4_gather")
@@ -674,8 +675,8 @@ def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Opt
 def _attend_out(out, q, rows: int, hq: int, dim: int):
     if out is None:
         return q.new_empty((rows, hq, dim))
-    if out.shape != (rows, hq, dim) or out.dtype is not q.dtype or not out.is_contiguous():
-        raise ValueError(f"out: a contiguous bfloat16 tensor of {(rows, hq, dim)}")
+    if out.shape != (rows, hq, dim) or out.dtype is not q.dtype or not out.is_contiguous() or not out.is_cuda:
+        raise ValueError(f"out: a contiguous bfloat16 tensor of {(rows, hq, dim)} on the GPU")
     return out
 
 
