@@ -480,144 +480,147 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
              * rows have one power for its value scales, which go to LDS scaled and rounded to f16.
              * Of another page they go there as they are. */
             const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
-#pragma unroll
-            for (int bb = 0; bb < NB; ++bb) {
-                sl[bb * KV4_PAGE + lane] = sw[bb];
-                const float v = sw[NB + bb];
-                if (whole) {
-                    if (__any(v >= vlimit[bb])) {
-                        const float top = glint_wave_max(v < INFINITY ? v : 0.f);
-                        if (top >= vlimit[bb])
-                            carry(bb, kv4_new_power(top, vdown[bb], vlimit[bb]));
+            glint_f32x4 sc[4]; /* scores, without the row's factor */
+            if (pg != KA_FAR) {
+    #pragma unroll
+                for (int bb = 0; bb < NB; ++bb) {
+                    sl[bb * KV4_PAGE + lane] = sw[bb];
+                    const float v = sw[NB + bb];
+                    if (whole) {
+                        if (__any(v >= vlimit[bb])) {
+                            const float top = glint_wave_max(v < INFINITY ? v : 0.f);
+                            if (top >= vlimit[bb])
+                                carry(bb, kv4_new_power(top, vdown[bb], vlimit[bb]));
+                        }
+                        ((kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE))[lane] = (_Float16)(v * vdown[bb]);
+                    } else {
+                        ((kv4_lds_f32 *)sl)[(NB + bb) * KV4_PAGE + lane] = v;
                     }
-                    ((kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE))[lane] = (_Float16)(v * vdown[bb]);
-                } else {
-                    ((kv4_lds_f32 *)sl)[(NB + bb) * KV4_PAGE + lane] = v;
                 }
-            }
 
-            /* scores, without the row's factor */
-            glint_f32x4 sc[4];
-#pragma unroll
-            for (int a = 0; a < 4; ++a) {
-                glint_f32x4 c[NB];
-#pragma unroll
-                for (int bb = 0; bb < NB; ++bb) {
-                    c[bb] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        Kv4Frag f;
-#pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            f.u[x] = pair(kw[a][2 * bb + st], x);
-                        c[bb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.f, qf[bb][st].f, c[bb], 0, 0, 0);
+    #pragma unroll
+                for (int a = 0; a < 4; ++a) {
+                    glint_f32x4 c[NB];
+    #pragma unroll
+                    for (int bb = 0; bb < NB; ++bb) {
+                        c[bb] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
+    #pragma unroll
+                        for (int st = 0; st < 2; ++st) {
+                            Kv4Frag f;
+    #pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                f.u[x] = pair(kw[a][2 * bb + st], x);
+                            c[bb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.f, qf[bb][st].f, c[bb], 0, 0, 0);
+                        }
                     }
-                }
-#pragma unroll
-                for (int bb = 0; bb < NB; ++bb) {
-                    const glint_f32x4 kscale = *(const glint_f32x4 *)(sl + bb * KV4_PAGE + 16 * g + 4 * a);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        sc[a][x] = bb ? fmaf(c[bb][x], kscale[x], sc[a][x]) : c[bb][x] * kscale[x];
+    #pragma unroll
+                    for (int bb = 0; bb < NB; ++bb) {
+                        const glint_f32x4 kscale = *(const glint_f32x4 *)(sl + bb * KV4_PAGE + 16 * g + 4 * a);
+    #pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            sc[a][x] = bb ? fmaf(c[bb][x], kscale[x], sc[a][x]) : c[bb][x] * kscale[x];
+                    }
                 }
             }
             load_k();
-            const int t0 = pg * KV4_PAGE + 16 * g;
-            if (!whole) { /* what the row does not see */
-#pragma unroll
-                for (int a = 0; a < 4; ++a)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        sc[a][x] = t0 + 4 * a + x <= last ? sc[a][x] : -INFINITY;
-            }
-
-            /* softmax weights */
-            float top = -INFINITY;
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    top = fmaxf(top, sc[a][x]);
-            top = kv4_over_row(top, GlintMax()) * factor;
-            if (__any(top > m)) {
-                const float mn = fmaxf(m, top);
-                const float keep = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
-                m = mn;
-                l *= keep;
-#pragma unroll
-                for (int bb = 0; bb < NB; ++bb)
-                    carry(bb, keep);
-            }
-            const float base = m == -INFINITY ? 0.f : m;
-            float sum = 0.f;
-#pragma unroll
-            for (int a = 0; a < 4; ++a)
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], factor, -base));
-                    sum += sc[a][x];
-                }
-            l += sum;
-
-            /* times the value scales, as f16 */
-            Kv4Frag pf[NB][2];
-            if (whole) {
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    kv4_f16x8 w;
-#pragma unroll
-                    for (int x = 0; x < 8; ++x)
-                        w[x] = (_Float16)sc[2 * st + (x >> 2)][x & 3];
-#pragma unroll
-                    for (int bb = 0; bb < NB; ++bb)
-                        pf[bb][st].f =
-                            w * *(const kv4_lds_f16x8 *)((const kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE) + 16 * g + 8 * st);
-                }
-            } else {
-#pragma unroll
-                for (int bb = 0; bb < NB; ++bb) {
-                    glint_f32x4 vscale[4];
-                    float any = 0.f, finite = 0.f;
-#pragma unroll
-                    for (int a = 0; a < 4; ++a) {
-                        vscale[a] = *(const kv4_lds_f32x4 *)(sl + (NB + bb) * KV4_PAGE + 16 * g + 4 * a);
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) { /* an unseen place counts as 0, whatever it holds */
-                            const float v = t0 + 4 * a + x <= last ? vscale[a][x] : 0.f;
-                            vscale[a][x] = v;
-                            any = fmaxf(any, v);
-                            finite = fmaxf(finite, v < INFINITY ? v : 0.f);
-                        }
-                    }
-                    if (__any(any >= vlimit[bb])) { /* outside f16's range under some row's power */
-                        finite = kv4_over_row(finite, GlintMax());
-                        if (finite >= vlimit[bb])
-                            carry(bb, kv4_new_power(finite, vdown[bb], vlimit[bb]));
-                    }
-#pragma unroll
+            if (pg != KA_FAR) {
+                const int t0 = pg * KV4_PAGE + 16 * g;
+                if (!whole) { /* what the row does not see */
+    #pragma unroll
                     for (int a = 0; a < 4; ++a)
-#pragma unroll
+    #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            pf[bb][a >> 1].f[4 * (a & 1) + x] = (_Float16)(sc[a][x] * (vscale[a][x] * vdown[bb]));
+                            sc[a][x] = t0 + 4 * a + x <= last ? sc[a][x] : -INFINITY;
                 }
-            }
 
-            /* outputs */
-#pragma unroll
-            for (int p = 0; p < D / 32; ++p)
-#pragma unroll
-                for (int st = 0; st < 2; ++st) {
-                    Kv4Frag lo, hi;
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const uint32_t w = vw[p][2 * st + (x >> 1)];
-                        const uint32_t e0 = pair(w, 2 * (x & 1)), e1 = pair(w, 2 * (x & 1) + 1);
-                        lo.u[x] = __builtin_amdgcn_perm(e1, e0, 0x05040100u);
-                        hi.u[x] = __builtin_amdgcn_perm(e1, e0, 0x07060302u);
-                    }
-                    o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.f, pf[p >> 1][st].f, o[2 * p], 0, 0, 0);
-                    o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.f, pf[p >> 1][st].f, o[2 * p + 1], 0, 0, 0);
+                /* softmax weights */
+                float top = -INFINITY;
+    #pragma unroll
+                for (int a = 0; a < 4; ++a)
+    #pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        top = fmaxf(top, sc[a][x]);
+                top = kv4_over_row(top, GlintMax()) * factor;
+                if (__any(top > m)) {
+                    const float mn = fmaxf(m, top);
+                    const float keep = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
+                    m = mn;
+                    l *= keep;
+    #pragma unroll
+                    for (int bb = 0; bb < NB; ++bb)
+                        carry(bb, keep);
                 }
+                const float base = m == -INFINITY ? 0.f : m;
+                float sum = 0.f;
+    #pragma unroll
+                for (int a = 0; a < 4; ++a)
+    #pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], factor, -base));
+                        sum += sc[a][x];
+                    }
+                l += sum;
+
+                /* times the value scales, as f16 */
+                Kv4Frag pf[NB][2];
+                if (whole) {
+    #pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        kv4_f16x8 w;
+    #pragma unroll
+                        for (int x = 0; x < 8; ++x)
+                            w[x] = (_Float16)sc[2 * st + (x >> 2)][x & 3];
+    #pragma unroll
+                        for (int bb = 0; bb < NB; ++bb)
+                            pf[bb][st].f =
+                                w * *(const kv4_lds_f16x8 *)((const kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE) + 16 * g + 8 * st);
+                    }
+                } else {
+    #pragma unroll
+                    for (int bb = 0; bb < NB; ++bb) {
+                        glint_f32x4 vscale[4];
+                        float any = 0.f, finite = 0.f;
+    #pragma unroll
+                        for (int a = 0; a < 4; ++a) {
+                            vscale[a] = *(const kv4_lds_f32x4 *)(sl + (NB + bb) * KV4_PAGE + 16 * g + 4 * a);
+    #pragma unroll
+                            for (int x = 0; x < 4; ++x) { /* an unseen place counts as 0, whatever it holds */
+                                const float v = t0 + 4 * a + x <= last ? vscale[a][x] : 0.f;
+                                vscale[a][x] = v;
+                                any = fmaxf(any, v);
+                                finite = fmaxf(finite, v < INFINITY ? v : 0.f);
+                            }
+                        }
+                        if (__any(any >= vlimit[bb])) { /* outside f16's range under some row's power */
+                            finite = kv4_over_row(finite, GlintMax());
+                            if (finite >= vlimit[bb])
+                                carry(bb, kv4_new_power(finite, vdown[bb], vlimit[bb]));
+                        }
+    #pragma unroll
+                        for (int a = 0; a < 4; ++a)
+    #pragma unroll
+                            for (int x = 0; x < 4; ++x)
+                                pf[bb][a >> 1].f[4 * (a & 1) + x] = (_Float16)(sc[a][x] * (vscale[a][x] * vdown[bb]));
+                    }
+                }
+
+                /* outputs */
+    #pragma unroll
+                for (int p = 0; p < D / 32; ++p)
+    #pragma unroll
+                    for (int st = 0; st < 2; ++st) {
+                        Kv4Frag lo, hi;
+    #pragma unroll
+                        for (int x = 0; x < 4; ++x) {
+                            const uint32_t w = vw[p][2 * st + (x >> 1)];
+                            const uint32_t e0 = pair(w, 2 * (x & 1)), e1 = pair(w, 2 * (x & 1) + 1);
+                            lo.u[x] = __builtin_amdgcn_perm(e1, e0, 0x05040100u);
+                            hi.u[x] = __builtin_amdgcn_perm(e1, e0, 0x07060302u);
+                        }
+                        o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.f, pf[p >> 1][st].f, o[2 * p], 0, 0, 0);
+                        o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.f, pf[p >> 1][st].f, o[2 * p + 1], 0, 0, 0);
+                    }
+            }
             load_v();
         }
         if (more_groups)
