@@ -11,10 +11,10 @@
  *   one 64-bit key, the value's order over the inverted index, so ties need no rule.
  *   Few long rows are split over workgroups, whose sums and lists meet in the last to arrive.
  *
- *   Long rows are bound by reading them once: 2047 rows of 128256 BF16 in 117 us, 4.5 TB/s, where a
+ *   Long rows are bound by reading them once: 2047 rows of 128256 BF16 in 117 to 124 us, 4.2 to 4.5 TB/s, where a
  *   copy reaches 5.1; a second pass over them for the list would double that. Short calls are bound
  *   by one chain of a workgroup's waits: first loads, wave and workgroup sums, the floor of the
- *   list, its candidates, their order; 8 rows of 128256 18 us. 1024 threads a row keep 64 KB of
+ *   list, its candidates, their order; 8 rows of 128256 13 us. 1024 threads a row keep 64 KB of
  *   loads in flight; LP_U loads a thread and as many ahead. */
 #include <algorithm>
 
@@ -212,21 +212,27 @@ __device__ __forceinline__ int lp_place(const uint64_t *keys, int n, uint64_t ke
         place += keys[i] > key ? 1 : 0;
     return place;
 }
-/* The elements that reach `least` of every thread whose maximum does: a load per lane of its wave,
- * 64 rounds at most (V <= LP_V_TOP). */
+/* The elements that reach `least` of every thread whose maximum does: the wave's lanes share those
+ * threads' loads out, `rounds` of each thread. */
 template <class E>
-__device__ __forceinline__ void lp_candidates(const LpRow<E> &r, int v0, int nvec, const int64_t (&ends)[2], uint64_t mine,
-                                              uint64_t least, uint64_t *cand, int *ncand) {
+__device__ __forceinline__ void lp_candidates(const LpRow<E> &r, int v0, int nvec, int rounds, const int64_t (&ends)[2],
+                                              uint64_t mine, uint64_t least, uint64_t *cand, int *ncand) {
     constexpr int PER = LpRow<E>::PER;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (uint64_t who = __ballot(mine != 0 && mine >= least); who; who &= who - 1) {
-        const int vec = wave * 64 + __builtin_ctzll(who) + lane * LP_T;
-        if (vec < nvec) {
+    const bool has = mine != 0 && mine >= least;
+    const uint64_t who = __ballot(has), below = who & ((1ull << lane) - 1);
+    const int n = __builtin_popcountll(who), rank = __builtin_popcountll(below);
+    /* lane i < n gets the i-th such thread's lane: every lane sends its own to a place of its own */
+    const int order = __builtin_amdgcn_ds_permute(4 * (has ? rank : n + lane - rank), lane);
+    for (int i0 = 0; i0 < n * rounds; i0 += 64) {
+        const int i = i0 + lane, k = i % rounds;
+        const int vec = wave * 64 + __shfl(order, min(i / rounds, 63), 64) + k * LP_T;
+        if (i < n * rounds && vec < nvec) {
             float w[PER];
             r.unpack(r.raw(v0 + vec), w);
 #pragma unroll
-            for (int i = 0; i < PER; ++i) {
-                const uint64_t key = lp_key(w[i], r.head + (int64_t)(v0 + vec) * PER + i);
+            for (int x = 0; x < PER; ++x) {
+                const uint64_t key = lp_key(w[x], r.head + (int64_t)(v0 + vec) * PER + x);
                 if (key >= least)
                     cand[atomicAdd(ncand, 1)] = key;
             }
@@ -255,7 +261,7 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
     constexpr int PER = LpRow<E>::PER;
     __shared__ float sm[LP_WAVES], ss[LP_WAVES], st[LP_WAVES];
     __shared__ int sr[LP_WAVES];
-    __shared__ uint32_t wave_reach[LP_WAVES];
+    __shared__ uint32_t wave_second[LP_WAVES];
     __shared__ uint64_t cand[LP_CAND];
     __shared__ uint64_t floor_key;
     __shared__ int ncand;
@@ -371,17 +377,15 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         st[wave] = wt;
         sr[wave] = wr;
     }
-    /* The top-th largest thread maximum: the largest value that `top` lanes of one wave reach is
-     * below it in no wave, so the maxima that reach the waves' largest such value hold it; each of
-     * them counts those before it. */
+    /* A value that the top-th largest thread maximum is not below: two lanes of a wave reach the
+     * second largest of its maxima, so where ceil(top / 2) waves reach a value by theirs, `top` lanes
+     * do. The maxima that reach it, some 30 for a list of 20, count those before each of them. */
     if (top > 0) {
-        const uint32_t value = (uint32_t)(mine >> 32);
-        uint32_t reach = 0; /* bit by bit */
-        for (uint32_t bit = 0x80000000u; bit; bit >>= 1)
-            if (__builtin_popcountll(__ballot(value >= (reach | bit))) >= top)
-                reach |= bit;
+        const uint32_t value = (uint32_t)(mine >> 32), first = lp_wave_max32(value);
+        const bool is_first = value == first;
+        const uint32_t second = lp_wave_max32(is_first ? 0u : value);
         if (lane == 0)
-            wave_reach[wave] = reach;
+            wave_second[wave] = __builtin_popcountll(__ballot(is_first)) > 1 ? first : second;
     }
     if (threadIdx.x == 0) {
         ncand = 0;
@@ -399,10 +403,15 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
             whole = LpPart{z, n};
     }
     if (top > 0) {
-        uint32_t reach = wave_reach[0];
+        const uint32_t own = wave_second[lane & 15];
+        int ahead = 0; /* waves */
 #pragma unroll
-        for (int i = 1; i < LP_WAVES; ++i)
-            reach = max(reach, wave_reach[i]);
+        for (int i = 0; i < LP_WAVES; ++i) {
+            const uint32_t v = wave_second[i];
+            ahead += v > own || (v == own && i < (lane & 15)) ? 1 : 0;
+        }
+        const uint64_t who = __ballot(ahead == (top - 1) / 2);
+        const uint32_t reach = (uint32_t)__builtin_amdgcn_readlane((int)own, __builtin_ctzll(who));
         if (mine != 0 && (uint32_t)(mine >> 32) >= reach)
             cand[atomicAdd(&ncand, 1)] = mine;
         __syncthreads();
@@ -411,16 +420,18 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
             if (lp_place(cand, n, cand[c]) == top - 1)
                 floor_key = cand[c];
         __syncthreads();
-        if (threadIdx.x == 0)
-            ncand = 0;
+        if (threadIdx.x == 0) { /* a list of one is that maximum */
+            cand[0] = floor_key;
+            ncand = top == 1 && floor_key != 0 ? 1 : 0;
+        }
     }
     __syncthreads();
     if (nsplit == 1 && wave == 0)
         lp_write(whole, tok, is_tok, xt, lane == 0, logprob + row, entropy ? entropy + row : nullptr, rank ? rank + row : nullptr,
                  s_ref, s_ls);
-    if (top > 0) {
+    if (top > 1) {
         const uint64_t least = floor_key;
-        lp_candidates(r, v0, nvec, ends, mine, least, cand, &ncand);
+        lp_candidates(r, v0, nvec, rounds, ends, mine, least, cand, &ncand);
     }
     __syncthreads();
     if (nsplit > 1) {
@@ -517,7 +528,7 @@ GLINT_API int glint_token_logprobs(const void *logits, int elt, int64_t stride, 
         return 0;
     /* Few rows are split, so that a workgroup per CU shares the reading, none with less than two loads
      * of every thread (as good as one, and fewer parts to join). Rows of 128256 BF16, split against
-     * whole, by kernel: 8 rows with a list of 20 18.2 and 24.7 us, 64 without a list 10.6 and 17.8. */
+     * whole, by kernel: 8 rows with a list of 20 13.4 and 21.0 us, 64 without a list 10.0 and 18.0. */
     const int64_t parts = V / (elt == GLINT_KV_BF16 ? 8 : 4) / (2 * LP_T);
     int nsplit = (int)std::min<int64_t>(std::min<int64_t>(LP_SPLIT, parts), glint_cu_count() / T);
     GlintSplitWs ws{nullptr, nullptr, 0, 0};
