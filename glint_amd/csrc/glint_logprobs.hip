@@ -11,8 +11,8 @@
  *   one 64-bit key, the value's order over the inverted index, so ties need no rule.
  *   Few long rows are split over workgroups, whose sums and lists meet in the last to arrive.
  *
- *   Long rows are bound by reading them once: 2047 rows of 128256 BF16 in 117 to 124 us, 4.2 to 4.5 TB/s, where a
- *   copy reaches 5.1; a second pass over them for the list would double that. Short calls are bound
+ *   Long rows are bound by reading them once: 2047 rows of 128256 BF16 in 115 us, 4.6 TB/s, where a copy
+ *   reaches 5.1, the vector units busy for 0.7 of it; a second pass for the list would double that. Short calls are bound
  *   by one chain of a workgroup's waits: first loads, wave and workgroup sums, the floor of the
  *   list, its candidates, their order; 8 rows of 128256 13 us. 1024 threads a row keep 64 KB of
  *   loads in flight; LP_U loads a thread and as many ahead. */
@@ -319,10 +319,15 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         }
         const int64_t j = r.head + (int64_t)vec * PER;
         const float reach = j < tok ? xt : xt_up;
-        if (__any(mx >= reach || (j < tok && tok < j + PER))) {
+        if (__any(mx >= reach)) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                before += w[i] >= (j + i < tok ? xt : xt_up) ? 1 : 0;
+                before += w[i] >= reach ? 1 : 0;
+            if (__any(j < tok && tok < j + PER)) { /* the token's own load: entries from it on that equal it */
+#pragma unroll
+                for (int i = 0; i < PER; ++i)
+                    before -= j < tok && j + i >= tok && w[i] == xt ? 1 : 0;
+            }
         }
         const bool more = mx > high || where < 0;
         high = fmaxf(high, mx);
