@@ -7,9 +7,11 @@
  *   elements a lane; 8 tokens of 8 heads in 3.5 us.
  * k_kv4_gather — a thread reads one byte of a key row (two adjacent dimensions) or of a value
  *   column (dimensions 16 apart) and writes its two BF16; 8 tokens in 2.8 us.
- * k_kv4_append_tile, k_kv4_gather_tile — 64 tokens of one head a workgroup, for prompts: without
+ * k_kv4_append_tile, k_kv4_gather_tile — 32 tokens of one head a workgroup, for prompts: without
  *   them a value's bytes are written and read one by one, 64 B apart. 4096 tokens of 8 heads of
- *   128: append 12.2 us (1.8 TB/s; 24 element-wise), gather 14.3 us (1.5 TB/s; 18). */
+ *   128: append 11.1 us (1.9 TB/s; 23 element-wise), gather 10.9 us (2.0 TB/s; 17). Each is a chain
+ *   of loads, LDS and stores, so the waves that a CU holds count: tiles of 64 tokens, half as many
+ *   workgroups, took 12.0 and 14.2. */
 #include "kv4.h"
 
 #define KV4_T 256
@@ -141,11 +143,11 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_gather(const int64_t *__restrict_
 }
 
 /* ------------------------------------------------------------------ tiles
- * 64 tokens of one head a workgroup. A value column lies a byte a token, 64 B apart, so values
+ * 32 tokens of one head a workgroup. A value column lies a byte a token, 64 B apart, so values
  * pass through LDS: columns there are shifted by the first token's place modulo 4, so that four
  * tokens whose slots follow each other, as a prompt's do, are one aligned word on both sides;
  * other tokens go byte by byte. */
-#define KT_TOKENS 64
+#define KT_TOKENS 32
 #define KT_COLS (KT_TOKENS + 4) /* the shift */
 #define KT_GROUPS (KT_COLS / 4)
 
@@ -341,16 +343,16 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_gather_tile(const int64_t *__rest
     }
 }
 
-/* When tiles are taken. A workgroup of them runs 7 to 10 us however little it has, so they want the
- * device's workgroups, and half their tokens. us, BF16, 128 dimensions, element-wise against tiles:
- *   tokens x heads   1024 x 8      1250 x 8      1536 x 8       2048 x 8       4096 x 8
- *   append           8.6, 9.7      9.8, 10.0     11.4, 10.1     14.5, 10.4     23.6, 12.2
- *   gather           6.6, 10.6     7.3, 11.1     8.5, 10.0      10.4, 10.3     18.0, 14.3
- *   tokens x heads   16 x 1024     32 x 512
- *   append           13.4, 15.2    12.9, 11.1 */
-#define KV4_TILE_APPEND 10240 /* tokens of one head */
-#define KV4_TILE_GATHER 16384
-#define KV4_TILE_T 32
+/* When tiles are taken. A workgroup of them runs 5 to 7 us however little it has, so they want most of
+ * the device's workgroups, and half their tokens. us, BF16, 128 dimensions, element-wise against tiles:
+ *   tokens x heads   700 x 8      850 x 8      1250 x 8     1536 x 8     2048 x 8      4096 x 8
+ *   append           6.7, 7.0     7.4, 7.0     9.8, 7.5     11.0, 7.7    13.7, 8.1     23.3, 11.1
+ *   gather           5.4, 7.5     5.9, 7.3     7.4, 8.2     8.4, 7.5     10.5, 7.8     17.4, 10.9
+ *   tokens x heads   16 x 512     16 x 1024
+ *   append           7.8, 7.5     12.6, 9.9 */
+#define KV4_TILE_APPEND 6144 /* tokens of one head */
+#define KV4_TILE_GATHER 10240
+#define KV4_TILE_T 16
 static bool kv4_tiles(int64_t T, int H, int64_t from) { return T >= KV4_TILE_T && T * H >= from; }
 
 /* Workgroups of KV4_T threads for n threads' work, or 0 where a grid cannot hold them. */
