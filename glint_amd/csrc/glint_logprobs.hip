@@ -11,11 +11,12 @@
  *   one 64-bit key, the value's order over the inverted index, so ties need no rule.
  *   Few long rows are split over workgroups, whose sums and lists meet in the last to arrive.
  *
- *   Long rows are bound by reading them once: 2047 rows of 128256 BF16 in 115 us, 4.6 TB/s, where a copy
- *   reaches 5.1, the vector units busy for 0.7 of it; a second pass for the list would double that. Short calls are bound
- *   by one chain of a workgroup's waits: first loads, wave and workgroup sums, the floor of the
- *   list, its candidates, their order; 8 rows of 128256 13 us. 1024 threads a row keep 64 KB of
- *   loads in flight; LP_U loads a thread and as many ahead. */
+ *   Long rows are bound by reading them once and, close behind, by some 13 vector instructions an
+ *   element: 2047 rows of 128256 BF16 in 111 us, 4.7 TB/s, where a copy reaches 5.1, the vector units
+ *   86% busy; a second pass for the list would add to both. Short calls are bound by one chain of a
+ *   workgroup's waits: first loads, wave and workgroup sums, the floor of the list, its
+ *   candidates, their order; 8 rows of 128256 13 us. 1024 threads a row keep 64 KB of loads in
+ *   flight; LP_U loads a thread and as many ahead. */
 #include <algorithm>
 
 #include "glint_common.h"
@@ -293,9 +294,11 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
     const float xt_up = lp_next_up(xt);
 
     LpSum a{-INFINITY, 0.f, 0.f};
-    int before = 0;
+    int before = 0;      /* this lane's ends */
+    int wave_before = 0; /* the wave's loads, by ballots: every lane takes part in every round */
     float high = -INFINITY;
-    int where = -1;
+    int where = (int)threadIdx.x < nvec ? v0 + (int)threadIdx.x : -1;
+    const uint32_t at = is_tok ? (uint32_t)tok : 0;
     auto take = [&](int vec, const glint_u32x4 raw) {
         float w[PER];
         r.unpack(raw, w);
@@ -317,30 +320,36 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
             for (int i = 0; i < PER; ++i)
                 a.s += w[i] != w[i] ? NAN : 0.f;
         }
-        const int64_t j = r.head + (int64_t)vec * PER;
-        const float reach = j < tok ? xt : xt_up;
+        const uint32_t j = (uint32_t)r.head + (uint32_t)vec * PER; /* V fits 31 bits */
+        const float reach = j < at ? xt : xt_up;
         if (__any(mx >= reach)) {
 #pragma unroll
             for (int i = 0; i < PER; ++i)
-                before += w[i] >= reach ? 1 : 0;
-            if (__any(j < tok && tok < j + PER)) { /* the token's own load: entries from it on that equal it */
+                wave_before += __builtin_popcountll(__ballot(w[i] >= reach));
+            if (__any(j < at && at < j + PER)) { /* the token's own load: entries from it on that equal it */
 #pragma unroll
                 for (int i = 0; i < PER; ++i)
-                    before -= j < tok && j + i >= tok && w[i] == xt ? 1 : 0;
+                    wave_before -= __builtin_popcountll(__ballot(j < at && j + i >= at && w[i] == xt));
             }
         }
-        const bool more = mx > high || where < 0;
+        where = mx > high ? vec : where;
         high = fmaxf(high, mx);
-        where = more ? vec : where;
     };
+    constexpr uint32_t NONE = sizeof(E) == 2 ? 0xFF80FF80u : 0xFF800000u; /* -inf adds nothing and comes before nothing */
     for (int k0 = 0; k0 < rounds; k0 += LP_U) {
         if (k0 + LP_U < rounds)
             fetch(k0 + LP_U, next);
 #pragma unroll
         for (int u = 0; u < LP_U; ++u) {
+            if (k0 + u >= rounds)
+                break;
             const int vec = (int)threadIdx.x + (k0 + u) * LP_T;
-            if (vec < nvec)
-                take(v0 + vec, now[u]);
+            if ((k0 + u + 1) * LP_T > nvec) { /* the last round */
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    now[u][i] = vec < nvec ? now[u][i] : NONE;
+            }
+            take(v0 + vec, now[u]);
         }
 #pragma unroll
         for (int u = 0; u < LP_U; ++u)
@@ -375,7 +384,7 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
     const float wm = lp_wave(a.m, LpMax());
     lp_refer(a, wm);
     const float ws = lp_wave(a.s, LpAdd()), wt = lp_wave(a.t, LpAdd());
-    const int wr = lp_wave_sum(before);
+    const int wr = lp_wave_sum(before) + wave_before;
     if (lane == 0) {
         sm[wave] = wm;
         ss[wave] = ws;
