@@ -12,10 +12,10 @@
  *   matrix instruction's operand; what few large weights lose is added back) and the output.
  *
  *   What bounds it: 4 D operations a row and key on the matrix units and, beside them, some 12
- *   vector operations for a score. 8192 tokens, 32 heads of 128 over 8: 550 GFLOP in 552 us, 1.0
+ *   vector operations for a score. 8192 tokens, 32 heads of 128 over 8: 550 GFLOP in 535 to 572 us, 1.0
  *   PFLOP/s, where an 8192^3 product of the library reaches 1.2; of 64 dimensions, where a score's
  *   vector work is twice a product's share, 310 us. Four waves of 32 rows, two workgroups a CU
- *   (D = 128: 202 registers, 66 KB of LDS), so that one wave's exponentials run under
+ *   (D = 128: 200 registers, 66 KB of LDS), so that one wave's exponentials run under
  *   another's products; loads a tile ahead, by the direct path to LDS, which needs no registers. A
  *   short prompt is bound by its longest row's tiles, one after another: 77 tokens 10 us. */
 #include <cfloat>

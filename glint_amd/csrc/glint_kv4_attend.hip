@@ -28,7 +28,7 @@
  *   seen, so that they stay inside f16's range whatever the scales' size.
  *
  *   What bounds it: reading the cache once, 4.5 bits an element. 32 sequences of 8192 tokens, 8 heads
- *   of 128, 4 rows a head: 303 MB in 66 us, 4.6 TB/s, where a copy reaches 5.1. Decoding codes in
+ *   of 128, 4 rows a head: 303 MB in 66 to 71 us, 4.3 to 4.6 TB/s, where a copy reaches 5.1. Decoding codes in
  *   LDS, its two products and 2^x hide behind that up to 16 rows a page, which is why a group
  *   has 16 (32 rows in registers spilled: 4 sequences of 8000 with 40 rows a head 57 us at best
  *   against 40). 8 waves share a table: 4 waves a workgroup were slower everywhere, by the
