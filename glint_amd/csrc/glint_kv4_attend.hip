@@ -327,6 +327,19 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         X.n = min(X.s.rounds - X.begin, run - X.k);
     };
     place(G);
+    /* The lane's rows of q. */
+    glint_u32x4 qw[NB][2];
+    auto load_q = [&](const Kv4Group &X) {
+        const int r = X.rb * KA_ROWS + col;
+        const bool live = r < X.s.rows;
+        const uint16_t *qr = A.q + (int64_t)(X.s.q0 + (live ? r / A.G : 0)) * A.q_st + (X.h * A.G + (live ? r % A.G : 0)) * A.q_sh;
+#pragma unroll
+        for (int bb = 0; bb < NB; ++bb)
+#pragma unroll
+            for (int st = 0; st < 2; ++st)
+                qw[bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
+    };
+    load_q(G); /* on its way while the pages are found */
     /* This wave's pages of the run's next rounds, from group X's first on, one a lane: as many as the
      * chunk's sequences hold, 64 at most. A page that is not there, past the sequence's end or not in
      * the pool, is read as the pool's first page and seen by nobody: its lane holds -1. */
@@ -336,10 +349,13 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             to_chunk(b);
         const int all = lane >= b - chunk ? kv4_seq(A, raw).all : 0;
         const int sum = scan(all) - at; /* rounds from here to the lane's sequence's end */
-        int j = 0;                        /* the lane whose sequence holds this lane's round */
+        int j = b - chunk;                /* the lane whose sequence holds this lane's round */
+        if (run - k > __builtin_amdgcn_readlane(sum, j)) {
+            j = 0;
 #pragma unroll
-        for (int step = 32; step; step >>= 1)
-            j += __shfl(sum, j + step - 1, 64) <= lane ? step : 0;
+            for (int step = 32; step; step >>= 1)
+                j += __shfl(sum, j + step - 1, 64) <= lane ? step : 0;
+        }
         /* every lane reads the others before any condition on its own */
         const int sum_j = __shfl(sum, j, 64);
         const Kv4Raw r{0, __shfl(raw.nq, j, 64), __shfl(raw.len, j, 64)};
@@ -360,18 +376,6 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     };
     float *sl = scales + wave * (2 * NB * KV4_PAGE);
 
-    /* The lane's rows of q. */
-    glint_u32x4 qw[NB][2];
-    auto load_q = [&](const Kv4Group &X) {
-        const int r = X.rb * KA_ROWS + col;
-        const bool live = r < X.s.rows;
-        const uint16_t *qr = A.q + (int64_t)(X.s.q0 + (live ? r / A.G : 0)) * A.q_st + (X.h * A.G + (live ? r % A.G : 0)) * A.q_sh;
-#pragma unroll
-        for (int bb = 0; bb < NB; ++bb)
-#pragma unroll
-            for (int st = 0; st < 2; ++st)
-                qw[bb][st] = *(const glint_u32x4 *)(qr + bb * 64 + 16 * g + 8 * st);
-    };
     /* A page's loads: this lane's 16-B pieces of the key rows and value columns, and one token's
      * scales, which go to the other lanes through LDS. `ph` is the page's place times the heads. */
     uint32_t kw[4][2 * NB];
@@ -402,7 +406,6 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         ph = (int64_t)max(pid, 0) * A.H + h;
         return pid >= 0;
     };
-    load_q(G);
     __syncthreads(); /* the table is written */
     bool there = page(0, G.h);
     load_k();
