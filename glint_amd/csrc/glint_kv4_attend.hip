@@ -485,7 +485,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
             glint_f32x4 sc[4]; /* scores, without the row's factor */
             if (pg != KA_FAR) {
-    #pragma unroll
+#pragma unroll
                 for (int bb = 0; bb < NB; ++bb) {
                     sl[bb * KV4_PAGE + lane] = sw[bb];
                     const float v = sw[NB + bb];
@@ -501,25 +501,30 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                     }
                 }
 
-    #pragma unroll
-                for (int a = 0; a < 4; ++a) {
-                    glint_f32x4 c[NB];
-    #pragma unroll
-                    for (int bb = 0; bb < NB; ++bb) {
+                constexpr int STEPS = 2 * NB; /* products of a score */
+                uint32_t e[2][4];
+                auto entries = [&](int n) {
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        e[n & 1][x] = pair(kw[n / STEPS][n % STEPS], x);
+                };
+                entries(0);
+                glint_f32x4 c[NB];
+#pragma unroll
+                for (int n = 0; n < 4 * STEPS; ++n) {
+                    const int a = n / STEPS, bb = n % STEPS >> 1, st = n & 1;
+                    if (n + 1 < 4 * STEPS)
+                        entries(n + 1);
+                    Kv4Frag f;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        f.u[x] = e[n & 1][x];
+                    if (st == 0)
                         c[bb] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
-    #pragma unroll
-                        for (int st = 0; st < 2; ++st) {
-                            Kv4Frag f;
-    #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                f.u[x] = pair(kw[a][2 * bb + st], x);
-                            c[bb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.f, qf[bb][st].f, c[bb], 0, 0, 0);
-                        }
-                    }
-    #pragma unroll
-                    for (int bb = 0; bb < NB; ++bb) {
+                    c[bb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f.f, qf[bb][st].f, c[bb], 0, 0, 0);
+                    if (st == 1) {
                         const glint_f32x4 kscale = *(const glint_f32x4 *)(sl + bb * KV4_PAGE + 16 * g + 4 * a);
-    #pragma unroll
+#pragma unroll
                         for (int x = 0; x < 4; ++x)
                             sc[a][x] = bb ? fmaf(c[bb][x], kscale[x], sc[a][x]) : c[bb][x] * kscale[x];
                     }
@@ -529,18 +534,18 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             if (pg != KA_FAR) {
                 const int t0 = pg * KV4_PAGE + 16 * g;
                 if (!whole) { /* what the row does not see */
-    #pragma unroll
+#pragma unroll
                     for (int a = 0; a < 4; ++a)
-    #pragma unroll
+#pragma unroll
                         for (int x = 0; x < 4; ++x)
                             sc[a][x] = t0 + 4 * a + x <= last ? sc[a][x] : -INFINITY;
                 }
 
                 /* softmax weights */
                 float top = -INFINITY;
-    #pragma unroll
+#pragma unroll
                 for (int a = 0; a < 4; ++a)
-    #pragma unroll
+#pragma unroll
                     for (int x = 0; x < 4; ++x)
                         top = fmaxf(top, sc[a][x]);
                 top = kv4_over_row(top, GlintMax()) * factor;
@@ -549,15 +554,15 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                     const float keep = __builtin_amdgcn_exp2f(m - (mn == -INFINITY ? 0.f : mn));
                     m = mn;
                     l *= keep;
-    #pragma unroll
+#pragma unroll
                     for (int bb = 0; bb < NB; ++bb)
                         carry(bb, keep);
                 }
                 const float base = m == -INFINITY ? 0.f : m;
                 float sum = 0.f;
-    #pragma unroll
+#pragma unroll
                 for (int a = 0; a < 4; ++a)
-    #pragma unroll
+#pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], factor, -base));
                         sum += sc[a][x];
@@ -567,26 +572,26 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                 /* times the value scales, as f16 */
                 Kv4Frag pf[NB][2];
                 if (whole) {
-    #pragma unroll
+#pragma unroll
                     for (int st = 0; st < 2; ++st) {
                         kv4_f16x8 w;
-    #pragma unroll
+#pragma unroll
                         for (int x = 0; x < 8; ++x)
                             w[x] = (_Float16)sc[2 * st + (x >> 2)][x & 3];
-    #pragma unroll
+#pragma unroll
                         for (int bb = 0; bb < NB; ++bb)
                             pf[bb][st].f =
                                 w * *(const kv4_lds_f16x8 *)((const kv4_lds_f16 *)(sl + (NB + bb) * KV4_PAGE) + 16 * g + 8 * st);
                     }
                 } else {
-    #pragma unroll
+#pragma unroll
                     for (int bb = 0; bb < NB; ++bb) {
                         glint_f32x4 vscale[4];
                         float any = 0.f, finite = 0.f;
-    #pragma unroll
+#pragma unroll
                         for (int a = 0; a < 4; ++a) {
                             vscale[a] = *(const kv4_lds_f32x4 *)(sl + (NB + bb) * KV4_PAGE + 16 * g + 4 * a);
-    #pragma unroll
+#pragma unroll
                             for (int x = 0; x < 4; ++x) { /* an unseen place counts as 0, whatever it holds */
                                 const float v = t0 + 4 * a + x <= last ? vscale[a][x] : 0.f;
                                 vscale[a][x] = v;
@@ -599,30 +604,36 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                             if (finite >= vlimit[bb])
                                 carry(bb, kv4_new_power(finite, vdown[bb], vlimit[bb]));
                         }
-    #pragma unroll
+#pragma unroll
                         for (int a = 0; a < 4; ++a)
-    #pragma unroll
+#pragma unroll
                             for (int x = 0; x < 4; ++x)
                                 pf[bb][a >> 1].f[4 * (a & 1) + x] = (_Float16)(sc[a][x] * (vscale[a][x] * vdown[bb]));
                     }
                 }
 
-                /* outputs */
-    #pragma unroll
-                for (int p = 0; p < D / 32; ++p)
-    #pragma unroll
-                    for (int st = 0; st < 2; ++st) {
-                        Kv4Frag lo, hi;
-    #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t w = vw[p][2 * st + (x >> 1)];
-                            const uint32_t e0 = pair(w, 2 * (x & 1)), e1 = pair(w, 2 * (x & 1) + 1);
-                            lo.u[x] = __builtin_amdgcn_perm(e1, e0, 0x05040100u);
-                            hi.u[x] = __builtin_amdgcn_perm(e1, e0, 0x07060302u);
-                        }
-                        o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.f, pf[p >> 1][st].f, o[2 * p], 0, 0, 0);
-                        o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.f, pf[p >> 1][st].f, o[2 * p + 1], 0, 0, 0);
+                    /* outputs: a product's table entries are read while the one before is multiplied */
+                uint32_t e[2][8];
+                auto entries = [&](int n) {
+#pragma unroll
+                    for (int x = 0; x < 8; ++x)
+                        e[n & 1][x] = pair(vw[n >> 1][2 * (n & 1) + (x >> 2)], x & 3);
+                };
+                entries(0);
+#pragma unroll
+                for (int n = 0; n < D / 16; ++n) {
+                    const int p = n >> 1, st = n & 1;
+                    if (n + 1 < D / 16)
+                        entries(n + 1);
+                    Kv4Frag lo, hi;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        lo.u[x] = __builtin_amdgcn_perm(e[n & 1][2 * x + 1], e[n & 1][2 * x], 0x05040100u);
+                        hi.u[x] = __builtin_amdgcn_perm(e[n & 1][2 * x + 1], e[n & 1][2 * x], 0x07060302u);
                     }
+                    o[2 * p] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lo.f, pf[p >> 1][st].f, o[2 * p], 0, 0, 0);
+                    o[2 * p + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(hi.f, pf[p >> 1][st].f, o[2 * p + 1], 0, 0, 0);
+                }
             }
             load_v();
         }
