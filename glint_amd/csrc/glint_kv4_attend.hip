@@ -28,13 +28,14 @@
  *   seen, so that they stay inside f16's range whatever the scales' size.
  *
  *   What bounds it: reading the cache once, 4.5 bits an element. 32 sequences of 8192 tokens, 8 heads
- *   of 128, 4 rows a head: 303 MB in 66 to 71 us, 4.3 to 4.6 TB/s, where a copy reaches 5.1. Decoding codes in
- *   LDS, its two products and 2^x hide behind that up to 16 rows a page, which is why a group
- *   has 16 (32 rows in registers spilled: 4 sequences of 8000 with 40 rows a head 57 us at best
- *   against 40). 8 waves share a table: 4 waves a workgroup were slower everywhere, by the
- *   table's filling. Short calls are bound by their start, some 7 us from the launch to the first
- *   page's scores: lengths, runs, table and page numbers one after another, then the pages; one
- *   sequence of 1000 tokens takes 13.8 us. */
+ *   of 128, 4 rows a head: 303 MB in 62 to 69 us, 4.4 to 4.9 TB/s, where a copy reaches 5.1. Decoding
+ *   codes in LDS, its two products and 2^x take some 700 vector instructions a page and hide behind
+ *   that up to 16 rows a page, which is why a group has 16 (32 rows in registers spilled: 4 sequences of
+ *   8000 with 40 rows a head 57 us at best, 38 now). A product's table entries are read while the one
+ *   before is multiplied (equal lengths 65 without, 62 with; ragged ones 42.5, 39). 8 waves share a
+ *   table: 4 waves a workgroup were slower everywhere, by the table's filling. Short calls are bound
+ *   by their start, some 5 us from the launch to the first page's loads: lengths, runs, table and
+ *   page numbers one after another; one sequence of 1000 tokens takes 12.8 us. */
 #include <algorithm>
 #include <cfloat>
 #include <cmath>
@@ -54,8 +55,9 @@ typedef glint_f32x4 kv4_lds_f32x4 __attribute__((may_alias));
 #define KA_T (64 * KA_WAVES)
 #define KA_ROWS 16 /* of q in a group */
 /* What turning to a group costs, in pages: its queries, its meeting in LDS, a join. Time at 0, 8, 16: 48
- * sequences of 1 to 4097 tokens and 10 heads 54, 43, 43 us; 64 of 1 to 2000, 8 heads of one query head
- * each, 39, 33, 35; 16 of 1 to 3001 with 4 new tokens 18, 14, 15; equal lengths 67 whatever it is. */
+ * sequences of 1 to 4097 tokens and 10 heads 50, 39, 39 us; 64 of 1 to 2000, 8 heads of one query head
+ * each, 35, 30, 32; 16 of 1 to 3001 with 4 new tokens 18, 14, 15; 4 of 8000 with 40 rows a head 38, 38,
+ * 34; 32 equal lengths 65 whatever it is. */
 #define KA_SWITCH 8
 #define KA_COPIES 32 /* of an entry; entries are 64 words apart, so that an address is one byte permute */
 #define KA_TABLE_WORDS (256 * 64)
