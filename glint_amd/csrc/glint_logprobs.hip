@@ -320,7 +320,7 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
             for (int i = 0; i < PER; ++i)
                 a.s += w[i] != w[i] ? NAN : 0.f;
         }
-        const uint32_t j = (uint32_t)r.head + (uint32_t)vec * PER; /* V fits 31 bits */
+        const uint32_t j = (uint32_t)r.head + (uint32_t)vec * PER; /* V fits 31 bits; vec = -1: past every token */
         const float reach = j < at ? xt : xt_up;
         if (__any(mx >= reach)) {
 #pragma unroll
@@ -335,7 +335,8 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         where = mx > high ? vec : where;
         high = fmaxf(high, mx);
     };
-    constexpr uint32_t NONE = sizeof(E) == 2 ? 0xFF80FF80u : 0xFF800000u; /* -inf adds nothing and comes before nothing */
+    /* past the last load: -inf adds nothing, and at vec = -1 comes before no token, not even one at -inf */
+    constexpr uint32_t NONE = sizeof(E) == 2 ? 0xFF80FF80u : 0xFF800000u;
     for (int k0 = 0; k0 < rounds; k0 += LP_U) {
         if (k0 + LP_U < rounds)
             fetch(k0 + LP_U, next);
@@ -343,13 +344,15 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         for (int u = 0; u < LP_U; ++u) {
             if (k0 + u >= rounds)
                 break;
-            const int vec = (int)threadIdx.x + (k0 + u) * LP_T;
+            int vec = v0 + (int)threadIdx.x + (k0 + u) * LP_T;
             if ((k0 + u + 1) * LP_T > nvec) { /* the last round */
+                const bool in = vec < v0 + nvec;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    now[u][i] = vec < nvec ? now[u][i] : NONE;
+                    now[u][i] = in ? now[u][i] : NONE;
+                vec = in ? vec : -1;
             }
-            take(v0 + vec, now[u]);
+            take(vec, now[u]);
         }
 #pragma unroll
         for (int u = 0; u < LP_U; ++u)
