@@ -1,9 +1,11 @@
 /* Log probabilities of given tokens (include/glint_serve.h).
  *
  * k_token_logprobs — one workgroup per row, one pass: a thread keeps a running maximum m,
- *   s = sum 2^(u - m) and t = sum 2^(u - m) (u - m) of its elements' u = x log2 e, counts those
- *   that come before the token, and remembers the 16-B load that held its largest element. Then
- *     lse = ln 2 (m + log2 s),  entropy = ln 2 (log2 s - t / s).
+ *   s = sum e^(x - m) and t = sum e^(x - m) (x - m) of its elements x, counts those that come
+ *   before the token, and remembers the 16-B load that held its largest element. Then
+ *     lse = m + ln s,  entropy = ln s - t / s.
+ *   m is subtracted before the factor log2 e of the hardware's 2^x is applied: x log2 e
+ *   overflows for the largest finite logits, which masks are made of.
  *   The top list needs no second pass over the row: with T the top-th largest of the threads'
  *   own maxima, every entry of the list is at least T and sits in one of the `top` threads
  *   whose maximum is at least T, so those threads look at their elements again and put
@@ -93,25 +95,26 @@ __device__ __forceinline__ float lp_next_up(float x) {
     return y != y ? y : __int_as_float(i >= 0 ? i + 1 : i - 1);
 }
 
-/* Running sums of a set of elements, in powers of two: with u = x log2 e and a reference m (not
- * below any u by more than LP_SLACK), s = sum 2^(u - m), t = sum 2^(u - m) (u - m). */
+/* Running sums of a set of elements: with a reference m (not below any x by more than LP_SLACK),
+ * s = sum e^(x - m), t = sum e^(x - m) (x - m). */
 #define LP_LOG2E 1.44269504088896341f
-#define LP_LN2 0.69314718055994531f
-#define LP_SLACK 20.f
+#define LP_SLACK 14.f
+#define LP_FAR -1024.f /* e to this is 0, and a sum times it is finite: 0 times what lies farther counts 0 */
+__device__ __forceinline__ float lp_exp(float d) { return __builtin_amdgcn_exp2f(d * LP_LOG2E); }
 struct LpSum {
     float m, s, t;
     __device__ void shift(float to) { /* to > m */
         if (m != -INFINITY) {
-            const float d = m - to, f = __builtin_amdgcn_exp2f(d);
+            const float d = fmaxf(m - to, LP_FAR), f = lp_exp(d);
             t = f * fmaf(d, s, t);
             s = f * s;
         }
         m = to;
     }
     __device__ void add(float x) { /* m is finite, or x makes s NaN */
-        const float d = fmaf(x, LP_LOG2E, -m), e = __builtin_amdgcn_exp2f(d);
+        const float d = x - m, e = lp_exp(d);
         s += e;
-        t = fmaf(e, fmaxf(d, -1024.f), t); /* 0 times -inf counts 0 */
+        t = fmaf(e, fmaxf(d, LP_FAR), t);
     }
 };
 /* Over each row of 16 lanes, left in every lane of the row. */
@@ -151,7 +154,7 @@ struct LpAdd {
 };
 /* The sums under another reference `to` >= m; nothing but NaN is left of a set without one. */
 __device__ __forceinline__ void lp_refer(LpSum &a, float to) {
-    const float d = a.m - to, f = a.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(d);
+    const float d = fmaxf(a.m - to, LP_FAR), f = a.m == -INFINITY ? 0.f : lp_exp(d);
     a.t = a.m == -INFINITY ? 0.f : f * fmaf(d, a.s, a.t);
     a.s = a.m == -INFINITY && a.s == a.s ? 0.f : f * a.s;
     a.m = to;
@@ -194,11 +197,11 @@ struct LpPart {
 __device__ __forceinline__ void lp_write(const LpPart &p, int64_t tok, bool is_tok, float xt, bool writes, float *logprob,
                                          float *entropy, int32_t *rank, float &ref, float &log_sum) {
     const float s = p.z.m == -INFINITY ? NAN : p.z.s; /* nothing is possible */
-    const float ls = log2f(s);
-    if (writes) { /* x - lse, in powers of two up to the last product */
-        *logprob = tok < 0 ? 0.f : is_tok ? (fmaf(xt, LP_LOG2E, -p.z.m) - ls) * LP_LN2 : NAN;
+    const float ls = logf(s);
+    if (writes) {
+        *logprob = tok < 0 ? 0.f : is_tok ? xt - p.z.m - ls : NAN;
         if (entropy)
-            *entropy = (ls - p.z.t / s) * LP_LN2;
+            *entropy = ls - p.z.t / s;
         if (rank)
             *rank = is_tok ? p.n : -1;
         ref = p.z.m;
@@ -306,10 +309,9 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
 #pragma unroll
         for (int i = 1; i < PER; ++i)
             mx = fmaxf(mx, w[i]);
-        if (__any(fmaf(mx, LP_LOG2E, -LP_SLACK) > a.m)) {
-            const float to = mx * LP_LOG2E;
-            if (to > a.m)
-                a.shift(to);
+        if (__any(mx - LP_SLACK > a.m)) {
+            if (mx > a.m)
+                a.shift(mx);
         }
         if (a.m != -INFINITY) {
 #pragma unroll
@@ -363,9 +365,9 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
 #pragma unroll
     for (int k = 0; k < 2; ++k)
         if (ends[k] >= 0) {
-            const float x = r.at(ends[k]), to = x * LP_LOG2E;
-            if (to > a.m)
-                a.shift(to);
+            const float x = r.at(ends[k]);
+            if (x > a.m)
+                a.shift(x);
             if (a.m != -INFINITY)
                 a.add(x);
             else
@@ -527,7 +529,7 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
         const uint64_t key = cand[c];
         const int place = lp_place(cand, n, key);
         if (place < top) {
-            top_logprob[row * top + place] = (fmaf(lp_key_value(key), LP_LOG2E, -m) - ls) * LP_LN2;
+            top_logprob[row * top + place] = lp_key_value(key) - m - ls;
             top_index[row * top + place] = (int32_t)lp_key_index(key);
         }
     }

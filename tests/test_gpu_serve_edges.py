@@ -1,4 +1,6 @@
 """The serving operators at masks, strides, defaults and batches where a call once went wrong."""
+import math
+
 import numpy as np
 import pytest
 
@@ -45,3 +47,55 @@ def test_rank_of_a_forbidden_token(T, V, shift, f32):
         r = {k: host(v) for k, v in H.token_logprobs(t, gpu(tok), top=2).items()}
         assert r["rank"].tolist() == want, first
         assert (r["logprob"] == -np.inf).all()
+
+
+def score_bound(x, tok):
+    """One row of finite logits, each lse' = log s from the maximum m: (x - m) - log s, entropy, and how far f32 may be off
+    log s: sums of a thread's elements and of the threads, and the exponents (x - r) log2 e, r within 14 of m, of three
+    roundings (2^-24 each, the constant's included)."""
+    m = x.max()
+    d = x - m
+    e = np.exp(d)
+    s = e.sum()
+    mean = -(e[e > 0] * d[e > 0]).sum() / s
+    off = (len(x) / 1024 + 40) * 2.0 ** -24 + (mean + 14) * 3 * 2.0 ** -24
+    return m, math.log(s), mean, off
+
+
+@pytest.mark.parametrize("f32", [False, True])
+@pytest.mark.parametrize("T,V", [(9, 500), (9, 32003), (9, 128256), (300, 2000)])
+def test_scores_of_the_largest_finite_logits(T, V, f32):
+    """Masks of the type's lowest value and logits as far out as the type goes: log probabilities stay those of the definition
+    (-log V in a row of nothing else) and become infinite only where they pass f32's range."""
+    torch_cuda()
+    print(f"finite extremes T={T} V={V} f32={f32}", flush=True)
+    rng = np.random.default_rng(V)
+    low = float(np.finfo(np.float32).min) if f32 else -3.3895313892515355e38
+    x = rng.normal(0, 3, (T, V))
+    x[0] = low                                       # nothing is allowed
+    x[1, rng.random(V) < 0.9] = low                  # a mask
+    x[2], x[2, 3] = low, 1.5                         # one entry is allowed
+    x[3] = -low                                      # the largest value everywhere
+    x[4, V // 2] = -low                              # and once
+    x[5] = rng.choice([2.5e38, 2.4e38, -2.5e38, 0.0], V)
+    x[6, : V // 2] = -1e38                           # long stretches far below what follows
+    x[7] = np.linspace(-3e38, 3e38, V)
+    x[8, :] = low
+    x[8, V // 4:] = -2.5e38
+    tok = rng.integers(0, V, T)
+    tok[1] = int(np.flatnonzero(x[1] == low)[0])
+    tok[2], tok[6] = 0, 1
+    top = 5
+    t, vals = logits_of(x, f32)
+    r = {k: host(v) for k, v in H.token_logprobs(t, gpu(tok), top=top).items()}
+    for i in range(T):
+        v = vals[i]
+        m, log_s, mean, off = score_bound(v, tok[i])
+        order = np.lexsort((np.arange(V), -v))[:top]
+        assert r["rank"][i] == np.count_nonzero(v > v[tok[i]]) + np.count_nonzero(v[: tok[i]] == v[tok[i]]), i
+        assert r["top_index"][i].tolist() == order.tolist(), i
+        for got, at in [(r["logprob"][i], tok[i])] + list(zip(r["top_logprob"][i], order)):
+            want = (v[at] - m) - log_s
+            with np.errstate(over="ignore"):
+                assert got == np.float32(want) or abs(float(got) - want) <= off + 2.0 ** -22 * (abs(want) + log_s), (i, at, got, want)
+        assert abs(r["entropy"][i] - (log_s + mean)) <= 4 * (off + 2.0 ** -22 * (log_s + mean)), (i, r["entropy"][i], log_s + mean)
