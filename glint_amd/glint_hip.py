@@ -557,16 +557,20 @@ def _planes(cache):
     return pages, heads, 2 * half, kh.data_ptr(), ka.data_ptr(), vh.data_ptr(), va.data_ptr()
 
 
-def _rows(t, align: int):
-    """A [tokens, heads, D] tensor whose rows the kernels can load: itself, or a copy where D is
-    strided or an address or stride is no multiple of `align` elements."""
-    s = t.stride()
-    if s[2] != 1 or s[0] % align or s[1] % align or t.data_ptr() % (align * t.element_size()):
+def _rows(t, align: int, low: int = 0, high: int = 0):
+    """A [tokens, heads, D] tensor whose rows the kernels can load, its tokens' and its heads' stride:
+    itself, or a copy where D is strided, an address or stride is no multiple of `align` elements or
+    (`high` given) the tokens' stride lies outside low .. high. A dimension of one has no stride: torch
+    leaves any number there, in what it calls contiguous too."""
+    n, heads, dim = t.shape
+    st, sh, sd = t.stride()
+    st, sh = st if n > 1 else heads * dim, sh if heads > 1 else dim
+    if sd != 1 or st % align or sh % align or t.data_ptr() % (align * t.element_size()) or (high and not low <= st <= high):
         t = t.contiguous()
         if t.data_ptr() % (align * t.element_size()):
             t = t.clone()
-        s = t.stride()
-    return t, s[0], s[1]
+        st, sh = heads * dim, dim
+    return t, st, sh
 
 
 def _kv_elt(t) -> int:
@@ -655,7 +659,7 @@ def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Opt
         raise TypeError(f"expected bfloat16, got {q.dtype}")
     if max_q < 1 or (cu_q is None and rows != B * max_q):
         raise ValueError(f"{rows} query rows, {B} sequences of {max_q}")
-    if page_table.dtype is not torch.int32 or page_table.stride(1) != 1:
+    if page_table.dtype is not torch.int32 or (page_table.stride(1) != 1 and wide > 1):
         raise ValueError("page_table: int32 with adjacent columns")
     q, qt, qh = _rows(q, 8)
     n = _ints(lens, torch.int32, B, "lens")
@@ -703,8 +707,8 @@ def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: 
     cq = _ints(cu_q, torch.int32, B + 1, "cu_q")
     ck = cq if cu_k is None else _ints(cu_k, torch.int32, B + 1, "cu_k")
     q, qt, qh = _rows(q, 8)
-    k, kt, kh = _rows(k if dim <= k.stride(0) <= 1 << 24 else k.contiguous(), 8)
-    v, vt, vh = _rows(v if dim <= v.stride(0) <= 1 << 24 else v.contiguous(), 8)
+    k, kt, kh = _rows(k, 8, dim, 1 << 24)
+    v, vt, vh = _rows(v, 8, dim, 1 << 24)
     out = _attend_out(out, q, Tq, hq, dim)
     if Tq == 0 or B <= 0:
         return out

@@ -99,3 +99,37 @@ def test_scores_of_the_largest_finite_logits(T, V, f32):
             with np.errstate(over="ignore"):
                 assert got == np.float32(want) or abs(float(got) - want) <= off + 2.0 ** -22 * (abs(want) + log_s), (i, at, got, want)
         assert abs(r["entropy"][i] - (log_s + mean)) <= 4 * (off + 2.0 ** -22 * (log_s + mean)), (i, r["entropy"][i], log_s + mean)
+
+
+# ------------------------------------------------------------------ strides of single rows
+@pytest.mark.parametrize("heads,T", [(8, 1), (1, 1), (1, 5)])
+def test_single_rows_of_any_stride(heads, T):
+    """Where there is one token, or one head, its stride means nothing, whatever it is."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(heads)
+    D, G = 128, 3
+    if T == 1:  # a row of a projection whose width is odd
+        buf = bf16(rng.normal(0, 1, (4, (G + 2) * heads * D + 5)).astype(np.float32))
+        q, k, v = (buf[:, at * heads * D:(at + n) * heads * D].unflatten(1, (n * heads, D))[:1] for at, n in ((0, G), (G, 1), (G + 1, 1)))
+    else:  # rows that follow each other; the one head's stride is odd
+        q = bf16(rng.normal(0, 1, (T, G, D)).astype(np.float32))
+        k, v = (torch.as_strided(bf16(rng.normal(0, 1, (T, D)).astype(np.float32)), (T, 1, D), (D, 13, 1)) for _ in range(2))
+    slots = torch.arange(T, device="cuda")
+    caches = []
+    for same in (lambda t: t, lambda t: torch.empty(t.shape, dtype=t.dtype, device="cuda").copy_(t)):
+        c = H.kv4_cache(2, heads, D)
+        H.kv4_append(same(k), same(v), slots, c)
+        H.kv4_append(same(k).float(), same(v).float(), slots + 64, c)
+        caches.append(c)
+    assert all(torch.equal(a, b) for a, b in zip(*caches))
+    assert any((p != 0).any() for p in caches[0])
+    cu = gpu(np.array([0, T], np.int32))
+    lens = gpu(np.array([T], np.int32))
+    want = H.attend_prompt(q.clone(memory_format=torch.contiguous_format), *(torch.empty(t.shape, dtype=t.dtype, device="cuda").copy_(t) for t in (k, v)), cu)
+    assert torch.equal(H.attend_prompt(q, k, v, cu), want)
+    if T == 1:
+        table = gpu(np.array([[0, 1], [1, 0]], np.int32)).t()[:1]
+        one = gpu(np.array([[0]], np.int32))
+        want = H.kv4_attend(torch.empty(q.shape, dtype=q.dtype, device="cuda").copy_(q), caches[0], one, lens)
+        assert torch.equal(H.kv4_attend(q, caches[0], one, lens), want)
+        assert torch.equal(H.kv4_attend(q, caches[0], table[:, :1], lens), want)
