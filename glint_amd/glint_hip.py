@@ -637,13 +637,15 @@ def kv4_gather(slots, cache, out=None, stream=None):
     return k, v
 
 
-def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Optional[float] = None, out=None,
+def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: Optional[int] = None, scale: Optional[float] = None, out=None,
                stream=None):
     """Attention of the newest tokens over the cache: q bf16 [rows, Hq, D] -> bf16 [rows, Hq, D].
 
     page_table int32 [B, max_pages] and lens int32 [B] (tokens in the cache, the new ones
     included) say what each sequence sees; its rows are cu_q[b] .. cu_q[b + 1] (int32, at most
-    max_q each), or max_q each where cu_q is None. A row sees the positions up to its own."""
+    max_q each: all rows where None), or max_q each (1 where None) where cu_q is None. A row sees
+    the positions up to its own. Rows past max_q, or of no sequence, are not written: they hold
+    what `out` held, anything where it is None."""
     if stream is not None:
         with _torch().cuda.stream(stream):
             return kv4_attend(q, cache, page_table, lens, cu_q, max_q, scale, out)
@@ -657,6 +659,8 @@ def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: int = 1, scale: Opt
         raise ValueError(f"q {tuple(q.shape)}, cache of {heads} heads of {dim}")
     if q.dtype is not torch.bfloat16:
         raise TypeError(f"expected bfloat16, got {q.dtype}")
+    if max_q is None:
+        max_q = max(rows, 1) if cu_q is not None else 1
     if max_q < 1 or (cu_q is None and rows != B * max_q):
         raise ValueError(f"{rows} query rows, {B} sequences of {max_q}")
     if page_table.dtype is not torch.int32 or (page_table.stride(1) != 1 and wide > 1):
@@ -690,7 +694,8 @@ def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: 
 
     cu_q, cu_k int32 [B + 1]: where each sequence's queries and keys start (cu_k is cu_q where
     None); a sequence's last query sees its last key. max_q: no sequence has more queries
-    (Tq where None)."""
+    (Tq where None). Queries past max_q, or of no sequence, are not written: they hold what `out`
+    held, anything where it is None."""
     if stream is not None:
         with _torch().cuda.stream(stream):
             return attend_prompt(q, k, v, cu_q, cu_k, max_q, scale, out)

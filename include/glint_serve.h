@@ -54,8 +54,8 @@ int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, const uint8_
  * q [Tq], at most max_q, or max_q rows each where cu_q is NULL (then Tq = B max_q). Row i of
  * its nq stands at position lens[b] - nq + i and sees the positions up to its own:
  *   out[row][hq][:] = sum_j softmax_j(scale q . k_j) v_j,   k, v of head hq / (Hq / H),
- * BF16 out [Tq][Hq][D]; a row that sees nothing is zero. Rows outside every sequence's are
- * left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores, softmax and
+ * BF16 out [Tq][Hq][D]; a row that sees nothing is zero. Rows past max_q, or outside every
+ * sequence, are left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores, softmax and
  * sums are f32; PARENT and the softmax weights times the value scales enter the matrix
  * products in f16. B H max_q max_pages is bounded: -2 where the list of work passes 2^30.
  * Long sequences are split over workgroups that meet in a workspace of the
@@ -78,9 +78,10 @@ int glint_serve_workspace_release(struct ihipStream_t *stream);
 /* Causal attention of B packed sequences. Sequence b has queries cu_q[b] .. cu_q[b + 1] of
  * q [Tq] (at most max_q) and keys cu_k[b] .. cu_k[b + 1] of k, v [Tk]; the last query sees
  * the last key, each earlier query one key less, and a query before the first key gives
- * zeros. Hq % H == 0; BF16 in and out, out [Tq][Hq][D]; strides multiples of 8, k's and v's
- * stride_t from D to 2^24, addresses 16-B aligned. f32 scores, softmax and sums; the softmax weights enter the second product
- * in BF16. */
+ * zeros. Queries past max_q, or outside every sequence, are left as they are. Hq % H == 0;
+ * BF16 in and out, out [Tq][Hq][D]; strides multiples of 8, k's and v's stride_t from D to 2^24,
+ * addresses 16-B aligned. f32 scores, softmax and sums; the softmax weights enter the second
+ * product in BF16. */
 int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
                         int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
                         int64_t v_stride_h, const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk, int B,

@@ -7,7 +7,7 @@ import pytest
 from glint_amd import glint_hip as H
 from tests import serve_util as S
 from tests.gpu_util import host, torch_cuda
-from tests.test_gpu_kv4 import bf16, gpu
+from tests.test_gpu_kv4 import bf16, gpu, random_planes
 
 pytestmark = pytest.mark.gpu
 
@@ -133,3 +133,22 @@ def test_single_rows_of_any_stride(heads, T):
         want = H.kv4_attend(torch.empty(q.shape, dtype=q.dtype, device="cuda").copy_(q), caches[0], one, lens)
         assert torch.equal(H.kv4_attend(q, caches[0], one, lens), want)
         assert torch.equal(H.kv4_attend(q, caches[0], table[:, :1], lens), want)
+
+
+# ------------------------------------------------------------------ defaults
+def test_rows_of_every_sequence_by_default():
+    """Where cu_q says how many rows a sequence has and max_q is left out, all of them are computed."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(40)
+    planes = tuple(gpu(p) for p in random_planes(rng, 20, 2, 128))
+    nqs = np.array([3, 0, 9, 1])
+    cu = gpu(np.concatenate([[0], np.cumsum(nqs)]).astype(np.int32))
+    q = bf16(rng.normal(0, 1, (13, 8, 128)).astype(np.float32))
+    table, lens = gpu(rng.permutation(20).astype(np.int32).reshape(4, 5)), gpu(np.array([300, 5, 64, 1], np.int32))
+    want = H.kv4_attend(q, planes, table, lens, cu, max_q=9)
+    out = torch.full_like(q, 7.0)
+    H.kv4_attend(q, planes, table, lens, cu, out=out)
+    assert torch.equal(out, want)
+    assert torch.equal(H.kv4_attend(q, planes, table, lens, cu), want)
+    single = H.kv4_attend(q[:4], planes, table, lens)
+    assert torch.equal(single, H.kv4_attend(q[:4], planes, table, lens, max_q=1))
