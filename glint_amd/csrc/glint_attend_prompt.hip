@@ -18,6 +18,7 @@
  *   (D = 128: 200 registers, 66 KB of LDS), so that one wave's exponentials run under
  *   another's products; loads a tile ahead, by the direct path to LDS, which needs no registers. A
  *   short prompt is bound by its longest row's tiles, one after another: 77 tokens 10 us. */
+#include <algorithm>
 #include <cfloat>
 #include <cmath>
 
@@ -401,18 +402,28 @@ GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t
         return -2;
     if (B == 0 || Tq == 0 || max_q == 0)
         return 0;
+    /* what one launch holds; max_q is a bound, so most row blocks of many sequences may be empty */
     const int nblk = (max_q + AP_ROWS - 1) / AP_ROWS;
-    const float scale2 = fabsf(scale) * 1.44269504088896341f;
-    const ApArgs a{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk,
-                   max_q, Hq, H, Hq / H, nblk, B * H, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out};
-    if ((int64_t)B * H > INT32_MAX || ((int64_t)nblk * Hq * B + 8) > INT32_MAX / AP_T)
+    const int64_t most = (INT32_MAX / AP_T - 8) / ((int64_t)nblk * Hq); /* sequences */
+    if (most < 1)
         return -2;
-    const int per = a.nblk * a.G, rest = a.ngroups & 7; /* 8 % rest == 0: whole rounds of 8 workgroups */
-    const int tail = rest == 0 ? 0 : 8 % rest == 0 ? (per + 8 / rest - 1) / (8 / rest) * 8 : rest * per;
-    const unsigned grid = (unsigned)((a.ngroups - rest) * per + tail);
-    if (D == 64)
-        k_attend_prompt<64><<<grid, AP_T, 0, stream>>>(a);
-    else
-        k_attend_prompt<128><<<grid, AP_T, 0, stream>>>(a);
-    return hipGetLastError() == hipSuccess ? 0 : -3;
+    const float scale2 = fabsf(scale) * 1.44269504088896341f;
+    ApArgs a{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk,
+             max_q, Hq, H, Hq / H, nblk, 0, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out};
+    const int per = a.nblk * a.G;
+    for (int64_t b = 0; b < B; b += most) {
+        a.cu_q = cu_q + b;
+        a.cu_k = cu_k + b;
+        a.ngroups = (int)std::min<int64_t>(B - b, most) * H;
+        const int rest = a.ngroups & 7; /* 8 % rest == 0: whole rounds of 8 workgroups */
+        const int tail = rest == 0 ? 0 : 8 % rest == 0 ? (per + 8 / rest - 1) / (8 / rest) * 8 : rest * per;
+        const unsigned grid = (unsigned)((a.ngroups - rest) * per + tail);
+        if (D == 64)
+            k_attend_prompt<64><<<grid, AP_T, 0, stream>>>(a);
+        else
+            k_attend_prompt<128><<<grid, AP_T, 0, stream>>>(a);
+        if (hipGetLastError() != hipSuccess)
+            return -3;
+    }
+    return 0;
 }

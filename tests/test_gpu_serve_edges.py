@@ -152,3 +152,18 @@ def test_rows_of_every_sequence_by_default():
     assert torch.equal(H.kv4_attend(q, planes, table, lens, cu), want)
     single = H.kv4_attend(q[:4], planes, table, lens)
     assert torch.equal(single, H.kv4_attend(q[:4], planes, table, lens, max_q=1))
+
+
+def test_many_prompts_without_a_longest():
+    """512 prompts of 65536 tokens in all and no max_q: more row blocks than a launch holds, most of them empty."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(41)
+    B, heads, G, D = 512, 1, 32, 64
+    cuts = np.sort(rng.choice(np.arange(1, 65536), B - 1, replace=False))
+    cu = gpu(np.concatenate([[0], cuts, [65536]]).astype(np.int32))
+    longest = int(np.diff(np.concatenate([[0], cuts, [65536]])).max())
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v = (torch.randn((65536, n, D), device="cuda", generator=g).bfloat16() for n in (heads * G, heads, heads))
+    want = H.attend_prompt(q, k, v, cu, max_q=longest)
+    print("without max_q", flush=True)
+    assert torch.equal(H.attend_prompt(q, k, v, cu), want)
