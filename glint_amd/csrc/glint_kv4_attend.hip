@@ -778,11 +778,13 @@ static bool ka_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
            max_pages <= KA_FAR && (int64_t)max_q * (Hq / H) <= (1 << 20);
 }
 
-/* Groups that the shape allows, or -1 where their units of cost leave 30 bits. */
-static int64_t ka_groups(int B, int max_q, int H, int G, int max_pages) {
-    const int64_t blocks = ((int64_t)max_q * G + KA_ROWS - 1) / KA_ROWS;
-    const double n = (double)B * H * (double)blocks * ((double)max_pages + KA_WAVES + KA_SWITCH);
-    return n > (double)(1 << 30) ? -1 : (int64_t)B * H * blocks;
+/* Groups that the shape allows a sequence, and how many sequences a launch takes so that all units of
+ * cost fit 30 bits (0: not even one). */
+static int64_t ka_groups(int max_q, int H, int G, int max_pages, int64_t &most) {
+    const int64_t groups = ((int64_t)max_q * G + KA_ROWS - 1) / KA_ROWS * H;
+    const int64_t units = (int64_t)max_pages + KA_WAVES + KA_SWITCH;
+    most = groups > (1 << 30) / units ? 0 : (1 << 30) / (groups * units);
+    return groups;
 }
 
 bool glint_serve_ws(hipStream_t stream, GlintSplitWs &ws) { return glint_split_ws_stream(stream, ws); }
@@ -814,22 +816,40 @@ GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_
     Kv4AttendArgs a{q, q_stride_t, q_stride_h, Tq, k_hole, v_hole, k_absmax, v_absmax, pages, table, table_stride,
                     max_pages, lens, cu_q, B, max_q, Hq, H, Hq / H, scale2 < FLT_MIN ? FLT_MIN : scale2,
                     scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr};
-    int64_t grid = ka_groups(B, max_q, H, a.G, max_pages);
-    if (grid < 0)
+    int64_t most;
+    const int64_t groups = ka_groups(max_q, H, a.G, max_pages, most), cus = glint_cu_count();
+    if (most < 1)
         return -2;
-    const int64_t cus = glint_cu_count();
     GlintSplitWs ws;
     if (glint_serve_ws(stream, ws) && ws.nctr >= (size_t)cus &&
         ws.part_floats >= (size_t)cus * 2 * KA_ROWS * (D + 4)) {
         a.part = ws.part;
         a.ctr = ws.ctr;
-        grid = std::min<int64_t>((grid * (max_pages + KA_WAVES + KA_SWITCH) + KA_WAVES - 1) / KA_WAVES, cus);
-    } else if (grid > INT32_MAX / KA_T) { /* a workgroup per group */
+    } else if (groups > INT32_MAX / KA_T) { /* a workgroup per group */
         return -2;
+    } else {
+        most = std::min<int64_t>(most, INT32_MAX / KA_T / groups);
     }
-    if (D == 64)
-        k_kv4_attend<64><<<(unsigned)grid, KA_T, 0, stream>>>(a);
-    else
-        k_kv4_attend<128><<<(unsigned)grid, KA_T, 0, stream>>>(a);
-    return hipGetLastError() == hipSuccess ? 0 : -3;
+    for (int64_t b = 0; b < B; b += most) {
+        a.B = (int)std::min<int64_t>(B - b, most);
+        a.table = table + b * table_stride;
+        a.lens = lens + b;
+        if (cu_q) {
+            a.cu_q = cu_q + b;
+        } else { /* rows by number: this launch's alone */
+            a.q = q + b * max_q * q_stride_t;
+            a.out = out + b * max_q * Hq * D;
+            a.Tq = (int64_t)a.B * max_q;
+        }
+        int64_t grid = a.B * groups;
+        if (a.part)
+            grid = std::min<int64_t>((grid * (max_pages + KA_WAVES + KA_SWITCH) + KA_WAVES - 1) / KA_WAVES, cus);
+        if (D == 64)
+            k_kv4_attend<64><<<(unsigned)grid, KA_T, 0, stream>>>(a);
+        else
+            k_kv4_attend<128><<<(unsigned)grid, KA_T, 0, stream>>>(a);
+        if (hipGetLastError() != hipSuccess)
+            return -3;
+    }
+    return 0;
 }

@@ -55,9 +55,10 @@ int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, const uint8_
  * its nq stands at position lens[b] - nq + i and sees the positions up to its own:
  *   out[row][hq][:] = sum_j softmax_j(scale q . k_j) v_j,   k, v of head hq / (Hq / H),
  * BF16 out [Tq][Hq][D]; a row that sees nothing is zero. Rows past max_q, or outside every
- * sequence, are left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores, softmax and
- * sums are f32; PARENT and the softmax weights times the value scales enter the matrix
- * products in f16. B H max_q max_pages is bounded: -2 where the list of work passes 2^30.
+ * sequence, are left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores,
+ * softmax and sums are f32; PARENT and the softmax weights times the value scales enter the
+ * matrix products in f16. A batch whose list of work passes 2^30 goes in several launches, and
+ * a sequence for which H max_q (Hq / H) max_pages / 16 does is -2.
  * Long sequences are split over workgroups that meet in a workspace of the
  * stream's (glint_serve_workspace_reserve): it is allocated by the first such call outside a
  * capture and never grows. A capture on a stream that has none runs unsplit. */

@@ -154,6 +154,33 @@ def test_rows_of_every_sequence_by_default():
     assert torch.equal(single, H.kv4_attend(q[:4], planes, table, lens, max_q=1))
 
 
+@pytest.mark.parametrize("packed", [False, True])
+def test_more_work_than_one_list(packed):
+    """Batches whose list of work, by the table's width and the rows that a sequence may have, is past one launch's bound:
+    the same as their parts, for lengths of one round of pages, which nothing splits."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(42)
+    pages, heads, G, D = 30, 8, 4, 64
+    planes = tuple(gpu(p) for p in random_planes(rng, pages, heads, D))
+    B, wide = (1024, 1024) if packed else (1100, 131072)
+    table = gpu(np.resize(rng.permutation(pages), wide).astype(np.int32))[None].expand(B, wide)
+    lens = rng.integers(0, 500, B).astype(np.int32)
+    nqs = rng.integers(0, 3, B) if packed else np.full(B, 2)
+    starts = np.concatenate([[0], np.cumsum(nqs)]).astype(np.int32)
+    wider = bf16(rng.normal(0, 1, (int(starts[-1]), (heads + 1) * G, D)).astype(np.float32))
+    q = wider[:, G:]
+    print(f"packed={packed} B={B} wide={wide}", flush=True)
+    if packed:
+        got = H.kv4_attend(q, planes, table, gpu(lens), gpu(starts))
+    else:
+        got = H.kv4_attend(q, planes, table, gpu(lens), max_q=2)
+    for a in range(0, B, 100):
+        z = min(a + 100, B)
+        rows = slice(int(starts[a]), int(starts[z]))
+        part = H.kv4_attend(q[rows], planes, table[a:z, :8], gpu(lens[a:z]), gpu(starts[a:z + 1] - starts[a]), max_q=2)
+        assert torch.equal(got[rows], part), a
+
+
 def test_many_prompts_without_a_longest():
     """512 prompts of 65536 tokens in all and no max_q: more row blocks than a launch holds, most of them empty."""
     torch = torch_cuda()
