@@ -671,8 +671,8 @@ def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: Optional[int] = Non
     out = _attend_out(out, q, rows, hq, dim)
     if rows == 0 or B == 0:
         return out
-    if wide == 0:
-        return out.zero_()
+    if wide == 0:  # nobody has a page
+        page_table, wide = page_table.new_full((B, 1), -1), 1
     _check(serve_lib().glint_kv4_attend(q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(),
                                         page_table.stride(0), wide, n, cu, B, max_q, hq, heads, dim,
                                         dim ** -0.5 if scale is None else scale, out.data_ptr(), _sh(None)),
@@ -717,8 +717,8 @@ def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: 
     out = _attend_out(out, q, Tq, hq, dim)
     if Tq == 0 or B <= 0:
         return out
-    if Tk == 0:
-        return out.zero_()
+    if Tk == 0:  # an address for the kernel, which reads no key
+        k, v = q, q
     _check(serve_lib().glint_attend_prompt(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cq, ck, Tq,
                                            Tk, B, Tq if max_q is None else max_q, hq, heads, dim,
                                            dim ** -0.5 if scale is None else scale, out.data_ptr(), _sh(None)),

@@ -194,3 +194,17 @@ def test_many_prompts_without_a_longest():
     want = H.attend_prompt(q, k, v, cu, max_q=longest)
     print("without max_q", flush=True)
     assert torch.equal(H.attend_prompt(q, k, v, cu), want)
+
+
+def test_rows_outside_stay_without_keys():
+    """Rows outside every sequence are left as they are where there is no key and no page either; those inside are zero."""
+    torch = torch_cuda()
+    q = torch.randn((9, 2, 64), device="cuda").bfloat16()
+    cu = gpu(np.array([2, 5, 6], np.int32))
+    none = q.new_empty((0, 1, 64))
+    for run in (lambda out: H.attend_prompt(q, none, none, cu, gpu(np.array([0, 0, 0], np.int32)), out=out),
+                lambda out: H.kv4_attend(q, H.kv4_cache(2, 1, 64), gpu(np.zeros((2, 0), np.int32)), gpu(np.array([0, 3], np.int32)),
+                                         cu, max_q=3, out=out)):
+        out = torch.full_like(q, 5.0)
+        run(out)
+        assert (out[:2] == 5).all() and (out[6:] == 5).all() and (out[2:6] == 0).all()
