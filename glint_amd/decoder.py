@@ -64,13 +64,23 @@ class Decoder:
         self.own = [[] for _ in range(requests)]
         self.free = list(range(pages))
 
+    def _pages(self, request, n):
+        """Pages that n more tokens of a request need."""
+        return max(0, (self.held[request] + n + H.KV_PAGE - 1) // H.KV_PAGE - len(self.own[request]))
+
+    def _refuse(self, news):
+        """Raises, before any request changes, where one of {request: tokens} does not exist or they do not all fit."""
+        for r in news:
+            if not 0 <= r < len(self.held):
+                raise IndexError(f"request {r} of {len(self.held)}")
+        want = {r: self._pages(r, len(some)) for r, some in news.items()}
+        if sum(want.values()) > len(self.free):
+            raise RuntimeError(f"requests {list(news)}: {list(want.values())} pages more, {len(self.free)} left")
+
     def _slots(self, request, n):
-        """Places for n more tokens of a request, with the pages that they need."""
+        """Places for n more tokens of a request, with the pages that they need; _refuse has seen that there are enough."""
         first = self.held[request]
-        want = (first + n + H.KV_PAGE - 1) // H.KV_PAGE - len(self.own[request])
-        if want > len(self.free):
-            raise RuntimeError(f"request {request}: {want} pages more, {len(self.free)} left")
-        for _ in range(want):
+        for _ in range(self._pages(request, n)):
             page = self.free.pop()
             self.table[request, len(self.own[request])] = page
             self.own[request].append(page)
@@ -95,7 +105,9 @@ class Decoder:
         return self.head(norm(x))
 
     def prefill(self, prompts):
-        """prompts: {request: tokens}, new prompts or further chunks. Logits [all tokens, vocab], in order."""
+        """prompts: {request: tokens}, new prompts or further chunks. Logits [all tokens, vocab], in order.
+        Where the tokens do not fit, no request changes."""
+        self._refuse(prompts)
         ints = lambda v, t=torch.int32: torch.tensor(v, dtype=t, device="cuda")
         tokens, pos, new, seen, keys_new, keys_old, old = [], [], [], [], [], [], []
         cu_q, cu_k = [0], [0]
@@ -125,7 +137,9 @@ class Decoder:
         return self._run(tokens, pos, attend)
 
     def step(self, news):
-        """news: {request: tokens}, the next token of each (or a few drafted ones). Logits [all tokens, vocab]."""
+        """news: {request: tokens}, the next token of each (or a few drafted ones). Logits [all tokens, vocab].
+        Where the tokens do not fit, no request changes."""
+        self._refuse(news)
         tokens, pos, slots, cu_q = [], [], [], [0]
         for r, some in news.items():
             pos += range(self.held[r], self.held[r] + len(some))

@@ -208,3 +208,23 @@ def test_rows_outside_stay_without_keys():
         out = torch.full_like(q, 5.0)
         run(out)
         assert (out[:2] == 5).all() and (out[6:] == 5).all() and (out[2:6] == 0).all()
+
+
+# ------------------------------------------------------------------ the decoder
+def test_a_refused_call_changes_nothing():
+    """Where a later request does not fit, or does not exist, the requests before it keep what they had."""
+    torch = torch_cuda()
+    from glint_amd.decoder import Decoder
+    shape = dict(vocab=97, dim=128, layers=1, heads=2, kv_heads=1, head_dim=64, ffn=128, pages=4, requests=3)
+    m, twin = Decoder(**shape), Decoder(**shape)
+    state = lambda d: (list(d.held), [list(o) for o in d.own], list(d.free), d.table.tolist())
+    for d in (m, twin):
+        d.prefill({0: list(range(60)), 1: [1, 2, 3]})
+    before = state(m)
+    for call, error in ((lambda: m.prefill({0: [5, 6], 2: [1] * 200}), RuntimeError), (lambda: m.step({0: [5] * 5, 1: [6] * 200}), RuntimeError),
+                        (lambda: m.step({0: [5] * 70, 1: [6] * 70}), RuntimeError), (lambda: m.prefill({1: [5], 9: [5]}), IndexError),
+                        (lambda: m.step({0: [5] * 10, 9: [5]}), IndexError)):
+        with pytest.raises(error):
+            call()
+        assert state(m) == before
+    assert torch.equal(m.step({0: [7], 1: [8]}), twin.step({0: [7], 1: [8]}))
