@@ -402,9 +402,10 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
     if (top > 0) {
         const uint32_t value = (uint32_t)(mine >> 32), first = lp_wave_max32(value);
         const bool is_first = value == first;
+        const bool tie = __builtin_popcountll(__ballot(is_first)) > 1; /* every lane takes part */
         const uint32_t second = lp_wave_max32(is_first ? 0u : value);
         if (lane == 0)
-            wave_second[wave] = __builtin_popcountll(__ballot(is_first)) > 1 ? first : second;
+            wave_second[wave] = tie ? first : second;
     }
     if (threadIdx.x == 0) {
         ncand = 0;

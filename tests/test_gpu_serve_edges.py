@@ -101,6 +101,38 @@ def test_scores_of_the_largest_finite_logits(T, V, f32):
         assert abs(r["entropy"][i] - (log_s + mean)) <= 4 * (off + 2.0 ** -22 * (log_s + mean)), (i, r["entropy"][i], log_s + mean)
 
 
+def test_ties_cost_no_more_than_their_order():
+    """Two threads of every wave share its largest value: the list's floor is that value, as where the two differ, and the
+    entries below it are no candidates (their search, quadratic over 1024 of them, took 2 times the call)."""
+    torch = torch_cuda()
+    T, V = 256, 8192  # a 16-B load of BF16 a thread
+    x = torch.zeros((T, 1024, 8), device="cuda")
+    x[:, 0::64, 0] = 10.0
+    x[:, 1::64, 3] = 10.0
+    apart = x.clone()
+    apart[:, 0::64, 0] = 11.0
+    tok = torch.zeros(T, dtype=torch.int64, device="cuda")
+    times = {}
+    rows = {"tie": x.view(T, V).bfloat16(), "apart": apart.view(T, V).bfloat16()}
+    for name in ("tie", "apart"):
+        r = H.token_logprobs(rows[name], tok, top=20)
+        want = torch.sort(rows[name].float(), dim=1, descending=True, stable=True).indices[:, :20]
+        assert torch.equal(r["top_index"].long(), want)
+    for _ in range(3):
+        for name, y in rows.items():
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            for _ in range(5):
+                H.token_logprobs(y, tok, top=20)
+            a.record()
+            for _ in range(30):
+                H.token_logprobs(y, tok, top=20)
+            b.record()
+            b.synchronize()
+            times[name] = min(times.get(name, 1e9), a.elapsed_time(b) / 30)
+    print({k: round(1e3 * v, 2) for k, v in times.items()}, flush=True)
+    assert times["tie"] < 1.25 * times["apart"]
+
+
 # ------------------------------------------------------------------ strides of single rows
 @pytest.mark.parametrize("heads,T", [(8, 1), (1, 1), (1, 5)])
 def test_single_rows_of_any_stride(heads, T):
