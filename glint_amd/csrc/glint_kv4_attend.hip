@@ -42,6 +42,8 @@
 
 #include "kv4.h"
 #include "serve_ws.h"
+/* two partials of 16 rows of 128 dimensions, a maximum and a sum per CU; token scores take fewer */
+#define GLINT_SPLIT_CU_FLOATS (2 * 16 * (128 + 4))
 #include "tile_mfma.h"
 
 typedef _Float16 kv4_f16x8 __attribute__((ext_vector_type(8)));

@@ -1015,6 +1015,9 @@ __global__ __launch_bounds__(512) void k_tile_big(P p, const uint16_t *__restric
  * tile_big_sk_launch check their plans against the capacity and fall back (unsplit, or
  * whole tiles) where they would not fit. */
 #define GLINT_SPLIT_TILE_FLOATS_MAX 65536
+#ifndef GLINT_SPLIT_CU_FLOATS /* partials' floats per CU; a source whose kernels need fewer defines it before this header */
+#define GLINT_SPLIT_CU_FLOATS (2 * GLINT_SPLIT_TILE_FLOATS_MAX)
+#endif
 static inline size_t glint_split_ctr_bytes(size_t nctr) { return (nctr * sizeof(unsigned) + 255) & ~(size_t)255; }
 
 /* Zero n counters on a stream (a kernel, not a memset node, so it is also safe to record
@@ -1064,7 +1067,7 @@ static inline bool glint_split_ws_key(hipStream_t st, uint64_t &key) {
 static inline size_t glint_split_ws_bytes(size_t &cb, size_t &nctr, size_t &part_floats) {
     const size_t cus = (size_t)glint_cu_count();
     nctr = 2 * cus;
-    part_floats = 2 * cus * GLINT_SPLIT_TILE_FLOATS_MAX;
+    part_floats = cus * GLINT_SPLIT_CU_FLOATS;
     cb = glint_split_ctr_bytes(nctr);
     return cb + part_floats * sizeof(float);
 }

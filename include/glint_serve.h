@@ -68,7 +68,7 @@ int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, 
                      const int32_t *cu_q, int B, int max_q, int Hq, int H, int D, float scale, uint16_t *out,
                      struct ihipStream_t *stream);
 
-/* The stream's workspace, 128 MiB on 256 CUs: one for eager calls and, once the stream was
+/* The stream's workspace, 4.1 MiB on 256 CUs: one for eager calls and, once the stream was
  * captured, one for the graphs captured on it, whose replays must not overlap one another.
  * reserve allocates the eager one ahead of time (0; -1: no memory, or the stream is being
  * captured). release waits for the stream and frees both (0, or -1); graphs captured before

@@ -242,6 +242,25 @@ def test_rows_outside_stay_without_keys():
         assert (out[:2] == 5).all() and (out[6:] == 5).all() and (out[2:6] == 0).all()
 
 
+def test_a_workspace_is_as_large_as_its_kernels_need():
+    """A stream's workspace takes some 4 MiB of the memory that cache pages want, not the matrix products' 128."""
+    torch = torch_cuda()
+    lib = H.serve_lib()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for s in streams:
+        assert lib.glint_serve_workspace_release(s.cuda_stream) == 0
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for s in streams:
+        assert lib.glint_serve_workspace_reserve(s.cuda_stream) == 0
+    torch.cuda.synchronize()
+    taken = free - torch.cuda.mem_get_info()[0]
+    for s in streams:
+        assert lib.glint_serve_workspace_release(s.cuda_stream) == 0
+    print(f"{taken / 2 ** 20:.1f} MiB for {len(streams)} streams", flush=True)
+    assert taken <= len(streams) * 16 << 20
+
+
 # ------------------------------------------------------------------ the decoder
 def test_a_refused_call_changes_nothing():
     """Where a later request does not fit, or does not exist, the requests before it keep what they had."""
