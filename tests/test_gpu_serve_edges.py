@@ -279,3 +279,20 @@ def test_a_refused_call_changes_nothing():
             call()
         assert state(m) == before
     assert torch.equal(m.step({0: [7], 1: [8]}), twin.step({0: [7], 1: [8]}))
+
+
+# ------------------------------------------------------------------ the order of prompt work
+@pytest.mark.parametrize("B,heads", [(3, 3), (5, 2), (2, 6), (13, 1), (11, 1)])
+def test_groups_past_whole_rounds_of_xcds(B, heads):
+    """More groups than XCDs, and a rest: 1, 2, 4, 5 and 3 of them."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(B)
+    G, D = 3, 64
+    n = rng.integers(1, 300, B)
+    cu = np.concatenate([[0], np.cumsum(n)]).astype(np.int32)
+    q, k, v = (bf16(rng.normal(0, 1, (cu[-1], c, D)).astype(np.float32)) for c in (heads * G, heads, heads))
+    got = H.attend_prompt(q, k, v, gpu(cu), max_q=300)
+    for b in range(B):
+        part = slice(int(cu[b]), int(cu[b + 1]))
+        one = gpu(np.array([0, n[b]], np.int32))
+        assert torch.equal(got[part], H.attend_prompt(q[part], k[part], v[part], one)), b
