@@ -195,7 +195,10 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
      * the longest rows come first. A workgroup's XCD is its index modulo 8, and each XCD's L2
      * should hold few groups' keys: as many groups as share out evenly go whole to one XCD
      * each; of the rest, where they divide 8, each goes to 8 / rest XCDs. 8192 tokens of 32
-     * heads over 8 key heads: 555 us, 773 with every group on every XCD. */
+     * heads over 8 key heads: 555 us, 773 with every group on every XCD. What it costs: groups of
+     * one XCD may be unlike, where a short sequence's heads fill the others. 4000 tokens and, in
+     * the same call, prompts of 60 until the groups are 8: 4 key heads 153 us, the long one alone
+     * 109; 2 key heads 148, 88; 1 key head 132, 86; 8 key heads (16 groups) 155, 163. */
     const int per = A.nblk * A.G, whole = A.ngroups & ~7, rest = A.ngroups & 7;
     int group, item;
     if ((int)blockIdx.x < whole * per) {

@@ -29,7 +29,7 @@
  *
  *   What bounds it: reading the cache once, 4.5 bits an element. 32 sequences of 8192 tokens, 8 heads
  *   of 128, 4 rows a head: 303 MB in 62 to 69 us, 4.4 to 4.9 TB/s, where a copy reaches 5.1. Decoding
- *   codes in LDS, its two products and 2^x take some 700 vector instructions a page and hide behind
+ *   codes in LDS, its two products and 2^x take some 620 vector instructions a page and hide behind
  *   that up to 16 rows a page, which is why a group has 16 (32 rows in registers spilled: 4 sequences of
  *   8000 with 40 rows a head 57 us at best, 38 now). A product's table entries are read while the one
  *   before is multiplied (equal lengths 65 without, 62 with; ragged ones 42.5, 39). 8 waves share a

@@ -13,9 +13,10 @@
  *   one 64-bit key, the value's order over the inverted index, so ties need no rule.
  *   Few long rows are split over workgroups, whose sums and lists meet in the last to arrive.
  *
- *   Long rows are bound by reading them once and, close behind, by some 13 vector instructions an
- *   element: 2047 rows of 128256 BF16 in 111 us, 4.7 TB/s, where a copy reaches 5.1, the vector units
- *   86% busy; a second pass for the list would add to both. Short calls are bound by one chain of a
+ *   Long rows are bound by reading them once and, close behind, by some 14 vector instructions an
+ *   element: 2047 rows of 128256 BF16 in 115 us, 4.6 TB/s, where a copy reaches 5.1, the vector units
+ *   90% busy (m in powers of two saved 1 of them, 3 us, and overflowed); a second pass for the list
+ *   would add to both. Short calls are bound by one chain of a
  *   workgroup's waits: first loads, wave and workgroup sums, the floor of the list, its
  *   candidates, their order; 8 rows of 128256 13 us. 1024 threads a row keep 64 KB of loads in
  *   flight; LP_U loads a thread and as many ahead. */
@@ -398,7 +399,8 @@ __global__ __launch_bounds__(LP_T, 8) void k_token_logprobs(const E *__restrict_
     }
     /* A value that the top-th largest thread maximum is not below: two lanes of a wave reach the
      * second largest of its maxima, so where ceil(top / 2) waves reach a value by theirs, `top` lanes
-     * do. The maxima that reach it, some 30 for a list of 20, count those before each of them. */
+     * do. The maxima that reach it, some 30 for a list of 20, count those before each of them: all 1024
+     * where they are equal, as in a row of one value (8 such rows of 128256 33 us, 13 of others). */
     if (top > 0) {
         const uint32_t value = (uint32_t)(mine >> 32), first = lp_wave_max32(value);
         const bool is_first = value == first;
@@ -548,7 +550,7 @@ GLINT_API int glint_token_logprobs(const void *logits, int elt, int64_t stride, 
         return 0;
     /* Few rows are split, so that a workgroup per CU shares the reading, none with less than two loads
      * of every thread (as good as one, and fewer parts to join). Rows of 128256 BF16, split against
-     * whole, by kernel: 8 rows with a list of 20 13.4 and 21.0 us, 64 without a list 10.0 and 18.0. */
+     * whole, by kernel: 8 rows with a list of 20 13.7 and 18.8 us, 64 without a list 9.8 and 15.7. */
     const int64_t parts = V / (elt == GLINT_KV_BF16 ? 8 : 4) / (2 * LP_T);
     int nsplit = (int)std::min<int64_t>(std::min<int64_t>(LP_SPLIT, parts), glint_cu_count() / T);
     GlintSplitWs ws{nullptr, nullptr, 0, 0};
