@@ -557,18 +557,17 @@ def _planes(cache):
     return pages, heads, 2 * half, kh.data_ptr(), ka.data_ptr(), vh.data_ptr(), va.data_ptr()
 
 
-def _rows(t, align: int, low: int = 0, high: int = 0):
-    """A [tokens, heads, D] tensor whose rows the kernels can load, its tokens' and its heads' stride:
-    itself, or a copy where D is strided, an address or stride is no multiple of `align` elements or
-    (`high` given) the tokens' stride lies outside low .. high. A dimension of one has no stride: torch
-    leaves any number there, in what it calls contiguous too."""
-    n, heads, dim = t.shape
+def _rows(t, align: int, low: int = 0, high: int = 1 << 62):
+    """A [tokens, heads, D] tensor whose rows the kernels can load, its tokens' and its heads' stride: itself, or a
+    contiguous one where D is strided, an address or stride is no multiple of `align` elements or the tokens' stride
+    lies outside low .. high. A contiguous tensor's strides are counted, not asked for: torch leaves any number on a
+    dimension of one."""
     st, sh, sd = t.stride()
-    st, sh = st if n > 1 else heads * dim, sh if heads > 1 else dim
-    if sd != 1 or st % align or sh % align or t.data_ptr() % (align * t.element_size()) or (high and not low <= st <= high):
+    if sd != 1 or st % align or sh % align or t.data_ptr() % (align * t.element_size()) or not low <= st <= high:
         t = t.contiguous()
         if t.data_ptr() % (align * t.element_size()):
             t = t.clone()
+        _, heads, dim = t.shape
         st, sh = heads * dim, dim
     return t, st, sh
 
