@@ -42,7 +42,8 @@ HIP_FLAGS = [
 LIBS = {
     "libglint_encode.so": ["glint_encode.hip", "glint_htile.hip", "glint_select.hip", "glint_noalloc.hip"],
     "libp7_kernels.so": ["int8_mma_gemm.hip", "int8_tile_gemm.hip", "p7_abi.cpp", "glint_plug_streamer.cpp", "p7_selftest.cpp"],
-    "libglint_serve.so": ["glint_kv4.hip", "glint_kv4_attend.hip", "glint_attend_prompt.hip", "glint_logprobs.hip"],
+    "libglint_serve.so": ["glint_kv4.hip", "glint_kv4_attend.hip", "glint_kv4_chunk.hip", "glint_attend_prompt.hip",
+                          "glint_rotate.hip", "glint_logprobs.hip"],
     # measurement only (bench.py's read ceiling), not part of the GLINT ABI
     "libglint_probe.so": ["hbm_probe.hip"],
     # measurement only (bench.py --timeline): libglint_encode.so with the decode GEMV's

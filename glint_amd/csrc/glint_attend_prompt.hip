@@ -22,27 +22,10 @@
 #include <cfloat>
 #include <cmath>
 
-#include "glint_common.h"
+#include "attend_tile.h"
 #include "glint_serve.h"
 
-typedef __bf16 ap_bf16x8 __attribute__((ext_vector_type(8)));
-typedef float ap_f32x16 __attribute__((ext_vector_type(16)));
-typedef short ap_s16x4 __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) ap_s16x4 ap_lds_s16x4;
-
-#define AP_WAVES 4
-#define AP_T (64 * AP_WAVES)
-#define AP_ROWS (32 * AP_WAVES)
-#define AP_KEYS 64
 #define AP_STRIDE (1 << 24) /* elements: a tile's bytes fit 32 bits */
-#define AP_SLACK 8.f /* a maximum may lag this far (in powers of two) before outputs are rescaled */
-
-union ApFrag {
-    uint32_t u[4];
-    glint_u32x4 v;
-    ap_s16x4 h[2];
-    ap_bf16x8 f;
-};
 
 struct ApArgs {
     const uint16_t *q, *k, *v;
@@ -55,132 +38,12 @@ struct ApArgs {
     uint32_t q_sign; /* 0x80008000 where the scale is negative */
     float scale2;    /* |scale| log2 e, above 0 */
     uint16_t *out;
+    ApBound bound; /* of the bounded form */
 };
 
-/* Where 16-B chunk c of row r lies in an LDS tile's row: keys so that 8 lanes reading one
- * chunk of 8 rows touch 8 places, values so that the 64-B pieces of 4 rows that one transposing
- * read takes lie in different 64-B quarters of 256 B. */
-__device__ __forceinline__ int ap_k_chunk(int r, int c) { return c ^ (r & 7); }
-template <int D>
-__device__ __forceinline__ int ap_v_chunk(int r, int c) { return D == 128 ? c ^ ((r & 3) << 2) : c ^ ((r & 2) << 1); }
-
-typedef __attribute__((address_space(3))) char ap_lds;
-
-/* 16 B per lane from the buffer to LDS at `to` + 16 lane (not in a template: the host pass refuses
- * the builtin where its arguments depend on one, and then leaves the kernel's stub out) */
-__device__ __forceinline__ void ap_dma(__amdgpu_buffer_rsrc_t from, ap_lds *to, uint32_t offset, uint32_t more) {
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (__attribute__((address_space(3))) void *)to, 16, offset, more, 0, 0);
-}
-
-/* What a wave carries from tile to tile for its 32 rows. */
-template <int D>
-struct ApRows {
-    ApFrag q[D / 16];
-    ap_f32x16 o[D / 32];
-    float m, l;
-    int last;        /* this lane's row sees the keys up to here */
-    uint32_t kat[4]; /* where the lane reads keys (by the chunk's low bits) and values (by dimension part) */
-    uint32_t vat[D / 32];
-};
-
-/* One tile of keys. */
-template <int D>
-__device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int t, ApRows<D> &w, float scale2, bool masked,
-                                        int half) {
-    ap_f32x16 sc[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            sc[a][i] = 0.f;
-#pragma unroll
-    for (int s = 0; s < D / 16; ++s)
-#pragma unroll
-        for (int a = 0; a < 2; ++a) {
-            ApFrag f;
-            f.v = *(const __attribute__((address_space(3))) glint_u32x4 *)(kl + w.kat[s & 3] + 128 * (s >> 2) + a * 32 * D * 2);
-            sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.f, w.q[s].f, sc[a], 0, 0, 0);
-        }
-    /* element i of part a is key 32 a + 8 (i / 4) + 4 half + i % 4 */
-    if (masked) {
-        const int first = t * AP_KEYS + 4 * half;
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                sc[a][i] = first + 32 * a + 8 * (i >> 2) + (i & 3) <= w.last ? sc[a][i] : -INFINITY;
-    }
-    float top = -INFINITY;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            top = fmaxf(top, sc[a][i]);
-    top = glint_xor32(top, GlintMax()) * scale2;
-    const bool more = top > w.m + AP_SLACK; /* a row's own test, here and below: its bits depend on no other row */
-    if (__any(more)) {
-        const float mn = more ? top : w.m;
-        const float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
-        w.m = mn;
-        w.l *= keep;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                w.o[d][i] *= keep;
-    }
-    const float base = w.m == -INFINITY ? 0.f : w.m;
-    ApFrag pf[4];
-    float sum = 0.f;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-#pragma unroll
-            for (int x = i; x < i + 2; ++x) {
-                sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], scale2, -base));
-                sum += sc[a][x];
-            }
-            pf[2 * a + (i >> 3)].u[(i & 7) >> 1] = glint_cvt_bf16x2(sc[a][i], sc[a][i + 1]);
-        }
-    w.l += sum;
-    /* Step s multiplies the keys that pf[s] holds: 16 s + 4 half + 0..3, and 8 on. */
-    auto values = [&](int s, int d) {
-        ApFrag f;
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-            f.h[x] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((ap_lds_s16x4 *)(vl + w.vat[d] + (16 * s + 8 * x) * D * 2));
-        return f;
-    };
-    /* A weight's bf16 rounding (2^-8) averages out over many keys and does not where few hold
-     * the sum: rows with a weight above 1 / 8 of their sum so far add what the rounding left. (8 equal
-     * weights leave 2^-10.8 of a value's size, rms.) 12 packed prompts: 45.0 us without, 47.6 with 1 / 8,
-     * 51.8 with 1 / 16; 8192 tokens 562, 565, 572. */
-    const bool few = __builtin_amdgcn_exp2f(top - base) * 8.f > glint_xor32(w.l, GlintAdd());
-    if (__any(few)) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            ApFrag rest;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int i = 8 * (s & 1) + 2 * x;
-                const uint32_t left =
-                    glint_cvt_bf16x2(sc[s >> 1][i] - glint_bf16lo(pf[s].u[x]), sc[s >> 1][i + 1] - glint_bf16hi(pf[s].u[x]));
-                rest.u[x] = few ? left : 0u;
-            }
-#pragma unroll
-            for (int d = 0; d < D / 32; ++d)
-                w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(s, d).f, rest.f, w.o[d], 0, 0, 0);
-        }
-    }
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-            w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(values(s, d).f, pf[s].f, w.o[d], 0, 0, 0);
-}
-
-template <int D>
+/* BOUNDED: rows see a window and sinks. A workgroup walks the sinks' tiles and those from its first row's window
+ * on; what lies between costs nothing. */
+template <int D, bool BOUNDED>
 __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs A) {
     constexpr int CH = D / 8;                  /* 16-B chunks of a row */
     constexpr int LOADS = AP_KEYS * CH / AP_T; /* of a thread, per tile of keys or values */
@@ -265,7 +128,21 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
         w.vat[d] = vkey * D * 2 + 16 * ap_v_chunk<D>(vkey, (32 * d + vdim) >> 3) + 2 * (vdim & 7);
 
     const int64_t far = min(r0 + AP_ROWS, nq) - 1 + gap; /* the last key of the last row */
-    const int ntiles = far < 0 ? 0 : (int)(far / AP_KEYS) + 1;
+    int ntiles = far < 0 ? 0 : (int)(far / AP_KEYS) + 1;
+    int sink_tiles = 0, skip = 0; /* step u of the walk is tile u, or, past the sinks', u + skip */
+    if (BOUNDED && ntiles > 0) {
+        sink_tiles = (int)(min((int64_t)A.bound.sinks, far + 1) + AP_KEYS - 1) / AP_KEYS;
+        skip = max(0, (int)(max((int64_t)0, r0 + gap - A.bound.window + 1) / AP_KEYS) - sink_tiles);
+        ntiles -= skip;
+    }
+    auto tile = [&](int u) { return BOUNDED && u >= sink_tiles ? u + skip : u; };
+    /* whether rows from `first` on see any of tile t, and rows up to `last` all of it, as far as the window goes */
+    auto bound_any = [&](int t, int first) {
+        return !BOUNDED || t * AP_KEYS + AP_KEYS - 1 > first - A.bound.window || t * AP_KEYS < A.bound.sinks;
+    };
+    auto bound_all = [&](int t, int last) {
+        return !BOUNDED || t * AP_KEYS > last - A.bound.window || t * AP_KEYS + AP_KEYS <= A.bound.sinks;
+    };
     const uint16_t *kb = A.k + k0 * A.k_st + h * A.k_sh, *vb = A.v + k0 * A.v_st + h * A.v_sh;
 
     /* Tiles go to LDS by the loads' direct path. Place p of a tile is chunk p % CH of row p / CH;
@@ -302,12 +179,13 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
      * an infinite or NaN one, of which a weight of 0 would make NaN, becomes 0 until the
      * end. */
     const int t_part = (int)max((int64_t)0, r0 + gap + 1) / AP_KEYS;
-    auto step = [&](int t, ap_lds *kt, ap_lds *vt, ap_lds *kn, ap_lds *vn) {
+    auto step = [&](int u, ap_lds *kt, ap_lds *vt, ap_lds *kn, ap_lds *vn) {
+        const int t = tile(u);
         __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0); /* this wave's part of tile t */
         __syncthreads();
-        if (t + 1 < ntiles)
-            fetch(t + 1, kn, vn); /* over tile t - 1, which every wave has left */
-        if (t >= t_part) {
+        if (u + 1 < ntiles)
+            fetch(tile(u + 1), kn, vn); /* over the tile before, which every wave has left */
+        if (t >= t_part || !bound_all(t, (int)far)) {
             typedef __attribute__((address_space(3))) glint_u32x4 lds_u32x4;
 #pragma unroll
             for (int i = 0; i < LOADS; ++i) {
@@ -327,17 +205,18 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
             }
             __syncthreads();
         }
-        if (t * AP_KEYS <= wave_high)
-            ap_tile<D>(kt, vt, t, w, A.scale2, t * AP_KEYS + AP_KEYS - 1 > wave_low, half);
+        if (t * AP_KEYS <= wave_high && bound_any(t, wave_low))
+            ap_tile<D, BOUNDED>(kt, vt, t * AP_KEYS, w, A.scale2,
+                                t * AP_KEYS + AP_KEYS - 1 > wave_low || !bound_all(t, wave_high), half, A.bound);
     };
     if (threadIdx.x == 0)
         apart = 0;
     if (ntiles > 0)
-        fetch(0, (ap_lds *)k0t, (ap_lds *)v0t);
-    for (int t = 0; t < ntiles; t += 2) {
-        step(t, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t, (ap_lds *)v1t);
-        if (t + 1 < ntiles)
-            step(t + 1, (ap_lds *)k1t, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t);
+        fetch(tile(0), (ap_lds *)k0t, (ap_lds *)v0t);
+    for (int u = 0; u < ntiles; u += 2) {
+        step(u, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t, (ap_lds *)v1t);
+        if (u + 1 < ntiles)
+            step(u + 1, (ap_lds *)k1t, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t);
     }
     const float l = glint_xor32(w.l, GlintAdd());
     /* A value that is not finite leaves itself or NaN in its dimension of the rows that see it,
@@ -360,7 +239,7 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const uint32_t v = from[8 * (i >> 2) + (i & 3)];
-                if ((v & 0x7F80u) == 0x7F80u && key <= w.last)
+                if ((v & 0x7F80u) == 0x7F80u && (BOUNDED ? A.bound.sees(key, w.last) : key <= w.last))
                     odd[i] += __uint_as_float(v << 16);
             }
         }
@@ -369,35 +248,17 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
             w.o[d][i] = odd[i] == 0.f ? w.o[d][i] : odd[i];
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    /* 8 dimensions in a lane once its halves have exchanged 4: 16-B stores */
-    uint16_t *dst = A.out + ((q0 + min(row, nq - 1)) * A.Hq + hq) * D + 8 * half;
-#pragma unroll
-    for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-        for (int i = 0; i < 16; i += 8) {
-            glint_u32x4 eight;
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const auto two = __builtin_amdgcn_permlane32_swap(
-                    glint_cvt_bf16x2(w.o[d][i + 2 * x] * inv, w.o[d][i + 2 * x + 1] * inv),
-                    glint_cvt_bf16x2(w.o[d][i + 4 + 2 * x] * inv, w.o[d][i + 5 + 2 * x] * inv), false, false);
-                eight[x] = two[0];
-                eight[2 + x] = two[1];
-            }
-            if (row < nq)
-                *(glint_u32x4 *)(dst + 32 * d + 2 * i) = eight;
-        }
+    ap_store<D>(A.out + ((q0 + min(row, nq - 1)) * A.Hq + hq) * D, w.o, inv, half, row < nq);
 }
 
-GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
-                                  int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
-                                  int64_t v_stride_h, const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk,
-                                  int B, int max_q, int Hq, int H, int D, float scale, uint16_t *out,
-                                  struct ihipStream_t *stream) {
+static int ap_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
+                     int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t, int64_t v_stride_h,
+                     const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk, int B, int max_q, int Hq, int H,
+                     int D, float scale, int window, int sinks, uint16_t *out, hipStream_t stream) {
     if (!q || !k || !v || !cu_q || !cu_k || !out)
         return -1;
     if (B < 0 || B > 65535 || max_q < 0 || max_q > (1 << 30) || H < 1 || Hq < H || Hq > 65535 || Hq % H ||
-        (D != 64 && D != 128) || Tq < 0 || Tk < 0)
+        (D != 64 && D != 128) || Tq < 0 || Tk < 0 || window < 0 || window > GLINT_WINDOW_MAX || sinks < 0)
         return -2;
     if (!glint_aligned(q, 16) || !glint_aligned(k, 16) || !glint_aligned(v, 16) || !glint_aligned(out, 16) ||
         ((q_stride_t | q_stride_h | k_stride_t | k_stride_h | v_stride_t | v_stride_h) & 7) || k_stride_t < D ||
@@ -412,7 +273,7 @@ GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t
         return -2;
     const float scale2 = fabsf(scale) * 1.44269504088896341f;
     ApArgs a{q, k, v, q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk,
-             max_q, Hq, H, Hq / H, nblk, 0, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out};
+             max_q, Hq, H, Hq / H, nblk, 0, scale < 0.f ? 0x80008000u : 0u, scale2 < FLT_MIN ? FLT_MIN : scale2, out, {window, sinks}};
     const int per = a.nblk * a.G;
     for (int64_t b = 0; b < B; b += most) {
         a.cu_q = cu_q + b;
@@ -421,12 +282,34 @@ GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t
         const int rest = a.ngroups & 7; /* 8 % rest == 0: whole rounds of 8 workgroups */
         const int tail = rest == 0 ? 0 : 8 % rest == 0 ? (per + 8 / rest - 1) / (8 / rest) * 8 : rest * per;
         const unsigned grid = (unsigned)((a.ngroups - rest) * per + tail);
-        if (D == 64)
-            k_attend_prompt<64><<<grid, AP_T, 0, stream>>>(a);
+        if (D == 64 && !window)
+            k_attend_prompt<64, false><<<grid, AP_T, 0, stream>>>(a);
+        else if (!window)
+            k_attend_prompt<128, false><<<grid, AP_T, 0, stream>>>(a);
+        else if (D == 64)
+            k_attend_prompt<64, true><<<grid, AP_T, 0, stream>>>(a);
         else
-            k_attend_prompt<128><<<grid, AP_T, 0, stream>>>(a);
+            k_attend_prompt<128, true><<<grid, AP_T, 0, stream>>>(a);
         if (hipGetLastError() != hipSuccess)
             return -3;
     }
     return 0;
+}
+
+GLINT_API int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
+                                  int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
+                                  int64_t v_stride_h, const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk,
+                                  int B, int max_q, int Hq, int H, int D, float scale, uint16_t *out,
+                                  struct ihipStream_t *stream) {
+    return ap_attend(q, q_stride_t, q_stride_h, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk, B,
+                     max_q, Hq, H, D, scale, 0, 0, out, stream);
+}
+
+GLINT_API int glint_attend_prompt_window(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
+                                  int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
+                                  int64_t v_stride_h, const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk,
+                                  int B, int max_q, int Hq, int H, int D, float scale, int window, int sinks, uint16_t *out,
+                                  struct ihipStream_t *stream) {
+    return ap_attend(q, q_stride_t, q_stride_h, k, k_stride_t, k_stride_h, v, v_stride_t, v_stride_h, cu_q, cu_k, Tq, Tk, B,
+                     max_q, Hq, H, D, scale, window, sinks, out, stream);
 }

@@ -12,9 +12,7 @@
  *   128: append 11.1 us (1.9 TB/s; 23 element-wise), gather 10.9 us (2.0 TB/s; 17). Each is a chain
  *   of loads, LDS and stores, so the waves that a CU holds count: tiles of 64 tokens, half as many
  *   workgroups, took 12.0 and 14.2. */
-#include "kv4.h"
-
-#define KV4_T 256
+#include "kv4_tile.h"
 
 template <class E>
 __device__ __forceinline__ void kv4_load4(const E *p, float (&w)[4]);
@@ -33,11 +31,6 @@ __device__ __forceinline__ void kv4_load4(const float *p, float (&w)[4]) {
     w[1] = u.y;
     w[2] = u.z;
     w[3] = u.w;
-}
-
-template <int CTRL>
-__device__ __forceinline__ float kv4_max_dpp(float v) {
-    return fmaxf(v, __int_as_float(glint_dpp<CTRL>(__float_as_int(v))));
 }
 
 template <class E, int D>
@@ -142,55 +135,7 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_gather(const int64_t *__restrict_
     }
 }
 
-/* ------------------------------------------------------------------ tiles
- * 32 tokens of one head a workgroup. A value column lies a byte a token, 64 B apart, so values
- * pass through LDS: columns there are shifted by the first token's place modulo 4, so that four
- * tokens whose slots follow each other, as a prompt's do, are one aligned word on both sides;
- * other tokens go byte by byte. */
-#define KT_TOKENS 32
-#define KT_COLS (KT_TOKENS + 4) /* the shift */
-#define KT_GROUPS (KT_COLS / 4)
-
-/* The slots of a tile, by shifted column; -1 where there is no token. */
-__device__ __forceinline__ int kt_slots(const int64_t *slots, int64_t t0, int64_t T, int64_t nslots, int64_t *place) {
-    const int64_t first = slots[t0];
-    const int shift = first >= 0 && first < nslots ? (int)(first & 3) : 0;
-    for (int c = threadIdx.x; c < KT_COLS; c += KV4_T) {
-        const int64_t t = t0 + c - shift;
-        const int64_t s = c >= shift && c - shift < KT_TOKENS && t < T ? slots[t] : -1;
-        place[c] = s < nslots ? s : -1;
-    }
-    return shift;
-}
-/* Whether columns c .. c + 3 are four slots in a row, the first a multiple of 4: its place, or -1. */
-__device__ __forceinline__ int64_t kt_word(const int64_t *place, int c) {
-    const int64_t s = place[c];
-    return s >= 0 && (s & 3) == 0 && place[c + 1] == s + 1 && place[c + 2] == s + 2 && place[c + 3] == s + 3 ? s : -1;
-}
-
-template <int D>
-__device__ __forceinline__ void kt_load8(const uint16_t *p, float (&w)[8]) {
-    const glint_u32x4 u = *(const glint_u32x4 *)p;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        w[2 * i] = glint_bf16lo(u[i]);
-        w[2 * i + 1] = glint_bf16hi(u[i]);
-    }
-}
-template <int D>
-__device__ __forceinline__ void kt_load8(const float *p, float (&w)[8]) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const glint_f32x4 u = ((const glint_f32x4 *)p)[i];
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-            w[4 * i + k] = u[k];
-    }
-}
-
-/* A row of 8 lanes encodes a 64-block, 8 dimensions a lane: their quotients by one multiply where the
- * input is BF16 and the absmax ordinary (no code differs from the divide's, see
- * tests/native/check_encode_quotient.c), by the divide elsewhere. */
+/* ------------------------------------------------------------------ tiles (kv4_tile.h) */
 template <class E, int D>
 __global__ __launch_bounds__(KV4_T) void k_kv4_append_tile(const E *__restrict__ k, const E *__restrict__ v, int64_t k_st,
                                                            int64_t k_sh, int64_t v_st, int64_t v_sh,
@@ -220,24 +165,8 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_append_tile(const E *__restrict__
 #pragma unroll
         for (int i = 0; i < PASSES; ++i) {
             const int item = r + i * ROWS, j = item / NB, b = item % NB, c = j + shift;
-            float s = 0.f; /* fmaxf leaves NaN out */
-#pragma unroll
-            for (int x = 0; x < 8; ++x)
-                s = fmaxf(s, fabsf(w[i][x]));
-            s = kv4_max_dpp<GLINT_DPP_QUAD_1032>(s);
-            s = kv4_max_dpp<GLINT_DPP_QUAD_2301>(s);
-            s = kv4_max_dpp<GLINT_DPP_ROW_HALF_MIRROR>(s);
-            uint32_t code = 0; /* 8 nibbles */
-            if (sizeof(E) == 2 && s >= 0x1p-90f && s < 0x1p90f) {
-                const float inv = 1.f / s;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) /* NaN among them: an absmax that leaves it out is no bound for it */
-                    code |= kv4_code(buckets, w[i][x] * inv) << (4 * x);
-            } else {
-#pragma unroll
-                for (int x = 0; x < 8; ++x)
-                    code |= kv4_code(buckets, s == 0.f ? 0.f : w[i][x] / s) << (4 * x);
-            }
+            float s;
+            const uint32_t code = kt_code8<sizeof(E) == 2>(buckets, w[i], s);
             const int64_t slot = place[c];
             if (e == 0)
                 scale[is_v][b][c] = s;
@@ -246,33 +175,12 @@ __global__ __launch_bounds__(KV4_T) void k_kv4_append_tile(const E *__restrict__
                     *(uint32_t *)(k_hole + (((slot >> 6) * H + h) * KV4_PAGE + (slot & 63)) * (D / 2) +
                                   kv4_k_byte<NB>(64 * b + 8 * e)) = code;
             } else {
-                /* dimensions 16 on are two lanes on; this lane writes four of the pair's rows */
-                const uint32_t other = (uint32_t)glint_dpp<GLINT_DPP_QUAD_2301>((int)code);
-                const int up = e & 2 ? 16 : 0;
-                const uint32_t lo = (e & 2 ? other : code) >> up, hi = (e & 2 ? code : other) >> up;
-                uint8_t *row = vt + (kv4_v_row(64 * b + 8 * (e & ~2)) + (e & 2 ? 4 : 0)) * KT_COLS + c;
-#pragma unroll
-                for (int x = 0; x < 4; ++x)
-                    row[x * KT_COLS] = (uint8_t)(((lo >> (4 * x)) & 15u) | ((hi >> (4 * x)) & 15u) << 4);
+                kt_put_value<KT_COLS>(vt + c, 64 * b, e, code);
             }
         }
     }
     __syncthreads();
-    for (int u = threadIdx.x; u < (D / 2) * KT_GROUPS; u += KV4_T) {
-        const int row = u / KT_GROUPS, c = 4 * (u % KT_GROUPS);
-        const uint32_t word = *(const uint32_t *)(vt + row * KT_COLS + c);
-        const int64_t s = kt_word(place, c);
-        if (s >= 0) {
-            *(uint32_t *)(v_hole + (((s >> 6) * H + h) * (D / 2) + row) * KV4_PAGE + (s & 63)) = word;
-        } else {
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int64_t p = place[c + x];
-                if (p >= 0)
-                    v_hole[(((p >> 6) * H + h) * (D / 2) + row) * KV4_PAGE + (p & 63)] = (uint8_t)(word >> (8 * x));
-            }
-        }
-    }
+    kt_store_values<D>(vt, place, h, H, v_hole);
     for (int u = threadIdx.x; u < 2 * NB * KT_COLS; u += KV4_T) {
         const int c = u % KT_COLS, b = u / KT_COLS % NB, is_v = u / (KT_COLS * NB);
         const int64_t p = place[c];

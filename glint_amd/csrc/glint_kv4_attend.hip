@@ -63,13 +63,6 @@ typedef glint_f32x4 kv4_lds_f32x4 __attribute__((may_alias));
 #define KA_SWITCH 8
 #define KA_COPIES 32 /* of an entry; entries are 64 words apart, so that an address is one byte permute */
 #define KA_TABLE_WORDS (256 * 64)
-/* The table holds PARENT * KA_ALPHA, whose f16 roundings are smaller and cancel: over the code
- * frequencies of normal values under a block-64 absmax (sigma 0.25 to 0.6 of it) and of even
- * ones, the mean error is at most 1.8e-6 of the absmax and the rms 3.9e-5, where PARENT's own
- * are 1.6e-5 and 9.5e-5. The mean counts: it is all that is left of the values' rounding in
- * the output of a long row, and at 8192 tokens of equal weight it alone was 0.8 of the bf16
- * output's rounding. */
-#define KA_ALPHA 1.458935f
 #define KA_VMAX 15 /* a scaled weight stays below 2^KA_VMAX */
 #define KA_VSTART 10
 #define KA_FAR (1 << 24) /* a page number past every sequence's: tables hold no more pages */
@@ -90,11 +83,12 @@ struct Kv4AttendArgs {
     int max_pages;
     const int32_t *lens, *cu_q;
     int B, max_q, Hq, H, G;
-    float scale2;    /* |scale| log2 e / KA_ALPHA, above 0 */
+    float scale2;    /* |scale| log2 e / KV4_ALPHA, above 0 */
     uint32_t q_sign; /* 0x80008000 where the scale is negative */
     uint16_t *out;
     float *part; /* two partials per workgroup; NULL: groups are not split */
     unsigned *ctr;
+    int window, sinks; /* of the bounded form: positions up to a row's own that it sees, and first ones */
 };
 
 /* A sequence's rows and length, with every device value bounded. */
@@ -116,11 +110,13 @@ __device__ __forceinline__ Kv4Raw kv4_raw(const Kv4AttendArgs &a, int b) {
 }
 struct Kv4Seq : Kv4Raw {
     int rows, npages;
+    int sink_pages, skip; /* of the bounded form: page i of the npages is the sequence's page i, or, past the sinks', i + skip */
     int rounds; /* of a group */
     int blocks; /* row blocks */
     int all;    /* rounds of all its groups */
     int cost;   /* of a group: KA_WAVES a round, and KA_SWITCH for turning to it */
 };
+template <bool BOUNDED>
 __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttendArgs &a, const Kv4Raw &r) {
     Kv4Seq s;
     s.q0 = r.q0;
@@ -128,6 +124,12 @@ __device__ __forceinline__ Kv4Seq kv4_seq(const Kv4AttendArgs &a, const Kv4Raw &
     s.len = r.len;
     s.rows = a.G * min(s.nq, a.max_q);
     s.npages = (s.len + KV4_PAGE - 1) / KV4_PAGE;
+    s.sink_pages = s.skip = 0;
+    if (BOUNDED) { /* up to the page that the first row's window begins in: a page at most of what is past */
+        s.sink_pages = (min(a.sinks, s.len) + KV4_PAGE - 1) / KV4_PAGE;
+        s.skip = max(0, (int)(max((int64_t)0, (int64_t)s.len - s.nq - a.window + 1) / KV4_PAGE) - s.sink_pages);
+        s.npages -= s.skip;
+    }
     s.rounds = (s.npages + KA_WAVES - 1) / KA_WAVES;
     s.blocks = (s.rows + KA_ROWS - 1) / KA_ROWS;
     s.all = s.rounds * s.blocks * a.H;
@@ -195,7 +197,10 @@ __device__ __forceinline__ uint16_t *kv4_out(const Kv4AttendArgs &a, int q0, int
     return a.out + ((int64_t)(q0 + r / a.G) * a.Hq + h * a.G + r % a.G) * D;
 }
 
-template <int D>
+/* BOUNDED: a row sees the last `window` positions up to its own and the first `sinks`. The list holds the
+ * pages that a sequence's rows see, so that what lies between costs nothing, and its numbers in the table are
+ * not read. */
+template <int D, bool BOUNDED>
 __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     constexpr int NB = D / 64;
     constexpr int ROW = D + 4; /* a row's output, then its maximum and sum */
@@ -213,7 +218,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     /* The table, while they are on their way: thread t writes four copies of the entries t / 8 + 64 i. */
     static_assert(KA_T == 512 && KA_COPIES == 32, "the table's shares");
     {
-        const float lo = kKv4Parent[(threadIdx.x >> 3) & 15] * KA_ALPHA;
+        const float lo = kKv4Parent[(threadIdx.x >> 3) & 15] * KV4_ALPHA;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             union {
@@ -221,7 +226,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                 uint32_t u;
             } e;
             e.f[0] = (_Float16)lo;
-            e.f[1] = (_Float16)(kKv4Parent[(wave >> 1) + 4 * i] * KA_ALPHA);
+            e.f[1] = (_Float16)(kKv4Parent[(wave >> 1) + 4 * i] * KV4_ALPHA);
             ((glint_u32x4 *)lds)[((threadIdx.x >> 3) + 64 * i) * 16 + (threadIdx.x & 7)] = glint_u32x4{e.u, e.u, e.u, e.u};
         }
     }
@@ -234,7 +239,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         r.q0 = __builtin_amdgcn_readlane(raw.q0, b - chunk);
         r.nq = __builtin_amdgcn_readlane(raw.nq, b - chunk);
         r.len = __builtin_amdgcn_readlane(raw.len, b - chunk);
-        return kv4_seq(A, r);
+        return kv4_seq<BOUNDED>(A, r);
     };
     auto scan = [](int v) { /* of the lanes up to this one: row_shr 1, 2, 4, 8, row_bcast 15, 31 */
         v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);
@@ -265,7 +270,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     auto weight = [&](const Kv4Seq &s) { return (A.part ? s.cost : s.cost > 0 ? 1 : 0) * s.blocks * A.H; };
     int mine = 0, mine_rounds = 0;
     for (int i = 0; i < per; ++i) {
-        const Kv4Seq s = kv4_seq(A, per == 1 ? raw : kv4_raw(A, lane * per + i));
+        const Kv4Seq s = kv4_seq<BOUNDED>(A, per == 1 ? raw : kv4_raw(A, lane * per + i));
         mine += weight(s);
         mine_rounds += s.all;
     }
@@ -351,7 +356,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
     auto open_window = [&](int b, int at, int k) {
         if (b < chunk || b - chunk >= 48)
             to_chunk(b);
-        const int all = lane >= b - chunk ? kv4_seq(A, raw).all : 0;
+        const int all = lane >= b - chunk ? kv4_seq<BOUNDED>(A, raw).all : 0;
         const int sum = scan(all) - at; /* rounds from here to the lane's sequence's end */
         int j = b - chunk;                /* the lane whose sequence holds this lane's round */
         if (run - k > __builtin_amdgcn_readlane(sum, j)) {
@@ -364,10 +369,11 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         const int sum_j = __shfl(sum, j, 64);
         const Kv4Raw r{0, __shfl(raw.nq, j, 64), __shfl(raw.len, j, 64)};
         const bool in = lane < run - k && lane < sum_j;
-        const Kv4Seq s = kv4_seq(A, r);
+        const Kv4Seq s = kv4_seq<BOUNDED>(A, r);
         const int in_seq = lane - (sum_j - s.all);
         const int pg = in_seq % max(s.rounds, 1) * KA_WAVES + wave;
-        pids = in && pg < s.npages ? A.table[(int64_t)(chunk + j) * A.table_stride + pg] : -1;
+        const int at_page = BOUNDED && pg >= s.sink_pages ? pg + s.skip : pg;
+        pids = in && pg < s.npages ? A.table[(int64_t)(chunk + j) * A.table_stride + at_page] : -1;
         pids = pids < A.pages ? pids : -1;
         window = k;
         window_n = __builtin_popcountll(__ballot(in));
@@ -472,7 +478,9 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
 
         for (int i = 0; i < G.n; ++i) {
             /* a page that nobody sees lies past every row's last position */
-            const int pg = there ? (G.begin + i) * KA_WAVES + wave : KA_FAR;
+            int pg = there ? (G.begin + i) * KA_WAVES + wave : KA_FAR;
+            if (BOUNDED && there && pg >= s.sink_pages)
+                pg += s.skip;
             /* The run's last page is loaded again: without a branch around them the next page's
              * loads can be counted, and this page's waits leave them in flight. */
             const int k = G.k + i + 1;
@@ -486,7 +494,8 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             /* A whole page lies below every row's last position: nothing of it is masked, and the
              * rows have one power for its value scales, which go to LDS scaled and rounded to f16.
              * Of another page they go there as they are. */
-            const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
+            const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1 &&
+                               (!BOUNDED || pg * KV4_PAGE >= s.len - A.window || (pg + 1) * KV4_PAGE <= A.sinks);
             glint_f32x4 sc[4]; /* scores, without the row's factor */
             if (pg != KA_FAR) {
 #pragma unroll
@@ -537,12 +546,13 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             load_k();
             if (pg != KA_FAR) {
                 const int t0 = pg * KV4_PAGE + 16 * g;
+                auto seen = [&](int t) { return t <= last && (!BOUNDED || t > last - A.window || t < A.sinks); };
                 if (!whole) { /* what the row does not see */
 #pragma unroll
                     for (int a = 0; a < 4; ++a)
 #pragma unroll
                         for (int x = 0; x < 4; ++x)
-                            sc[a][x] = t0 + 4 * a + x <= last ? sc[a][x] : -INFINITY;
+                            sc[a][x] = seen(t0 + 4 * a + x) ? sc[a][x] : -INFINITY;
                 }
 
                 /* softmax weights */
@@ -597,7 +607,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                             vscale[a] = *(const kv4_lds_f32x4 *)(sl + (NB + bb) * KV4_PAGE + 16 * g + 4 * a);
 #pragma unroll
                             for (int x = 0; x < 4; ++x) { /* an unseen place counts as 0, whatever it holds */
-                                const float v = t0 + 4 * a + x <= last ? vscale[a][x] : 0.f;
+                                const float v = seen(t0 + 4 * a + x) ? vscale[a][x] : 0.f;
                                 vscale[a][x] = v;
                                 any = fmaxf(any, v);
                                 finite = fmaxf(finite, v < INFINITY ? v : 0.f);
@@ -654,7 +664,7 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
         float *row = meet + (wave * KA_ROWS + col) * ROW;
 #pragma unroll
         for (int d = 0; d < D / 16; ++d) {
-            const float back = 1.f / vdown[d >> 2] * (1.f / KA_ALPHA); /* a power of two, inverted exactly */
+            const float back = 1.f / vdown[d >> 2] * (1.f / KV4_ALPHA); /* a power of two, inverted exactly */
             *(glint_f32x4 *)(row + 16 * d + 4 * g) = glint_f32x4{o[d][0] * back, o[d][1] * back, o[d][2] * back, o[d][3] * back};
         }
         if (g == 0) {
@@ -799,25 +809,25 @@ GLINT_API int glint_serve_workspace_reserve(struct ihipStream_t *stream) {
 }
 GLINT_API int glint_serve_workspace_release(struct ihipStream_t *stream) { return glint_split_ws_release(stream); }
 
-GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq,
+static int ka_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq,
                                const uint8_t *k_hole, const float *k_absmax, const uint8_t *v_hole,
                                const float *v_absmax, int64_t pages, const int32_t *table, int64_t table_stride,
                                int max_pages, const int32_t *lens, const int32_t *cu_q, int B, int max_q, int Hq, int H,
-                               int D, float scale, uint16_t *out, struct ihipStream_t *stream) {
+                               int D, float scale, int window, int sinks, uint16_t *out, hipStream_t stream) {
     if (!q || !k_hole || !k_absmax || !v_hole || !v_absmax || !table || !lens || !out)
         return -1;
     if (!ka_shape(B, max_q, Hq, H, D, max_pages) || Tq < 0 || Tq > INT32_MAX || pages < 1 || pages >= (int64_t)1 << 40 ||
-        (!cu_q && Tq != (int64_t)B * max_q))
+        (!cu_q && Tq != (int64_t)B * max_q) || window < 0 || window > GLINT_WINDOW_MAX || sinks < 0)
         return -2;
     if (!glint_aligned(q, 16) || !glint_aligned(out, 8) || !glint_aligned(k_hole, 16) || !glint_aligned(v_hole, 16) ||
         !glint_aligned(k_absmax, 16) || !glint_aligned(v_absmax, 16) || ((q_stride_t | q_stride_h) & 7))
         return -2;
     if (B == 0 || Tq == 0)
         return 0;
-    const float scale2 = fabsf(scale) * (1.44269504088896341f / KA_ALPHA);
+    const float scale2 = fabsf(scale) * (1.44269504088896341f / KV4_ALPHA);
     Kv4AttendArgs a{q, q_stride_t, q_stride_h, Tq, k_hole, v_hole, k_absmax, v_absmax, pages, table, table_stride,
                     max_pages, lens, cu_q, B, max_q, Hq, H, Hq / H, scale2 < FLT_MIN ? FLT_MIN : scale2,
-                    scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr};
+                    scale < 0.f ? 0x80008000u : 0u, out, nullptr, nullptr, window, sinks};
     int64_t most;
     const int64_t groups = ka_groups(max_q, H, a.G, max_pages, most), cus = glint_cu_count();
     if (most < 1)
@@ -846,12 +856,35 @@ GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_
         int64_t grid = a.B * groups;
         if (a.part)
             grid = std::min<int64_t>((grid * (max_pages + KA_WAVES + KA_SWITCH) + KA_WAVES - 1) / KA_WAVES, cus);
-        if (D == 64)
-            k_kv4_attend<64><<<(unsigned)grid, KA_T, 0, stream>>>(a);
+        const unsigned g = (unsigned)grid;
+        if (D == 64 && !window)
+            k_kv4_attend<64, false><<<g, KA_T, 0, stream>>>(a);
+        else if (!window)
+            k_kv4_attend<128, false><<<g, KA_T, 0, stream>>>(a);
+        else if (D == 64)
+            k_kv4_attend<64, true><<<g, KA_T, 0, stream>>>(a);
         else
-            k_kv4_attend<128><<<(unsigned)grid, KA_T, 0, stream>>>(a);
+            k_kv4_attend<128, true><<<g, KA_T, 0, stream>>>(a);
         if (hipGetLastError() != hipSuccess)
             return -3;
     }
     return 0;
+}
+
+GLINT_API int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq,
+                               const uint8_t *k_hole, const float *k_absmax, const uint8_t *v_hole,
+                               const float *v_absmax, int64_t pages, const int32_t *table, int64_t table_stride,
+                               int max_pages, const int32_t *lens, const int32_t *cu_q, int B, int max_q, int Hq, int H,
+                               int D, float scale, uint16_t *out, struct ihipStream_t *stream) {
+    return ka_attend(q, q_stride_t, q_stride_h, Tq, k_hole, k_absmax, v_hole, v_absmax, pages, table, table_stride, max_pages,
+                     lens, cu_q, B, max_q, Hq, H, D, scale, 0, 0, out, stream);
+}
+
+GLINT_API int glint_kv4_attend_window(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq,
+                               const uint8_t *k_hole, const float *k_absmax, const uint8_t *v_hole,
+                               const float *v_absmax, int64_t pages, const int32_t *table, int64_t table_stride,
+                               int max_pages, const int32_t *lens, const int32_t *cu_q, int B, int max_q, int Hq, int H,
+                               int D, float scale, int window, int sinks, uint16_t *out, struct ihipStream_t *stream) {
+    return ka_attend(q, q_stride_t, q_stride_h, Tq, k_hole, k_absmax, v_hole, v_absmax, pages, table, table_stride, max_pages,
+                     lens, cu_q, B, max_q, Hq, H, D, scale, window, sinks, out, stream);
 }

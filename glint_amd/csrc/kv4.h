@@ -58,6 +58,14 @@ __device__ __forceinline__ uint32_t kv4_code(const Kv4Bucket *t, float v) { /* |
     return e.base + (v > e.edge ? 1u : 0u);
 }
 
+/* The attention kernels' table holds PARENT * KV4_ALPHA, whose f16 roundings are smaller and cancel: over the code
+ * frequencies of normal values under a block-64 absmax (sigma 0.25 to 0.6 of it) and of even
+ * ones, the mean error is at most 1.8e-6 of the absmax and the rms 3.9e-5, where PARENT's own
+ * are 1.6e-5 and 9.5e-5. The mean counts: it is all that is left of the values' rounding in
+ * the output of a long row, and at 8192 tokens of equal weight it alone was 0.8 of the bf16
+ * output's rounding. */
+#define KV4_ALPHA 1.458935f
+
 /* Byte of dimension pair (d, d + 1), d even, in a key row of NB blocks. */
 template <int NB>
 __host__ __device__ __forceinline__ int kv4_k_byte(int d) {

@@ -121,10 +121,21 @@ _SERVE_SIGS = {
     "glint_kv4_gather": ([VP, I64, I32, I32, VP, VP, VP, VP, I64, VP, VP, VP], I32),
     "glint_kv4_attend": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32,
                           _c.c_float, VP, VP], I32),
+    "glint_kv4_attend_window": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32,
+                                 _c.c_float, I32, I32, VP, VP], I32),
+    "glint_kv4_attend_chunk_scratch": ([I32, I32, I32, I32, I32, I32], I64),
+    "glint_kv4_attend_chunk": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32, VP, I64,
+                                I64, VP, I64, I64, _c.c_float, I32, I32, VP, VP, I64, VP], I32),
     "glint_serve_workspace_reserve": ([VP], I32),
     "glint_serve_workspace_release": ([VP], I32),
     "glint_attend_prompt": ([VP, I64, I64, VP, I64, I64, VP, I64, I64, VP, VP, I64, I64, I32, I32, I32, I32, I32,
                              _c.c_float, VP, VP], I32),
+    "glint_attend_prompt_window": ([VP, I64, I64, VP, I64, I64, VP, I64, I64, VP, VP, I64, I64, I32, I32, I32, I32, I32,
+                                    _c.c_float, I32, I32, VP, VP], I32),
+    "glint_rotate_qk": ([VP, I64, I64, VP, I64, I64, I32, VP, VP, I64, I32, I32, I32, I32, I32, _c.c_double, VP, VP, I32,
+                         _c.c_float, VP, VP, VP], I32),
+    "glint_kv4_append_rotated": ([VP, I64, I64, VP, I64, I64, VP, I64, I64, I32, VP, VP, VP, I64, I32, I32, I32, I32, I32,
+                                  _c.c_double, VP, VP, I32, _c.c_float, VP, VP, VP, VP, VP, VP, I64, VP], I32),
     "glint_token_logprobs": ([VP, I32, I64, VP, I64, I64, I32, VP, VP, VP, VP, VP, VP], I32),
 }
 
@@ -636,18 +647,31 @@ def kv4_gather(slots, cache, out=None, stream=None):
     return k, v
 
 
+def _bounds(window: Optional[int], sinks: int):
+    """window and sinks as the C entry points take them."""
+    if window is None:
+        if sinks:
+            raise ValueError(f"{sinks} sinks without a window")
+        return 0, 0
+    if not 1 <= window <= 1 << 30 or sinks < 0:
+        raise ValueError(f"window {window}, sinks {sinks}: a window of 1 .. 2^30, sinks of 0 or more")
+    return window, min(sinks, (1 << 31) - 1)
+
+
 def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: Optional[int] = None, scale: Optional[float] = None, out=None,
-               stream=None):
+               stream=None, *, window: Optional[int] = None, sinks: int = 0):
     """Attention of the newest tokens over the cache: q bf16 [rows, Hq, D] -> bf16 [rows, Hq, D].
 
     page_table int32 [B, max_pages] and lens int32 [B] (tokens in the cache, the new ones
     included) say what each sequence sees; its rows are cu_q[b] .. cu_q[b + 1] (int32, at most
     max_q each: all rows where None), or max_q each (1 where None) where cu_q is None. A row sees
-    the positions up to its own. Rows past max_q, or of no sequence, are not written: they hold
-    what `out` held, anything where it is None."""
+    the positions up to its own; with a window, the last `window` of them and the first `sinks`
+    positions, and pages that no row sees may have left the table. Rows past max_q, or of no sequence,
+    are not written: they hold what `out` held, anything where it is None."""
     if stream is not None:
         with _torch().cuda.stream(stream):
-            return kv4_attend(q, cache, page_table, lens, cu_q, max_q, scale, out)
+            return kv4_attend(q, cache, page_table, lens, cu_q, max_q, scale, out, window=window, sinks=sinks)
+    window, sinks = _bounds(window, sinks)
     torch = _TORCH or _torch()
     pages, heads, dim, *planes = _planes(cache)
     rows, hq, d = q.shape
@@ -672,10 +696,65 @@ def kv4_attend(q, cache, page_table, lens, cu_q=None, max_q: Optional[int] = Non
         return out
     if wide == 0:  # nobody has a page
         page_table, wide = page_table.new_full((B, 1), -1), 1
-    _check(serve_lib().glint_kv4_attend(q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(),
-                                        page_table.stride(0), wide, n, cu, B, max_q, hq, heads, dim,
-                                        dim ** -0.5 if scale is None else scale, out.data_ptr(), _sh(None)),
-           "glint_kv4_attend")
+    _check(serve_lib().glint_kv4_attend_window(q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(),
+                                               page_table.stride(0), wide, n, cu, B, max_q, hq, heads, dim,
+                                               dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                               _sh(None)), "glint_kv4_attend")
+    return out
+
+
+def kv4_attend_chunk(q, cache, page_table, lens, cu_q=None, max_q: Optional[int] = None, scale: Optional[float] = None,
+                     out=None, stream=None, *, k=None, v=None, window: Optional[int] = None, sinks: int = 0):
+    """kv4_attend for many new tokens a sequence: arguments, masks and result as there.
+
+    k, v bf16 [rows, H, D], both or neither: the new tokens' own keys and values, seen in place of what the
+    cache holds of them (which may then be nothing)."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return kv4_attend_chunk(q, cache, page_table, lens, cu_q, max_q, scale, out, k=k, v=v, window=window, sinks=sinks)
+    torch = _TORCH or _torch()
+    window, sinks = _bounds(window, sinks)
+    _here(q, page_table, lens, cu_q, k, v, out, *cache)
+    pages, heads, dim, *planes = _planes(cache)
+    rows, hq, d = q.shape
+    B, wide = page_table.shape
+    if d != dim or hq % heads:
+        raise ValueError(f"q {tuple(q.shape)}, cache of {heads} heads of {dim}")
+    if (k is None) != (v is None):
+        raise ValueError("k and v: both or neither")
+    if k is not None and not k.shape == v.shape == (rows, heads, dim):
+        raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)}: both {(rows, heads, dim)}")
+    if any(t is not None and t.dtype is not torch.bfloat16 for t in (q, k, v)):
+        raise TypeError(f"expected bfloat16, got {', '.join(str(t.dtype) for t in (q, k, v) if t is not None)}")
+    if max_q is None:
+        max_q = max(rows, 1) if cu_q is not None else 1
+    if max_q < 1 or (cu_q is None and rows != B * max_q):
+        raise ValueError(f"{rows} query rows, {B} sequences of {max_q}")
+    if page_table.dtype is not torch.int32 or (page_table.stride(1) != 1 and wide > 1):
+        raise ValueError("page_table: int32 with adjacent columns")
+    n = _ints(lens, torch.int32, B, "lens")
+    cu = None if cu_q is None else _ints(cu_q, torch.int32, B + 1, "cu_q")
+    q, qt, qh = _rows(q, 8)
+    kt = kh = vt = vh = 0
+    if k is not None:
+        k, kt, kh = _rows(k, 8, dim, 1 << 24)
+        v, vt, vh = _rows(v, 8, dim, 1 << 24)
+    if out is not None and out.data_ptr() % 16:
+        raise ValueError("out: 16-B aligned")
+    out = _attend_out(out, q, rows, hq, dim)
+    if rows == 0 or B == 0:
+        return out
+    if wide == 0:  # nobody has a page
+        page_table, wide = page_table.new_full((B, 1), -1), 1
+    size = serve_lib().glint_kv4_attend_chunk_scratch(B, max_q, hq, heads, dim, wide)
+    if size < 0:
+        raise ValueError(f"{max_q} new tokens a sequence, {hq} heads over {heads}, {wide} pages: more than a launch can hold")
+    scratch = q.new_empty(size, dtype=torch.uint8)
+    _check(serve_lib().glint_kv4_attend_chunk(
+        q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(), page_table.stride(0), wide, n, cu, B, max_q, hq,
+        heads, dim, None if k is None else k.data_ptr(), kt, kh, None if v is None else v.data_ptr(), vt, vh,
+        dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), scratch.data_ptr(), size, _sh(None)),
+        "glint_kv4_attend_chunk")
     return out
 
 
@@ -688,16 +767,17 @@ def _attend_out(out, q, rows: int, hq: int, dim: int):
 
 
 def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: Optional[float] = None, out=None,
-                  stream=None):
+                  stream=None, *, window: Optional[int] = None, sinks: int = 0):
     """Causal attention over packed sequences: q bf16 [Tq, Hq, D], k and v bf16 [Tk, H, D] -> bf16 [Tq, Hq, D].
 
     cu_q, cu_k int32 [B + 1]: where each sequence's queries and keys start (cu_k is cu_q where
-    None); a sequence's last query sees its last key. max_q: no sequence has more queries
-    (Tq where None). Queries past max_q, or of no sequence, are not written: they hold what `out`
+    None); a sequence's last query sees its last key. With a window a query sees the last `window`
+    keys up to its own and its sequence's first `sinks`. max_q: no sequence has more queries (Tq where None). Queries past max_q, or of no sequence, are not written: they hold what `out`
     held, anything where it is None."""
     if stream is not None:
         with _torch().cuda.stream(stream):
-            return attend_prompt(q, k, v, cu_q, cu_k, max_q, scale, out)
+            return attend_prompt(q, k, v, cu_q, cu_k, max_q, scale, out, window=window, sinks=sinks)
+    window, sinks = _bounds(window, sinks)
     torch = _TORCH or _torch()
     Tq, hq, dim = q.shape
     Tk, heads, _ = k.shape
@@ -718,11 +798,125 @@ def attend_prompt(q, k, v, cu_q, cu_k=None, max_q: Optional[int] = None, scale: 
         return out
     if Tk == 0:  # an address for the kernel, which reads no key
         k, v = q, q
-    _check(serve_lib().glint_attend_prompt(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cq, ck, Tq,
-                                           Tk, B, Tq if max_q is None else max_q, hq, heads, dim,
-                                           dim ** -0.5 if scale is None else scale, out.data_ptr(), _sh(None)),
-           "glint_attend_prompt")
+    _check(serve_lib().glint_attend_prompt_window(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, cq, ck,
+                                                  Tq, Tk, B, Tq if max_q is None else max_q, hq, heads, dim,
+                                                  dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+                                                  _sh(None)), "glint_attend_prompt")
     return out
+
+
+def rotary_freqs(rot: int, base: float = 10000.0, factor: float = 1.0, trained: Optional[int] = None, slow: float = 1.0,
+                 fast: float = 4.0, device="cuda"):
+    """Frequencies for rotate_qk, float64 [rot / 2] in radians a position: base^(-2 i / rot), divided by
+    `factor`; with `trained` (a context length) only those that turn less than `slow` times in it, while those
+    that turn `fast` times or more stay and the ones between are mixed. Any others do as well."""
+    torch = _torch()
+    if rot < 16 or rot % 16:
+        raise ValueError(f"{rot} turned dimensions: a multiple of 16")
+    f = base ** (torch.arange(rot // 2, dtype=torch.float64) * (-2.0 / rot))
+    keep = torch.zeros_like(f)
+    if trained is not None:
+        if not fast > slow:
+            raise ValueError(f"turns from {slow} to {fast}")
+        keep = ((trained * f / 6.283185307179586 - slow) / (fast - slow)).clamp(0, 1)
+    return (f * keep + f / factor * (1 - keep)).to(device)
+
+
+def _here(*tensors) -> None:
+    """Refuses tensors that are not on the current device; None among them is no tensor."""
+    at = (_TORCH or _torch()).cuda.current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t is not None and (at < 0 or t.get_device() != at):
+            raise ValueError(f"a tensor on {t.device}: all must be on the current GPU")
+
+
+def _turn_args(q, k, pos, freqs, q_norm, k_norm):
+    """What rotate_qk and kv4_append_rotated have in common: (elt, T, Hq, H, D, rot, pos, freqs, the norms' pointers and type)."""
+    torch = _TORCH or _torch()
+    T, hq, dim = q.shape
+    if k.dim() != 3 or k.shape[0] != T or k.shape[2] != dim or k.dtype is not q.dtype:
+        raise ValueError(f"q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}")
+    elt, rot = _kv_elt(q), 2 * freqs.numel()
+    if dim % 16 or not 16 <= dim <= 256 or rot % 16 or not 16 <= rot <= dim:
+        raise ValueError(f"head dimension {dim}, {rot} of it turned: multiples of 16, at most 256")
+    at, fr = _ints(pos, torch.int64, T, "pos"), _ints(freqs, torch.float64, rot // 2, "freqs")
+    norm_elt = 0
+    for w in (q_norm, k_norm):
+        if w is not None:
+            if w.shape != (dim,) or not w.is_contiguous() or w.data_ptr() % 16:
+                raise ValueError(f"a norm: a contiguous, 16-B aligned vector of {dim}, got {tuple(w.shape)}")
+            norm_elt = _kv_elt(w)
+    if q_norm is not None and k_norm is not None and q_norm.dtype is not k_norm.dtype:
+        raise TypeError(f"norms of {q_norm.dtype} and {k_norm.dtype}")
+    return (elt, T, hq, k.shape[1], dim, rot, at, fr, None if q_norm is None else q_norm.data_ptr(),
+            None if k_norm is None else k_norm.data_ptr(), norm_elt)
+
+
+def _turn_out(out, like, shape):
+    if out is None:
+        return like.new_empty(shape)
+    if out.shape != shape or out.dtype is not like.dtype or not out.is_contiguous() or out.data_ptr() % 16 or \
+            out.device != like.device:
+        raise ValueError(f"out: a contiguous, 16-B aligned {like.dtype} tensor of {shape} beside q and k")
+    return out
+
+
+def rotate_qk(q, k, pos, freqs, *, interleaved: bool = False, magnitude: float = 1.0, q_norm=None, k_norm=None,
+              eps: float = 1e-6, out=None, stream=None):
+    """Queries [T, Hq, D] and keys [T, H, D] (bf16 or f32), normed per head and turned to positions pos [T]
+    (int64): (q, k) of the same types and shapes.
+
+    freqs float64 [rot / 2] (rotary_freqs, or any): the first rot dimensions turn, pair i by the angle
+    pos * freqs[i], pairs being (i, i + rot / 2), or (2 i, 2 i + 1) where interleaved; turned dimensions are
+    multiplied by `magnitude`. q_norm, k_norm [D] (bf16 or f32): each row is first divided by the root of its mean
+    square (plus eps) and multiplied by them; None: as it is. out: (q, k) to write, which may be the inputs
+    where those are contiguous."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return rotate_qk(q, k, pos, freqs, interleaved=interleaved, magnitude=magnitude, q_norm=q_norm, k_norm=k_norm,
+                             eps=eps, out=out)
+    _here(q, k, pos, freqs, q_norm, k_norm)
+    elt, T, hq, heads, dim, rot, at, fr, qn, kn, ne = _turn_args(q, k, pos, freqs, q_norm, k_norm)
+    q_out, k_out = (None, None) if out is None else out
+    q_out, k_out = _turn_out(q_out, q, (T, hq, dim)), _turn_out(k_out, k, (T, heads, dim))
+    if T == 0:
+        return q_out, k_out
+    q, qt, qh = _rows(q, 4 if elt else 8)
+    k, kt, kh = _rows(k, 4 if elt else 8)
+    _check(serve_lib().glint_rotate_qk(q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, elt, at, fr, T, hq, heads, dim, rot,
+                                       interleaved, magnitude, qn, kn, ne, eps, q_out.data_ptr(), k_out.data_ptr(),
+                                       _sh(None)), "glint_rotate_qk")
+    return q_out, k_out
+
+
+def kv4_append_rotated(q, k, v, pos, freqs, slots, cache, *, interleaved: bool = False, magnitude: float = 1.0, q_norm=None,
+                       k_norm=None, eps: float = 1e-6, keys: bool = False, out=None, stream=None):
+    """rotate_qk and kv4_append in one launch: the turned keys, and the values [T, H, D], go into the cache at slots
+    [T] (int64; negative ones are skipped). The turned queries, or (queries, keys) with keys=True; out: the
+    tensor, or both, to write."""
+    if stream is not None:
+        with _torch().cuda.stream(stream):
+            return kv4_append_rotated(q, k, v, pos, freqs, slots, cache, interleaved=interleaved, magnitude=magnitude,
+                                      q_norm=q_norm, k_norm=k_norm, eps=eps, keys=keys, out=out)
+    torch = _TORCH or _torch()
+    _here(q, k, v, pos, freqs, slots, q_norm, k_norm, *cache)
+    pages, cache_heads, cache_dim, *planes = _planes(cache)
+    elt, T, hq, heads, dim, rot, at, fr, qn, kn, ne = _turn_args(q, k, pos, freqs, q_norm, k_norm)
+    if heads != cache_heads or dim != cache_dim or v.shape != k.shape or v.dtype is not k.dtype:
+        raise ValueError(f"k {tuple(k.shape)}, v {tuple(v.shape)} {v.dtype}, cache of {cache_heads} heads of {cache_dim}")
+    sl = _ints(slots, torch.int64, T, "slots")
+    q_out, k_out = out if keys and out is not None else (out, None)
+    q_out = _turn_out(q_out, q, (T, hq, dim))
+    k_out = _turn_out(k_out, k, (T, heads, dim)) if keys else None
+    if T:
+        q, qt, qh = _rows(q, 4 if elt else 8)
+        k, kt, kh = _rows(k, 4 if elt else 8)
+        v, vt, vh = _rows(v, 4 if elt else 8)
+        _check(serve_lib().glint_kv4_append_rotated(
+            q.data_ptr(), qt, qh, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, elt, at, fr, sl, T, hq, heads, dim, rot,
+            interleaved, magnitude, qn, kn, ne, eps, q_out.data_ptr(), k_out.data_ptr() if keys else None, *planes, pages,
+            _sh(None)), "glint_kv4_append_rotated")
+    return (q_out, k_out) if keys else q_out
 
 
 def token_logprobs(logits, tokens, top: int = 0, stream=None) -> dict:

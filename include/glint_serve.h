@@ -1,6 +1,7 @@
 /* What a served model runs between its pinned linears, MI355X (gfx950), in
- * libglint_serve.so: a paged key/value cache held in 4 bits, attention over that cache,
- * causal attention over packed prompts, and log probabilities of given tokens.
+ * libglint_serve.so: queries and keys normed and turned to their positions, a paged key/value
+ * cache held in 4 bits, attention over that cache for single tokens and for chunks, causal
+ * attention over packed prompts, both also bounded to a window, and log probabilities of given tokens.
  * The reference keeps attention and scoring in its model harness (tests/arm0_forward.h);
  * these entry points have no counterpart in its ABI.
  *
@@ -68,6 +69,35 @@ int glint_kv4_attend(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, 
                      const int32_t *cu_q, int B, int max_q, int Hq, int H, int D, float scale, uint16_t *out,
                      struct ihipStream_t *stream);
 
+/* The same, bounded: the row at position p sees the positions j up to p with j > p - window or
+ * j < sinks. window 1 .. GLINT_WINDOW_MAX, or 0: no bound (sinks mean nothing then); sinks >= 0. What
+ * no row of a sequence sees is not read, nor are its pages' numbers in the table, so that a caller may
+ * give such pages back. */
+#define GLINT_WINDOW_MAX (1 << 30)
+int glint_kv4_attend_window(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq, const uint8_t *k_hole,
+                            const float *k_absmax, const uint8_t *v_hole, const float *v_absmax, int64_t pages,
+                            const int32_t *table, int64_t table_stride, int max_pages, const int32_t *lens,
+                            const int32_t *cu_q, int B, int max_q, int Hq, int H, int D, float scale, int window,
+                            int sinks, uint16_t *out, struct ihipStream_t *stream);
+
+/* Attention of B sequences' newest tokens over the cache, for many of them a sequence: arguments and result as
+ * glint_kv4_attend_window, out 16-B aligned. Where k and v are given [Tq], BF16, rows as q's, strides
+ * multiples of 8, stride_t from D to 2^24, 16-B aligned, they are the new tokens' keys and values, and what the
+ * cache holds of these tokens is not read (it need not hold them; its max_pages bound the tokens before them
+ * alone). Scores, softmax and sums are f32; held keys, values and softmax weights enter the matrix products in
+ * f16 (an absmax below 2^-25 of the largest that a workgroup has met loses bits), given ones as in
+ * glint_attend_prompt. A value that is not finite leaves itself or NaN in its dimension of the rows that see it.
+ * max_q (Hq / H) is at most 2^19. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a shape that is
+ * refused) for the current device; the call's alone until it has run. */
+int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H, int D, int max_pages);
+int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq, const uint8_t *k_hole,
+                           const float *k_absmax, const uint8_t *v_hole, const float *v_absmax, int64_t pages,
+                           const int32_t *table, int64_t table_stride, int max_pages, const int32_t *lens,
+                           const int32_t *cu_q, int B, int max_q, int Hq, int H, int D, const uint16_t *k,
+                           int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
+                           int64_t v_stride_h, float scale, int window, int sinks, uint16_t *out, void *scratch,
+                           int64_t scratch_bytes, struct ihipStream_t *stream);
+
 /* The stream's workspace, 4.1 MiB on 256 CUs: one for eager calls and, once the stream was
  * captured, one for the graphs captured on it, whose replays must not overlap one another.
  * reserve allocates the eager one ahead of time (0; -1: no memory, or the stream is being
@@ -87,6 +117,38 @@ int glint_attend_prompt(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_
                         int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
                         int64_t v_stride_h, const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk, int B,
                         int max_q, int Hq, int H, int D, float scale, uint16_t *out, struct ihipStream_t *stream);
+
+/* The same, bounded as glint_kv4_attend_window; positions are a sequence's keys. */
+int glint_attend_prompt_window(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, const uint16_t *k,
+                               int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v, int64_t v_stride_t,
+                               int64_t v_stride_h, const int32_t *cu_q, const int32_t *cu_k, int64_t Tq, int64_t Tk,
+                               int B, int max_q, int Hq, int H, int D, float scale, int window, int sinks, uint16_t *out,
+                               struct ihipStream_t *stream);
+
+/* Rows of T tokens, q of Hq heads and k of H, normed (where a norm is given) and turned to the tokens'
+ * positions pos [T]:
+ *   x_d = row_d (1 / sqrt(mean_d row_d^2 + eps)) norm_d;
+ *   pair i of the first `rot` dimensions turns by a = pos[t] freqs[i], freqs [rot / 2] in radians a position:
+ *   (x, y) -> magnitude (x cos a - y sin a, y cos a + x sin a), pairs being dimensions (i, i + rot / 2), or
+ *   (2 i, 2 i + 1) where interleaved is not 0; the others stay.
+ * f32 arithmetic, rounded once at the end; a is formed in f64, so that its error is 2^-52 of its size (past
+ * 2^51 it means nothing). D a multiple of 16, 16 .. 256, rot one too, 16 .. D. q, k and the outputs
+ * q_out [T][Hq][D], k_out [T][H][D] are of type elt (GLINT_KV_BF16 or GLINT_KV_F32); an output may be its
+ * own input where that is as contiguous. q_norm and k_norm [D], each or NULL, are of type norm_elt. Addresses
+ * are 16-B aligned, strides multiples of 16 B. */
+int glint_rotate_qk(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
+                    int64_t k_stride_h, int elt, const int64_t *pos, const double *freqs, int64_t T, int Hq, int H, int D,
+                    int rot, int interleaved, double magnitude, const void *q_norm, const void *k_norm, int norm_elt,
+                    float eps, void *q_out, void *k_out, struct ihipStream_t *stream);
+
+/* The same on the way into the cache: the keys that glint_rotate_qk gives, and v, are encoded as
+ * glint_kv4_append does. D is 64 or 128; k_out may be NULL. */
+int glint_kv4_append_rotated(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
+                             int64_t k_stride_h, const void *v, int64_t v_stride_t, int64_t v_stride_h, int elt,
+                             const int64_t *pos, const double *freqs, const int64_t *slots, int64_t T, int Hq, int H,
+                             int D, int rot, int interleaved, double magnitude, const void *q_norm, const void *k_norm,
+                             int norm_elt, float eps, void *q_out, void *k_out, uint8_t *k_hole, float *k_absmax,
+                             uint8_t *v_hole, float *v_absmax, int64_t pages, struct ihipStream_t *stream);
 
 /* Scores of T rows of V logits (BF16 bits or f32, row t at t * stride), with
  * lse = log sum_j exp x_j:
