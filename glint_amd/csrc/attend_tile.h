@@ -22,10 +22,11 @@ union ApFrag {
     ap_bf16x8 f;
 };
 
-/* Where 16-B chunk c of row r lies in an LDS tile's row: keys so that 8 lanes reading one
- * chunk of 8 rows touch 8 places, values so that the 64-B pieces of 4 rows that one transposing
+/* Where 16-B chunk c of row r lies in an LDS tile's row: keys so that 16 lanes reading one
+ * chunk of 16 rows touch every bank once, values so that the 64-B pieces of 4 rows that one transposing
  * read takes lie in different 64-B quarters of 256 B. */
-__device__ __forceinline__ int ap_k_chunk(int r, int c) { return c ^ (r & 7); }
+template <int D>
+__device__ __forceinline__ int ap_k_chunk(int r, int c) { return c ^ (D == 128 ? r & 15 : (r >> 1) & 7); }
 template <int D>
 __device__ __forceinline__ int ap_v_chunk(int r, int c) { return D == 128 ? c ^ ((r & 3) << 2) : c ^ ((r & 2) << 1); }
 
@@ -69,7 +70,7 @@ __device__ __forceinline__ void ap_tile(const ap_lds *kl, const ap_lds *vl, int 
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
             ApFrag f;
-            f.v = *(const __attribute__((address_space(3))) glint_u32x4 *)(kl + w.kat[s & 3] + 128 * (s >> 2) + a * 32 * D * 2);
+            f.v = *(const __attribute__((address_space(3))) glint_u32x4 *)(kl + (w.kat[s & 3] ^ (128 * (s >> 2))) + a * 32 * D * 2);
             sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(f.f, w.q[s].f, sc[a], 0, 0, 0);
         }
     /* element i of part a is key 32 a + 8 (i / 4) + 4 half + i % 4 */

@@ -121,7 +121,7 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
      * receives dimension i of the 4 keys. */
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-        w.kat[j] = col * D * 2 + 16 * ap_k_chunk(col, 2 * j + half);
+        w.kat[j] = col * D * 2 + 16 * ap_k_chunk<D>(col, 2 * j + half);
     const int vkey = 4 * half + ((lane & 15) >> 2), vdim = 16 * ((lane >> 4) & 1) + 4 * (lane & 3);
 #pragma unroll
     for (int d = 0; d < D / 32; ++d)
@@ -149,7 +149,7 @@ __global__ __launch_bounds__(AP_T, D == 64 ? 4 : 2) void k_attend_prompt(ApArgs 
      * thread t fills places t + i AP_T, so its lane's global chunk carries the swizzle (the same
      * for every i). Rows past the sequence take an offset past the buffer's end: zeros. */
     const int my_row = threadIdx.x / CH, my_chunk = threadIdx.x % CH;
-    const uint32_t ko = (uint32_t)(my_row * A.k_st * 2) + 16 * ap_k_chunk(my_row, my_chunk);
+    const uint32_t ko = (uint32_t)(my_row * A.k_st * 2) + 16 * ap_k_chunk<D>(my_row, my_chunk);
     const uint32_t vo = (uint32_t)(my_row * A.v_st * 2) + 16 * ap_v_chunk<D>(my_row, my_chunk);
     const uint32_t kstep = (uint32_t)(STEP * A.k_st * 2), vstep = (uint32_t)(STEP * A.v_st * 2);
     auto fetch = [&](int t, ap_lds *kt, ap_lds *vt) {

@@ -123,7 +123,7 @@ _SERVE_SIGS = {
                           _c.c_float, VP, VP], I32),
     "glint_kv4_attend_window": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32,
                                  _c.c_float, I32, I32, VP, VP], I32),
-    "glint_kv4_attend_chunk_scratch": ([I32, I32, I32, I32, I32, I32], I64),
+    "glint_kv4_attend_chunk_scratch": ([I32, I32, I32, I32, I32, I32, I32], I64),
     "glint_kv4_attend_chunk": ([VP, I64, I64, I64, VP, VP, VP, VP, I64, VP, I64, I32, VP, VP, I32, I32, I32, I32, I32, VP, I64,
                                 I64, VP, I64, I64, _c.c_float, I32, I32, VP, VP, I64, VP], I32),
     "glint_serve_workspace_reserve": ([VP], I32),
@@ -746,7 +746,7 @@ def kv4_attend_chunk(q, cache, page_table, lens, cu_q=None, max_q: Optional[int]
         return out
     if wide == 0:  # nobody has a page
         page_table, wide = page_table.new_full((B, 1), -1), 1
-    size = serve_lib().glint_kv4_attend_chunk_scratch(B, max_q, hq, heads, dim, wide)
+    size = serve_lib().glint_kv4_attend_chunk_scratch(B, max_q, hq, heads, dim, wide, k is not None)
     if size < 0:
         raise ValueError(f"{max_q} new tokens a sequence, {hq} heads over {heads}, {wide} pages: more than a launch can hold")
     scratch = q.new_empty(size, dtype=torch.uint8)

@@ -81,13 +81,15 @@ def test_empty_calls_do_nothing():
 
 
 def test_scratch():
-    """Two parts of 256 rows a workgroup: outputs, maxima and sums."""
+    """Parts, sums, and tiles: 4 * 64 * D bytes for each page and for each 64 own keys of a sequence and head."""
     size = H.serve_lib().glint_kv4_attend_chunk_scratch
-    assert size(0, 4, 8, 2, 128, 4) == 0
-    assert size(1, 1, 8, 2, 128, 1) % (2 * 256 * 130 * 4) == 0 < size(1, 1, 8, 2, 128, 1)
-    assert size(64, 512, 32, 8, 64, 1 << 10) % (2 * 256 * 66 * 4) == 0
-    for bad in ((1, 4, 8, 3, 128, 4), (1, 4, 8, 2, 96, 4), (1, 0, 8, 2, 128, 4), (1, 4, 8, 2, 128, 1 << 25), (1, 1 << 18, 8, 2, 128, 1 << 24)):
-        assert size(*bad) == -2, bad
+    assert size(0, 4, 8, 2, 128, 4, 0) == 0
+    small, wide = size(1, 64, 8, 2, 128, 4, 0), size(1, 64, 8, 2, 128, 1004, 0)
+    assert 0 < 2 * 4 * 4 * 64 * 128 < small and wide - small > 1000 * 2 * 4 * 64 * 128
+    assert size(1, 64, 8, 2, 128, 4, 1) > small
+    assert size(64, 512, 32, 8, 64, 1 << 16, 0) < 3 << 30  # cut into launches
+    for bad in ((1, 4, 8, 3, 128, 4), (1, 4, 8, 2, 96, 4), (1, 0, 8, 2, 128, 4), (1, 4, 8, 2, 128, 1 << 25), (1, 1 << 16, 8, 2, 128, 1 << 24)):
+        assert size(*bad, 0) == -2, bad
 
 
 def test_helpers_refuse():
