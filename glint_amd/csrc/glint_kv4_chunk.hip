@@ -33,7 +33,7 @@ typedef _Float16 kc_f16x2 __attribute__((ext_vector_type(2)));
 #define KC_T (64 * KC_WAVES)
 #define KC_ROWS (32 * KC_WAVES)
 #define KC_PAIRS 2048 /* of a sequence and a row block, in a launch */
-#define KC_SHARE 2    /* tiles that a workgroup takes at least */
+#define KC_SHARE 4    /* tiles that a workgroup takes at least */
 #define KC_UP 7.f     /* weights are 2^KC_UP times the softmax's: f16 has room above, and its small ones keep more bits */
 #define KC_CAP ((int64_t)1 << 31) /* bytes of tiles of a launch */
 
@@ -45,6 +45,16 @@ struct KcMeta {
 #define KC_EXP 1024
 #define KC_ABSENT 0x80000000u /* the page is not in the pool: nothing was written */
 #define KC_ODD 0x40000000u    /* a value that is not finite was taken out */
+
+/* Where a workgroup's run of the list begins: sequence, key head, row block, tile; how many tiles it has (0: none), and
+ * how many the runs have that a group goes on in. */
+struct KcStart {
+    int b, h, rb, at, left, step, pad[2];
+};
+/* A group that begins in a workgroup's run and goes on in those up to w_last's (0: there is none). */
+struct KcJoin {
+    int w_last, q0, head, rb, rows, pad[3];
+};
 
 struct KcArgs {
     const uint16_t *q;
@@ -67,6 +77,8 @@ struct KcArgs {
     ApBound bound;
     float *part; /* outputs of two parts per workgroup, [KC_ROWS][D] each, */
     float *sums; /* and their rows' maxima and sums */
+    KcStart *starts; /* of the attention's workgroups */
+    KcJoin *joins;
     KcMeta *meta;
     char *tiles;
 };
@@ -129,8 +141,7 @@ __device__ __forceinline__ int kc_cost(const KcArgs &a, const KcSeq &s, int rb) 
  * (sequence, row block) before pair i. */
 struct KcPlan {
     int pre[KC_PAIRS + 1];
-    int wave[KC_WAVES];
-    int b, rb, at;
+    int wave[4]; /* of the scanning workgroup's waves */
 };
 template <class F> /* pairs, and the cost of pair i */
 __device__ __forceinline__ void kc_scan(KcPlan &p, int pairs, F cost_of) {
@@ -167,33 +178,84 @@ __device__ __forceinline__ void kc_scan(KcPlan &p, int pairs, F cost_of) {
         p.pre[pairs] = before;
     __syncthreads();
 }
-__device__ __forceinline__ void kc_plan(const KcArgs &a, KcPlan &p) {
-    kc_scan(p, a.B * a.nblk, [&](int i) { return kc_cost(a, kc_seq(a, i / a.nblk), i % a.nblk); });
+/* The last i of lo .. hi - 1 with v(i) <= x, where v(lo) is. */
+template <class F>
+__device__ __forceinline__ int kc_last(int lo, int hi, int x, F v) {
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (v(mid) <= x)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
 }
-/* The group that unit u of the list lies in, and where in it. */
-__device__ __forceinline__ void kc_find(const KcArgs &a, KcPlan &p, int u, int &b, int &h, int &rb, int &at) {
-    for (int i = threadIdx.x; i < a.B; i += blockDim.x)
-        if (a.Hn * p.pre[i * a.nblk] <= u && u < a.Hn * p.pre[(i + 1) * a.nblk])
-            p.b = i;
+/* One workgroup finds where the attention's `grid` workgroups begin. Runs are equal shares of the list, or, where the
+ * longest is then not much longer, whole groups or equal parts of groups: workgroups of one key head then walk
+ * its tiles side by side, which the XCD's L2 serves. 2048 tokens over 16384, 512 groups: X us so, Y with equal
+ * shares (41% of L2 reads missed). */
+__device__ __forceinline__ void kc_starts(const KcArgs &a, KcPlan &p, int *cnt, int grid) {
+    const int pairs = a.B * a.nblk;
+    auto blocks = [&](int b) { return (kc_seq(a, b).rows + KC_ROWS - 1) / KC_ROWS; };
+    kc_scan(p, a.B, blocks);
+    for (int i = threadIdx.x; i <= a.B; i += blockDim.x)
+        cnt[i] = p.pre[i];
     __syncthreads();
-    b = __builtin_amdgcn_readfirstlane(p.b);
-    const int *pre = p.pre + b * a.nblk;
-    const int each = pre[a.nblk] - pre[0], in = u - a.Hn * pre[0];
-    h = __builtin_amdgcn_readfirstlane(in / each);
-    const int r = in % each + pre[0];
-    for (int i = threadIdx.x; i < a.nblk; i += blockDim.x)
-        if (pre[i] <= r && r < pre[i + 1]) {
-            p.rb = i;
-            p.at = r - pre[i];
+    int most = 0;
+    kc_scan(p, pairs, [&](int i) {
+        const int c = kc_cost(a, kc_seq(a, i / a.nblk), i % a.nblk);
+        most = max(most, c);
+        return c;
+    });
+    most = (int)glint_wave_max((float)min(most, 1 << 24));
+    if ((threadIdx.x & 63) == 0)
+        p.wave[threadIdx.x >> 6] = most;
+    __syncthreads();
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w)
+        most = max(most, p.wave[w]);
+    const int total = a.Hn * p.pre[pairs], groups = a.Hn * cnt[a.B];
+    const int share = max(KC_SHARE, (total + grid - 1) / grid);
+    const int parts = groups ? max(1, grid / groups) : 1, each_wg = (groups + grid - 1) / grid;
+    const int step = (most + parts - 1) / parts;
+    const bool whole = (int64_t)each_wg * step * 8 <= (int64_t)share * 9 && step >= KC_SHARE;
+    auto at_group = [&](int g, KcStart &s) {
+        s.b = kc_last(0, a.B, g, [&](int b) { return a.Hn * cnt[b]; });
+        const int n = cnt[s.b + 1] - cnt[s.b], in = g - a.Hn * cnt[s.b];
+        s.h = in / n;
+        s.rb = in % n;
+        const int *pre = p.pre + s.b * a.nblk;
+        return a.Hn * pre[0] + s.h * (pre[a.nblk] - pre[0]) + pre[s.rb] - pre[0]; /* units before it */
+    };
+    for (int w = threadIdx.x; w < grid; w += blockDim.x) {
+        KcStart s{0, 0, 0, 0, 0, share, {0, 0}};
+        if (whole) {
+            const int g = parts > 1 ? w / parts : w * each_wg;
+            if (g < groups) {
+                const int u = at_group(g, s);
+                if (parts > 1) {
+                    const int cost = p.pre[s.b * a.nblk + s.rb + 1] - p.pre[s.b * a.nblk + s.rb];
+                    s.step = (cost + parts - 1) / parts;
+                    s.at = w % parts * s.step;
+                    s.left = max(0, min(s.step, cost - s.at));
+                } else {
+                    KcStart next;
+                    s.left = (g + each_wg < groups ? at_group(g + each_wg, next) : total) - u;
+                }
+            }
+        } else if ((int64_t)w * share < total) {
+            const int u = w * share;
+            s.left = min(share, total - u);
+            s.b = kc_last(0, a.B, u, [&](int b) { return a.Hn * p.pre[b * a.nblk]; });
+            const int *pre = p.pre + s.b * a.nblk;
+            const int each = pre[a.nblk] - pre[0], in = u - a.Hn * pre[0];
+            s.h = in / each;
+            const int r = in % each + pre[0];
+            s.rb = kc_last(0, a.nblk, r, [&](int i) { return pre[i]; });
+            s.at = r - pre[s.rb];
         }
-    __syncthreads();
-    rb = __builtin_amdgcn_readfirstlane(p.rb);
-    at = __builtin_amdgcn_readfirstlane(p.at);
+        a.starts[w] = s;
+    }
 }
-__device__ __forceinline__ int kc_total(const KcArgs &a, const KcPlan &p) {
-    return __builtin_amdgcn_readfirstlane(a.Hn * p.pre[a.B * a.nblk]);
-}
-__device__ __forceinline__ int kc_share(int total, int grid) { return max(KC_SHARE, (total + grid - 1) / grid); }
 
 union KcFrag {
     uint32_t u[4];
@@ -211,7 +273,6 @@ __device__ __forceinline__ int kc_v_at(int d, int c) { return d * 128 + 16 * (c 
 
 /* ------------------------------------------------------------------ tiles */
 #define KU_T 256
-#define KU_COPIES 16 /* of an entry, 8 B each */
 
 /* The exponent e of a power of two 2^(14 - e) that brings `top` (finite) under 2^15, in steps of `step`. */
 __device__ __forceinline__ int ku_exponent(float top, int step) {
@@ -219,16 +280,22 @@ __device__ __forceinline__ int ku_exponent(float top, int step) {
     return (e + step - 1) & -step;
 }
 
-template <int D>
-__global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
+/* The last workgroup lays out the attention's work; the others take tiles in turn. */
+template <int D, bool OWN>
+__global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
     constexpr int NB = D / 64, TILE = AP_KEYS * D * 2, CH = D / 8;
-    __shared__ __attribute__((aligned(16))) glint_f32x2 entries[256 * KU_COPIES]; /* a byte's two parents */
-    __shared__ __attribute__((aligned(16))) uint16_t rows[AP_KEYS][D + 2];        /* own values, to be turned */
+    __shared__ float parents[16 * 64]; /* a copy for every lane's bank */
+    __shared__ __attribute__((aligned(16))) uint16_t rows[OWN ? AP_KEYS : 1][D + 2]; /* own values, to be turned */
     __shared__ float tops[2][KU_T / 64];
     __shared__ uint32_t odds;
     __shared__ KcPlan plan;
-    for (int i = threadIdx.x; i < 256 * KU_COPIES; i += KU_T)
-        entries[i] = glint_f32x2{kKv4Parent[i / KU_COPIES & 15], kKv4Parent[i / KU_COPIES >> 4]};
+    __shared__ int counts[KC_PAIRS + 1];
+    if (blockIdx.x + 1 == gridDim.x) {
+        kc_starts(A, plan, counts, grid);
+        return;
+    }
+    for (int i = threadIdx.x; i < 16 * 64; i += KU_T)
+        parents[i] = kKv4Parent[i >> 6];
     /* the list: a sequence's tiles, head after head */
     kc_scan(plan, A.B, [&](int b) {
         const KcTiles t = kc_tiles(A, kc_seq(A, b), 0, A.nblk);
@@ -237,7 +304,7 @@ __global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int total = A.Hn * plan.pre[A.B];
     int b = 0;
-    for (int u = blockIdx.x; u < total; u += gridDim.x) {
+    for (int u = blockIdx.x; u < total; u += gridDim.x - 1) {
         while (A.Hn * plan.pre[b + 1] <= u) /* u only grows */
             ++b;
         b = __builtin_amdgcn_readfirstlane(b);
@@ -300,18 +367,15 @@ __global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
             meta = KcMeta{ldexpf(1.f, ke - 14), (uint32_t)(ve + KC_EXP) | (__any(mine && odd) ? KC_ODD : 0u)};
             if (threadIdx.x == 0)
                 A.meta[slot] = meta;
-            const glint_f32x2 *entry = entries + (lane & (KU_COPIES - 1));
-            auto pair = [&](uint32_t word, int byte) { return entry[(word >> (8 * byte) & 255u) * KU_COPIES]; };
+            auto parent = [&](uint32_t word, int nibble) { return parents[(word >> (4 * nibble) & 15u) * 64 + lane]; };
 #pragma unroll
             for (int x = 0; x < NB; ++x)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) {
                     glint_u32x4 eight;
 #pragma unroll
-                    for (int z = 0; z < 4; ++z) {
-                        const glint_f32x2 e = pair(kw[x][y], z);
-                        eight[z] = kc_f16pair(e.x * (ks[x] * kdown), e.y * (ks[x] * kdown));
-                    }
+                    for (int z = 0; z < 4; ++z)
+                        eight[z] = kc_f16pair(parent(kw[x][y], 2 * z) * (ks[x] * kdown), parent(kw[x][y], 2 * z + 1) * (ks[x] * kdown));
                     *(glint_u32x4 *)(kt + tok * (D * 2) + 16 * ap_k_chunk<D>(tok, 8 * x + 2 * part + y)) = eight;
                 }
             if (has_v) {
@@ -327,9 +391,8 @@ __global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
                             const int at = key + 16 * part + 4 * j + k;
                             /* what nobody sees is 0: a weight of 0 does not undo an infinity */
                             const float f = fabsf(vs[j][k]) <= FLT_MAX && at < s.held && seen(at) ? vs[j][k] * vdown : 0.f;
-                            const glint_f32x2 e = pair(vw[j], k);
-                            a[k] = e.x * f;
-                            z[k] = e.y * f;
+                            a[k] = parent(vw[j], 2 * k) * f;
+                            z[k] = parent(vw[j], 2 * k + 1) * f;
                         }
                         lo[2 * x] = kc_f16pair(a[0], a[1]);
                         lo[2 * x + 1] = kc_f16pair(a[2], a[3]);
@@ -340,7 +403,7 @@ __global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
                     *(glint_u32x4 *)(vt + kc_v_at(dim + 16, 2 * part + y)) = hi;
                 }
             }
-        } else {
+        } else if constexpr (OWN) {
             /* own keys: positions s.own + 64 f ..; rows past the sequence's last are 0 */
             const int f = i - t.np < t.fsinks ? i - t.np : i - t.np + t.fskip;
             const int64_t slot = kc_slot(A, b, hl, A.max_pages + f);
@@ -348,67 +411,65 @@ __global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
             const int key = s.own + f * AP_KEYS;
             const int64_t row0 = (int64_t)s.q0 + s.nq - s.len + key;
             constexpr int PER = AP_KEYS * CH / KU_T; /* 16-B chunks of a thread */
-            glint_u32x4 kx[PER], vx[PER];
-            float ktop = 0.f, vtop = 0.f;
-            bool odd = false;
-            __syncthreads(); /* the tile before has been turned, odds and tops are read */
+            int e[2];
             if (threadIdx.x == 0)
                 odds = 0;
+#pragma unroll 1
+            for (int is_v = 0; is_v < 2; ++is_v) {
+                const uint16_t *from = is_v ? A.v + row0 * A.v_st + h * A.v_sh : A.k + row0 * A.k_st + h * A.k_sh;
+                const int64_t st = is_v ? A.v_st : A.k_st;
+                glint_u32x4 in[PER];
+                float top = 0.f;
+                bool odd = false;
 #pragma unroll
-            for (int x = 0; x < PER; ++x) {
-                const int r = (threadIdx.x + x * KU_T) / CH, c = (threadIdx.x + x * KU_T) % CH;
-                const bool mine = key + r < s.len && seen(key + r);
-                kx[x] = vx[x] = glint_u32x4{0, 0, 0, 0};
-                if (mine) {
-                    kx[x] = *(const glint_u32x4 *)(A.k + (row0 + r) * A.k_st + h * A.k_sh + 8 * c);
-                    vx[x] = *(const glint_u32x4 *)(A.v + (row0 + r) * A.v_st + h * A.v_sh + 8 * c);
-                }
+                for (int x = 0; x < PER; ++x) {
+                    const int r = (threadIdx.x + x * KU_T) / CH, c = (threadIdx.x + x * KU_T) % CH;
+                    in[x] = glint_u32x4{0, 0, 0, 0};
+                    if (key + r < s.len && seen(key + r))
+                        in[x] = *(const glint_u32x4 *)(from + r * st + 8 * c);
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const float a = fabsf(k ? glint_bf16hi(kx[x][j]) : glint_bf16lo(kx[x][j]));
-                        const float z = fabsf(k ? glint_bf16hi(vx[x][j]) : glint_bf16lo(vx[x][j]));
-                        ktop = a <= FLT_MAX ? fmaxf(ktop, a) : ktop;
-                        if (z <= FLT_MAX) {
-                            vtop = fmaxf(vtop, z);
-                        } else {
-                            odd = true;
-                            vx[x][j] &= k ? 0xFFFFu : 0xFFFF0000u;
+                        for (int k = 0; k < 2; ++k) {
+                            const float a = fabsf(k ? glint_bf16hi(in[x][j]) : glint_bf16lo(in[x][j]));
+                            if (a <= FLT_MAX) {
+                                top = fmaxf(top, a);
+                            } else if (is_v) { /* a key's stays: what sees it is NaN */
+                                odd = true;
+                                in[x][j] &= k ? 0xFFFFu : 0xFFFF0000u;
+                            }
                         }
-                    }
-            }
-            ktop = glint_wave_max(ktop);
-            vtop = glint_wave_max(vtop);
-            if (lane == 0) {
-                tops[0][wave] = ktop;
-                tops[1][wave] = vtop;
-            }
-            __syncthreads();
-            if (odd)
-                odds = 1;
-#pragma unroll
-            for (int x = 0; x < KU_T / 64; ++x) {
-                ktop = fmaxf(ktop, tops[0][x]);
-                vtop = fmaxf(vtop, tops[1][x]);
-            }
-            const int ke = ku_exponent(ktop, 1), ve = ku_exponent(vtop, 8);
-            const float kdown = ldexpf(1.f, 14 - ke), vdown = ldexpf(1.f, 14 - ve);
-#pragma unroll
-            for (int x = 0; x < PER; ++x) {
-                const int r = (threadIdx.x + x * KU_T) / CH, c = (threadIdx.x + x * KU_T) % CH;
-                glint_u32x4 eight;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    eight[j] = kc_f16pair(glint_bf16lo(kx[x][j]) * kdown, glint_bf16hi(kx[x][j]) * kdown);
-                    const uint32_t two = kc_f16pair(glint_bf16lo(vx[x][j]) * vdown, glint_bf16hi(vx[x][j]) * vdown);
-                    *(uint32_t *)&rows[r][8 * c + 2 * j] = two;
                 }
-                *(glint_u32x4 *)(kt + r * (D * 2) + 16 * ap_k_chunk<D>(r, c)) = eight;
+                top = glint_wave_max(top);
+                if (lane == 0)
+                    tops[is_v][wave] = top;
+                __syncthreads(); /* also: the tile before has been turned */
+                if (odd)
+                    odds = 1;
+#pragma unroll
+                for (int x = 0; x < KU_T / 64; ++x)
+                    top = fmaxf(top, tops[is_v][x]);
+                e[is_v] = ku_exponent(top, is_v ? 8 : 1);
+                const float down = ldexpf(1.f, 14 - e[is_v]);
+#pragma unroll
+                for (int x = 0; x < PER; ++x) {
+                    const int r = (threadIdx.x + x * KU_T) / CH, c = (threadIdx.x + x * KU_T) % CH;
+                    glint_u32x4 eight;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        eight[j] = kc_f16pair(glint_bf16lo(in[x][j]) * down, glint_bf16hi(in[x][j]) * down);
+                    if (!is_v) {
+                        *(glint_u32x4 *)(kt + r * (D * 2) + 16 * ap_k_chunk<D>(r, c)) = eight;
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            *(uint32_t *)&rows[r][8 * c + 2 * j] = eight[j];
+                    }
+                }
             }
             __syncthreads();
             if (threadIdx.x == 0)
-                A.meta[slot] = KcMeta{ldexpf(1.f, ke - 14), (uint32_t)(ve + KC_EXP) | (odds ? KC_ODD : 0u)};
+                A.meta[slot] = KcMeta{ldexpf(1.f, e[0] - 14), (uint32_t)(e[1] + KC_EXP) | (odds ? KC_ODD : 0u)};
 #pragma unroll
             for (int x = 0; x < PER; ++x) {
                 const int d = (threadIdx.x + x * KU_T) / 8, c = (threadIdx.x + x * KU_T) % 8;
@@ -426,114 +487,86 @@ __global__ __launch_bounds__(KU_T) void k_kv4_unpack(KcArgs A) {
 }
 
 /* ------------------------------------------------------------------ attention */
-/* A page's scores: as ap_tile's, in f16. Products in groups of four: the next group's operands are read ahead of a
- * group's products, whose time covers the reads' latency; left to itself the compiler waits for every read. */
 typedef const __attribute__((address_space(3))) glint_u32x4 kc_lds_u32x4;
-template <int D>
-__device__ __forceinline__ void kc_scores(const ap_lds *kl, const ApRows<D> &w, ap_f32x16 (&sc)[2]) {
-    KcFrag f[2][4];
-    auto read = [&](int g) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int s = 2 * g + (x >> 1), a = x & 1;
-            f[g & 1][x].v = *(kc_lds_u32x4 *)(kl + (w.kat[s & 3] ^ (128 * (s >> 2))) + a * 32 * D * 2);
-        }
+
+/* A wave issues in order, and a product occupies the matrix unit for 32 cycles: the vector work of one tile's
+ * weights stands between the products of the next tile's scores, product by product, and operands are read
+ * from LDS some products ahead. The compiler would put all products first and wait for every read, so the order
+ * is fixed by scheduling barriers. */
+#define KC_FIXED() __builtin_amdgcn_sched_barrier(0)
+
+/* The scores of a tile of keys, sc; where NOW, also the weights pf (f16) and their sum l of the tile before, whose scores
+ * `now` holds. */
+template <int D, bool NEXT, bool NOW>
+__device__ __forceinline__ void kc_scores(const ap_lds *kl, const ApRows<D> &w, ap_f32x16 (&sc)[2], ap_f32x16 (&now)[2],
+                                          float factor, float base, KcFrag (&pf)[4], float &l) {
+    constexpr int N = D / 8, AHEAD = 4; /* products */
+    KcFrag f[AHEAD];
+    auto read = [&](int n) {
+        const int s = n >> 1, a = n & 1;
+        f[n % AHEAD].v = *(kc_lds_u32x4 *)(kl + (w.kat[s & 3] ^ (128 * (s >> 2))) + a * 32 * D * 2);
     };
-    read(0);
+    if constexpr (NEXT) {
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-            sc[a][i] = 0.f;
-#pragma unroll
-    for (int g = 0; g < D / 32; ++g) {
-        if (g + 1 < D / 32)
-            read(g + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            KcFrag q;
-            q.v = w.q[2 * g + (x >> 1)].v;
-            sc[x & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[g & 1][x].f, q.f, sc[x & 1], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
-}
-/* What the scores weigh: `upto` is the last key of the tile that the lane's row may see. Values are V^T; the weights are
- * multiplied by `less`, a power of two, where it is not 1. */
-template <int D>
-__device__ __forceinline__ void kc_weigh(const ap_lds *vl, int at, ApRows<D> &w, ap_f32x16 (&sc)[2], const uint32_t (&vat)[4],
-                                         float factor, float less, bool masked, int upto, int half, const ApBound &bound) {
-    if (masked) {
-        const int first = at + 4 * half;
+        for (int n = 0; n < AHEAD; ++n)
+            read(n);
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int key = first + 32 * a + 8 * (i >> 2) + (i & 3);
-                sc[a][i] = key <= upto && bound.sees(key, w.last) ? sc[a][i] : -INFINITY;
-            }
+            for (int i = 0; i < 16; ++i)
+                sc[a][i] = 0.f;
     }
+    const kc_f16x2 ones = {(_Float16)1.f, (_Float16)1.f};
+    KC_FIXED();
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        if constexpr (NEXT) {
+            KcFrag q;
+            q.v = w.q[n >> 1].v;
+            sc[n & 1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[n % AHEAD].f, q.f, sc[n & 1], 0, 0, 0);
+            KC_FIXED();
+            if (n + AHEAD < N)
+                read(n + AHEAD);
+        }
+        if constexpr (NOW) {
+#pragma unroll
+            for (int e = 32 / N * n; e < 32 / N * (n + 1); e += 2) { /* two elements, or four */
+                const int a = e >> 4, i = e & 15;
+                const float x = __builtin_amdgcn_exp2f(fmaf(now[a][i], factor, -base));
+                const float y = __builtin_amdgcn_exp2f(fmaf(now[a][i + 1], factor, -base));
+                const uint32_t two = kc_f16pair(x, y);
+                pf[2 * a + (i >> 3)].u[(i & 7) >> 1] = two;
+                l = __builtin_amdgcn_fdot2(__builtin_bit_cast(kc_f16x2, two), ones, l, false);
+            }
+        }
+        KC_FIXED();
+    }
+}
+/* Outputs of a tile of values, and the largest of the next tile's scores meanwhile. */
+template <int D>
+__device__ __forceinline__ float kc_outputs(const ap_lds *vl, ApRows<D> &w, const uint32_t (&vat)[4], const KcFrag (&pf)[4],
+                                            const ap_f32x16 (&sc)[2]) {
+    constexpr int N = D / 8, AHEAD = 5, PARTS = D / 32; /* products; parts of the outputs */
+    KcFrag f[AHEAD];
+    auto read = [&](int n) { f[n % AHEAD].v = *(kc_lds_u32x4 *)(vl + vat[n / PARTS] + n % PARTS * 32 * 128); };
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n)
+        read(n);
+    KC_FIXED();
     float top = -INFINITY;
 #pragma unroll
-    for (int a = 0; a < 2; ++a)
+    for (int n = 0; n < N; ++n) {
+        const int s = n / PARTS, d = n % PARTS;
+        w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[n % AHEAD].f, pf[s].f, w.o[d], 0, 0, 0);
+        KC_FIXED();
+        if (n + AHEAD < N)
+            read(n + AHEAD);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            top = fmaxf(top, sc[a][i]);
-    top = glint_xor32(top, GlintMax()) * factor;
-    const bool more = top > w.m + AP_SLACK;
-    if (__any(more)) {
-        const float mn = more ? top : w.m;
-        const float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
-        w.m = mn;
-        w.l *= keep;
-#pragma unroll
-        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                w.o[d][i] *= keep;
+        for (int e = 32 / N * n; e < 32 / N * (n + 1); ++e)
+            top = fmaxf(top, sc[e >> 4][e & 15]);
+        KC_FIXED();
     }
-    constexpr int PARTS = D / 32; /* of the outputs */
-    KcFrag f[2][4];
-    auto read = [&](int g) {
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-            f[g & 1][x].v = *(kc_lds_u32x4 *)(vl + vat[(4 * g + x) / PARTS] + (4 * g + x) % PARTS * 32 * 128);
-    };
-    read(0);
-    __builtin_amdgcn_sched_barrier(0);
-    const float base = w.m == -INFINITY ? 0.f : w.m - KC_UP;
-    KcFrag pf[4];
-    float sum = 0.f;
-#pragma unroll
-    for (int a = 0; a < 2; ++a)
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-#pragma unroll
-            for (int x = i; x < i + 2; ++x) {
-                sc[a][x] = __builtin_amdgcn_exp2f(fmaf(sc[a][x], factor, -base));
-                sum += sc[a][x];
-            }
-            pf[2 * a + (i >> 3)].u[(i & 7) >> 1] = kc_f16pair(sc[a][i], sc[a][i + 1]);
-        }
-    w.l += sum;
-    if (less != 1.f) {
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-            pf[s].f *= (_Float16)less;
-    }
-#pragma unroll
-    for (int g = 0; g < PARTS; ++g) {
-        if (g + 1 < PARTS)
-            read(g + 1);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int s = (4 * g + x) / PARTS, d = (4 * g + x) % PARTS;
-            w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f[g & 1][x].f, pf[s].f, w.o[d], 0, 0, 0);
-        }
-        __builtin_amdgcn_sched_barrier(0);
-    }
+    return top;
 }
 
 template <int D>
@@ -541,18 +574,17 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
     constexpr int TILE = AP_KEYS * D * 2, LOADS = TILE / (16 * KC_T);
     /* arrays of their own, so that reads of one do not wait for loads into the other */
     __shared__ __attribute__((aligned(16))) char k0t[TILE], k1t[TILE], v0t[TILE], v1t[TILE];
-    __shared__ KcPlan plan;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    kc_plan(A, plan);
-    const int grid = gridDim.x, total = kc_total(A, plan), share = kc_share(total, grid);
     /* neighbours in the list share keys: they go to one XCD, a workgroup's being its index modulo 8 */
-    const int me = grid & 7 ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (grid >> 3) + ((int)blockIdx.x >> 3);
-    if ((int64_t)me * share >= total)
+    const int grid = gridDim.x, me = grid & 7 ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (grid >> 3) + ((int)blockIdx.x >> 3);
+    int left = A.starts[me].left; /* of this workgroup's run */
+    if (left == 0) {
+        if (threadIdx.x == 0)
+            A.joins[me].w_last = 0;
         return;
-    int left = min(share, total - me * share); /* of this workgroup's run */
-    int b, h, rb, at;
-    kc_find(A, plan, me * share, b, h, rb, at);
+    }
+    int b = A.starts[me].b, h = A.starts[me].h, rb = A.starts[me].rb, at = A.starts[me].at;
 
     ApRows<D> w;
 #pragma unroll
@@ -591,18 +623,41 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
             };
             const int64_t slot0 = kc_slot(A, b, h, 0);
             const uint32_t my = threadIdx.x * 16;
-            auto fetch = [&](int i, ap_lds *kt, ap_lds *vt) {
-                const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
-                    (void *)(A.tiles + (slot0 + place(i)) * (2 * TILE)), (short)0, 2 * TILE, GLINT_BUF_DWORD3);
+            auto tile_of = [&](int i) {
+                return __builtin_amdgcn_make_buffer_rsrc((void *)(A.tiles + (slot0 + place(i)) * (2 * TILE)), (short)0, 2 * TILE,
+                                                         GLINT_BUF_DWORD3);
+            };
+            auto fetch_k = [&](int i, ap_lds *kt) {
+                const __amdgpu_buffer_rsrc_t r = tile_of(i);
 #pragma unroll
                 for (int x = 0; x < LOADS; ++x)
                     ap_dma(r, kt + (x * KC_T + wave * 64) * 16, my, x * (KC_T * 16));
+            };
+            auto fetch_v = [&](int i, ap_lds *vt) {
+                const __amdgpu_buffer_rsrc_t r = tile_of(i);
 #pragma unroll
                 for (int x = 0; x < LOADS; ++x)
                     ap_dma(r, vt + (x * KC_T + wave * 64) * 16, my, TILE + x * (KC_T * 16));
             };
+            /* what a step has to know of its tile */
+            struct {
+                int key, ends; /* its first position, and the last one that it may show */
+                bool want;     /* whether the wave has scores to form */
+                KcMeta meta;
+            } T, N;
+            auto look = [&](int i, auto &X) {
+                const int to = place(i);
+                const bool own = i >= tiles.np;
+                X.key = own ? s.own + (to - A.max_pages) * AP_KEYS : to * AP_KEYS;
+                X.ends = own ? INT32_MAX : s.held - 1;
+                X.meta = A.meta[slot0 + to];
+                X.want = wave_live && X.key <= min(wave_high, X.ends) &&
+                         (X.key + AP_KEYS - 1 > wave_low - A.bound.window || X.key < A.bound.sinks);
+            };
+            ap_lds *const ka = (ap_lds *)(at & 1 ? k1t : k0t);
             __syncthreads(); /* the last group's tiles are read */
-            fetch(at, (ap_lds *)k0t, (ap_lds *)v0t);
+            fetch_k(at, ka);
+            look(at, T);
             /* q as f16, scaled to 2^14 .. 2^15 by a power of two of the row's */
             const uint16_t *qr = A.q + (int64_t)(s.q0 + (live ? row / A.G : 0)) * A.q_st + (head + (live ? row % A.G : 0)) * A.q_sh;
             uint32_t high = 0;
@@ -624,41 +679,107 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                     w.q[x].u[i] = kc_f16pair(ldexpf(glint_bf16lo(w.q[x].u[i]), -ex), ldexpf(glint_bf16hi(w.q[x].u[i]), -ex));
             const float factor = ldexpf(A.scale2, ex);
 
-            auto step = [&](int i, ap_lds *kt, ap_lds *vt, ap_lds *kn, ap_lds *vn) {
-                const int to = place(i);
-                const bool own = i >= tiles.np;
-                const int key = own ? s.own + (to - A.max_pages) * AP_KEYS : to * AP_KEYS;
-                const int ends = own ? INT32_MAX : s.held - 1; /* the last position that the tile may show */
-                const KcMeta meta = A.meta[slot0 + to];
-                __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0); /* this wave's part of the tile */
-                __syncthreads();
-                if (i + 1 < end)
-                    fetch(i + 1, kn, vn); /* over the tile before, which every wave has left */
-                apart |= (meta.vexp & KC_ODD) != 0;
-                if ((meta.vexp & KC_ABSENT) || !wave_live || key > min(wave_high, ends) ||
-                    !(key + AP_KEYS - 1 > wave_low - A.bound.window || key < A.bound.sinks))
-                    return;
-                ap_f32x16 sc[2];
-                kc_scores<D>(kt, w, sc);
-                const int ve = (int)(meta.vexp & 0xFFFFu) - KC_EXP;
-                if (ve > oexp) {
-                    const float by = ldexpf(1.f, max(oexp - ve, -300));
+            /* Step i weighs tile i, whose scores step i - 1 has formed, and forms tile i + 1's: keys are fetched two
+             * tiles ahead and values one. */
+            ap_f32x16 sa[2], sb[2];
+            KcFrag pf[4];
+            float top = -INFINITY, l = 0.f;
+            __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
+            __syncthreads();
+            T.want = T.want && !(T.meta.vexp & KC_ABSENT);
+            if (at + 1 < end)
+                fetch_k(at + 1, (ap_lds *)(at & 1 ? k0t : k1t));
+            fetch_v(at, (ap_lds *)(at & 1 ? v1t : v0t));
+            auto largest = [&](const ap_f32x16 (&sc)[2]) {
+                float m = -INFINITY;
 #pragma unroll
-                    for (int d = 0; d < D / 32; ++d)
+                for (int a = 0; a < 2; ++a)
 #pragma unroll
-                        for (int x = 0; x < 16; ++x)
-                            w.o[d][x] *= by;
-                    oexp = ve;
-                }
-                const bool all = key > wave_high - A.bound.window || key + AP_KEYS <= A.bound.sinks;
-                kc_weigh<D>(vt, key, w, sc, vat, fminf(fmaxf(factor * meta.kback, FLT_MIN), FLT_MAX), ldexpf(1.f, max(ve - oexp, -30)),
-                            key + AP_KEYS - 1 > min(wave_low, ends) || !all, min(w.last, ends), half, A.bound);
+                    for (int i = 0; i < 16; ++i)
+                        m = fmaxf(m, sc[a][i]);
+                return m;
             };
-            for (int i = at; i < end; i += 2) {
-                step(i, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t, (ap_lds *)v1t);
-                if (i + 1 < end)
-                    step(i + 1, (ap_lds *)k1t, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t);
+            auto first = [&](ap_f32x16 (&sc)[2]) {
+                if (T.want) {
+                    kc_scores<D, true, false>(ka, w, sc, sc, 0.f, 0.f, pf, l);
+                    top = largest(sc);
+                }
+            };
+            auto step = [&](int i, ap_f32x16 (&sc)[2], ap_f32x16 (&next)[2], ap_lds *vt, ap_lds *kn, ap_lds *vn, ap_lds *knn) {
+                const bool more = i + 1 < end;
+                if (more)
+                    look(i + 1, N);
+                __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0); /* this wave's part of what was fetched a step before */
+                __syncthreads();
+                if (i + 2 < end)
+                    fetch_k(i + 2, knn); /* over tile i's, which every wave has left */
+                if (more)
+                    fetch_v(i + 1, vn);
+                N.want = more && N.want && !(N.meta.vexp & KC_ABSENT);
+                apart |= (T.meta.vexp & (KC_ODD | KC_ABSENT)) == KC_ODD;
+                if (T.want) {
+                    const float f = fminf(fmaxf(factor * T.meta.kback, FLT_MIN), FLT_MAX);
+                    if (T.key + AP_KEYS - 1 > min(wave_low, T.ends) ||
+                        !(T.key > wave_high - A.bound.window || T.key + AP_KEYS <= A.bound.sinks)) { /* what a row does not see */
+                        const int from = T.key + 4 * half, upto = min(w.last, T.ends);
+#pragma unroll
+                        for (int a = 0; a < 2; ++a)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x) { /* element x of part a is key 32 a + 8 (x / 4) + 4 half + x % 4 */
+                                const int key = from + 32 * a + 8 * (x >> 2) + (x & 3);
+                                sc[a][x] = key <= upto && A.bound.sees(key, w.last) ? sc[a][x] : -INFINITY;
+                            }
+                        top = largest(sc);
+                    }
+                    top = glint_xor32(top, GlintMax()) * f;
+                    const bool up = top > w.m + AP_SLACK; /* a row's own test: its bits depend on no other row */
+                    const int ve = (int)(T.meta.vexp & 0xFFFFu) - KC_EXP;
+                    if (__any(up) || ve > oexp) {
+                        const float mn = up ? top : w.m;
+                        float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
+                        w.m = mn;
+                        l *= keep;
+                        keep *= ldexpf(1.f, max(min(oexp - ve, 0), -300));
+                        oexp = max(oexp, ve);
+#pragma unroll
+                        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                w.o[d][x] *= keep;
+                    }
+                    const float base = w.m == -INFINITY ? 0.f : w.m - KC_UP;
+                    if (N.want)
+                        kc_scores<D, true, true>(kn, w, next, sc, f, base, pf, l);
+                    else
+                        kc_scores<D, false, true>(kn, w, next, sc, f, base, pf, l);
+                    if (ve < oexp) {
+                        const _Float16 less = (_Float16)ldexpf(1.f, max(ve - oexp, -30));
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            pf[x].f *= less;
+                    }
+                    top = kc_outputs<D>(vt, w, vat, pf, next);
+                } else if (N.want) {
+                    kc_scores<D, true, false>(kn, w, next, sc, 0.f, 0.f, pf, l);
+                    top = largest(next);
+                }
+                T = N;
+            };
+            if (at & 1)
+                first(sb);
+            else
+                first(sa);
+            int i = at;
+            if (at & 1) {
+                step(i, sb, sa, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t);
+                ++i;
             }
+            for (; i < end; i += 2) {
+                step(i, sa, sb, (ap_lds *)v0t, (ap_lds *)k1t, (ap_lds *)v1t, (ap_lds *)k0t);
+                if (i + 1 < end)
+                    step(i + 1, sb, sa, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t);
+            }
+            w.l = l;
             const float back = ldexpf(1.f, max(oexp - 14, -300));
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
@@ -734,10 +855,18 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                 *(glint_f32x2 *)(A.sums + (slot * KC_ROWS + 32 * wave + col) * 2) = glint_f32x2{w.m, l};
         }
         left -= take;
-        if (left == 0)
+        if (left == 0) {
+            if (at == 0 && take < cost) {
+                const int step = A.starts[me].step, w_last = me + (cost - take + step - 1) / step;
+                if (threadIdx.x == 0)
+                    A.joins[me] = KcJoin{w_last, s.q0, head, rb, s.rows, {0, 0, 0}};
+            } else if (threadIdx.x == 0) {
+                A.joins[me].w_last = 0;
+            }
             break;
+        }
         at = 0;
-        do { /* the next group that has work */
+        for (;;) { /* the next group that has rows */
             if (++rb == A.nblk) {
                 rb = 0;
                 if (++h == A.Hn) {
@@ -745,59 +874,62 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                     ++b;
                 }
             }
-        } while (plan.pre[b * A.nblk + rb + 1] == plan.pre[b * A.nblk + rb]);
-        b = __builtin_amdgcn_readfirstlane(b);
-        h = __builtin_amdgcn_readfirstlane(h);
-        rb = __builtin_amdgcn_readfirstlane(rb);
+            if (rb * KC_ROWS < kc_seq(A, b).rows)
+                break;
+            rb = A.nblk - 1; /* no further block of this head has */
+        }
     }
 }
 
-/* The group that begins in workgroup w's run and ends in a later one's: its parts, added in the list's order.
- * Blocks (w, y); a block takes 32 rows, and lists are found as there. */
+/* The group that begins in workgroup w's run and ends in a later one's: its parts, added in the list's order. Blocks
+ * (w, y); a block takes KJ_ROWS rows, D / 4 lanes one, each 4 dimensions. */
 #define KJ_T 256
-#define KJ_ROWS 32
+#define KJ_ROWS 8
 template <int D>
-__global__ __launch_bounds__(KJ_T) void k_kv4_chunk_join(KcArgs A, int grid) {
-    __shared__ KcPlan plan;
-    kc_plan(A, plan);
-    const int total = kc_total(A, plan), share = kc_share(total, grid), me = blockIdx.x;
-    const int64_t last = (int64_t)(me + 1) * share - 1; /* of the run */
-    if (last >= total - 1)
+__global__ __launch_bounds__(KJ_T) void k_kv4_chunk_join(KcArgs A) {
+    constexpr int LANES = D / 4, AHEAD = 4;
+    const int me = blockIdx.x;
+    const KcJoin J = A.joins[me];
+    if (J.w_last == 0 || J.rb * KC_ROWS + (int)blockIdx.y * KJ_ROWS >= J.rows)
         return;
-    int b, h, rb, at;
-    kc_find(A, plan, (int)last, b, h, rb, at);
-    const int *pre = plan.pre + b * A.nblk + rb;
-    const int cost = pre[1] - pre[0];
-    if (at >= share || at == cost - 1) /* it began before this run, or ends with it */
-        return;
-    const KcSeq s = kc_seq(A, b);
-    const int w_last = (int)((last + cost - 1 - at) / share);
-    constexpr int LANES = D / 4;
-    const int d = 4 * (threadIdx.x % LANES);
+    const int lane = threadIdx.x % LANES, parts = J.w_last - me + 1;
     for (int r = threadIdx.x / LANES; r < KJ_ROWS; r += KJ_T / LANES) {
-        const int in = blockIdx.y * KJ_ROWS + r, row = rb * KC_ROWS + in;
-        if (row >= s.rows)
-            break;
-        auto slot = [&](int w) { return (int64_t)(2 * w + (w == me)) * KC_ROWS + in; };
+        const int in = blockIdx.y * KJ_ROWS + r, row = J.rb * KC_ROWS + in;
+        const bool live = row < J.rows;
+        auto slot = [&](int p) { return (int64_t)(2 * (me + p) + (p == 0)) * KC_ROWS + in; };
         float m = -INFINITY;
-        for (int w = me; w <= w_last; ++w)
-            m = fmaxf(m, A.sums[slot(w) * 2]);
+        for (int p = lane; p < parts; p += LANES)
+            m = live ? fmaxf(m, A.sums[slot(p) * 2]) : m;
+#pragma unroll
+        for (int x = 1; x < LANES; x *= 2)
+            m = fmaxf(m, __shfl_xor(m, x, 64));
         const float base = m == -INFINITY ? 0.f : m;
         float l = 0.f;
         glint_f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 4
-        for (int w = me; w <= w_last; ++w) {
-            const glint_f32x2 ml = *(const glint_f32x2 *)(A.sums + slot(w) * 2);
-            const glint_f32x4 v = *(const glint_f32x4 *)(A.part + slot(w) * D + d);
-            const float f = __builtin_amdgcn_exp2f(ml.x - base);
-            l = fmaf(f, ml.y, l);
+        for (int p0 = 0; p0 < parts; p0 += AHEAD) {
+            glint_f32x4 v[AHEAD];
+            glint_f32x2 ml[AHEAD];
 #pragma unroll
-            for (int x = 0; x < 4; ++x)
-                o[x] = fmaf(f, v[x], o[x]);
+            for (int p = 0; p < AHEAD; ++p) {
+                ml[p] = glint_f32x2{0.f, 0.f};
+                if (live && p0 + p < parts) {
+                    ml[p] = *(const glint_f32x2 *)(A.sums + slot(p0 + p) * 2);
+                    v[p] = *(const glint_f32x4 *)(A.part + slot(p0 + p) * D + 4 * lane);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < AHEAD; ++p) {
+                const float f = p0 + p < parts ? __builtin_amdgcn_exp2f(ml[p].x - base) : 0.f;
+                l = p0 + p < parts ? fmaf(f, ml[p].y, l) : l;
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+                    o[x] = p0 + p < parts ? fmaf(f, v[p][x], o[x]) : o[x];
+            }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        *(glint_u32x2 *)(A.out + ((int64_t)(s.q0 + row / A.G) * A.Hq + (A.h0 + h) * A.G + row % A.G) * D + d) =
-            glint_u32x2{glint_cvt_bf16x2(o[0] * inv, o[1] * inv), glint_cvt_bf16x2(o[2] * inv, o[3] * inv)};
+        if (live)
+            *(glint_u32x2 *)(A.out + ((int64_t)(J.q0 + row / A.G) * A.Hq + J.head + row % A.G) * D + 4 * lane) =
+                glint_u32x2{glint_cvt_bf16x2(o[0] * inv, o[1] * inv), glint_cvt_bf16x2(o[2] * inv, o[3] * inv)};
     }
 }
 
@@ -806,7 +938,8 @@ __global__ __launch_bounds__(KJ_T) void k_kv4_chunk_join(KcArgs A, int grid) {
 struct KcCut {
     int64_t seqs;
     int heads, slots, nblk, grid;
-    int64_t sums, meta, tiles, bytes; /* offsets; all of it */
+    int unpack; /* workgroups of k_kv4_unpack */
+    int64_t sums, starts, joins, meta, tiles, bytes; /* offsets; all of it */
 };
 static KcCut kc_cut(int B, int max_q, int H, int G, int D, int max_pages, bool own) {
     KcCut c{};
@@ -821,8 +954,11 @@ static KcCut kc_cut(int B, int max_q, int H, int G, int D, int max_pages, bool o
     c.seqs = std::max<int64_t>(1, std::min<int64_t>(c.seqs, KC_CAP / (tile * c.heads)));
     c.grid = (int)std::min<int64_t>(2 * glint_cu_count(), (c.seqs * c.nblk * c.heads * units + KC_SHARE - 1) / KC_SHARE);
     c.sums = (int64_t)c.grid * 2 * KC_ROWS * D * 4;
-    c.meta = c.sums + (int64_t)c.grid * 2 * KC_ROWS * 2 * 4;
+    c.starts = c.sums + (int64_t)c.grid * 2 * KC_ROWS * 2 * 4;
+    c.joins = c.starts + c.grid * (int64_t)sizeof(KcStart);
+    c.meta = c.joins + c.grid * (int64_t)sizeof(KcJoin);
     const int64_t slots = c.seqs * c.heads * c.slots;
+    c.unpack = (int)std::min<int64_t>(4 * glint_cu_count(), slots) + 1;
     c.tiles = (c.meta + slots * (int64_t)sizeof(KcMeta) + 255) & -256;
     c.bytes = c.tiles + slots * 4 * AP_KEYS * D;
     return c;
@@ -842,10 +978,13 @@ GLINT_API int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H
 }
 
 template <int D>
-static void kc_run(const KcArgs &a, int grid, hipStream_t stream) {
-    k_kv4_unpack<D><<<grid, KU_T, 0, stream>>>(a);
-    k_kv4_chunk<D><<<grid, KC_T, 0, stream>>>(a);
-    k_kv4_chunk_join<D><<<dim3(grid, KC_ROWS / KJ_ROWS), KJ_T, 0, stream>>>(a, grid);
+static void kc_run(const KcArgs &a, const KcCut &c, hipStream_t stream) {
+    if (a.k)
+        k_kv4_unpack<D, true><<<c.unpack, KU_T, 0, stream>>>(a, c.grid);
+    else
+        k_kv4_unpack<D, false><<<c.unpack, KU_T, 0, stream>>>(a, c.grid);
+    k_kv4_chunk<D><<<c.grid, KC_T, 0, stream>>>(a);
+    k_kv4_chunk_join<D><<<dim3(c.grid, KC_ROWS / KJ_ROWS), KJ_T, 0, stream>>>(a);
 }
 
 GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq,
@@ -878,7 +1017,7 @@ GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int6
              cu_q, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, B, max_q, Hq, H, Hq / H, c.nblk, 0, 0, c.slots,
              scale2 < FLT_MIN ? FLT_MIN : scale2, scale < 0.f ? 0x80008000u : 0u, out,
              {window ? window : GLINT_WINDOW_MAX, window ? sinks : 0}, (float *)mem, (float *)(mem + c.sums),
-             (KcMeta *)(mem + c.meta), mem + c.tiles};
+             (KcStart *)(mem + c.starts), (KcJoin *)(mem + c.joins), (KcMeta *)(mem + c.meta), mem + c.tiles};
     for (int64_t b = 0; b < B; b += c.seqs) {
         a.B = (int)std::min<int64_t>(B - b, c.seqs);
         a.table = table + b * table_stride;
@@ -898,9 +1037,9 @@ GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int6
         for (a.h0 = 0; a.h0 < H; a.h0 += c.heads) {
             a.Hn = std::min(c.heads, H - a.h0);
             if (D == 64)
-                kc_run<64>(a, c.grid, stream);
+                kc_run<64>(a, c, stream);
             else
-                kc_run<128>(a, c.grid, stream);
+                kc_run<128>(a, c, stream);
             if (hipGetLastError() != hipSuccess)
                 return -3;
         }
