@@ -2,9 +2,8 @@
  * cache (include/glint_serve.h).
  *
  * k_rotate — a workgroup takes rows (a token's heads, queries first) of one token: its rot / 2 angles are
- *   formed once, one a thread, and shared through LDS; then LPR lanes take a row, 8 dimensions each, and read
- *   the 8 that theirs are paired with a second time (the same cache lines), so a row needs no exchange but
- *   the sum of its squares. Angles, sines and cosines are formed in 64 bits, right at any position.
+ *   formed once, one a thread, and shared through LDS; then LPR lanes take a row, 8 dimensions each, and
+ *   exchange the sum of its squares and what is paired across lanes. Angles, sines and cosines are formed in 64 bits, right at any position.
  *
  *   k_rotate of the cache's form encodes a key after its rounding, as kv4_append would encode what rotate_qk
  *   returns, in the lanes that hold it. Values of few tokens are further rows; of many, tiles of 32 tokens
@@ -25,7 +24,7 @@ struct RotateArgs {
     int64_t T;
     int Hq, H, D, rot, interleaved;
     double magnitude;
-    float eps;
+    float eps, inv_d;
     const void *q_norm, *k_norm;
     int norm_f32;
     void *q_out, *k_out;
@@ -35,7 +34,7 @@ struct RotateArgs {
     float *k_absmax, *v_absmax;
     int64_t nslots;
     int value_rows;  /* of a token among its rows: H, or 0 where tiles take them */
-    unsigned tiles;  /* value tiles, the launch's first workgroups */
+    unsigned tiles;  /* value tiles, the launch's last workgroups */
     int tile_blocks; /* of 32 tokens */
     int parts;       /* workgroups of a token */
 };
@@ -80,12 +79,17 @@ __device__ __forceinline__ void kr_store8(float *p, const float (&w)[8]) {
     for (int i = 0; i < 2; ++i)
         ((glint_f32x4 *)p)[i] = glint_f32x4{w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]};
 }
-/* A norm's 8 weights, 16-B aligned. */
+/* A norm's 8 weights from dimension d on; ones where there is no norm. */
 __device__ __forceinline__ void kr_norm8(const void *norm, int f32, int d, float (&g)[8]) {
-    if (f32)
+    if (!norm) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            g[i] = 1.f;
+    } else if (f32) {
         kt_load8<0>((const float *)norm + d, g);
-    else
+    } else {
         kt_load8<0>((const uint16_t *)norm + d, g);
+    }
 }
 
 /* 32 tokens' values of one head into the cache. */
@@ -93,8 +97,9 @@ template <class E, int D>
 __device__ __forceinline__ void kr_value_tile(const RotateArgs &A, const Kv4Bucket *buckets, int64_t *place, uint8_t *vt,
                                               float *scale) {
     constexpr int NB = D / 64, ROWS = KR_T / 8, PASSES = KT_TOKENS * NB / ROWS;
-    const int64_t t0 = (int64_t)(blockIdx.x % A.tile_blocks) * KT_TOKENS;
-    const int h = blockIdx.x / A.tile_blocks, e = threadIdx.x & 7, r = threadIdx.x >> 3;
+    const unsigned at = blockIdx.x - (gridDim.x - A.tiles);
+    const int64_t t0 = (int64_t)(at % A.tile_blocks) * KT_TOKENS;
+    const int h = at / A.tile_blocks, e = threadIdx.x & 7, r = threadIdx.x >> 3;
     float w[PASSES][8];
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) { /* every load first */
@@ -135,13 +140,17 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
     __shared__ float scale[CACHE ? (NB + 1) * KT_COLS : 1];
     if constexpr (CACHE) {
         kv4_fill_buckets(buckets);
-        if (blockIdx.x < A.tiles) {
+        if (blockIdx.x >= gridDim.x - A.tiles) {
             kr_value_tile<E, CD>(A, buckets, place, vt, scale);
             return;
         }
     }
-    const int64_t t = (int64_t)(blockIdx.x - A.tiles) / A.parts;
-    const int part = (int)((blockIdx.x - A.tiles) % A.parts);
+    int64_t t = (int64_t)blockIdx.x / A.parts;
+    const int part = (int)(blockIdx.x % A.parts);
+    if (A.parts == 1) { /* neighbours' places in the cache share lines: neighbours go to one XCD, the workgroup's index modulo 8 */
+        const int64_t per = A.T >> 3;
+        t = t < 8 * per ? (t & 7) * per + (t >> 3) : t;
+    }
     const int half = A.rot / 2, rows = A.Hq + A.H + (CACHE ? A.value_rows : 0);
     const double p = (double)A.pos[t];
     if ((int)threadIdx.x < half)
@@ -154,9 +163,11 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
     __syncthreads();
     const int c = threadIdx.x % LPR, d = 8 * c;
     const bool in = d < A.D, turned = d < A.rot;
-    /* y_i = w_i cs_i + p_i sn_i, p_i the dimension that i is paired with */
-    float cs[8], sn[8];
-    int other = d;
+    /* y_i = w_i cs_i + p_i sn_i, p_i the dimension that i is paired with, in lane `other` of the row */
+    float cs[8], sn[8], gq[8], gk[8];
+    kr_norm8(A.q_norm, A.norm_f32, in ? d : 0, gq);
+    kr_norm8(A.k_norm, A.norm_f32, in ? d : 0, gk);
+    int other = threadIdx.x & 63;
     if (!turned) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -173,10 +184,10 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
         }
     } else {
         const bool first = d < half;
-        other = first ? d + half : d - half;
+        other += first ? half / 8 : -half / 8;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const glint_f32x2 x = turn[(first ? d : other) + i];
+            const glint_f32x2 x = turn[(first ? d : d - half) + i];
             cs[i] = x.x;
             sn[i] = first ? -x.y : x.y;
         }
@@ -194,10 +205,7 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
         if (live)
             kt_load8<0>(from + d, w);
         if (!is_v) {
-            if (live && turned && !A.interleaved)
-                kt_load8<0>(from + other, y);
-            const void *norm = is_k ? A.k_norm : A.q_norm;
-            if (norm) { /* for all rows of a kind */
+            if (is_k ? A.k_norm : A.q_norm) { /* for all rows of a kind */
                 /* The order of the sum is that of torch's mean over a row (neighbours by pairs, from 128
                  * dimensions on by fours in turn first), and no product is fused, so that f32 rows have the bits of
                  * the same formula written there. */
@@ -214,26 +222,22 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
                     sum = glint_add_dpp<GLINT_DPP_ROW_MIRROR>(sum);
                 if constexpr (LPR >= 32)
                     sum += __shfl_xor(sum, 16, 64);
-                const float r = rsqrtf(sum / (float)A.D + A.eps);
-                float g[8];
-                if (in) {
-                    kr_norm8(norm, A.norm_f32, d, g);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        w[i] = w[i] * r * g[i];
-                    if (turned && !A.interleaved) {
-                        kr_norm8(norm, A.norm_f32, other, g);
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            y[i] = y[i] * r * g[i];
-                    }
-                }
-            }
-            if (turned && A.interleaved) {
+                const float r = rsqrtf(sum * A.inv_d + A.eps);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
-                    y[i] = w[i ^ 1];
+                    w[i] = w[i] * r * (is_k ? gk[i] : gq[i]);
             }
+        }
+        if (A.interleaved) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                y[i] = w[i ^ 1];
+        } else { /* every lane of the wave, also of rows that do not turn */
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                y[i] = __shfl(w[i], other, 64);
+        }
+        if (!is_v) {
             if (turned) {
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
@@ -323,7 +327,7 @@ GLINT_API int glint_rotate_qk(const void *q, int64_t q_stride_t, int64_t q_strid
     a.q = q, a.q_st = q_stride_t, a.q_sh = q_stride_h;
     a.k = k, a.k_st = k_stride_t, a.k_sh = k_stride_h;
     a.pos = pos, a.freqs = freqs, a.T = T, a.Hq = Hq, a.H = H, a.D = D, a.rot = rot, a.interleaved = interleaved != 0;
-    a.magnitude = magnitude, a.eps = eps, a.q_norm = q_norm, a.k_norm = k_norm, a.norm_f32 = norm_elt == GLINT_KV_F32;
+    a.magnitude = magnitude, a.eps = eps, a.inv_d = 1.f / (float)D, a.q_norm = q_norm, a.k_norm = k_norm, a.norm_f32 = norm_elt == GLINT_KV_F32;
     a.q_out = q_out, a.k_out = k_out;
     const int rc = kr_refuse(a, elt, norm_elt, 1);
     if (rc || T == 0)
@@ -343,7 +347,7 @@ GLINT_API int glint_kv4_append_rotated(const void *q, int64_t q_stride_t, int64_
     a.k = k, a.k_st = k_stride_t, a.k_sh = k_stride_h;
     a.v = v, a.v_st = v_stride_t, a.v_sh = v_stride_h;
     a.pos = pos, a.freqs = freqs, a.T = T, a.Hq = Hq, a.H = H, a.D = D, a.rot = rot, a.interleaved = interleaved != 0;
-    a.magnitude = magnitude, a.eps = eps, a.q_norm = q_norm, a.k_norm = k_norm, a.norm_f32 = norm_elt == GLINT_KV_F32;
+    a.magnitude = magnitude, a.eps = eps, a.inv_d = 1.f / (float)D, a.q_norm = q_norm, a.k_norm = k_norm, a.norm_f32 = norm_elt == GLINT_KV_F32;
     a.q_out = q_out, a.k_out = k_out;
     a.slots = slots, a.k_hole = k_hole, a.k_absmax = k_absmax, a.v_hole = v_hole, a.v_absmax = v_absmax;
     a.nslots = pages * KV4_PAGE;

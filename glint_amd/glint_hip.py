@@ -824,9 +824,9 @@ def rotary_freqs(rot: int, base: float = 10000.0, factor: float = 1.0, trained: 
 
 def _here(*tensors) -> None:
     """Refuses tensors that are not on the current device; None among them is no tensor."""
-    at = (_TORCH or _torch()).cuda.current_device() if tensors[0].is_cuda else -1
+    at = (_TORCH or _torch())._C._cuda_getDevice() if tensors[0].is_cuda else -2
     for t in tensors:
-        if t is not None and (at < 0 or t.get_device() != at):
+        if t is not None and t.get_device() != at:
             raise ValueError(f"a tensor on {t.device}: all must be on the current GPU")
 
 
@@ -834,22 +834,29 @@ def _turn_args(q, k, pos, freqs, q_norm, k_norm):
     """What rotate_qk and kv4_append_rotated have in common: (elt, T, Hq, H, D, rot, pos, freqs, the norms' pointers and type)."""
     torch = _TORCH or _torch()
     T, hq, dim = q.shape
-    if k.dim() != 3 or k.shape[0] != T or k.shape[2] != dim or k.dtype is not q.dtype:
+    kT, heads, kdim = k.shape if k.dim() == 3 else (-1, 0, 0)
+    if kT != T or kdim != dim or k.dtype is not q.dtype:
         raise ValueError(f"q {tuple(q.shape)} {q.dtype}, k {tuple(k.shape)} {k.dtype}")
     elt, rot = _kv_elt(q), 2 * freqs.numel()
-    if dim % 16 or not 16 <= dim <= 256 or rot % 16 or not 16 <= rot <= dim:
+    if dim & 15 or not 16 <= dim <= 256 or rot & 15 or not 16 <= rot <= dim:
         raise ValueError(f"head dimension {dim}, {rot} of it turned: multiples of 16, at most 256")
     at, fr = _ints(pos, torch.int64, T, "pos"), _ints(freqs, torch.float64, rot // 2, "freqs")
+    qn = kn = None
     norm_elt = 0
-    for w in (q_norm, k_norm):
-        if w is not None:
-            if w.shape != (dim,) or not w.is_contiguous() or w.data_ptr() % 16:
-                raise ValueError(f"a norm: a contiguous, 16-B aligned vector of {dim}, got {tuple(w.shape)}")
-            norm_elt = _kv_elt(w)
-    if q_norm is not None and k_norm is not None and q_norm.dtype is not k_norm.dtype:
-        raise TypeError(f"norms of {q_norm.dtype} and {k_norm.dtype}")
-    return (elt, T, hq, k.shape[1], dim, rot, at, fr, None if q_norm is None else q_norm.data_ptr(),
-            None if k_norm is None else k_norm.data_ptr(), norm_elt)
+    if q_norm is not None:
+        qn, norm_elt = _norm(q_norm, dim)
+    if k_norm is not None:
+        kn, norm_elt = _norm(k_norm, dim)
+        if q_norm is not None and q_norm.dtype is not k_norm.dtype:
+            raise TypeError(f"norms of {q_norm.dtype} and {k_norm.dtype}")
+    return elt, T, hq, heads, dim, rot, at, fr, qn, kn, norm_elt
+
+
+def _norm(w, dim: int):
+    at = w.data_ptr()
+    if w.dim() != 1 or w.numel() != dim or not w.is_contiguous() or at & 15:
+        raise ValueError(f"a norm: a contiguous, 16-B aligned vector of {dim}, got {tuple(w.shape)}")
+    return at, _kv_elt(w)
 
 
 def _turn_out(out, like, shape):
