@@ -963,6 +963,18 @@ static KcCut kc_cut(int B, int max_q, int H, int G, int D, int max_pages, bool o
     c.bytes = c.tiles + slots * 4 * AP_KEYS * D;
     return c;
 }
+/* Calls that glint_kv4_attend.hip's kernel takes, whose waves decode the pages that they read and whose start is one
+ * launch: few rows, or few products in all (as far as the call's bounds say). us, there against here, 8 key heads of
+ * 128 dimensions:
+ *   rows of a key head       128       256       512       1024
+ *   1 sequence of 4000       21, 43    27, 52    33, 73    60, 75
+ *   1 sequence of 16000      40, 70    61, 121   101, 104  193, 129
+ *   8 sequences of 4000      66, 101   122, 100  224, 127  435, 177
+ *   8 sequences of 16000     198, 330  390, 358  758, 475  1497, 707 */
+static bool kc_few(int B, int max_q, int H, int G, int max_pages) {
+    const int64_t rows = (int64_t)max_q * G;
+    return rows <= 256 || rows * B * H <= ((int64_t)1 << 26) / KV4_PAGE / max_pages;
+}
 static bool kc_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
     return B >= 0 && max_q >= 1 && H >= 1 && Hq >= H && Hq % H == 0 && Hq <= 65535 && (D == 64 || D == 128) &&
            max_pages >= 1 && max_pages <= 1 << 24 && (int64_t)max_q * (Hq / H) <= (int64_t)KC_PAIRS * KC_ROWS;
@@ -971,7 +983,7 @@ static bool kc_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
 GLINT_API int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H, int D, int max_pages, int own) {
     if (!kc_shape(B, max_q, Hq, H, D, max_pages))
         return -2;
-    if (B == 0)
+    if (B == 0 || (!own && kc_few(B, max_q, H, Hq / H, max_pages)))
         return 0;
     const KcCut c = kc_cut(B, max_q, H, Hq / H, D, max_pages, own != 0);
     return c.seqs ? c.bytes : -2;
@@ -994,7 +1006,7 @@ GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int6
                                      int D, const uint16_t *k, int64_t k_stride_t, int64_t k_stride_h, const uint16_t *v,
                                      int64_t v_stride_t, int64_t v_stride_h, float scale, int window, int sinks,
                                      uint16_t *out, void *scratch, int64_t scratch_bytes, struct ihipStream_t *stream) {
-    if (!q || !k_hole || !k_absmax || !v_hole || !v_absmax || !table || !lens || !out || !scratch || !k != !v)
+    if (!q || !k_hole || !k_absmax || !v_hole || !v_absmax || !table || !lens || !out || !k != !v)
         return -1;
     if (!kc_shape(B, max_q, Hq, H, D, max_pages) || Tq < 0 || Tq > INT32_MAX || pages < 1 || pages >= (int64_t)1 << 40 ||
         (!cu_q && Tq != (int64_t)B * max_q) || window < 0 || window > GLINT_WINDOW_MAX || sinks < 0)
@@ -1008,6 +1020,11 @@ GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int6
         return -2;
     if (B == 0 || Tq == 0)
         return 0;
+    if (!k && kc_few(B, max_q, H, Hq / H, max_pages))
+        return glint_kv4_attend_window(q, q_stride_t, q_stride_h, Tq, k_hole, k_absmax, v_hole, v_absmax, pages, table,
+                                       table_stride, max_pages, lens, cu_q, B, max_q, Hq, H, D, scale, window, sinks, out, stream);
+    if (!scratch)
+        return -1;
     const float scale2 = fabsf(scale) * 1.44269504088896341f;
     const KcCut c = kc_cut(B, max_q, H, Hq / H, D, max_pages, k != nullptr);
     if (!c.seqs || scratch_bytes < c.bytes)

@@ -749,11 +749,12 @@ def kv4_attend_chunk(q, cache, page_table, lens, cu_q=None, max_q: Optional[int]
     size = serve_lib().glint_kv4_attend_chunk_scratch(B, max_q, hq, heads, dim, wide, k is not None)
     if size < 0:
         raise ValueError(f"{max_q} new tokens a sequence, {hq} heads over {heads}, {wide} pages: more than a launch can hold")
-    scratch = q.new_empty(size, dtype=torch.uint8)
+    scratch = q.new_empty(size, dtype=torch.uint8) if size else None
     _check(serve_lib().glint_kv4_attend_chunk(
         q.data_ptr(), qt, qh, rows, *planes, pages, page_table.data_ptr(), page_table.stride(0), wide, n, cu, B, max_q, hq,
         heads, dim, None if k is None else k.data_ptr(), kt, kh, None if v is None else v.data_ptr(), vt, vh,
-        dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(), scratch.data_ptr(), size, _sh(None)),
+        dim ** -0.5 if scale is None else scale, window, sinks, out.data_ptr(),
+        scratch.data_ptr() if size else None, size, _sh(None)),
         "glint_kv4_attend_chunk")
     return out
 

@@ -87,7 +87,8 @@ int glint_kv4_attend_window(const uint16_t *q, int64_t q_stride_t, int64_t q_str
  * alone). Scores, softmax and sums are f32; held keys, values and softmax weights enter the matrix products in
  * f16 (an absmax below 2^-25 of the largest that a workgroup has met loses bits), given ones as in
  * glint_attend_prompt. A value that is not finite leaves itself or NaN in its dimension of the rows that see it.
- * max_q (Hq / H) is at most 2^18. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a shape that is
+ * max_q (Hq / H) is at most 2^18. Few rows without own keys go as glint_kv4_attend_window does, its refusals and its
+ * workspace included, and _scratch gives 0. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a shape that is
  * refused) for the current device; the call's alone until it has run. */
 int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H, int D, int max_pages, int own);
 int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq, const uint8_t *k_hole,

@@ -5,7 +5,7 @@ import pytest
 from glint_amd import glint_hip as H
 from tests import bounded_util as R
 from tests import serve_util as S
-from tests.gpu_util import torch_cuda
+from tests.gpu_util import host, torch_cuda
 from tests.test_gpu_kv4 import bf16, gpu, random_planes
 from tests.test_gpu_window import paged, spoil, values
 
@@ -13,15 +13,23 @@ pytestmark = pytest.mark.gpu
 
 
 def bound(own):
-    """The cache's: f16 tables, scales and their products, three roundings of 2^-12 for a key and for a value element (half of
-    2^-11 where it is even once scaled) and one for a weight; f32 scores. Own keys: as attend_prompt's. A mix: both."""
+    """f16 products: as kv4_attend's, whose one rounding of a value, of a weight and of a key element they share (2^-12 there, half
+    of what f16's worst is; all of it here), twice for the weights, whose sum is of the rounded ones. An own key or value
+    is bf16 and rounds no more in f16."""
     def far(out, mass, size):
-        cache = 2.0 ** -8 * np.abs(out) + mass * (4 * 2.0 ** -12 + np.expm1(2 * (3 * 2.0 ** -12 + 2.0 ** -18) * size)[:, None] + 2.0 ** -16)
-        return np.maximum(cache, S.prompt_bound(out, mass, size)) if own else cache
+        return 2.0 ** -8 * np.abs(out) + mass * (3 * 2.0 ** -11 + np.expm1(2 * (2.0 ** -11 + 2.0 ** -18) * size)[:, None] + 2.0 ** -16)
     return far
 
 
-def check(lens, nqs, heads, G, D, window=0, sinks=0, own=False, seed=0, max_q=None, spread=None, scale=None, **kw):
+def many(table, rows):
+    """The table with further columns and a max_q that bounds more rows: both only bounds, for which the call takes the
+    kernels for many rows."""
+    wide = np.full((table.shape[0], 4200), -3, np.int32)
+    wide[:, :table.shape[1]] = table
+    return wide, max(rows, 257)
+
+
+def check(lens, nqs, heads, G, D, window=0, sinks=0, own=False, seed=0, spread=None, scale=None):
     rng = np.random.default_rng(seed)
     planes, table, pages = paged(rng, lens, heads, D)
     if spread is not None:
@@ -37,9 +45,10 @@ def check(lens, nqs, heads, G, D, window=0, sinks=0, own=False, seed=0, max_q=No
             j = np.arange(max(0, n - nq), n)
             for plane in (planes[1], planes[3]):
                 plane[table[b, j // 64], :, :, j % 64] = np.nan
-    out = H.kv4_attend_chunk(q, tuple(gpu(p) for p in planes), gpu(table), gpu(np.array(lens, np.int32)), gpu(cu),
-                             max_q=max_q or max(nqs), k=k if own else None, v=v if own else None, window=window or None, sinks=sinks,
-                             scale=scale, **kw)
+    wide, max_q = many(table, max(nqs))
+    assert H.serve_lib().glint_kv4_attend_chunk_scratch(len(lens), max_q, heads * G, heads, D, wide.shape[1], own) > 0
+    out = H.kv4_attend_chunk(q, tuple(gpu(p) for p in planes), gpu(wide), gpu(np.array(lens, np.int32)), gpu(cu), max_q=max_q,
+                             k=k if own else None, v=v if own else None, window=window or None, sinks=sinks, scale=scale)
     got, qf, kf, vf = values(out), values(q), values(k), values(v)
     for b, (n, nq) in enumerate(zip(lens, nqs)):
         if nq == 0:
@@ -116,9 +125,20 @@ def test_rows_outside_stay():
     assert got is out
     assert (out[:3] == 7).all() and (out[23:33] == 7).all() and (out[53:] == 7).all()
     assert torch.equal(out[3:23], full[3:23]) and torch.equal(out[33:53], full[33:53])
+    assert torch.equal(full[3:53], H.kv4_attend(q, cache, gpu(table), lens, gpu(np.array([3, 33, 53], np.int32)))[3:53])
+    wide, _ = many(table, 0)
+    k = bf16(rng.normal(0, 1, (60, 1, 64)))
+    for own in (None, k):
+        out.fill_(7.0)
+        H.kv4_attend_chunk(q, cache, gpu(wide), lens, gpu(np.array([3, 33, 53], np.int32)), max_q=260, k=own, v=own, out=out)
+        assert (out[:3] == 7).all() and (out[53:] == 7).all() and (out[3:53] != 7).any()
+    out.fill_(7.0)
+    H.kv4_attend_chunk(q, cache, gpu(table), lens, gpu(np.array([3, 33, 53], np.int32)), max_q=20, k=k, v=k, out=out)
+    assert (out[:3] == 7).all() and (out[23:33] == 7).all() and (out[53:] == 7).all()
     for cu in ([-1, 5, 70], [5, 5, 4]):  # bounds that lie outside: nothing is written
         out.fill_(7.0)
         H.kv4_attend_chunk(q, cache, gpu(table), lens, gpu(np.array(cu, np.int32)), max_q=20, out=out)
+        H.kv4_attend_chunk(q, cache, gpu(wide), lens, gpu(np.array(cu, np.int32)), max_q=260, out=out)
         assert (out == 7).all(), cu
 
 
@@ -133,11 +153,13 @@ def test_missing_pages_are_not_seen():
     k, v = S.held(planes, table[0][np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64)
     t = table.copy()
     t[0, 1], t[0, 3], t[0, 7] = -1, pages, 1 << 30
-    got = values(H.kv4_attend_chunk(q, cache, gpu(t), lens, cu, max_q=nq))
+    wide, max_q = many(t, nq)
+    got = values(H.kv4_attend_chunk(q, cache, gpu(wide), lens, cu, max_q=max_q))
     there = ~np.isin(np.arange(n) // 64, (1, 3, 7))
     ok = R.seen(np.arange(nq) + n - nq, n, 0, 0) & there
     for h in range(2):
         assert R.far(got[:, h], *R.attend(values(q)[:, h], k[:, 0], v[:, 0], ok, D ** -0.5), bound(False)) <= 0
+    assert (H.kv4_attend_chunk(q, cache, gpu(np.full_like(wide, -1)), lens, cu, max_q=max_q) == 0).all()
     assert (H.kv4_attend_chunk(q, cache, gpu(np.full_like(table, -1)), lens, cu, max_q=nq) == 0).all()
     assert (H.kv4_attend_chunk(q, cache, gpu(table[:, :0]), lens, cu, max_q=nq) == 0).all()
 
@@ -154,7 +176,8 @@ def test_what_is_not_finite_stays_with_its_rows(D, own):
         q = bf16(rng.normal(0, 1, (nq, 2, D)))
         lens, cu = gpu(np.array([n], np.int32)), gpu(np.array([0, nq], np.int32))
         k, v = (bf16(rng.normal(0, 1, (nq, 1, D))) for _ in range(2))
-        run = lambda p, k, v: H.kv4_attend_chunk(q, tuple(gpu(x) for x in p), gpu(table), lens, cu, max_q=nq,
+        wide, max_q = many(table, nq)
+        run = lambda p, k, v: H.kv4_attend_chunk(q, tuple(gpu(x) for x in p), gpu(wide), lens, cu, max_q=max_q,
                                                  k=k if own else None, v=v if own else None)
         clean = run(planes, k, v)
         assert torch.isfinite(clean).all()
@@ -210,7 +233,8 @@ def test_captured():
     cache, table, lens = tuple(gpu(p) for p in planes), gpu(table), gpu(np.array([2900, 300], np.int32))
     q, k, v = (bf16(rng.normal(0, 1, (80, h, 64))) for h in (4, 2, 2))
     cu = gpu(np.array([0, 30, 80], np.int32))
-    calls = [lambda: H.kv4_attend_chunk(q, cache, table, lens, cu, max_q=50),
+    broad = gpu(many(host(table), 0)[0])
+    calls = [lambda: H.kv4_attend_chunk(q, cache, broad, lens, cu, max_q=260),
              lambda: H.kv4_attend_chunk(q, cache, table, lens, cu, max_q=50, k=k, v=v, window=700, sinks=4)]
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
@@ -233,10 +257,20 @@ def test_captured():
             assert torch.equal(y, c()), i
 
 
-def test_many_sequences():
-    """More sequences than a launch's list holds, most of them short."""
+@pytest.mark.parametrize("own", [False, True])
+def test_many_sequences(own):
+    """More sequences than a launch's list holds, most of them short, and (where the table's width bounds their tiles)
+    than its scratch memory does."""
     torch_cuda()
     rng = np.random.default_rng(14)
-    nqs = rng.integers(0, 4, 2100).tolist()
-    lens = [n + int(x) for n, x in zip(nqs, rng.integers(0, 90, 2100))]
-    check(lens, nqs, 1, 1, 64, seed=14)
+    B = 700 if own else 130
+    nqs = rng.integers(0, 4, B).tolist()
+    lens = [n + int(x) for n, x in zip(nqs, rng.integers(0, 90, B))]
+    check(lens, nqs, 1, 1, 64, own=own, seed=14)
+
+
+def test_equal_groups():
+    """Groups that come out even over the device's workgroups: whole ones, and equal parts."""
+    torch_cuda()
+    check([900], [300], 2, 8, 64, seed=15)
+    check([1300] * 3, [200] * 3, 1, 4, 128, seed=16)

@@ -39,7 +39,7 @@ def prompt(lib, **kw):
 
 
 def chunk(lib, **kw):
-    a = dict(q=P, qt=1024, qh=128, Tq=8, kh=P, ka=P, vh=P, va=P, pages=2, table=P, ts=4, wide=4, lens=P, cu=None, B=2, max_q=4, Hq=8,
+    a = dict(q=P, qt=1024, qh=128, Tq=600, kh=P, ka=P, vh=P, va=P, pages=2, table=P, ts=4, wide=4000, lens=P, cu=None, B=2, max_q=300, Hq=8,
              H=2, D=128, k=None, kt=256, kh_=128, v=None, vt=256, vh_=128, scale=1.0, window=0, sinks=0, out=P, scratch=P,
              size=1 << 40, stream=None)
     a.update(kw)
@@ -57,7 +57,7 @@ TURN = [("q", None, -1), ("k", None, -1), ("pos", None, -1), ("freqs", None, -1)
     (append, TURN + [("v", None, -1), ("slots", None, -1), ("va", None, -1), ("D", 96, -2), ("D", 256, -2), ("pages", 0, -2),
                      ("v", ODD, -2), ("vt", 132, -2), ("kh_", ODD, -2)]),
     (attend, [("q", None, -1), ("window", -1, -2), ("window", (1 << 30) + 1, -2), ("sinks", -1, -2), ("D", 96, -2)]),
-    (chunk, [("q", None, -1), ("k", P, -1), ("v", P, -1), ("scratch", None, -1), ("D", 96, -2), ("H", 3, -2), ("Tq", 9, -2), ("out", ODD, -2),
+    (chunk, [("q", None, -1), ("k", P, -1), ("v", P, -1), ("D", 96, -2), ("H", 3, -2), ("Tq", 601, -2), ("out", ODD, -2),
              ("scratch", ODD, -2), ("size", 1000, -2), ("window", -1, -2), ("sinks", -1, -2), ("max_q", (1 << 18) + 1, -2), ("max_q", 0, -2),
              ("wide", 0, -2), ("pages", 0, -2), ("qh", 129, -2)]),
     (prompt, [("q", None, -1), ("window", -1, -2), ("window", (1 << 30) + 1, -2), ("sinks", -1, -2), ("D", 96, -2)]),
@@ -67,6 +67,7 @@ def test_refusals(call, bad):
     for name, value, code in bad:
         assert call(lib, **{name: value}) == code, (name, value)
     if call is chunk:
+        assert chunk(lib, scratch=None, size=0) == -1
         for name, value in (("kt", 120), ("vh_", 129), ("k", ODD), ("vt", (1 << 24) + 8)):
             assert chunk(lib, **{"k": P, "v": P, name: value}) == -2, name
     if call is rotate:
@@ -84,9 +85,9 @@ def test_scratch():
     """Parts, sums, and tiles: 4 * 64 * D bytes for each page and for each 64 own keys of a sequence and head."""
     size = H.serve_lib().glint_kv4_attend_chunk_scratch
     assert size(0, 4, 8, 2, 128, 4, 0) == 0
-    small, wide = size(1, 64, 8, 2, 128, 4, 0), size(1, 64, 8, 2, 128, 1004, 0)
+    small, wide = size(1, 64, 8, 2, 128, 4, 1), size(1, 64, 8, 2, 128, 1004, 1)
     assert 0 < 2 * 4 * 4 * 64 * 128 < small and wide - small > 1000 * 2 * 4 * 64 * 128
-    assert size(1, 64, 8, 2, 128, 4, 1) > small
+    assert size(1, 64, 8, 2, 128, 4, 0) == 0 and size(1, 1 << 12, 8, 2, 128, 4, 0) == 0  # few rows; few products
     assert size(64, 512, 32, 8, 64, 1 << 16, 0) < 3 << 30  # cut into launches
     for bad in ((1, 4, 8, 3, 128, 4), (1, 4, 8, 2, 96, 4), (1, 0, 8, 2, 128, 4), (1, 4, 8, 2, 128, 1 << 25), (1, 1 << 16, 8, 2, 128, 1 << 24)):
         assert size(*bad, 0) == -2, bad
