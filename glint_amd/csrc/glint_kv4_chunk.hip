@@ -5,7 +5,7 @@
  *   scratch memory, K as [64][D] and V^T as [D][64], in the very order in which the next kernel's LDS holds
  *   them. A tile is scaled by a power of two, so that f16 keeps 11 bits of PARENT * absmax (one rounding) and
  *   all bits of a BF16 element. Decoding in the attention kernel itself, once for 256 query rows, took 586 us
- *   for 2048 tokens over 16384 where this takes X: its LDS round trips lie in every wave's way, and a
+ *   for 2048 tokens over 16384 where this takes 528: its LDS round trips lie in every wave's way, and a
  *   document's chunk has many row blocks.
  *
  * k_kv4_chunk — a group is one sequence, key head and block of up to 128 query rows (the heads that share the
@@ -192,8 +192,8 @@ __device__ __forceinline__ int kc_last(int lo, int hi, int x, F v) {
 }
 /* One workgroup finds where the attention's `grid` workgroups begin. Runs are equal shares of the list, or, where the
  * longest is then not much longer, whole groups or equal parts of groups: workgroups of one key head then walk
- * its tiles side by side, which the XCD's L2 serves. 2048 tokens over 16384, 512 groups: X us so, Y with equal
- * shares (41% of L2 reads missed). */
+ * its tiles side by side, which the XCD's L2 serves. 2048 tokens over 16384, 512 groups: 555 us so, 577 with equal
+ * shares (3% and 41% of L2 reads missed). */
 __device__ __forceinline__ void kc_starts(const KcArgs &a, KcPlan &p, int *cnt, int grid) {
     const int pairs = a.B * a.nblk;
     auto blocks = [&](int b) { return (kc_seq(a, b).rows + KC_ROWS - 1) / KC_ROWS; };
