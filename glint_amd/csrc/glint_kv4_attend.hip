@@ -493,9 +493,15 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
             }
             /* A whole page lies below every row's last position: nothing of it is masked, and the
              * rows have one power for its value scales, which go to LDS scaled and rounded to f16.
-             * Of another page they go there as they are. */
-            const bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1 &&
-                               (!BOUNDED || pg * KV4_PAGE >= s.len - A.window || (pg + 1) * KV4_PAGE <= A.sinks);
+             * Of another page they go there as they are. Behind a page that rows saw in part, as a bound's first
+             * ones, their powers may differ: then every page is another one. */
+            bool whole = (pg + 1) * KV4_PAGE <= s.len - s.nq + 1;
+            if (BOUNDED) {
+                whole = whole && (pg * KV4_PAGE >= s.len - A.window || (pg + 1) * KV4_PAGE <= A.sinks);
+#pragma unroll
+                for (int bb = 0; bb < NB; ++bb)
+                    whole = whole && !__any(__float_as_int(vdown[bb]) != __builtin_amdgcn_readfirstlane(__float_as_int(vdown[bb])));
+            }
             glint_f32x4 sc[4]; /* scores, without the row's factor */
             if (pg != KA_FAR) {
 #pragma unroll
@@ -615,6 +621,10 @@ __global__ __launch_bounds__(KA_T) void k_kv4_attend(Kv4AttendArgs A) {
                         }
                         if (__any(any >= vlimit[bb])) { /* outside f16's range under some row's power */
                             finite = kv4_over_row(finite, GlintMax());
+                            if (BOUNDED) { /* columns without a row go with the largest */
+                                const float most = glint_wave_max(finite);
+                                finite = last < 0 ? most : finite;
+                            }
                             if (finite >= vlimit[bb])
                                 carry(bb, kv4_new_power(finite, vdown[bb], vlimit[bb]));
                         }

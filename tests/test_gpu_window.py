@@ -82,6 +82,31 @@ def test_long_sequences_are_split():
     check_cache([70 + 40 * i for i in range(70)], [1] * 70, 1, 2, 64, 90, 66, seed=3)
 
 
+@pytest.mark.parametrize("sink_scale,edge_scale,rest_scale", [(1, 1, 8), (8, 1, 1), (1, 8, 1), (1 / 64, 1, 30), (30, 1 / 64, 1), (1, 1 / 30, 64)])
+def test_scales_of_unlike_pages(sink_scale, edge_scale, rest_scale):
+    """Pages seen in part come before whole ones whose values are larger or smaller, and a wave has several of them: 80
+    sequences with the same pages."""
+    torch_cuda()
+    for D, heads, G, nq, window, sinks in ((128, 2, 4, 1, 2048, 4), (64, 2, 5, 3, 2000, 70), (128, 1, 3, 5, 2001, 3)):
+        rng = np.random.default_rng(D + nq)
+        B, n = 80, 4096 + 17
+        planes, table, _ = paged(rng, [n], heads, D)
+        at = table[0]
+        planes[3][:] *= np.float32(rest_scale)
+        planes[3][at[:(sinks + 63) // 64]] *= np.float32(sink_scale / rest_scale)
+        low = (n - nq - window + 1) // 64
+        planes[3][at[low:low + 1]] *= np.float32(edge_scale / rest_scale)
+        q = bf16(rng.normal(0, 0.3, (nq, heads * G, D)).astype(np.float32))
+        out = H.kv4_attend(q.repeat(B, 1, 1), tuple(gpu(p) for p in planes), gpu(table).repeat(B, 1), gpu(np.full(B, n, np.int32)),
+                           max_q=nq, window=window, sinks=sinks)
+        got, qf = values(out).reshape(B, nq, heads * G, D), values(q)
+        k, v = S.held(planes, at[np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64)
+        ok = R.seen(np.arange(nq) + n - nq, n, window, sinks)
+        for h in range(heads * G):
+            worst = R.far(got[:, :, h], *R.attend(qf[:, h], k[:, h // G], v[:, h // G], ok, D ** -0.5), R.KV4)
+            assert worst <= 0, (D, nq, h, worst)
+
+
 def test_dropped_pages_are_not_read():
     """Pages between sinks and window may be -1 or any other number."""
     torch = torch_cuda()
