@@ -897,33 +897,35 @@ __global__ __launch_bounds__(KJ_T) void k_kv4_chunk_join(KcArgs A) {
         const int in = blockIdx.y * KJ_ROWS + r, row = J.rb * KC_ROWS + in;
         const bool live = row < J.rows;
         auto slot = [&](int p) { return (int64_t)(2 * (me + p) + (p == 0)) * KC_ROWS + in; };
-        float m = -INFINITY;
-        for (int p = lane; p < parts; p += LANES)
-            m = live ? fmaxf(m, A.sums[slot(p) * 2]) : m;
-#pragma unroll
-        for (int x = 1; x < LANES; x *= 2)
-            m = fmaxf(m, __shfl_xor(m, x, 64));
-        const float base = m == -INFINITY ? 0.f : m;
-        float l = 0.f;
+        float m = -INFINITY, l = 0.f;
         glint_f32x4 o = {0.f, 0.f, 0.f, 0.f};
         for (int p0 = 0; p0 < parts; p0 += AHEAD) {
             glint_f32x4 v[AHEAD];
             glint_f32x2 ml[AHEAD];
 #pragma unroll
             for (int p = 0; p < AHEAD; ++p) {
-                ml[p] = glint_f32x2{0.f, 0.f};
+                ml[p] = glint_f32x2{-INFINITY, 0.f};
+                v[p] = glint_f32x4{0.f, 0.f, 0.f, 0.f};
                 if (live && p0 + p < parts) {
                     ml[p] = *(const glint_f32x2 *)(A.sums + slot(p0 + p) * 2);
                     v[p] = *(const glint_f32x4 *)(A.part + slot(p0 + p) * D + 4 * lane);
                 }
             }
+            float top = m;
+#pragma unroll
+            for (int p = 0; p < AHEAD; ++p)
+                top = fmaxf(top, ml[p].x);
+            const float base = top == -INFINITY ? 0.f : top, keep = __builtin_amdgcn_exp2f(m - base);
+            m = top;
+            l *= keep;
+            o *= keep;
 #pragma unroll
             for (int p = 0; p < AHEAD; ++p) {
-                const float f = p0 + p < parts ? __builtin_amdgcn_exp2f(ml[p].x - base) : 0.f;
-                l = p0 + p < parts ? fmaf(f, ml[p].y, l) : l;
+                const float f = __builtin_amdgcn_exp2f(ml[p].x - base);
+                l = fmaf(f, ml[p].y, l);
 #pragma unroll
                 for (int x = 0; x < 4; ++x)
-                    o[x] = p0 + p < parts ? fmaf(f, v[p][x], o[x]) : o[x];
+                    o[x] = fmaf(f, v[p][x], o[x]);
             }
         }
         const float inv = l == 0.f ? 0.f : 1.f / l;
