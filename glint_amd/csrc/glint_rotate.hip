@@ -67,6 +67,14 @@ __device__ __forceinline__ glint_f32x2 kr_turn(double angle, double magnitude) {
     return glint_f32x2{(quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b};
 }
 
+/* 1 / sqrt(x) rounded once: a step of Newton's in 64 bits behind the instruction, which is off by a bit in one
+ * value of ten. */
+__device__ __forceinline__ float kr_rsqrt(float x) {
+    const float r = rsqrtf(x);
+    const double y = fma(0.5 * r, fma(-(double)x * r, (double)r, 1.0), (double)r);
+    return r > 0.f && r < INFINITY ? (float)y : r; /* of 0 and of infinity as they are */
+}
+
 __device__ __forceinline__ void kr_store8(uint16_t *p, const float (&w)[8]) {
     glint_u32x4 u;
 #pragma unroll
@@ -222,7 +230,7 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
                     sum = glint_add_dpp<GLINT_DPP_ROW_MIRROR>(sum);
                 if constexpr (LPR >= 32)
                     sum += __shfl_xor(sum, 16, 64);
-                const float r = rsqrtf(sum * A.inv_d + A.eps);
+                const float r = kr_rsqrt(sum * A.inv_d + A.eps);
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
                     w[i] = w[i] * r * (is_k ? gk[i] : gq[i]);

@@ -54,6 +54,22 @@ def test_rotate(T, Hq, heads, D, rot, norm, dtype, interleaved):
         check(got, want, off, dtype)
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_root_is_rounded_once(D):
+    """Small whole numbers, whose mean square is exact: a row of f32 holds its elements times the nearest f32 to the root's inverse."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(D)
+    x = rng.integers(-9, 10, (3000, 5, D)).astype(np.float32)
+    x[:, :, 0] = 1
+    x[0] = 0
+    eps = np.float32(2.0 ** -12)  # exact beside a mean of up to 81 in steps of 1 / D
+    one = torch.ones(D, device="cuda")
+    got, _ = H.rotate_qk(gpu(x), gpu(x), gpu(np.zeros(3000, np.int64)), torch.zeros(D // 2, dtype=torch.float64, device="cuda"),
+                         q_norm=one, k_norm=one, eps=float(eps))
+    r = (1 / np.sqrt((x.astype(np.float64) ** 2).mean(-1, keepdims=True) + float(eps))).astype(np.float32)
+    assert np.array_equal(got.cpu().numpy(), x * r)
+
+
 def test_far_and_negative_positions():
     """Angles of positions up to 2^40 and below 0, and of any frequency."""
     torch_cuda()
