@@ -35,7 +35,9 @@
  *   before is multiplied (equal lengths 65 without, 62 with; ragged ones 42.5, 39). 8 waves share a
  *   table: 4 waves a workgroup were slower everywhere, by the table's filling. Short calls are bound
  *   by their start, some 5 us from the launch to the first page's loads: lengths, runs, table and
- *   page numbers one after another; one sequence of 1000 tokens takes 12.8 us. */
+ *   page numbers one after another; one sequence of 1000 tokens takes 12.8 us.
+ *   Of a bounded call too: 32 sequences of 8192 under a window of 1024 and 4 first tokens read 38 MB in 17.8 us,
+ *   two to three pages a wave. */
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

@@ -18,7 +18,10 @@
  * k_kv4_chunk_join — parts of a group that lies in several runs, added in the list's order.
  *
  *   What bounds it: 4 D operations a row and key on the matrix units, the vector operations of a score beside
- *   them, and LDS, from which each wave reads every tile. */
+ *   them, and LDS, from which each wave reads every tile. 2048 tokens of 32 heads of 128 over 8 after 14336: 515
+ *   GFLOP in 528 to 558 us, of which unpacking takes 24 (its writes; 15 without them), the join 4 and
+ *   the rest 0.97 PFLOP/s at some 2.0 GHz, where an 8192^3 product of the library reaches 1.2 to 1.3. 512 tokens
+ *   in 4 parts a row block with their own BF16 keys: 189 to 196 us, 31 of them unpacking and 18 the join. */
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

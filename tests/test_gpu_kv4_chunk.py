@@ -274,3 +274,22 @@ def test_equal_groups():
     torch_cuda()
     check([900], [300], 2, 8, 64, seed=15)
     check([1300] * 3, [200] * 3, 1, 4, 128, seed=16)
+
+
+def test_heads_in_several_launches():
+    """A table so wide that its scratch memory holds 3 of 4 heads."""
+    torch_cuda()
+    rng = np.random.default_rng(17)
+    n, nq, heads, D = 300, 260, 4, 64
+    planes, table, _ = paged(rng, [n], heads, D)
+    wide = np.full((1, 50000), -1, np.int32)
+    wide[:, :table.shape[1]] = table
+    q = bf16(rng.normal(0, 1, (nq, heads, D)).astype(np.float32))
+    size = H.serve_lib().glint_kv4_attend_chunk_scratch(1, nq, heads, heads, D, wide.shape[1], 0)
+    assert 2 * 50000 * 256 * D < size < 4 * 50000 * 256 * D
+    got = values(H.kv4_attend_chunk(q, tuple(gpu(p) for p in planes), gpu(wide), gpu(np.array([n], np.int32)), max_q=nq))
+    k, v = S.held(planes, table[0][np.arange(n) // 64].astype(np.int64) * 64 + np.arange(n) % 64)
+    ok, qf = R.seen(np.arange(nq) + n - nq, n, 0, 0), values(q)
+    for h in range(heads):
+        worst = R.far(got[:, h], *R.attend(qf[:, h], k[:, h], v[:, h], ok, D ** -0.5), bound(False))
+        assert worst <= 0, (h, worst)
