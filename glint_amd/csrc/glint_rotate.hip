@@ -203,7 +203,8 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
             sn[i] = first ? -x.y : x.y;
         }
     }
-    for (int row = part * ROWS + (int)threadIdx.x / LPR; row - (int)threadIdx.x / LPR < rows; row += A.parts * ROWS) {
+    /* a wave ends with its own last row: 40 rows are 10 waves' */
+    for (int row = part * ROWS + (int)threadIdx.x / LPR; row - (int)(threadIdx.x & 63) / LPR < rows; row += A.parts * ROWS) {
         const bool is_v = CACHE && row >= A.Hq + A.H, is_k = row >= A.Hq && !is_v, live = in && row < rows;
         const int h = is_v ? row - A.Hq - A.H : is_k ? row - A.Hq : row;
         const E *from = is_v   ? (const E *)A.v + t * A.v_st + h * A.v_sh
