@@ -70,12 +70,12 @@ __device__ __forceinline__ glint_f32x2 kr_turn(double angle, double magnitude) {
     return glint_f32x2{(quarter + 1) & 2 ? -a : a, quarter & 2 ? -b : b};
 }
 
-/* 1 / sqrt(x) rounded once: a step of Newton's in 64 bits behind the instruction, which is off by a bit in one
- * value of ten. */
+/* 1 / sqrt(x) rounded once: a step of Newton's behind the instruction, which is off by a bit in one value of ten. What
+ * x r r leaves of 1 is formed from exact products, good to 2^-47. */
 __device__ __forceinline__ float kr_rsqrt(float x) {
-    const float r = rsqrtf(x);
-    const double y = fma(0.5 * r, fma(-(double)x * r, (double)r, 1.0), (double)r);
-    return r > 0.f && r < INFINITY ? (float)y : r; /* of 0 and of infinity as they are */
+    const float r = rsqrtf(x), h = x * r, l = fmaf(x, r, -h);
+    const float y = fmaf(0.5f * r, fmaf(-l, r, fmaf(-h, r, 1.f)), r);
+    return r > 0.f && r < INFINITY ? y : r; /* of 0 and of infinity as they are */
 }
 
 __device__ __forceinline__ void kr_store8(uint16_t *p, const float (&w)[8]) {
