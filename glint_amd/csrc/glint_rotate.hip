@@ -11,7 +11,7 @@
  *
  *   What bounds it: bytes, each read and written once, or the launch. 4095 tokens of 32 and 8 heads of 128: 84 MB
  *   in 16.3 to 17.6 us, 4.8 to 5.1 TB/s, the rate of a copy; with another lane's dimensions read from memory
- *   again instead of exchanged 18.0. 4096 tokens into the cache 28 us for 92 MB, 3.3 TB/s: codes and the value
+ *   again instead of exchanged 18.0. 4096 tokens into the cache 27 us for 88 MB, 3.3 TB/s: codes and the value
  *   tiles' LDS between loads and stores. 8 tokens: the kernel 3.8 us, a call from Python 14.5. */
 #include <algorithm>
 
