@@ -293,3 +293,23 @@ def test_heads_in_several_launches():
     for h in range(heads):
         worst = R.far(got[:, h], *R.attend(qf[:, h], k[:, h], v[:, h], ok, D ** -0.5), bound(False))
         assert worst <= 0, (h, worst)
+
+
+def test_two_calls_at_once():
+    """Calls on two streams, several in turn, each with scratch memory of its own."""
+    torch = torch_cuda()
+    rng = np.random.default_rng(18)
+    planes, table, _ = paged(rng, [2900, 700], 2, 64)
+    cache, lens = tuple(gpu(p) for p in planes), gpu(np.array([2900, 700], np.int32))
+    wide, cu = gpu(many(table, 0)[0]), gpu(np.array([0, 300, 420], np.int32))
+    qs = [bf16(rng.normal(0, 1, (420, 8, 64))) for _ in range(2)]
+    bounds = [{}, {"window": 900, "sinks": 5}]
+    want = [H.kv4_attend_chunk(q, cache, wide, lens, cu, max_q=300, **b) for q, b in zip(qs, bounds)]
+    streams = [torch.cuda.Stream() for _ in qs]
+    torch.cuda.synchronize()
+    got = [[] for _ in qs]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            got[i].append(H.kv4_attend_chunk(qs[i], cache, wide, lens, cu, max_q=300, stream=s, **bounds[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, w) for ys, w in zip(got, want) for y in ys)
