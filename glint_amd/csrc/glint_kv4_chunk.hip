@@ -39,6 +39,7 @@ typedef _Float16 kc_f16x2 __attribute__((ext_vector_type(2)));
 #define KC_SHARE 4    /* tiles that a workgroup takes at least */
 #define KC_UP 7.f     /* weights are 2^KC_UP times the softmax's: f16 has room above, and its small ones keep more bits */
 #define KC_CAP ((int64_t)1 << 31) /* bytes of tiles of a launch */
+#define KC_LENGTH (INT32_MAX - AP_KEYS) /* tokens of a sequence: a tile's last position is an int wherever it begins */
 
 /* What a tile's elements were multiplied by. */
 struct KcMeta {
@@ -99,7 +100,7 @@ __device__ __forceinline__ KcSeq kc_seq(const KcArgs &a, int b) {
         s.rows = a.G * min(s.nq, a.max_q);
     }
     const int most = (int)min((int64_t)INT32_MAX, (int64_t)a.max_pages * KV4_PAGE);
-    s.len = max(a.lens[b], 0);
+    s.len = min(max(a.lens[b], 0), KC_LENGTH);
     if (a.k) {
         s.own = max(0, s.len - s.nq);
         s.held = min(s.own, most);
