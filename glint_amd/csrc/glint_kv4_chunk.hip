@@ -317,7 +317,7 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
         const KcSeq s = kc_seq(A, b);
         const KcTiles t = kc_tiles(A, s, 0, A.nblk);
         const int gap = s.len - s.nq;
-        const int low = gap - A.bound.window + 1, high = gap + (s.rows - 1) / A.G; /* what some row sees */
+        const int low = (int)max((int64_t)0, (int64_t)gap - A.bound.window + 1), high = gap + (s.rows - 1) / A.G; /* what some row sees */
         auto seen = [&](int key) { return key <= high && (key >= low || key < A.bound.sinks); };
         KcMeta meta{1.f, KC_EXP};
         if (i < t.np) {
@@ -607,11 +607,12 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
         const int row = rb * KC_ROWS + 32 * wave + col, head = (A.h0 + h) * A.G;
         const bool live = row < s.rows, wave_live = rb * KC_ROWS + 32 * wave < s.rows;
         const int gap = s.len - s.nq;
-        const int wave_low = gap + (rb * KC_ROWS + 32 * wave) / A.G;
-        const int wave_high = gap + min(s.rows - 1, rb * KC_ROWS + 32 * wave + 31) / A.G;
+        /* rows before the sequence's first position see nothing, as one at -1 does; less any window is an int then */
+        const int wave_low = max(-1, gap + (rb * KC_ROWS + 32 * wave) / A.G);
+        const int wave_high = max(-1, gap + min(s.rows - 1, rb * KC_ROWS + 32 * wave + 31) / A.G);
         w.m = -INFINITY;
         w.l = 0.f;
-        w.last = live ? gap + row / A.G : -1;
+        w.last = live ? max(-1, gap + row / A.G) : -1;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -1039,7 +1040,7 @@ GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int6
     KcArgs a{q, q_stride_t, q_stride_h, Tq, k_hole, v_hole, k_absmax, v_absmax, pages, table, table_stride, max_pages, lens,
              cu_q, k, v, k_stride_t, k_stride_h, v_stride_t, v_stride_h, B, max_q, Hq, H, Hq / H, c.nblk, 0, 0, c.slots,
              scale2 < FLT_MIN ? FLT_MIN : scale2, scale < 0.f ? 0x80008000u : 0u, out,
-             {window ? window : GLINT_WINDOW_MAX, window ? sinks : 0}, (float *)mem, (float *)(mem + c.sums),
+             {window ? window : INT32_MAX, window ? sinks : 0}, (float *)mem, (float *)(mem + c.sums),
              (KcStart *)(mem + c.starts), (KcJoin *)(mem + c.joins), (KcMeta *)(mem + c.meta), mem + c.tiles};
     for (int64_t b = 0; b < B; b += c.seqs) {
         a.B = (int)std::min<int64_t>(B - b, c.seqs);

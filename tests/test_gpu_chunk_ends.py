@@ -39,3 +39,11 @@ def test_a_window_at_the_last_positions(length, D):
     torch_cuda()
     print(f"length={length} D={D}", flush=True)
     far_chunk(length, 70, 5, D)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 30 + 100, 2 ** 30 + 5])
+def test_without_a_window_every_position_is_seen(length, D):
+    torch_cuda()
+    print(f"length={length} D={D}", flush=True)
+    far_chunk(length, None, 0, D)
