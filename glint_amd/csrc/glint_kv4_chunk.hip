@@ -47,6 +47,7 @@ struct KcMeta {
     uint32_t vexp; /* the values': 2^(14 - e), e + KC_EXP here; and */
 };
 #define KC_EXP 1024
+#define KC_LIFT 64
 #define KC_ABSENT 0x80000000u /* the page is not in the pool: nothing was written */
 #define KC_ODD 0x40000000u    /* a value that is not finite was taken out */
 
@@ -619,7 +620,8 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
             for (int i = 0; i < 16; ++i)
                 w.o[d][i] = 0.f;
         bool apart = false;
-        int oexp = -4096; /* the outputs are 2^(14 - oexp) times themselves */
+        int oexp = -4096; /* the outputs are 2^(14 - oexp) times themselves: the last tile's power */
+        int most = -4096; /* of the tiles so far; oexp stays within KC_LIFT of it, so that outputs stay finite */
         if (at < end) {
             /* the place of tile i: pages, then own keys; its first position and, of what it holds, the end */
             auto place = [&](int i) {
@@ -739,13 +741,17 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                     top = glint_xor32(top, GlintMax()) * f;
                     const bool up = top > w.m + AP_SLACK; /* a row's own test: its bits depend on no other row */
                     const int ve = (int)(T.meta.vexp & 0xFFFFu) - KC_EXP;
-                    if (__any(up) || ve > oexp) {
+                    /* The outputs go to the tile's power, up or down, and not the weights, whose f16 has no bits to spare:
+                     * at 2^-17 of the largest value met, weights times 2^-24 lost half of themselves. */
+                    most = max(most, ve);
+                    const int to = max(ve, most - KC_LIFT);
+                    if (__any(up) || to != oexp) {
                         const float mn = up ? top : w.m;
                         float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
                         w.m = mn;
                         l *= keep;
-                        keep *= ldexpf(1.f, max(min(oexp - ve, 0), -300));
-                        oexp = max(oexp, ve);
+                        keep *= ldexpf(1.f, max(oexp - to, -300));
+                        oexp = to;
 #pragma unroll
                         for (int d = 0; d < D / 32; ++d)
 #pragma unroll

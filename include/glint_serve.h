@@ -85,7 +85,7 @@ int glint_kv4_attend_window(const uint16_t *q, int64_t q_stride_t, int64_t q_str
  * multiples of 8, stride_t from D to 2^24, 16-B aligned, they are the new tokens' keys and values, and what the
  * cache holds of these tokens is not read (it need not hold them; its max_pages bound the tokens before them
  * alone; a length past 2^31 - 65 counts as that). Scores, softmax and sums are f32; held keys, values and softmax weights enter the matrix products in
- * f16 (an absmax below 2^-25 of the largest that a workgroup has met loses bits), given ones as in
+ * f16 (an absmax below 2^-64 of the largest that a workgroup has met loses bits), given ones as in
  * glint_attend_prompt. A value that is not finite leaves itself or NaN in its dimension of the rows that see it.
  * max_q (Hq / H) is at most 2^18. Few rows without own keys go as glint_kv4_attend_window does, its refusals and its
  * workspace included, and _scratch gives 0. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a shape that is
