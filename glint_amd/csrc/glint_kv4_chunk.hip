@@ -4,7 +4,7 @@
  *   pages' codes, and, where the call brings them, the new tokens' own BF16 rows, become f16 operands in
  *   scratch memory, K as [64][D] and V^T as [D][64], in the very order in which the next kernel's LDS holds
  *   them. A tile is scaled by a power of two, so that f16 keeps 11 bits of PARENT * absmax (one rounding) and
- *   all bits of a BF16 element. Decoding in the attention kernel itself, once for 256 query rows, took 586 us
+ *   all bits of a BF16 element; what one power does not hold is marked (KC_WIDE) and taken as pairs of BF16. Decoding in the attention kernel itself, once for 256 query rows, took 586 us
  *   for 2048 tokens over 16384 where this takes 528: its LDS round trips lie in every wave's way, and a
  *   document's chunk has many row blocks.
  *
@@ -27,7 +27,7 @@
 #include <cmath>
 
 #include "attend_tile.h"
-#include "kv4.h"
+#include "kv4_tile.h"
 
 typedef _Float16 kc_f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 kc_f16x2 __attribute__((ext_vector_type(2)));
@@ -47,9 +47,19 @@ struct KcMeta {
     uint32_t vexp; /* the values': 2^(14 - e), e + KC_EXP here; and */
 };
 #define KC_EXP 1024
-#define KC_LIFT 64
+/* What one power a tile does not keep in f16, or an output in f32 while it goes from tile to tile, makes a tile wide:
+ * it is left out of these products and taken by kc_wide_tile. The size of a key or value then costs the rows nothing that do not
+ * see it or give it no weight.
+ *   Keys: f16 is off by 2^-25 of what an element is scaled to, q's likewise, and a score by 2^-9 D times its factor at most. A
+ *   factor of KC_KEYS leaves 2^-18; a wave's rows have powers of their own, so a wave asks for itself.
+ *   Values: a token's 64 dimensions whose largest is KC_SPAN of the tile's, which is 2^7 to 2^15 once scaled, keep 2^-20 of that.
+ *   Powers past KC_BAND either way: tiles within are 2^64 apart at most, by which an output may be lifted. */
+#define KC_KEYS 0x1p-16f
+#define KC_SPAN 0x1p-12f
+#define KC_BAND 32
 #define KC_ABSENT 0x80000000u /* the page is not in the pool: nothing was written */
 #define KC_ODD 0x40000000u    /* a value that is not finite was taken out */
+#define KC_WIDE 0x20000000u   /* by its values */
 
 /* Where a workgroup's run of the list begins: sequence, key head, row block, tile; how many tiles it has (0: none), and
  * how many the runs have that a group goes on in. */
@@ -267,6 +277,7 @@ union KcFrag {
     glint_u32x4 v;
     kc_f16x8 f;
 };
+__device__ __forceinline__ uint32_t kc_uniform(uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
 __device__ __forceinline__ uint32_t kc_f16pair(float lo, float hi) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(glint_f32x2{lo, hi}, kc_f16x2));
 }
@@ -285,6 +296,13 @@ __device__ __forceinline__ int ku_exponent(float top, int step) {
     return (e + step - 1) & -step;
 }
 
+/* The values' power of a tile, of which `top` is the largest, as KcMeta holds it; low: some token's lie below KC_SPAN of it. */
+__device__ __forceinline__ uint32_t ku_values(float top, bool low, int &e) {
+    const int at = ku_exponent(top, 8);
+    e = max(at, -KC_BAND); /* also of a tile of zeros */
+    return (uint32_t)(e + KC_EXP) | (low || (top > 0.f && (at < -KC_BAND || at > KC_BAND)) ? KC_WIDE : 0u);
+}
+
 /* The last workgroup lays out the attention's work; the others take tiles in turn. */
 template <int D, bool OWN>
 __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
@@ -292,7 +310,7 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
     __shared__ float parents[16 * 64]; /* a copy for every lane's bank */
     __shared__ __attribute__((aligned(16))) uint16_t rows[OWN ? AP_KEYS : 1][D + 2]; /* own values, to be turned */
     __shared__ float tops[2][KU_T / 64];
-    __shared__ uint32_t odds;
+    __shared__ uint32_t odds; /* KC_ODD, KC_WIDE of own values */
     __shared__ KcPlan plan;
     __shared__ int counts[KC_PAIRS + 1];
     if (blockIdx.x + 1 == gridDim.x) {
@@ -367,9 +385,16 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
                 vtop = fabsf(vl[x]) <= FLT_MAX ? fmaxf(vtop, fabsf(vl[x])) : vtop;
                 odd |= !(fabsf(vl[x]) <= FLT_MAX);
             }
-            const int ke = ku_exponent(glint_wave_max(mine ? ktop : 0.f), 1), ve = ku_exponent(glint_wave_max(mine ? vtop : 0.f), 8);
+            const float vmost = glint_wave_max(mine ? vtop : 0.f);
+            bool below = false;
+#pragma unroll
+            for (int x = 0; x < NB; ++x)
+                below |= vl[x] != 0.f && fabsf(vl[x]) < vmost * KC_SPAN;
+            int ve;
+            const int ke = ku_exponent(glint_wave_max(mine ? ktop : 0.f), 1);
+            const uint32_t vexp = ku_values(vmost, __any(mine && below), ve);
             const float kdown = ldexpf(1.f, 14 - ke), vdown = ldexpf(1.f, 14 - ve);
-            meta = KcMeta{ldexpf(1.f, ke - 14), (uint32_t)(ve + KC_EXP) | (__any(mine && odd) ? KC_ODD : 0u)};
+            meta = KcMeta{ldexpf(1.f, ke - 14), vexp | (__any(mine && odd) ? KC_ODD : 0u)};
             if (threadIdx.x == 0)
                 A.meta[slot] = meta;
             auto parent = [&](uint32_t word, int nibble) { return parents[(word >> (4 * nibble) & 15u) * 64 + lane]; };
@@ -416,7 +441,8 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
             const int key = s.own + f * AP_KEYS;
             const int64_t row0 = (int64_t)s.q0 + s.nq - s.len + key;
             constexpr int PER = AP_KEYS * CH / KU_T; /* 16-B chunks of a thread */
-            int e[2];
+            int ke = 0, ve = 0;
+            uint32_t vexp = 0;
             if (threadIdx.x == 0)
                 odds = 0;
 #pragma unroll 1
@@ -424,11 +450,12 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
                 const uint16_t *from = is_v ? A.v + row0 * A.v_st + h * A.v_sh : A.k + row0 * A.k_st + h * A.k_sh;
                 const int64_t st = is_v ? A.v_st : A.k_st;
                 glint_u32x4 in[PER];
-                float top = 0.f;
+                float top = 0.f, least = INFINITY; /* least: the smallest of the rows' 64-blocks' largest, but for zeros */
                 bool odd = false;
 #pragma unroll
                 for (int x = 0; x < PER; ++x) {
                     const int r = (threadIdx.x + x * KU_T) / CH, c = (threadIdx.x + x * KU_T) % CH;
+                    float block = 0.f;
                     in[x] = glint_u32x4{0, 0, 0, 0};
                     if (key + r < s.len && seen(key + r))
                         in[x] = *(const glint_u32x4 *)(from + r * st + 8 * c);
@@ -438,24 +465,34 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
                         for (int k = 0; k < 2; ++k) {
                             const float a = fabsf(k ? glint_bf16hi(in[x][j]) : glint_bf16lo(in[x][j]));
                             if (a <= FLT_MAX) {
-                                top = fmaxf(top, a);
+                                block = fmaxf(block, a);
                             } else if (is_v) { /* a key's stays: what sees it is NaN */
                                 odd = true;
                                 in[x][j] &= k ? 0xFFFFu : 0xFFFF0000u;
                             }
                         }
+                    top = fmaxf(top, block);
+                    block = kv4_max_dpp<GLINT_DPP_QUAD_1032>(block); /* of 8 lanes, a row's 64 dimensions */
+                    block = kv4_max_dpp<GLINT_DPP_QUAD_2301>(block);
+                    block = kv4_max_dpp<GLINT_DPP_ROW_HALF_MIRROR>(block);
+                    least = block > 0.f ? fminf(least, block) : least;
                 }
                 top = glint_wave_max(top);
                 if (lane == 0)
                     tops[is_v][wave] = top;
                 __syncthreads(); /* also: the tile before has been turned */
-                if (odd)
-                    odds = 1;
 #pragma unroll
                 for (int x = 0; x < KU_T / 64; ++x)
                     top = fmaxf(top, tops[is_v][x]);
-                e[is_v] = ku_exponent(top, is_v ? 8 : 1);
-                const float down = ldexpf(1.f, 14 - e[is_v]);
+                if (odd)
+                    atomicOr(&odds, KC_ODD);
+                if (is_v && least < top * KC_SPAN)
+                    atomicOr(&odds, KC_WIDE);
+                if (is_v)
+                    vexp = ku_values(top, false, ve);
+                else
+                    ke = ku_exponent(top, 1);
+                const float down = ldexpf(1.f, 14 - (is_v ? ve : ke));
 #pragma unroll
                 for (int x = 0; x < PER; ++x) {
                     const int r = (threadIdx.x + x * KU_T) / CH, c = (threadIdx.x + x * KU_T) % CH;
@@ -474,7 +511,7 @@ __global__ __launch_bounds__(KU_T, 4) void k_kv4_unpack(KcArgs A, int grid) {
             }
             __syncthreads();
             if (threadIdx.x == 0)
-                A.meta[slot] = KcMeta{ldexpf(1.f, e[0] - 14), (uint32_t)(e[1] + KC_EXP) | (odds ? KC_ODD : 0u)};
+                A.meta[slot] = KcMeta{ldexpf(1.f, ke - 14), vexp | odds};
 #pragma unroll
             for (int x = 0; x < PER; ++x) {
                 const int d = (threadIdx.x + x * KU_T) / 8, c = (threadIdx.x + x * KU_T) % 8;
@@ -574,20 +611,273 @@ __device__ __forceinline__ float kc_outputs(const ap_lds *vl, ApRows<D> &w, cons
     return top;
 }
 
+/* What a wave has to know of its 32 rows: this lane's, whether it and whether any is there; what their first and their last
+ * one see up to, and this lane's. Rows before the sequence's first position see nothing, as one at -1 does; less any window
+ * is an int then. */
+struct KcWave {
+    int row;
+    bool live, any;
+    int low, high, last;
+};
+__device__ __forceinline__ KcWave kc_wave(const KcArgs &a, const KcSeq &s, int rb, int wave, int col) {
+    const int first = rb * KC_ROWS + 32 * wave, row = first + col, gap = s.len - s.nq;
+    return KcWave{row, row < s.rows, first < s.rows, max(-1, gap + first / a.G), max(-1, gap + min(s.rows - 1, first + 31) / a.G),
+                  row < s.rows ? max(-1, gap + row / a.G) : -1};
+}
+/* The place of step i's tile: pages, then own keys. */
+__device__ __forceinline__ int kc_place(const KcArgs &a, const KcTiles &t, int i) {
+    return i < t.np ? (i < t.psinks ? i : i + t.pskip) : a.max_pages + (i - t.np < t.fsinks ? i - t.np : i - t.np + t.fskip);
+}
+/* What a step has to know of its tile. */
+struct KcStep {
+    int key, ends; /* its first position, and the last one that it may show */
+    bool want;     /* whether the wave has scores to form */
+    KcMeta meta;
+};
+__device__ __forceinline__ KcStep kc_look(const KcArgs &a, const KcSeq &s, const KcTiles &t, const KcWave &w, int64_t slot0, int i) {
+    KcStep x;
+    const int to = kc_place(a, t, i);
+    const bool own = i >= t.np;
+    x.key = own ? s.own + (to - a.max_pages) * AP_KEYS : to * AP_KEYS;
+    x.ends = own ? INT32_MAX : s.held - 1;
+    x.meta = a.meta[slot0 + to];
+    x.want = w.any && x.key <= min(w.high, x.ends) && (x.key + AP_KEYS - 1 > w.low - a.bound.window || x.key < a.bound.sinks);
+    return x;
+}
+/* A row of q, its sign the scale's: the power of two that brings it to 2^14 .. 2^15 is 2^-(what is returned). */
 template <int D>
-__global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
+__device__ __forceinline__ int kc_load_q(const KcArgs &a, const uint16_t *qr, ApFrag (&q)[D / 16], int half) {
+    uint32_t high = 0;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
+        q[x].v = *(const glint_u32x4 *)(qr + 16 * x + 8 * half);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q[x].u[i] ^= a.q_sign;
+            high = max(high, max((q[x].u[i] & 0x7FFFu) << 16, q[x].u[i] & 0x7FFF0000u));
+        }
+    }
+    high = __float_as_uint(glint_xor32(__uint_as_float(min(high, 0x7F800000u)), GlintMax()));
+    return high >= 0x7F800000u ? 0 : (int)(high >> 23) - 127 - 14;
+}
+/* What scores of a tile are multiplied by, `factor` being the row's part. */
+__device__ __forceinline__ float kc_factor(float factor, const KcMeta &meta) { return fminf(fmaxf(factor * meta.kback, FLT_MIN), FLT_MAX); }
+/* The largest kback, in bits (of two floats above 0 the larger has the larger), that leaves the wave's factors below KC_KEYS. */
+__device__ __forceinline__ uint32_t kc_keys(float factor) { return kc_uniform(__float_as_uint(KC_KEYS / glint_wave_max(factor))); }
+__device__ __forceinline__ bool kc_wide(const KcMeta &meta, uint32_t keys) {
+    return !(meta.vexp & KC_ABSENT) && ((meta.vexp & KC_WIDE) || __float_as_uint(meta.kback) > keys);
+}
+
+/* A wide tile, from where it came: every operand as two of bf16, which has f32's range, one the other's rest: 2^-16 of each
+ * element is left out. Rows `from` on of own keys and values, or the page and head of that place; the first is position `at`, and
+ * past element `there` nothing is read of own ones. f is the scores' factor, keys are multiplied by kdown, q holds bf16. */
+template <int D>
+__device__ __forceinline__ void kc_wide_tile(const KcArgs &A, ApRows<D> &w, int h, bool own, int64_t from, int at,
+                                             int last, int upto, int there, float f, float kdown, int half) {
+    const int lane = threadIdx.x & 63, col = lane & 31;
+    const float my_parent = kKv4Parent[lane & 15];
+    auto parent = [&](uint32_t code) { return __shfl(my_parent, (int)(code & 15u), 64); };
+    auto split = [](const float (&x)[8], ApFrag &hi, ApFrag &lo) { /* hi is cut off, so that it stays finite */
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t a = __float_as_uint(x[2 * j]), b = __float_as_uint(x[2 * j + 1]);
+            hi.u[j] = (a >> 16) | (b & 0xFFFF0000u);
+            lo.u[j] = glint_cvt_bf16x2(x[2 * j] - __uint_as_float(a & 0xFFFF0000u), x[2 * j + 1] - __uint_as_float(b & 0xFFFF0000u));
+        }
+    };
+    ap_f32x16 sc[2];
+    float x[8];
+    ApFrag hi, lo;
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+        const int r = 32 * a + col;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            sc[a][i] = 0.f;
+#pragma unroll
+        for (int n = 0; n < D / 16; ++n) { /* dimensions 16 n + 8 half .. of key r */
+            if (own) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = 0.f;
+                if (r <= there)
+                    kt_load8<D>(A.k + (from + r) * A.k_st + h * A.k_sh + 16 * n + 8 * half, x);
+            } else {
+                const uint32_t c = *(const uint32_t *)(A.k_hole + (from * KV4_PAGE + r) * (D / 2) + kv4_k_byte<D / 64>(16 * n + 8 * half));
+                const float sk = A.k_absmax[(from * (D / 64) + (n >> 2)) * KV4_PAGE + r];
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    x[e] = parent(c >> (4 * e)) * sk;
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] *= kdown;
+            split(x, hi, lo);
+            sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi.f, w.q[n].f, sc[a], 0, 0, 0);
+            sc[a] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo.f, w.q[n].f, sc[a], 0, 0, 0);
+        }
+    }
+    float top = -INFINITY;
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int key = at + 32 * a + 8 * (i >> 2) + 4 * half + (i & 3);
+            sc[a][i] = key <= upto && A.bound.sees(key, last) ? sc[a][i] * f : -INFINITY;
+            top = fmaxf(top, sc[a][i]);
+        }
+    top = glint_xor32(top, GlintMax());
+    if (top > w.m + AP_SLACK) {
+        const float keep = __builtin_amdgcn_exp2f(w.m - top);
+        w.m = top;
+        w.l *= keep;
+#pragma unroll
+        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                w.o[d][i] *= keep;
+    }
+    /* not a fused product: a score far from 0 then lies as far above the maximum as that says */
+    const float base = w.m == -INFINITY ? 0.f : w.m - KC_UP;
+    ApFrag ph[4], pl[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            x[e] = __builtin_amdgcn_exp2f(sc[n >> 1][8 * (n & 1) + e] - base);
+            w.l += x[e];
+        }
+        split(x, ph[n], pl[n]);
+    }
+#pragma unroll
+    for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+        for (int n = 0; n < 4; ++n) { /* keys 16 n + 4 half + 0..3, and 8 on, of dimension 32 d + col */
+            const int r = 16 * n + 4 * half;
+            if (own) {
+                const uint16_t *v = A.v + (from + r) * A.v_st + h * A.v_sh + 32 * d + col;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int k = (e & 3) + 2 * (e & 4);
+                    x[e] = r + k <= there ? __uint_as_float((uint32_t)v[k * A.v_st] << 16) : 0.f;
+                }
+            } else {
+                const uint8_t *v = A.v_hole + (from * (D / 2) + 16 * d + (col & 15)) * KV4_PAGE + r;
+                const float *sv = A.v_absmax + (from * (D / 64) + (d >> 1)) * KV4_PAGE + r;
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const uint32_t c = *(const uint32_t *)(v + 8 * y) >> (col & 16 ? 4 : 0);
+                    const glint_f32x4 scale = *(const glint_f32x4 *)(sv + 8 * y);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        x[4 * y + e] = parent(c >> (8 * e)) * scale[e];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                x[e] = fabsf(x[e]) <= FLT_MAX ? x[e] : 0.f;
+            split(x, hi, lo);
+            w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi.f, ph[n].f, w.o[d], 0, 0, 0);
+            w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(hi.f, pl[n].f, w.o[d], 0, 0, 0);
+            w.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(lo.f, ph[n].f, w.o[d], 0, 0, 0);
+        }
+}
+
+/* What the steps at .. end - 1 of a row block leave out. */
+template <int D>
+__device__ __forceinline__ void kc_rare(const KcArgs &A, ApRows<D> &w, const KcSeq &s, const KcTiles &tiles, const KcWave &W, int b, int h,
+                                        int at, int end, bool wide, bool apart, int lane) {
+    const int half = lane >> 5;
+    if (wide) {
+        const int64_t slot0 = kc_slot(A, b, h, 0);
+        ApFrag (&q)[D / 16] = w.q;
+        const int row = W.live ? W.row : 0;
+        const int ex = kc_load_q<D>(A, A.q + (int64_t)(s.q0 + row / A.G) * A.q_st + ((A.h0 + h) * A.G + row % A.G) * A.q_sh, q, half);
+#pragma unroll
+        for (int x = 0; x < D / 16; ++x)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                q[x].u[i] = glint_cvt_bf16x2(ldexpf(glint_bf16lo(q[x].u[i]), -ex), ldexpf(glint_bf16hi(q[x].u[i]), -ex));
+        const float factor = ldexpf(A.scale2, ex);
+        const uint32_t keys = kc_keys(factor);
+#pragma unroll 1
+        for (int i = at; i < end; ++i) {
+            const KcStep T = kc_look(A, s, tiles, W, slot0, i);
+            if (!T.want || !kc_wide(T.meta, keys))
+                continue;
+            int64_t from = (int64_t)s.q0 + s.nq - s.len + T.key; /* row of the first own key, or place of the page and head */
+            if (i < tiles.np)
+                from = (int64_t)A.table[(int64_t)b * A.table_stride + T.key / KV4_PAGE] * A.H + A.h0 + h;
+            kc_wide_tile<D>(A, w, A.h0 + h, i >= tiles.np, from, T.key, W.last, min(W.last, T.ends), min(W.high - T.key, AP_KEYS - 1),
+                            kc_factor(factor, T.meta), 1.f / T.meta.kback, half);
+        }
+    }
+    /* A value that is not finite leaves itself or NaN in its dimension of the rows that see it, whatever its
+     * weight. */
+    if (apart) {
+#pragma unroll 1
+        for (int d = 0; d < D / 32; ++d) {
+            ap_f32x16 odd;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                odd[i] = 0.f;
+            for (int i = at; i < min(end, tiles.np); ++i) {
+                const int page = i < tiles.psinks ? i : i + tiles.pskip;
+                const int pid = A.table[(int64_t)b * A.table_stride + page];
+                if (pid < 0 || pid >= A.pages)
+                    continue;
+                const int64_t ph = (int64_t)pid * A.H + A.h0 + h;
+                const float sv = A.v_absmax[ph * (D / 64 * KV4_PAGE) + (d >> 1) * KV4_PAGE + lane];
+                uint64_t hit = __ballot(!(fabsf(sv) <= FLT_MAX) && page * KV4_PAGE + lane < s.held);
+                for (; hit; hit &= hit - 1) {
+                    const int j = __builtin_ctzll(hit), key = page * KV4_PAGE + j;
+                    const float sj = __shfl(sv, j, 64);
+                    if (!A.bound.sees(key, W.last))
+                        continue;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const int dim = 32 * d + 8 * (x >> 2) + 4 * half + (x & 3);
+                        const uint32_t c = A.v_hole[ph * (KV4_PAGE * D / 2) + kv4_v_row(dim) * KV4_PAGE + j];
+                        odd[x] += kKv4Parent[c >> (dim & 16 ? 4 : 0) & 15] * sj;
+                    }
+                }
+            }
+            for (int i = max(at, tiles.np); i < end; ++i) {
+                const int f = i - tiles.np < tiles.fsinks ? i - tiles.np : i - tiles.np + tiles.fskip;
+                const int first = s.own + f * AP_KEYS;
+                for (int key = first; key < min(first + AP_KEYS, min(W.high + 1, s.len)); ++key) {
+                    const uint16_t *from = A.v + ((int64_t)s.q0 + s.nq - s.len + key) * A.v_st + (A.h0 + h) * A.v_sh + 32 * d + 4 * half;
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) {
+                        const uint32_t v = from[8 * (x >> 2) + (x & 3)];
+                        if ((v & 0x7F80u) == 0x7F80u && A.bound.sees(key, W.last))
+                            odd[x] += __uint_as_float(v << 16);
+                    }
+                }
+            }
+#pragma unroll
+            for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+                for (int x = 0; x < 16; ++x)
+                    w.o[k][x] = k != d || odd[x] == 0.f ? w.o[k][x] : odd[x];
+        }
+    }
+}
+
+/* A workgroup's run. Returns whether the wave left something out: wide tiles and values that are not finite, which a pass that
+ * is RARE takes at the end of each row block (kc_rare). */
+template <int D, bool RARE>
+__device__ __forceinline__ bool kc_pass(const KcArgs &A, int me, char (&k0t)[AP_KEYS * D * 2], char (&k1t)[AP_KEYS * D * 2],
+                                        char (&v0t)[AP_KEYS * D * 2], char (&v1t)[AP_KEYS * D * 2]) {
     constexpr int TILE = AP_KEYS * D * 2, LOADS = TILE / (16 * KC_T);
-    /* arrays of their own, so that reads of one do not wait for loads into the other */
-    __shared__ __attribute__((aligned(16))) char k0t[TILE], k1t[TILE], v0t[TILE], v1t[TILE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int col = lane & 31, half = lane >> 5;
-    /* neighbours in the list share keys: they go to one XCD, a workgroup's being its index modulo 8 */
-    const int grid = gridDim.x, me = grid & 7 ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (grid >> 3) + ((int)blockIdx.x >> 3);
+    bool rare = false;
     int left = A.starts[me].left; /* of this workgroup's run */
     if (left == 0) {
         if (threadIdx.x == 0)
             A.joins[me].w_last = 0;
-        return;
+        return false;
     }
     int b = A.starts[me].b, h = A.starts[me].h, rb = A.starts[me].rb, at = A.starts[me].at;
 
@@ -605,15 +895,12 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
         const KcTiles tiles = kc_tiles(A, s, rb, 1);
         const int n = tiles.np + tiles.nf, cost = max(1, n);
         const int take = min(left, cost - at), end = min(at + take, n); /* tiles at .. end - 1 */
-        const int row = rb * KC_ROWS + 32 * wave + col, head = (A.h0 + h) * A.G;
-        const bool live = row < s.rows, wave_live = rb * KC_ROWS + 32 * wave < s.rows;
-        const int gap = s.len - s.nq;
-        /* rows before the sequence's first position see nothing, as one at -1 does; less any window is an int then */
-        const int wave_low = max(-1, gap + (rb * KC_ROWS + 32 * wave) / A.G);
-        const int wave_high = max(-1, gap + min(s.rows - 1, rb * KC_ROWS + 32 * wave + 31) / A.G);
+        const KcWave W = kc_wave(A, s, rb, wave, col);
+        const int row = W.row, head = (A.h0 + h) * A.G, wave_low = W.low, wave_high = W.high;
+        const bool live = W.live, wave_live = W.any;
         w.m = -INFINITY;
         w.l = 0.f;
-        w.last = live ? max(-1, gap + row / A.G) : -1;
+        w.last = W.last;
 #pragma unroll
         for (int d = 0; d < D / 32; ++d)
 #pragma unroll
@@ -621,17 +908,12 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                 w.o[d][i] = 0.f;
         bool apart = false;
         int oexp = -4096; /* the outputs are 2^(14 - oexp) times themselves: the last tile's power */
-        int most = -4096; /* of the tiles so far; oexp stays within KC_LIFT of it, so that outputs stay finite */
+        bool wide = false; /* there are wide tiles among those that the wave sees */
         if (at < end) {
-            /* the place of tile i: pages, then own keys; its first position and, of what it holds, the end */
-            auto place = [&](int i) {
-                return i < tiles.np ? (i < tiles.psinks ? i : i + tiles.pskip)
-                                    : A.max_pages + (i - tiles.np < tiles.fsinks ? i - tiles.np : i - tiles.np + tiles.fskip);
-            };
             const int64_t slot0 = kc_slot(A, b, h, 0);
             const uint32_t my = threadIdx.x * 16;
             auto tile_of = [&](int i) {
-                return __builtin_amdgcn_make_buffer_rsrc((void *)(A.tiles + (slot0 + place(i)) * (2 * TILE)), (short)0, 2 * TILE,
+                return __builtin_amdgcn_make_buffer_rsrc((void *)(A.tiles + (slot0 + kc_place(A, tiles, i)) * (2 * TILE)), (short)0, 2 * TILE,
                                                          GLINT_BUF_DWORD3);
             };
             auto fetch_k = [&](int i, ap_lds *kt) {
@@ -646,39 +928,15 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                 for (int x = 0; x < LOADS; ++x)
                     ap_dma(r, vt + (x * KC_T + wave * 64) * 16, my, TILE + x * (KC_T * 16));
             };
-            /* what a step has to know of its tile */
-            struct {
-                int key, ends; /* its first position, and the last one that it may show */
-                bool want;     /* whether the wave has scores to form */
-                KcMeta meta;
-            } T, N;
-            auto look = [&](int i, auto &X) {
-                const int to = place(i);
-                const bool own = i >= tiles.np;
-                X.key = own ? s.own + (to - A.max_pages) * AP_KEYS : to * AP_KEYS;
-                X.ends = own ? INT32_MAX : s.held - 1;
-                X.meta = A.meta[slot0 + to];
-                X.want = wave_live && X.key <= min(wave_high, X.ends) &&
-                         (X.key + AP_KEYS - 1 > wave_low - A.bound.window || X.key < A.bound.sinks);
-            };
+            KcStep T, N;
+            auto look = [&](int i, KcStep &X) { X = kc_look(A, s, tiles, W, slot0, i); };
             ap_lds *const ka = (ap_lds *)(at & 1 ? k1t : k0t);
             __syncthreads(); /* the last group's tiles are read */
             fetch_k(at, ka);
             look(at, T);
             /* q as f16, scaled to 2^14 .. 2^15 by a power of two of the row's */
             const uint16_t *qr = A.q + (int64_t)(s.q0 + (live ? row / A.G : 0)) * A.q_st + (head + (live ? row % A.G : 0)) * A.q_sh;
-            uint32_t high = 0;
-#pragma unroll
-            for (int x = 0; x < D / 16; ++x) {
-                w.q[x].v = *(const glint_u32x4 *)(qr + 16 * x + 8 * half);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    w.q[x].u[i] ^= A.q_sign;
-                    high = max(high, max((w.q[x].u[i] & 0x7FFFu) << 16, w.q[x].u[i] & 0x7FFF0000u));
-                }
-            }
-            high = __float_as_uint(glint_xor32(__uint_as_float(min(high, 0x7F800000u)), GlintMax()));
-            const int ex = high >= 0x7F800000u ? 0 : (int)(high >> 23) - 127 - 14;
+            const int ex = kc_load_q<D>(A, qr, w.q, half);
 #pragma unroll
             for (int x = 0; x < D / 16; ++x)
 #pragma unroll
@@ -691,9 +949,15 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
             ap_f32x16 sa[2], sb[2];
             KcFrag pf[4];
             float top = -INFINITY, l = 0.f;
+            const uint32_t keys = kc_keys(factor);
+            auto decide = [&](KcStep &X) { /* whether the wave takes the tile into its products */
+                const bool fits = !(X.meta.vexp & (KC_ABSENT | KC_WIDE)) && __float_as_uint(X.meta.kback) <= keys;
+                wide |= X.want && !fits;
+                X.want = X.want && fits;
+            };
             __builtin_amdgcn_s_waitcnt(GLINT_WAIT_VMCNT0);
             __syncthreads();
-            T.want = T.want && !(T.meta.vexp & KC_ABSENT);
+            decide(T);
             if (at + 1 < end)
                 fetch_k(at + 1, (ap_lds *)(at & 1 ? k0t : k1t));
             fetch_v(at, (ap_lds *)(at & 1 ? v1t : v0t));
@@ -722,10 +986,11 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                     fetch_k(i + 2, knn); /* over tile i's, which every wave has left */
                 if (more)
                     fetch_v(i + 1, vn);
-                N.want = more && N.want && !(N.meta.vexp & KC_ABSENT);
+                N.want = more && N.want;
+                decide(N);
                 apart |= (T.meta.vexp & (KC_ODD | KC_ABSENT)) == KC_ODD;
                 if (T.want) {
-                    const float f = fminf(fmaxf(factor * T.meta.kback, FLT_MIN), FLT_MAX);
+                    const float f = kc_factor(factor, T.meta);
                     if (T.key + AP_KEYS - 1 > min(wave_low, T.ends) ||
                         !(T.key > wave_high - A.bound.window || T.key + AP_KEYS <= A.bound.sinks)) { /* what a row does not see */
                         const int from = T.key + 4 * half, upto = min(w.last, T.ends);
@@ -742,32 +1007,30 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                     const bool up = top > w.m + AP_SLACK; /* a row's own test: its bits depend on no other row */
                     const int ve = (int)(T.meta.vexp & 0xFFFFu) - KC_EXP;
                     /* The outputs go to the tile's power, up or down, and not the weights, whose f16 has no bits to spare:
-                     * at 2^-17 of the largest value met, weights times 2^-24 lost half of themselves. */
-                    most = max(most, ve);
-                    const int to = max(ve, most - KC_LIFT);
-                    if (__any(up) || to != oexp) {
+                     * at 2^-17 of the largest value met, weights times 2^-24 lost half of themselves. They do once the weights are
+                     * formed: without this branch between them and the products the compiler copies the weights, 2048 tokens over
+                     * 16384 559 us so, 592 with it before the weights. */
+                    const bool other = __any(up) || ve != oexp;
+                    float keep = 1.f;
+                    if (other) {
                         const float mn = up ? top : w.m;
-                        float keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
+                        keep = __builtin_amdgcn_exp2f(w.m - (mn == -INFINITY ? 0.f : mn));
                         w.m = mn;
                         l *= keep;
-                        keep *= ldexpf(1.f, max(oexp - to, -300));
-                        oexp = to;
-#pragma unroll
-                        for (int d = 0; d < D / 32; ++d)
-#pragma unroll
-                            for (int x = 0; x < 16; ++x)
-                                w.o[d][x] *= keep;
+                        keep *= ldexpf(1.f, max(oexp - ve, -300));
+                        oexp = ve;
                     }
                     const float base = w.m == -INFINITY ? 0.f : w.m - KC_UP;
                     if (N.want)
                         kc_scores<D, true, true>(kn, w, next, sc, f, base, pf, l);
                     else
                         kc_scores<D, false, true>(kn, w, next, sc, f, base, pf, l);
-                    if (ve < oexp) {
-                        const _Float16 less = (_Float16)ldexpf(1.f, max(ve - oexp, -30));
+                    if (other) {
 #pragma unroll
-                        for (int x = 0; x < 4; ++x)
-                            pf[x].f *= less;
+                        for (int d = 0; d < D / 32; ++d)
+#pragma unroll
+                            for (int x = 0; x < 16; ++x)
+                                w.o[d][x] *= keep;
                     }
                     top = kc_outputs<D>(vt, w, vat, pf, next);
                 } else if (N.want) {
@@ -799,55 +1062,11 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                     w.o[d][x] *= back;
         }
 
-        /* A value that is not finite leaves itself or NaN in its dimension of the rows that see it, whatever its
-         * weight. */
-        if (apart) {
-#pragma unroll 1
-            for (int d = 0; d < D / 32; ++d) {
-                ap_f32x16 odd;
-#pragma unroll
-                for (int i = 0; i < 16; ++i)
-                    odd[i] = 0.f;
-                for (int i = at; i < min(end, tiles.np); ++i) {
-                    const int page = i < tiles.psinks ? i : i + tiles.pskip;
-                    const int pid = A.table[(int64_t)b * A.table_stride + page];
-                    if (pid < 0 || pid >= A.pages)
-                        continue;
-                    const int64_t ph = (int64_t)pid * A.H + A.h0 + h;
-                    const float sv = A.v_absmax[ph * (D / 64 * KV4_PAGE) + (d >> 1) * KV4_PAGE + lane];
-                    uint64_t hit = __ballot(!(fabsf(sv) <= FLT_MAX) && page * KV4_PAGE + lane < s.held);
-                    for (; hit; hit &= hit - 1) {
-                        const int j = __builtin_ctzll(hit), key = page * KV4_PAGE + j;
-                        const float sj = __shfl(sv, j, 64);
-                        if (!A.bound.sees(key, w.last))
-                            continue;
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            const int dim = 32 * d + 8 * (x >> 2) + 4 * half + (x & 3);
-                            const uint32_t c = A.v_hole[ph * (KV4_PAGE * D / 2) + kv4_v_row(dim) * KV4_PAGE + j];
-                            odd[x] += kKv4Parent[c >> (dim & 16 ? 4 : 0) & 15] * sj;
-                        }
-                    }
-                }
-                for (int i = max(at, tiles.np); i < end; ++i) {
-                    const int f = i - tiles.np < tiles.fsinks ? i - tiles.np : i - tiles.np + tiles.fskip;
-                    const int first = s.own + f * AP_KEYS;
-                    for (int key = first; key < min(first + AP_KEYS, min(wave_high + 1, s.len)); ++key) {
-                        const uint16_t *from = A.v + ((int64_t)s.q0 + s.nq - s.len + key) * A.v_st + (A.h0 + h) * A.v_sh + 32 * d + 4 * half;
-#pragma unroll
-                        for (int x = 0; x < 16; ++x) {
-                            const uint32_t v = from[8 * (x >> 2) + (x & 3)];
-                            if ((v & 0x7F80u) == 0x7F80u && A.bound.sees(key, w.last))
-                                odd[x] += __uint_as_float(v << 16);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-                    for (int x = 0; x < 16; ++x)
-                        w.o[k][x] = k != d || odd[x] == 0.f ? w.o[k][x] : odd[x];
-            }
+        if (wide || apart) {
+            if constexpr (RARE)
+                kc_rare<D>(A, w, s, tiles, W, b, h, at, end, wide, apart, lane);
+            else
+                rare = true;
         }
         const float l = glint_xor32(w.l, GlintAdd());
         if (take == cost) {
@@ -889,6 +1108,32 @@ __global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
                 break;
             rb = A.nblk - 1; /* no further block of this head has */
         }
+    }
+    return rare;
+}
+
+template <int D>
+__global__ __launch_bounds__(KC_T, 2) void k_kv4_chunk(KcArgs A) {
+    constexpr int TILE = AP_KEYS * D * 2;
+    /* arrays of their own, so that reads of one do not wait for loads into the other */
+    __shared__ __attribute__((aligned(16))) char k0t[TILE], k1t[TILE], v0t[TILE], v1t[TILE];
+    __shared__ int left_out;
+    /* neighbours in the list share keys: they go to one XCD, a workgroup's being its index modulo 8 */
+    const int grid = gridDim.x, me = grid & 7 ? (int)blockIdx.x : ((int)blockIdx.x & 7) * (grid >> 3) + ((int)blockIdx.x >> 3);
+    if (threadIdx.x == 0)
+        left_out = 0;
+    __syncthreads();
+    if (kc_pass<D, false>(A, me, k0t, k1t, v0t, v1t))
+        left_out = 1;
+    __syncthreads();
+    /* A run that left something out is gone through once more. What is rare has registers of its own so: at the end of each row
+     * block it cost the loop 2048 tokens over 16384 561 us where this takes 532, as a launch of its own 549. The arguments are
+     * read again for the same reason. */
+    if (left_out) {
+        typedef const __attribute__((address_space(4))) KcArgs KernArgs;
+        KernArgs *again = (KernArgs *)__builtin_amdgcn_kernarg_segment_ptr();
+        asm volatile("" : "+s"(again));
+        kc_pass<D, true>(*(const KcArgs *)again, me, k0t, k1t, v0t, v1t);
     }
 }
 

@@ -68,7 +68,8 @@ class Chunk:
         q = values(self.q)
         for h in range(HEADS * G):
             z = R.attend(q[rows, h], k[:, h // G], v[:, h // G], ok[rows], self.D ** -0.5)
-            worst = R.far(self.got[rows, h], *z, bound(self.own))
+            with np.errstate(over="ignore"):  # a key past every bound of f32 scores: finite is all that is asked
+                worst = R.far(self.got[rows, h], *z, bound(self.own))
             assert worst <= 0, (h, worst)
 
 
@@ -90,3 +91,72 @@ def test_a_large_value_that_weighs_nothing(power, D, own):
         c.key(100, 0.7)
         c.run()
         c.check(range(j, j + 64))
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [14, 27, 36, 100])
+def test_a_later_token_takes_nothing_from_earlier_rows(power, D, own):
+    """A key or value of 2^power times the others' in the middle of the chunk: rows before it do not see it, however near
+    their own tokens lie to it. Rows from it on hold what it gives them."""
+    torch_cuda()
+    for n, nq in ((300, 100), (3000, 100)):
+        for which in (0, 1):
+            print(f"power={power} D={D} own={own} n={n} which={which}", flush=True)
+            c = Chunk(n, nq, D, own, power + D + which)
+            j = n - nq + 37
+            c.times(which, j, 2.0 ** power)
+            c.key(100, 0.7)
+            c.run()
+            c.check(rows=slice(0, 37))
+            c.check(rows=slice(37, nq))
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("power", [14, 26, 100])
+def test_one_large_value_beside_others(power, D, own):
+    """As above for a value that every row sees and that weighs nothing: the tokens of its own tile keep theirs. A power of 100
+    also leaves the tiles behind it more than f32 could carry an output up by."""
+    torch_cuda()
+    for n, nq, window, sinks in ((500, 70, 0, 0), (3000, 150, 0, 0), (900, 200, 400, 70)):
+        print(f"power={power} D={D} own={own} n={n} window={window}", flush=True)
+        c = Chunk(n, nq, D, own, power + n)
+        j = n - nq if own else 20 if sinks else 0
+        c.key(j, -30.0)
+        c.times(1, j, 2.0 ** power)
+        c.key(50, 0.7)
+        c.run(window, sinks)
+        c.check([j], window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("own", [False, True])
+def test_blocks_of_unlike_size(own):
+    """128 dimensions whose first 64 are 2^40 times the others', where the queries hold nothing there; values likewise."""
+    torch_cuda()
+    c = Chunk(400, 90, 128, own, 3)
+    c.q[..., :64] = 0
+    c.planes[1][:, :, 0] *= np.float32(2.0 ** 40)
+    c.planes[3][:, :, 1] *= np.float32(2.0 ** -40)
+    c.k[..., :64] *= np.float32(2.0 ** 40)
+    c.v[..., 64:] *= np.float32(2.0 ** -40)
+    c.run()
+    c.check()
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("power", [-60, -34, 30, 41, 90])
+def test_values_far_from_one(power, own):
+    """All values 2^power, but for a tile of zeros and one of ordinary size with no weight."""
+    torch_cuda()
+    for D, n, nq in ((64, 500, 100), (128, 3000, 40)):
+        c = Chunk(n, nq, D, own, 1000 + power)
+        c.planes[3] *= np.float32(2.0 ** power)
+        c.v *= np.float32(2.0 ** power)
+        for j in range(64, 128):
+            c.planes[3][c.place(j)] = 0
+        for j in range(192, 256):
+            c.times(1, j, 2.0 ** -power)
+            c.key(j, -30.0)
+        c.run()
+        c.check(range(192, 256))
