@@ -727,7 +727,7 @@ __device__ __forceinline__ void kc_wide_tile(const KcArgs &A, ApRows<D> &w, int 
             top = fmaxf(top, sc[a][i]);
         }
     top = glint_xor32(top, GlintMax());
-    if (top > w.m + AP_SLACK) {
+    if (top > w.m) { /* no slack: no weight is above 1 */
         const float keep = __builtin_amdgcn_exp2f(w.m - top);
         w.m = top;
         w.l *= keep;
@@ -738,7 +738,7 @@ __device__ __forceinline__ void kc_wide_tile(const KcArgs &A, ApRows<D> &w, int 
                 w.o[d][i] *= keep;
     }
     /* not a fused product: a score far from 0 then lies as far above the maximum as that says */
-    const float base = w.m == -INFINITY ? 0.f : w.m - KC_UP;
+    const float base = w.m == -INFINITY ? 0.f : w.m;
     ApFrag ph[4], pl[4];
 #pragma unroll
     for (int n = 0; n < 4; ++n) {
@@ -1053,8 +1053,9 @@ __device__ __forceinline__ bool kc_pass(const KcArgs &A, int me, char (&k0t)[AP_
                 if (i + 1 < end)
                     step(i + 1, sb, sa, (ap_lds *)v1t, (ap_lds *)k0t, (ap_lds *)v0t, (ap_lds *)k1t);
             }
-            w.l = l;
-            const float back = ldexpf(1.f, max(oexp - 14, -300));
+            /* to the values' own size and the softmax's weights, so that no sum is far above the values */
+            w.l = ldexpf(l, -(int)KC_UP);
+            const float back = ldexpf(1.f, max(oexp - 14 - (int)KC_UP, -300));
 #pragma unroll
             for (int d = 0; d < D / 32; ++d)
 #pragma unroll

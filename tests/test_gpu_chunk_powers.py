@@ -160,3 +160,15 @@ def test_values_far_from_one(power, own):
             c.key(j, -30.0)
         c.run()
         c.check(range(192, 256))
+
+
+@pytest.mark.parametrize("own", [False, True])
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_largest_values(D, own):
+    """Sums of some 500 weights times 2^116: in f32 as long as no weight counts as more than 1."""
+    torch_cuda()
+    c = Chunk(500, 100, D, own, 77)
+    c.planes[3] *= np.float32(2.0 ** 116)
+    c.v *= np.float32(2.0 ** 116)
+    c.run()
+    c.check()
