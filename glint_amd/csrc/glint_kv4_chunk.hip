@@ -1225,14 +1225,18 @@ static KcCut kc_cut(int B, int max_q, int H, int G, int D, int max_pages, bool o
 /* Calls that glint_kv4_attend.hip's kernel takes, whose waves decode the pages that they read and whose start is one
  * launch: few rows, or few products in all (as far as the call's bounds say). us, there against here, 8 key heads of
  * 128 dimensions:
- *   rows of a key head       128       256       512       1024
- *   1 sequence of 4000       21, 43    27, 52    33, 73    60, 75
- *   1 sequence of 16000      40, 70    61, 121   101, 104  193, 129
- *   8 sequences of 4000      66, 101   122, 100  224, 127  435, 177
- *   8 sequences of 16000     198, 330  390, 358  758, 475  1497, 707 */
-static bool kc_few(int B, int max_q, int H, int G, int max_pages) {
+ *   rows of a key head       128         192         256        512        1024
+ *   1 sequence of 4000       20, 40      29, 49      27, 49     34, 68     60, 72
+ *   1 sequence of 16000      37, 68      55, 98      61, 116    104, 101   190, 132
+ *   2 sequences of 16000     60, 136     94, 112     101, 116   195, 146   376, 198
+ *   8 sequences of 1000      26, 47      35, 55      45, 58     85, 57     159, 66
+ *   8 sequences of 4000      61, 102     94, 95      118, 100   225, 129   436, 182
+ *   8 sequences of 16000     205, 330    296, 341    389, 353   766, 467   1538, 725
+ *   32 sequences of 1000     80, 89      119, 82     155, 85    302, 131   597, 216
+ * and of 64 dimensions 1 of 16000 24, 49; 33, 71; 36, 79; 58, 75; 109, 94 and 8 of 4000 36, 67; 53, 67; 66, 69; 130, 88; 247, 129. */
+static bool kc_few(int B, int max_q, int H, int G, int D, int max_pages) {
     const int64_t rows = (int64_t)max_q * G;
-    return rows <= 256 || rows * B * H <= ((int64_t)1 << 26) / KV4_PAGE / max_pages;
+    return rows <= 192 || (double)rows * B * H * max_pages * D < 0x1p26; /* a double: the product may pass 2^63 */
 }
 static bool kc_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
     return B >= 0 && max_q >= 1 && H >= 1 && Hq >= H && Hq % H == 0 && Hq <= 65535 && (D == 64 || D == 128) &&
@@ -1242,7 +1246,7 @@ static bool kc_shape(int B, int max_q, int Hq, int H, int D, int max_pages) {
 GLINT_API int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H, int D, int max_pages, int own) {
     if (!kc_shape(B, max_q, Hq, H, D, max_pages))
         return -2;
-    if (B == 0 || (!own && kc_few(B, max_q, H, Hq / H, max_pages)))
+    if (B == 0 || (!own && kc_few(B, max_q, H, Hq / H, D, max_pages)))
         return 0;
     const KcCut c = kc_cut(B, max_q, H, Hq / H, D, max_pages, own != 0);
     return c.seqs ? c.bytes : -2;
@@ -1279,7 +1283,7 @@ GLINT_API int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int6
         return -2;
     if (B == 0 || Tq == 0)
         return 0;
-    if (!k && kc_few(B, max_q, H, Hq / H, max_pages))
+    if (!k && kc_few(B, max_q, H, Hq / H, D, max_pages))
         return glint_kv4_attend_window(q, q_stride_t, q_stride_h, Tq, k_hole, k_absmax, v_hole, v_absmax, pages, table,
                                        table_stride, max_pages, lens, cu_q, B, max_q, Hq, H, D, scale, window, sinks, out, stream);
     if (!scratch)
