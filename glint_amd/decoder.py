@@ -63,6 +63,13 @@ class Decoder:
             raise ValueError(f"{heads} heads over {kv_heads}")
         if window is not None and rotary is None:
             raise ValueError("a window goes with rotary frequencies")
+        H._bounds(window, sinks)  # refused here, where no request has begun
+        if rotary is not None:
+            rot = 2 * rotary.numel()
+            if rotary.dtype is not torch.float64 or rotary.dim() != 1 or not rotary.is_contiguous() or not rotary.is_cuda:
+                raise ValueError(f"rotary frequencies: a contiguous float64 vector on the GPU, got {rotary.dtype} {tuple(rotary.shape)}")
+            if rot % 16 or not 16 <= rot <= head_dim:
+                raise ValueError(f"{rot} of {head_dim} dimensions turned: a multiple of 16")
         self.rotary, self.window, self.sinks = rotary, window, sinks
         self.dim, self.heads, self.kv_heads, self.head_dim, self.ffn, self.pages = dim, heads, kv_heads, head_dim, ffn, pages
         gen = torch.Generator(device="cuda").manual_seed(seed)
