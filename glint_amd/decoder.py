@@ -9,6 +9,7 @@ Weights are random; `python -m glint_amd.decoder` serves a few requests and prin
 """
 from __future__ import annotations
 
+import contextlib
 import time
 
 import torch
@@ -108,6 +109,21 @@ class Decoder:
         self.held[request] = first + n
         return [self.own[request][t // H.KV_PAGE] * H.KV_PAGE + t % H.KV_PAGE for t in range(first, first + n)]
 
+    @contextlib.contextmanager
+    def _undone(self, news):
+        """Requests are as they were where what is within raises: an operator may refuse what _refuse does not know of, or memory
+        run out. What layers wrote belongs to tokens that nobody holds then."""
+        before = {r: (self.held[r], len(self.own[r])) for r in news}
+        try:
+            yield
+        except BaseException:
+            for r, (held, pages) in reversed(before.items()):
+                self.free += reversed(self.own[r][pages:])
+                del self.own[r][pages:]
+                self.table[r, pages:] = -1
+                self.held[r] = held
+            raise
+
     def _slide(self, requests):
         """Pages that no later token of the requests sees are free."""
         if self.window is None:
@@ -169,16 +185,18 @@ class Decoder:
                 return H.attend_prompt(q, k, v, cu, max_q=most, **bounds)
             return H.kv4_attend_chunk(q, layer.cache, table, lens, cu, max_q=most, k=k, v=v, **bounds)
 
-        logits = self._rotated(tokens, pos, slots, attend, True)
-        self._slide(rows)
-        return logits
+        return self._rotated(tokens, pos, slots, attend, True)
 
     def prefill(self, prompts):
-        """prompts: {request: tokens}, new prompts or further chunks. Logits [all tokens, vocab], in order.
-        Where the tokens do not fit, no request changes."""
+        """prompts: {request: tokens}, new prompts or further chunks. Logits [all tokens, vocab], in order. Where the tokens
+        do not fit, or are more than attention takes in a call, no request changes."""
         self._refuse(prompts)
-        if self.rotary is not None:
-            return self._prefill_rotated(prompts)
+        with self._undone(prompts):
+            logits = (self._prefill if self.rotary is None else self._prefill_rotated)(prompts)
+        self._slide(prompts)
+        return logits
+
+    def _prefill(self, prompts):
         ints = lambda v, t=torch.int32: torch.tensor(v, dtype=t, device="cuda")
         tokens, pos, new, seen, keys_new, keys_old, old = [], [], [], [], [], [], []
         cu_q, cu_k = [0], [0]
@@ -208,9 +226,15 @@ class Decoder:
         return self._run(tokens, pos, attend)
 
     def step(self, news):
-        """news: {request: tokens}, the next token of each (or a few drafted ones). Logits [all tokens, vocab].
-        Where the tokens do not fit, no request changes."""
+        """news: {request: tokens}, the next token of each (or a few drafted ones). Logits [all tokens, vocab]. Where the tokens
+        do not fit, or are more than attention takes in a call, no request changes."""
         self._refuse(news)
+        with self._undone(news):
+            logits = self._step(news)
+        self._slide(news)
+        return logits
+
+    def _step(self, news):
         tokens, pos, slots, cu_q = [], [], [], [0]
         for r, some in news.items():
             pos += range(self.held[r], self.held[r] + len(some))
@@ -224,10 +248,8 @@ class Decoder:
 
         most = max(len(t) for t in news.values())
         if self.rotary is not None:
-            logits = self._rotated(tokens, pos, slots, lambda layer, q: H.kv4_attend(
+            return self._rotated(tokens, pos, slots, lambda layer, q: H.kv4_attend(
                 q, layer.cache, table, lens, cu, max_q=most, window=self.window, sinks=self.sinks), False)
-            self._slide(rows)
-            return logits
 
         def attend(layer, q, k, v):
             H.kv4_append(k, v, slots, layer.cache)
