@@ -218,9 +218,10 @@ __global__ __launch_bounds__(KR_T) void k_rotate(RotateArgs A) {
             kt_load8<0>(from + d, w);
         if (!is_v) {
             if (is_k ? A.k_norm : A.q_norm) { /* for all rows of a kind */
-                /* The order of the sum is that of torch's mean over a row (neighbours by pairs, from 128
-                 * dimensions on by fours in turn first), and no product is fused, so that f32 rows have the bits of
-                 * the same formula written there. */
+                /* The sum goes over neighbours by pairs, in rows of more than 64 dimensions by fours in turn first, and no
+                 * product is fused. Rows of 64, 128 and 256 dimensions then have the bits of the formula in elementary f32
+                 * operations whose mean sums in that order, as torch's here does: a key's code, where a quotient lies on
+                 * an edge, is the formula's. Other widths are summed as if zeros followed, and may differ by a rounding. */
                 float q2[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i)
