@@ -4,9 +4,9 @@
  *   pages' codes, and, where the call brings them, the new tokens' own BF16 rows, become f16 operands in
  *   scratch memory, K as [64][D] and V^T as [D][64], in the very order in which the next kernel's LDS holds
  *   them. A tile is scaled by a power of two, so that f16 keeps 11 bits of PARENT * absmax (one rounding) and
- *   all bits of a BF16 element; what one power does not hold is marked (KC_WIDE) and taken as pairs of BF16. Decoding in the attention kernel itself, once for 256 query rows, took 586 us
- *   for 2048 tokens over 16384 where this takes 528: its LDS round trips lie in every wave's way, and a
- *   document's chunk has many row blocks.
+ *   all bits of a BF16 element; what one power does not hold is marked (KC_WIDE) and taken as pairs of BF16.
+ *   Decoding in the attention kernel itself, once for 256 query rows, took 586 us for 2048 tokens over 16384
+ *   where this took 528: its LDS round trips lie in every wave's way, and a document's chunk has many row blocks.
  *
  * k_kv4_chunk — a group is one sequence, key head and block of up to 128 query rows (the heads that share the
  *   key head, times the new tokens), its work the tiles that its rows see. The groups' tiles form one list, and
@@ -19,9 +19,10 @@
  *
  *   What bounds it: 4 D operations a row and key on the matrix units, the vector operations of a score beside
  *   them, and LDS, from which each wave reads every tile. 2048 tokens of 32 heads of 128 over 8 after 14336: 515
- *   GFLOP in 528 to 558 us, of which unpacking takes 24 (its writes; 15 without them), the join 4 and
+ *   GFLOP in 531 to 581 us by device, of which unpacking takes 23 (its writes; 15 without them), the join 4 and
  *   the rest 0.97 PFLOP/s at some 2.0 GHz, where an 8192^3 product of the library reaches 1.2 to 1.3. 512 tokens
- *   in 4 parts a row block with their own BF16 keys: 189 to 196 us, 31 of them unpacking and 18 the join. */
+ *   in 4 parts a row block with their own BF16 keys: 190 to 201 us, 34 of them unpacking (where the form for own
+ *   keys spills 18 registers) and 17 the join; with a window of 1024 57 to 60. */
 #include <algorithm>
 #include <cfloat>
 #include <cmath>

@@ -708,7 +708,8 @@ def kv4_attend_chunk(q, cache, page_table, lens, cu_q=None, max_q: Optional[int]
     """kv4_attend for many new tokens a sequence: arguments, masks and result as there.
 
     k, v bf16 [rows, H, D], both or neither: the new tokens' own keys and values, seen in place of what the
-    cache holds of them (which may then be nothing)."""
+    cache holds of them (which may then be nothing). max_q times the query heads of a key head: at most 2^18. out overlaps
+    no input."""
     if stream is not None:
         with _torch().cuda.stream(stream):
             return kv4_attend_chunk(q, cache, page_table, lens, cu_q, max_q, scale, out, k=k, v=v, window=window, sinks=sinks)

@@ -58,7 +58,9 @@ int glint_kv4_gather(const int64_t *slots, int64_t T, int H, int D, const uint8_
  * BF16 out [Tq][Hq][D]; a row that sees nothing is zero. Rows past max_q, or outside every
  * sequence, are left as they are. q: BF16 bits, strides multiples of 8, 16-B aligned. Scores,
  * softmax and sums are f32; PARENT and the softmax weights times the value scales enter the
- * matrix products in f16. A batch whose list of work passes 2^30 goes in several launches, and
+ * matrix products in f16, under a power of two that follows the largest value scale met: a weight times its
+ * value scale loses bits below 2^-24 of that scale, and below 2^-35, or a weight below 2^-25, adds nothing but to the
+ * weights' sum. A batch whose list of work passes 2^30 goes in several launches, and
  * a sequence for which H max_q (Hq / H) max_pages / 16 does is -2.
  * Long sequences are split over workgroups that meet in a workspace of the
  * stream's (glint_serve_workspace_reserve): it is allocated by the first such call outside a
@@ -89,8 +91,9 @@ int glint_kv4_attend_window(const uint16_t *q, int64_t q_stride_t, int64_t q_str
  * and of elements below 2^-14 of the largest of the token's 64 dimensions 2^-20 of that largest may be lost. 64 tokens whose
  * values span more (2^12 and more from one token's largest to another's, or sizes past 2^+-32), or whose scores might pass 2^21,
  * enter as pairs of BF16, at some ten times the cost and a second pass over what their workgroup has: what a row gives
- * no weight, or does not see, costs it no bits. out overlaps no input. A value that is not finite leaves itself or NaN in its dimension of the rows that see it.
- * max_q (Hq / H) is at most 2^18. Few rows without own keys go as glint_kv4_attend_window does, its refusals and its
+ * no weight, or does not see, costs it no bits. A weight below 2^-32 of its row's largest adds nothing but to the weights'
+ * sum. out overlaps no input. A value that is not finite leaves itself or NaN in its dimension of the rows that see it.
+ * max_q (Hq / H) is at most 2^18. Few rows without own keys go as glint_kv4_attend_window does, its limits, refusals and
  * workspace included, and _scratch gives 0. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a shape that is
  * refused) for the current device; the call's alone until it has run. */
 int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H, int D, int max_pages, int own);
@@ -139,7 +142,8 @@ int glint_attend_prompt_window(const uint16_t *q, int64_t q_stride_t, int64_t q_
  * 2^51 it means nothing). D a multiple of 16, 16 .. 256, rot one too, 16 .. D. q, k and the outputs
  * q_out [T][Hq][D], k_out [T][H][D] are of type elt (GLINT_KV_BF16 or GLINT_KV_F32); an output may be its
  * own input where that is as contiguous. q_norm and k_norm [D], each or NULL, are of type norm_elt. Addresses
- * are 16-B aligned, strides multiples of 16 B. */
+ * are 16-B aligned, strides multiples of 16 B. A launch holds 2^23 - 1 workgroups (from 2048 tokens on one a token, and
+ * into the cache one for 32 tokens' values of a head): more is -2. */
 int glint_rotate_qk(const void *q, int64_t q_stride_t, int64_t q_stride_h, const void *k, int64_t k_stride_t,
                     int64_t k_stride_h, int elt, const int64_t *pos, const double *freqs, int64_t T, int Hq, int H, int D,
                     int rot, int interleaved, double magnitude, const void *q_norm, const void *k_norm, int norm_elt,
