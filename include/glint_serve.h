@@ -83,19 +83,21 @@ int glint_kv4_attend_window(const uint16_t *q, int64_t q_stride_t, int64_t q_str
                             int sinks, uint16_t *out, struct ihipStream_t *stream);
 
 /* Attention of B sequences' newest tokens over the cache, for many of them a sequence: arguments and result as
- * glint_kv4_attend_window, out 16-B aligned. Where k and v are given [Tq], BF16, rows as q's, strides
- * multiples of 8, stride_t from D to 2^24, 16-B aligned, they are the new tokens' keys and values, and what the
- * cache holds of these tokens is not read (it need not hold them; its max_pages bound the tokens before them
- * alone; a length past 2^31 - 65 counts as that). Scores, softmax and sums are f32; keys, values and softmax weights enter the matrix products in
- * f16, 64 tokens' keys under one power of two and their values under another: a held element is rounded by 2^-11 of itself,
- * and of elements below 2^-14 of the largest of the token's 64 dimensions 2^-20 of that largest may be lost. 64 tokens whose
- * values span more (2^12 and more from one token's largest to another's, or sizes past 2^+-32), or whose scores might pass 2^21,
- * enter as pairs of BF16, at some ten times the cost and a second pass over what their workgroup has: what a row gives
- * no weight, or does not see, costs it no bits. A weight below 2^-32 of its row's largest adds nothing but to the weights'
- * sum. out overlaps no input. A value that is not finite leaves itself or NaN in its dimension of the rows that see it.
- * max_q (Hq / H) is at most 2^18. Few rows without own keys go as glint_kv4_attend_window does, its limits, refusals and
- * workspace included, and _scratch gives 0. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a shape that is
- * refused) for the current device; the call's alone until it has run. */
+ * glint_kv4_attend_window, out 16-B aligned and apart from every input. Where k and v are given [Tq], BF16, rows as
+ * q's, strides multiples of 8, stride_t from D to 2^24, 16-B aligned, they are the new tokens' keys and values, and
+ * what the cache holds of these tokens is not read (it need not hold them; its max_pages bound the tokens before
+ * them alone; a length past 2^31 - 65 counts as that).
+ * Scores, softmax and sums are f32; keys, values and softmax weights enter the matrix products in f16, 64 tokens'
+ * keys under one power of two and their values under another: a held element is rounded by 2^-11 of itself, and of
+ * elements below 2^-14 of the largest of the token's 64 dimensions 2^-20 of that largest may be lost. 64 tokens
+ * whose values span more (2^12 and more from one token's largest to another's, or sizes past 2^+-32), or whose scores
+ * might pass 2^21, enter as pairs of BF16, at some ten times the cost and a second pass over what their workgroup has:
+ * what a row gives no weight, or does not see, costs it no bits. A weight below 2^-32 of its row's largest adds
+ * nothing but to the weights' sum. A value that is not finite leaves itself or NaN in its dimension of the rows that
+ * see it.
+ * max_q (Hq / H) is at most 2^18. Few rows without own keys go as glint_kv4_attend_window does, its limits, refusals
+ * and workspace included, and _scratch gives 0. scratch: 16-B aligned, at least as many bytes as _scratch gives (-2: a
+ * shape that is refused) for the current device; the call's alone until it has run. */
 int64_t glint_kv4_attend_chunk_scratch(int B, int max_q, int Hq, int H, int D, int max_pages, int own);
 int glint_kv4_attend_chunk(const uint16_t *q, int64_t q_stride_t, int64_t q_stride_h, int64_t Tq, const uint8_t *k_hole,
                            const float *k_absmax, const uint8_t *v_hole, const float *v_absmax, int64_t pages,
